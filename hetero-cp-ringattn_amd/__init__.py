@@ -11,6 +11,8 @@ The operator names mirror the reference's ring-attention backend
   ``hcp_paged_decode_partial``
 * :func:`paged_kv_gather` / :func:`paged_kv_scatter`  the vLLM block extract / insert of
   python/hcp_vllm_block_ring_plugin.py:143-174, 304-337 -> ``hcp_paged_kv_*``
+* :func:`kv_plan_step`  block tables, slots and positions of a step from request lengths ->
+  ``hcp_kv_plan_step`` (no reference counterpart)
 * :func:`ring_attention_replay`             ring.rs:861-1398 for every domain on one GPU ->
   ``hcp_ring_prefill_replay`` (``_paged`` variant stages K/V from a block pool)
 
@@ -22,6 +24,7 @@ ABI status code and the library's message.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -282,6 +285,9 @@ def lib() -> ctypes.CDLL:
         "hcp_block_poll_transfers": ([vp, ctypes.POINTER(BlockCompletionC), ctypes.c_size_t,
                                       ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
         "hcp_block_wire_bytes": ([vp, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)], ctypes.c_int),
+        "hcp_kv_plan_workspace_size": ([i32], ctypes.c_size_t),
+        "hcp_kv_plan_step": ([i32, i32, i64, vp, vp, vp, i64, i64, vp, vp, i64, vp, vp, vp, vp, vp, vp,
+                              ctypes.c_size_t, vp], ctypes.c_int),
         "hcp_ring_trace_attach": ([vp, ctypes.c_size_t], ctypes.c_int),
         "hcp_ring_trace_record_bytes": ([ctypes.POINTER(ReplayDesc)], ctypes.c_size_t),
         "hcp_ring_trace_read": ([vp, ctypes.POINTER(TraceDomain), i32, ctypes.POINTER(i32),
@@ -603,6 +609,79 @@ def decode_ring_replay(q, pool, shards, seed_domain, scale=None, out=None, lse_o
     _check(lib().hcp_decode_ring_replay(ctypes.byref(desc), ctypes.byref(pp), qv, n, arr, seed_domain, ov,
                                         _ptr(lse_out), _ptr(workspace), workspace.numel(), _stream(stream)))
     return out, lse_out
+
+
+# ---------------------------------------------------------------------------------
+# (9) step plan of a paged cache
+# ---------------------------------------------------------------------------------
+def _want(name, t, dtype, shape, device):
+    """Refuses a tensor that a kernel could not read as ``dtype`` [shape] on ``device``."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+
+
+def _on(device):
+    """Context in which ``device`` is the current one (kernels and error flags go by it)."""
+    torch = _torch()
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a GPU, not on {device}")
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def kv_plan_workspace_size(batch: int) -> int:
+    """Workspace bytes of :func:`kv_plan_step`."""
+    return lib().hcp_kv_plan_workspace_size(batch)
+
+
+def kv_plan_step(seq_lens, new_lens, block_tables, free_blocks, free_count, block_size: int, capacity=None, slots=None,
+                 positions=None, token_starts=None, seq_lens_out=None, free_count_out=None, workspace=None, stream=None):
+    """Block tables, slots and positions of a step, built on the GPU from request lengths.
+
+    seq_lens / new_lens [B] int32: tokens held and tokens to add (negative: the sequence
+    ended and gives its blocks back); block_tables [B, n] int32 and free_blocks
+    [num_blocks] int32, a stack of height free_count [1] int32, are updated in place.
+    Returns (slots [capacity] int64, positions [capacity] int64, token_starts [B + 1]
+    int32, seq_lens_out [B] int32, free_count_out [1] int32); pass seq_lens and free_count
+    as the last two to have them updated in place.  A sequence that cannot be served (too
+    few free blocks, a full table, a token past ``capacity``) keeps its length, and its
+    tokens get slot -1, as the places past the last token do."""
+    torch = _torch()
+    b, dev = seq_lens.shape[0], seq_lens.device
+    if slots is not None:
+        capacity = slots.shape[0]
+    elif capacity is None:
+        raise ValueError("kv_plan_step needs a capacity or slots")
+    i32, i64 = torch.int32, torch.int64
+    new = lambda n, dt: torch.empty(n, dtype=dt, device=dev)  # noqa: E731
+    slots = new(capacity, i64) if slots is None else slots
+    positions = new(capacity, i64) if positions is None else positions
+    token_starts = new(b + 1, i32) if token_starts is None else token_starts
+    seq_lens_out = new(b, i32) if seq_lens_out is None else seq_lens_out
+    free_count_out = new(1, i32) if free_count_out is None else free_count_out
+    for name, t, dt, n in (("seq_lens", seq_lens, i32, b), ("new_lens", new_lens, i32, b),
+                           ("free_blocks", free_blocks, i32, free_blocks.numel()), ("free_count", free_count, i32, 1),
+                           ("slots", slots, i64, capacity), ("positions", positions, i64, capacity),
+                           ("token_starts", token_starts, i32, b + 1), ("seq_lens_out", seq_lens_out, i32, b),
+                           ("free_count_out", free_count_out, i32, 1)):
+        _want(name, t, dt, (n,), dev)
+    if block_tables.dtype != i32 or block_tables.dim() != 2 or block_tables.shape[0] != b or block_tables.device != dev \
+            or (block_tables.stride(1) != 1 and block_tables.shape[1] > 1):
+        raise ValueError(f"block_tables must be an int32 tensor of {b} contiguous rows on {dev}")
+    if workspace is None:
+        workspace = torch.empty(max(kv_plan_workspace_size(b), 1), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev:
+        raise ValueError(f"workspace must be on {dev}")
+    with _on(dev):
+        _check(lib().hcp_kv_plan_step(b, block_size, free_blocks.numel(), seq_lens.data_ptr(), new_lens.data_ptr(),
+                                      block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
+                                      free_blocks.data_ptr(), free_count.data_ptr(), capacity, token_starts.data_ptr(),
+                                      slots.data_ptr(), positions.data_ptr(), seq_lens_out.data_ptr(),
+                                      free_count_out.data_ptr(), workspace.data_ptr(),
+                                      workspace.numel() * workspace.element_size(), _stream(stream)))
+    return slots, positions, token_starts, seq_lens_out, free_count_out
 
 
 # ---------------------------------------------------------------------------------

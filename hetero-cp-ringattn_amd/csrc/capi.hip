@@ -1777,6 +1777,34 @@ int hcp_ring_trace_perf_log(void* stream, int32_t layer_idx, const char* path) {
   });
 }
 
+// ---- (9) step plan of a paged cache ----
+size_t hcp_kv_plan_workspace_size(int32_t batch) { return batch > 0 ? kv_plan_workspace_bytes(batch) : 0; }
+
+int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, const int32_t* seq_lens,
+                     const int32_t* new_lens, int32_t* block_tables, int64_t table_stride, int64_t table_len,
+                     int32_t* free_blocks, const int32_t* free_count, int64_t capacity, int32_t* token_starts,
+                     int64_t* slots, int64_t* positions, int32_t* seq_lens_out, int32_t* free_count_out,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded(__func__, [&] {
+    require(batch > 0, "batch must be positive");
+    require(block_size > 0, "block_size must be positive");
+    require(num_blocks > 0 && num_blocks <= INT32_MAX, "num_blocks must be in [1, 2^31)");
+    require(capacity >= 0 && capacity <= INT32_MAX, "capacity must be in [0, 2^31)");
+    require(table_len >= 1 && table_stride >= table_len, "bad table shape");
+    require(seq_lens != nullptr && new_lens != nullptr && block_tables != nullptr && free_blocks != nullptr &&
+                free_count != nullptr && token_starts != nullptr && seq_lens_out != nullptr && free_count_out != nullptr,
+            "null pointer");
+    require(capacity == 0 || (slots != nullptr && positions != nullptr), "null slots or positions");
+    const size_t need = kv_plan_workspace_bytes(batch);
+    require(workspace != nullptr && workspace_bytes >= need, "workspace too small: need " + std::to_string(need) + " bytes");
+    require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
+    launch_kv_plan(KvPlan{batch, block_size, num_blocks, seq_lens, new_lens, block_tables, table_stride, table_len,
+                          free_blocks, free_count, capacity, token_starts, seq_lens_out, free_count_out, slots, positions,
+                          device_error_flags()},
+                   workspace, as_stream(stream));
+  });
+}
+
 int hcp_ring_replay_timing(int32_t enable) {
   return guarded(__func__, [&] {
     ReplayTiming& t = timing();

@@ -135,6 +135,24 @@ void launch_paged_decode(int dtype, int batch, int hq, int hkv, int d, const voi
                          const DecodeSpan* spans, float scale, int out_dtype, void* out, int64_t out_rs, float* lse,
                          void* ws, size_t ws_bytes, int* err, hipStream_t stream);
 
+// The plan of one step of a paged cache (kv_plan.hip); pointers and their meaning as in
+// hcp_kv_plan_step.
+struct KvPlan {
+  int32_t batch, bs;
+  int64_t num_blocks;
+  const int32_t *seq_lens, *new_lens;
+  int32_t* block_tables;
+  int64_t table_stride, table_len;
+  int32_t* free_blocks;
+  const int32_t* free_count;
+  int64_t capacity;
+  int32_t *token_starts, *seq_lens_out, *free_count_out;
+  int64_t *slots, *positions;
+  int* err;
+};
+size_t kv_plan_workspace_bytes(int batch);
+void launch_kv_plan(const KvPlan& p, void* ws, hipStream_t stream);
+
 // Scheduling strategies (strategy.rs:14-24) and their closed-form positions; see
 // positions.hip.
 enum Strategy : int32_t { kStrategyVanilla = 0, kStrategyStriped = 1, kStrategyZigZag = 2 };

@@ -109,7 +109,8 @@ int hcp_ring_last_key_parts(void);
  * bit 1: a replay's generated key positions were not non-decreasing (an internal
  *        consistency check; hcp_ring_block_partial_positioned takes keys in any order
  *        and never sets it);
- * bit 2: a RoPE position outside the cos / sin table).
+ * bit 2: a RoPE position outside the cos / sin table;
+ * bit 3: lengths or a free-block count that hcp_kv_plan_step cannot follow).
  * Synchronises `stream`.
  */
 int hcp_ring_fetch_device_errors(void* stream, int* flags);
@@ -683,6 +684,44 @@ int hcp_block_submit_transfer(hcp_block_agent* agent, uint64_t local_block_id,
 int hcp_block_poll_transfers(hcp_block_agent* agent, hcp_block_completion* out, size_t capacity,
                              size_t* n);
 int hcp_block_wire_bytes(const hcp_block_agent* agent, uint64_t* sent, uint64_t* recv);
+
+/* ---------------------------------------------------------------------------------
+ * (9) Step plan of a paged cache from request lengths (no reference counterpart: its
+ * block tables are built on the host, one sequence at a time).
+ *
+ * Sequence b holds seq_lens[b] tokens in the blocks of row b of block_tables and adds
+ * new_lens[b] tokens; a negative new_lens[b] says that it ended.  free_blocks (num_blocks
+ * entries) is a stack of free block ids of height *free_count.  With used = ceil(seq_lens /
+ * block_size) and need = ceil((seq_lens + new_lens) / block_size) - used:
+ *   1. the blocks of the ended sequences go on the stack, in order of b and of their row;
+ *   2. blocks are taken from the stack's top in order of b, each into entry used, used + 1,
+ *      ... of its sequence's row.  A sequence is served if (seq_lens + new_lens) fits
+ *      table_len entries, its tokens lie within the first `capacity` of all, and need is 0
+ *      or the needs up to and including it fit the stack.  One that is not served keeps its
+ *      length and its row.
+ * Written: token_starts [batch + 1] (token i of the step belongs to the b with
+ * token_starts[b] <= i < token_starts[b + 1], served or not); for i < capacity slots[i] =
+ * block * block_size + (position mod block_size), -1 for a token that was not served and
+ * from token_starts[batch] on; positions[i] = the token's position in its sequence (0 from
+ * token_starts[batch] on); seq_lens_out [batch] (0 for an ended sequence) and
+ * *free_count_out, which may be seq_lens and free_count themselves; new entries of
+ * block_tables, and of free_blocks the ended sequences' blocks that lie above the old
+ * height and below the new one.  Nothing else of the two is touched.
+ * A negative length, one beyond its table, a free_count outside [0, num_blocks] or more
+ * blocks than free_blocks holds set device error bit 3 (such a sequence is not served, what
+ * does not fit the stack is dropped); a table or stack entry outside [0, num_blocks) sets
+ * bit 0 and its tokens get slot -1.  All arrays are DEVICE memory; nothing is read on the
+ * host, so a captured graph follows the lengths.  No two sequences may hold a block in
+ * common.  Workspace: hcp_kv_plan_workspace_size(batch) bytes, 256-byte aligned.
+ * ------------------------------------------------------------------------------- */
+size_t hcp_kv_plan_workspace_size(int32_t batch);
+
+int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, const int32_t* seq_lens,
+                     const int32_t* new_lens, int32_t* block_tables, int64_t table_stride,
+                     int64_t table_len, int32_t* free_blocks, const int32_t* free_count,
+                     int64_t capacity, int32_t* token_starts, int64_t* slots, int64_t* positions,
+                     int32_t* seq_lens_out, int32_t* free_count_out, void* workspace,
+                     size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * Replay kernel timing (no reference counterpart; benchmark instrumentation; the
