@@ -13,6 +13,9 @@ The operator names mirror the reference's ring-attention backend
   python/hcp_vllm_block_ring_plugin.py:143-174, 304-337 -> ``hcp_paged_kv_*``
 * :func:`kv_plan_step`  block tables, slots and positions of a step from request lengths ->
   ``hcp_kv_plan_step`` (no reference counterpart)
+* :func:`kv8_append` / :func:`kv8_gather` / :func:`kv8_ring_attention_replay_paged`  a paged
+  K/V cache in 8 bits with a scale per block and head -> ``hcp_kv8_*`` (no reference
+  counterpart)
 * :func:`ring_attention_replay`             ring.rs:861-1398 for every domain on one GPU ->
   ``hcp_ring_prefill_replay`` (``_paged`` variant stages K/V from a block pool)
 
@@ -288,6 +291,11 @@ def lib() -> ctypes.CDLL:
         "hcp_kv_plan_workspace_size": ([i32], ctypes.c_size_t),
         "hcp_kv_plan_step": ([i32, i32, i64, vp, vp, vp, i64, i64, vp, vp, i64, vp, vp, vp, vp, vp, vp,
                               ctypes.c_size_t, vp], ctypes.c_int),
+        "hcp_kv8_append": ([ctypes.POINTER(PagedPool), vp, i32, i32, View, View, i64, vp, vp], ctypes.c_int),
+        "hcp_kv8_gather": ([ctypes.POINTER(PagedPool), vp, i32, i32, vp, i64, i64, i64, i64, View, View, vp],
+                           ctypes.c_int),
+        "hcp_kv8_prefill_replay_paged": ([ctypes.POINTER(ReplayDesc), View, ctypes.POINTER(PagedPool), vp, i32, vp,
+                                          i64, View, vp, vp, ctypes.c_size_t, vp], ctypes.c_int),
         "hcp_ring_trace_attach": ([vp, ctypes.c_size_t], ctypes.c_int),
         "hcp_ring_trace_record_bytes": ([ctypes.POINTER(ReplayDesc)], ctypes.c_size_t),
         "hcp_ring_trace_read": ([vp, ctypes.POINTER(TraceDomain), i32, ctypes.POINTER(i32),
@@ -751,6 +759,104 @@ def ring_attention_replay_paged(q, pool, block_table, chunks, causal=True, scale
                                                _ptr(block_table), block_table.numel(), view(out),
                                                _ptr(lse_out), _ptr(workspace), workspace.numel(),
                                                _stream(stream)))
+    del arr
+    return out, lse_out
+
+
+# ---------------------------------------------------------------------------------
+# (10) 8-bit paged K/V cache
+# ---------------------------------------------------------------------------------
+KV8_E4M3, KV8_INT8 = 1, 2
+
+
+def kv8_pool(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int, dtype=None, device="cuda"):
+    """An empty 8-bit cache: (pool [2, num_blocks, block_size, Hkv, D] float8_e4m3fn (default)
+    or int8, scales [2, num_blocks, Hkv] fp32); a code stands for scale * code."""
+    torch = _torch()
+    pool = torch.zeros(2, num_blocks, block_size, num_kv_heads, head_dim, dtype=torch.uint8, device=device)
+    return (pool.view(dtype or torch.float8_e4m3fn),
+            torch.zeros(2, num_blocks, num_kv_heads, dtype=torch.float32, device=device))
+
+
+def _kv8(pool, scales):
+    """(hcp_paged_pool, HCP_KV8_* of the pool's type)."""
+    torch = _torch()
+    fmt = {torch.float8_e4m3fn: KV8_E4M3, torch.int8: KV8_INT8}.get(pool.dtype)
+    if fmt is None:
+        raise ValueError("an 8-bit pool is float8_e4m3fn or int8")
+    pp = paged_pool(pool)
+    _want("scales", scales, torch.float32, (2, pool.shape[1], pool.shape[3]), pool.device)
+    return pp, fmt
+
+
+def _rows_of(name, t, shape, pool, dtype=None):
+    if tuple(t.shape) != tuple(shape) or t.device != pool.device or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name} must be [{', '.join(str(n) for n in shape)}] on {pool.device}"
+                         + (f" in {dtype}" if dtype is not None else ""))
+
+
+def kv8_append(pool, scales, k, v, slots, stream=None):
+    """Quantise the rows of k / v [Hkv, T, D] into the slots [T] int64 of an 8-bit cache
+    (:func:`kv_plan_step`; negative: skipped).  A block's scale is a power of two that only
+    grows while the block fills; rows held already are rounded to the new one."""
+    torch = _torch()
+    pp, fmt = _kv8(pool, scales)
+    tokens = slots.shape[0]
+    shape = (pool.shape[3], tokens, pool.shape[4])
+    _rows_of("k", k, shape, pool)
+    _rows_of("v", v, shape, pool, k.dtype)
+    _want("slots", slots, torch.int64, (tokens,), pool.device)
+    with _on(pool.device):
+        _check(lib().hcp_kv8_append(ctypes.byref(pp), scales.data_ptr(), fmt, dtype_code(k.dtype), view(k), view(v),
+                                    tokens, slots.data_ptr(), _stream(stream)))
+
+
+def kv8_gather(pool, scales, block_table, table_seq_offset, t0, t1, dtype=None, k_out=None, v_out=None, stream=None):
+    """As :func:`paged_kv_gather` from an 8-bit cache: scale * code rounded to ``dtype``
+    (default bfloat16) -> k, v [Hkv, t1 - t0, D]."""
+    torch = _torch()
+    pp, fmt = _kv8(pool, scales)
+    shape = (pool.shape[3], t1 - t0, pool.shape[4])
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=dtype or torch.bfloat16, device=pool.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=k_out.dtype, device=pool.device)
+    _rows_of("k_out", k_out, shape, pool, dtype)
+    _rows_of("v_out", v_out, shape, pool, k_out.dtype)
+    _want("block_table", block_table, torch.int32, (block_table.numel(),), pool.device)
+    with _on(pool.device):
+        _check(lib().hcp_kv8_gather(ctypes.byref(pp), scales.data_ptr(), fmt, dtype_code(k_out.dtype),
+                                    block_table.data_ptr(), block_table.numel(), table_seq_offset, t0, t1, view(k_out),
+                                    view(v_out), _stream(stream)))
+    return k_out, v_out
+
+
+def kv8_ring_attention_replay_paged(q, pool, scales, block_table, chunks, causal=True, scale=None, out=None,
+                                    lse_out=None, workspace=None, stream=None, strategy="vanilla", schedule="auto"):
+    """As :func:`ring_attention_replay_paged`, K/V staged from an 8-bit cache in q's type."""
+    torch = _torch()
+    pp, fmt = _kv8(pool, scales)
+    hq, s, d = q.shape
+    hkv = pool.shape[3]
+    desc, arr = replay_desc(q.dtype, hq, hkv, d, chunks, causal, scale, strategy, schedule)
+    _want("block_table", block_table, torch.int32, (block_table.numel(),), pool.device)
+    if s != sum(chunks):
+        raise ValueError(f"invalid chunk sum: actual {sum(chunks)}, expected {s}")
+    if workspace is None:
+        need = lib().hcp_ring_replay_workspace_size(ctypes.byref(desc), 1)
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+    if out is None:
+        out = torch.empty((hq, s, d), dtype=q.dtype, device=q.device)
+    if lse_out is None:
+        lse_out = torch.empty((hq, s), dtype=torch.float32, device=q.device)
+    _rows_of("q", q, (hq, s, d), pool)
+    _rows_of("out", out, (hq, s, d), pool, q.dtype)
+    _want("lse_out", lse_out, torch.float32, (hq, s), pool.device)
+    with _on(pool.device):
+        _check(lib().hcp_kv8_prefill_replay_paged(ctypes.byref(desc), view(q), ctypes.byref(pp), scales.data_ptr(), fmt,
+                                                  block_table.data_ptr(), block_table.numel(), view(out),
+                                                  lse_out.data_ptr(), workspace.data_ptr(),
+                                                  workspace.numel() * workspace.element_size(), _stream(stream)))
     del arr
     return out, lse_out
 

@@ -564,9 +564,11 @@ void trace_stats(hipStream_t stream, std::vector<hcp_ring_trace_domain>& doms, h
   }
 }
 
+// codes8: the pool's codes and scales where it is an 8-bit one (staged in the descriptor's dtype).
 void run_replay(const hcp_ring_replay_desc* d, hcp_ring_view q, hcp_ring_view k, hcp_ring_view v,
                 const hcp_paged_pool* pool, const int32_t* table, int64_t table_len,
-                hcp_ring_view out, float* lse_out, void* ws, size_t ws_bytes, hipStream_t stream) {
+                hcp_ring_view out, float* lse_out, void* ws, size_t ws_bytes, hipStream_t stream,
+                const Kv8Pool* codes8 = nullptr) {
   const bool paged = pool != nullptr;
   ReplayPlan p = plan_replay(d, paged);
   g_last_path = HCP_PATH_NONE;
@@ -583,13 +585,23 @@ void run_replay(const hcp_ring_replay_desc* d, hcp_ring_view q, hcp_ring_view k,
     require(pool->data != nullptr && table != nullptr, "null pool or block table");
     require(pool->num_kv_heads == d->num_kv_heads && pool->head_dim == d->head_dim,
             "pool shape does not match the descriptor");
-    require(pool->elem_bytes == es, "pool element size does not match dtype");
+    require(codes8 != nullptr || pool->elem_bytes == es, "pool element size does not match dtype");
     require(pool->block_size >= 1, "block_size must be >= 1");
     require((p.seq - 1) / pool->block_size < table_len, "block table shorter than the sequence");
   } else {
     check_view(k, "k", p.seq);
     check_view(v, "v", p.seq);
   }
+  auto stage = [&](const std::vector<PagedRangeDesc>& rs) {
+    timed(kTimedGather, stream, [&] {
+      if (codes8 != nullptr)
+        launch_kv8_gather(*codes8, d->dtype, static_cast<int>(rs.size()), rs.data(), err, stream);
+      else
+        launch_paged_copy_batch(true, pool->data, pool->num_blocks, pool->block_size, pool->num_kv_heads,
+                                pool->head_dim, pool->elem_bytes, static_cast<int>(rs.size()), rs.data(), 0, err,
+                                stream);
+    });
+  };
   // Fused schedule: one matrix-core launch for the whole replay -- BF16/F16 (head_dim a
   // multiple of 8 up to 128, 16-byte rows): the fused ring for vanilla positions, one
   // positions-mode block over the sequence otherwise; FP32 (head_dim a multiple of 4 up
@@ -618,11 +630,7 @@ void run_replay(const hcp_ring_replay_desc* d, hcp_ring_view q, hcp_ring_view k,
         rs.push_back(PagedRangeDesc{table, 0, p.off[s], p.off[s] + p.len[s], static_cast<char*>(kk.data) + o * es,
                                     static_cast<char*>(vv.data) + o * es, hs, d->head_dim});
       }
-      timed(kTimedGather, stream, [&] {
-        launch_paged_copy_batch(true, pool->data, pool->num_blocks, pool->block_size, pool->num_kv_heads,
-                                pool->head_dim, pool->elem_bytes, static_cast<int>(rs.size()), rs.data(), 0, err,
-                                stream);
-      });
+      stage(rs);
     }
     if (p.positioned) {
       run_replay_fused_positioned(d, p, q, kk, vv, out, lse_out, base, stream);
@@ -677,11 +685,7 @@ void run_replay(const hcp_ring_replay_desc* d, hcp_ring_view q, hcp_ring_view k,
         rs.push_back(PagedRangeDesc{table, 0, p.off[src], p.off[src] + p.len[src], ks[t].data, vs[t].data, hs,
                                     d->head_dim});
       }
-      timed(kTimedGather, stream, [&] {
-        launch_paged_copy_batch(true, pool->data, pool->num_blocks, pool->block_size, pool->num_kv_heads,
-                                pool->head_dim, pool->elem_bytes, static_cast<int>(rs.size()), rs.data(), 0, err,
-                                stream);
-      });
+      stage(rs);
     }
     // The step's blocks write distinct targets' state: one grouped launch.
     std::vector<BlockLaunch> step_launches;
@@ -1802,6 +1806,87 @@ int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, cons
                           free_blocks, free_count, capacity, token_starts, seq_lens_out, free_count_out, slots, positions,
                           device_error_flags()},
                    workspace, as_stream(stream));
+  });
+}
+
+// ---- (10) 8-bit paged cache ----
+}  // extern "C": internal helpers below have C++ linkage
+namespace {
+Kv8Pool check_kv8(const hcp_paged_pool* pool, const float* scales, int32_t format) {
+  require(pool != nullptr && pool->data != nullptr, "null pool");
+  require(pool->num_blocks > 0 && pool->block_size > 0 && pool->num_kv_heads > 0, "pool dimensions must be positive");
+  require(pool->num_blocks <= INT32_MAX, "num_blocks must be in [1, 2^31)");
+  require(pool->elem_bytes == 1, "an 8-bit pool has elem_bytes 1");
+  require(pool->head_dim > 0 && pool->head_dim <= 256 && pool->head_dim % 8 == 0,
+          "head_dim must be a multiple of 8 up to 256");
+  require(reinterpret_cast<uintptr_t>(pool->data) % 16 == 0, "the pool must be 16-byte aligned");
+  require(scales != nullptr && reinterpret_cast<uintptr_t>(scales) % 4 == 0, "null or unaligned scales");
+  require(format == HCP_KV8_E4M3 || format == HCP_KV8_INT8, "format must be 1 (E4M3) or 2 (INT8)");
+  return Kv8Pool{static_cast<uint8_t*>(pool->data), const_cast<float*>(scales), format, pool->num_blocks,
+                 pool->block_size, pool->num_kv_heads, pool->head_dim};
+}
+
+// Element accesses of a view: its rows start on element boundaries.
+void check_rows(const hcp_ring_view& v, const char* name, int64_t len, int dtype) {
+  check_view(v, name, len);
+  require(reinterpret_cast<uintptr_t>(v.data) % elem_size(dtype) == 0, std::string(name) + ": not aligned to its elements");
+}
+}  // namespace
+extern "C" {
+
+int hcp_kv8_append(const hcp_paged_pool* pool, float* scales, int32_t format, int32_t dtype, hcp_ring_view k,
+                   hcp_ring_view v, int64_t tokens, const int64_t* slots, void* stream) {
+  return guarded(__func__, [&] {
+    const Kv8Pool c = check_kv8(pool, scales, format);
+    elem_size(dtype);
+    require(tokens >= 0 && tokens <= INT32_MAX, "tokens must be in [0, 2^31)");
+    if (tokens == 0) return;
+    check_rows(k, "k", tokens, dtype);
+    check_rows(v, "v", tokens, dtype);
+    require(slots != nullptr, "null slots");
+    Kv8Append p;
+    p.pool = c.codes;
+    p.scales = c.scales;
+    p.num_blocks = c.num_blocks;
+    p.bs = c.bs;
+    p.hkv = c.hkv;
+    p.d = c.d;
+    p.src[0] = k.data; p.src[1] = v.data;
+    p.hs[0] = k.head_stride; p.hs[1] = v.head_stride;
+    p.ss[0] = k.seq_stride; p.ss[1] = v.seq_stride;
+    p.tokens = tokens;
+    p.slots = slots;
+    p.err = device_error_flags();
+    launch_kv8_append(format, dtype, p, as_stream(stream));
+  });
+}
+
+int hcp_kv8_gather(const hcp_paged_pool* pool, const float* scales, int32_t format, int32_t dtype,
+                   const int32_t* block_table, int64_t table_len, int64_t table_seq_offset, int64_t t0, int64_t t1,
+                   hcp_ring_view k_out, hcp_ring_view v_out, void* stream) {
+  return guarded(__func__, [&] {
+    const Kv8Pool c = check_kv8(pool, scales, format);
+    elem_size(dtype);
+    check_paged_range(pool, block_table, table_len, table_seq_offset, t0, t1);
+    check_rows(k_out, "k_out", t1 - t0, dtype);
+    check_rows(v_out, "v_out", t1 - t0, dtype);
+    require(k_out.head_stride == v_out.head_stride && k_out.seq_stride == v_out.seq_stride,
+            "k_out and v_out must share strides");
+    const PagedRangeDesc r{block_table, table_seq_offset, t0, t1, k_out.data, v_out.data, k_out.head_stride,
+                           k_out.seq_stride};
+    launch_kv8_gather(c, dtype, 1, &r, device_error_flags(), as_stream(stream));
+  });
+}
+
+int hcp_kv8_prefill_replay_paged(const hcp_ring_replay_desc* desc, hcp_ring_view q, const hcp_paged_pool* pool,
+                                 const float* scales, int32_t format, const int32_t* block_table, int64_t table_len,
+                                 hcp_ring_view out, float* lse_out, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  return guarded(__func__, [&] {
+    const Kv8Pool c = check_kv8(pool, scales, format);
+    hcp_ring_view none{nullptr, 0, 1};
+    run_replay(desc, q, none, none, pool, block_table, table_len, out, lse_out, workspace, workspace_bytes,
+               as_stream(stream), &c);
   });
 }
 

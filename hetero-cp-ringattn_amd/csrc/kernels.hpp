@@ -153,6 +153,44 @@ struct KvPlan {
 size_t kv_plan_workspace_bytes(int batch);
 void launch_kv_plan(const KvPlan& p, void* ws, hipStream_t stream);
 
+// The 8-bit paged cache (kv8.hpp): append through a slot map, gather to contiguous rows.
+struct Kv8Pool {
+  uint8_t* codes;
+  float* scales;
+  int32_t format;
+  int64_t num_blocks;
+  int32_t bs, hkv, d;
+};
+struct Kv8Append {
+  uint8_t* pool;
+  float* scales;
+  int64_t num_blocks;
+  int32_t bs, hkv, d, lanes_per_row;
+  const void* src[2];  // k, v views [hkv, tokens, d]
+  int64_t hs[2], ss[2];
+  int64_t tokens;
+  const int64_t* slots;
+  int* err;
+};
+void launch_kv8_append(int format, int dtype, Kv8Append p, hipStream_t stream);
+constexpr int kKv8Ranges = 16;
+struct Kv8Range {
+  const int32_t* table;
+  int64_t at0;  // place in the table's blocks of the range's first token
+  void *k, *v;
+  int64_t hs, ss;
+};
+struct Kv8Gather {
+  const uint8_t* pool;
+  const float* scales;
+  int64_t num_blocks;
+  int32_t bs, hkv, d, lanes_per_row, n;
+  int64_t tokens, begin[kKv8Ranges];  // tokens of all ranges; those before a range
+  Kv8Range r[kKv8Ranges];
+  int* err;
+};
+void launch_kv8_gather(const Kv8Pool& pool, int dtype, int n, const PagedRangeDesc* ranges, int* err, hipStream_t stream);
+
 // Scheduling strategies (strategy.rs:14-24) and their closed-form positions; see
 // positions.hip.
 enum Strategy : int32_t { kStrategyVanilla = 0, kStrategyStriped = 1, kStrategyZigZag = 2 };

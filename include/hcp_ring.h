@@ -724,6 +724,49 @@ int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, cons
                      size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * (10) 8-bit paged K/V cache (no reference counterpart; its caches are in the model's type).
+ *
+ * The pool of (3) with elem_bytes 1: codes [2, num_blocks, block_size, Hkv, D], and beside
+ * it a scale for each plane, block and head, scales [2, num_blocks, Hkv] fp32 (DEVICE).  A
+ * code c of the block stands for scale * c.  Formats: E4M3 (the OCP 8-bit float with 4
+ * exponent and 3 mantissa bits, largest value 448) and INT8 (symmetric, -127 .. 127, about
+ * three times nearer than E4M3 where a block's values are of one size; E4M3 keeps small ones
+ * beside large ones).  head_dim a multiple of 8 up to 256 (decode: 128), the pool 16-byte
+ * aligned.
+ *
+ * hcp_kv8_append writes the rows of k / v [Hkv, tokens, D] (BF16, F16 or F32 views) to
+ * slots[t] = block * block_size + place (DEVICE int64 [tokens], e.g. of hcp_kv_plan_step; a
+ * negative one is skipped, one past the pool sets device error bit 0).  Tokens that follow
+ * each other into following places of one block are a run; the rows of the block before the
+ * run's first place are held already, those after its last stay as they are.  The block's
+ * scale becomes the least power of two (2^-100 at least) under which the run's largest
+ * magnitude fits the format, or stays if it is larger and rows are held (a run from place 0
+ * starts the block anew); where it grows the held codes are rounded to it.  New codes are
+ * the nearest to x / scale, ties to even.  A run with a value that is not finite makes the
+ * scale NaN, and with it all that the block and head stand for, until it is started anew.
+ * A block takes one run per call: of two, either may be lost.
+ *
+ * hcp_kv8_gather: as hcp_paged_kv_gather, out = scale * code rounded to dtype.
+ * hcp_kv8_prefill_replay_paged: as hcp_ring_prefill_replay_paged, K/V staged that way
+ * (workspace: hcp_ring_replay_workspace_size(desc, 1)).
+ * ------------------------------------------------------------------------------- */
+enum hcp_kv8_format { HCP_KV8_E4M3 = 1, HCP_KV8_INT8 = 2 };
+
+int hcp_kv8_append(const hcp_paged_pool* pool, float* scales, int32_t format, int32_t dtype,
+                   hcp_ring_view k, hcp_ring_view v, int64_t tokens, const int64_t* slots,
+                   void* stream);
+
+int hcp_kv8_gather(const hcp_paged_pool* pool, const float* scales, int32_t format, int32_t dtype,
+                   const int32_t* block_table, int64_t table_len, int64_t table_seq_offset,
+                   int64_t t0, int64_t t1, hcp_ring_view k_out, hcp_ring_view v_out, void* stream);
+
+int hcp_kv8_prefill_replay_paged(const hcp_ring_replay_desc* desc, hcp_ring_view q,
+                                 const hcp_paged_pool* pool, const float* scales, int32_t format,
+                                 const int32_t* block_table, int64_t table_len, hcp_ring_view out,
+                                 float* lse_out, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* ---------------------------------------------------------------------------------
  * Replay kernel timing (no reference counterpart; benchmark instrumentation; the
  * reference logs wall-clock compute per phase to HCP_PERF_LOG, ring.rs:820-844).
  *
