@@ -13,8 +13,8 @@ The operator names mirror the reference's ring-attention backend
   python/hcp_vllm_block_ring_plugin.py:143-174, 304-337 -> ``hcp_paged_kv_*``
 * :func:`kv_plan_step`  block tables, slots and positions of a step from request lengths ->
   ``hcp_kv_plan_step`` (no reference counterpart)
-* :func:`kv8_append` / :func:`kv8_gather` / :func:`kv8_ring_attention_replay_paged`  a paged
-  K/V cache in 8 bits with a scale per block and head -> ``hcp_kv8_*`` (no reference
+* :func:`kv8_append` / :func:`kv8_decode_partial` / :func:`kv8_decode_ring_replay` /
+  :func:`kv8_gather` / :func:`kv8_ring_attention_replay_paged`  a paged K/V cache in 8 bits with a scale per block and head -> ``hcp_kv8_*`` (no reference
   counterpart)
 * :func:`ring_attention_replay`             ring.rs:861-1398 for every domain on one GPU ->
   ``hcp_ring_prefill_replay`` (``_paged`` variant stages K/V from a block pool)
@@ -294,6 +294,14 @@ def lib() -> ctypes.CDLL:
         "hcp_kv8_append": ([ctypes.POINTER(PagedPool), vp, i32, i32, View, View, i64, vp, vp], ctypes.c_int),
         "hcp_kv8_gather": ([ctypes.POINTER(PagedPool), vp, i32, i32, vp, i64, i64, i64, i64, View, View, vp],
                            ctypes.c_int),
+        "hcp_kv8_decode_workspace_size": ([ctypes.POINTER(DecodeDesc), ctypes.POINTER(PagedPool)], ctypes.c_size_t),
+        "hcp_kv8_decode_partial": ([ctypes.POINTER(DecodeDesc), ctypes.POINTER(PagedPool), vp, i32, View, vp, vp, vp,
+                                    vp, vp, ctypes.c_size_t, vp], ctypes.c_int),
+        "hcp_kv8_decode_ring_workspace_size": ([ctypes.POINTER(DecodeDesc), ctypes.POINTER(PagedPool), i32,
+                                                ctypes.POINTER(DecodeShard)], ctypes.c_size_t),
+        "hcp_kv8_decode_ring_replay": ([ctypes.POINTER(DecodeDesc), ctypes.POINTER(PagedPool), vp, i32, View, i32,
+                                        ctypes.POINTER(DecodeShard), i32, View, vp, vp, ctypes.c_size_t, vp],
+                                       ctypes.c_int),
         "hcp_kv8_prefill_replay_paged": ([ctypes.POINTER(ReplayDesc), View, ctypes.POINTER(PagedPool), vp, i32, vp,
                                           i64, View, vp, vp, ctypes.c_size_t, vp], ctypes.c_int),
         "hcp_ring_trace_attach": ([vp, ctypes.c_size_t], ctypes.c_int),
@@ -779,14 +787,18 @@ def kv8_pool(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
 
 
 def _kv8(pool, scales):
-    """(hcp_paged_pool, HCP_KV8_* of the pool's type)."""
+    """(hcp_paged_pool, HCP_KV8_* of the pool's type), the scales checked against it."""
+    pp, fmt = _kv8_shape(pool)
+    _want("scales", scales, _torch().float32, (2, pool.shape[1], pool.shape[3]), pool.device)
+    return pp, fmt
+
+
+def _kv8_shape(pool):
     torch = _torch()
     fmt = {torch.float8_e4m3fn: KV8_E4M3, torch.int8: KV8_INT8}.get(pool.dtype)
     if fmt is None:
         raise ValueError("an 8-bit pool is float8_e4m3fn or int8")
-    pp = paged_pool(pool)
-    _want("scales", scales, torch.float32, (2, pool.shape[1], pool.shape[3]), pool.device)
-    return pp, fmt
+    return paged_pool(pool), fmt
 
 
 def _rows_of(name, t, shape, pool, dtype=None):
@@ -829,6 +841,85 @@ def kv8_gather(pool, scales, block_table, table_seq_offset, t0, t1, dtype=None, 
                                     block_table.data_ptr(), block_table.numel(), table_seq_offset, t0, t1, view(k_out),
                                     view(v_out), _stream(stream)))
     return k_out, v_out
+
+
+def _decode_tables(name, tables, lens, b, device):
+    torch = _torch()
+    if tables is not None and (tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != b
+                               or tables.device != device or (tables.stride(1) != 1 and tables.shape[1] > 1)):
+        raise ValueError(f"{name} must be an int32 tensor of {b} contiguous rows on {device}")
+    if lens is not None:
+        _want("seq_lens", lens, torch.int32, (b,), device)
+
+
+def _decode_rows(q, pool, o, lse, o_dtype):
+    """Outputs [B, Hq, D] and [B, Hq] (made where None), and q checked against the pool."""
+    torch = _torch()
+    b, hq, d = q.shape
+    if d != pool.shape[4] or q.device != pool.device or (q.stride(2) != 1 and d > 1):
+        raise ValueError(f"q must be [B, Hq, {pool.shape[4]}] with contiguous rows on {pool.device}")
+    if o is None:
+        o = torch.empty((b, hq, d), dtype=o_dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((b, hq), dtype=torch.float32, device=q.device)
+    _rows_of("o", o, (b, hq, d), pool, o_dtype)
+    _want("lse", lse, torch.float32, (b, hq), pool.device)
+    return o, lse
+
+
+def kv8_decode_workspace_size(q, pool, block_tables, t0, t1) -> int:
+    """Workspace bytes of :func:`kv8_decode_partial` (for any shorter range, too)."""
+    desc, (pp, _) = decode_desc(q, pool, block_tables, t0, t1), _kv8_shape(pool)
+    return lib().hcp_kv8_decode_workspace_size(ctypes.byref(desc), ctypes.byref(pp))
+
+
+def kv8_decode_partial(q, pool, scales, block_tables, t0, t1, seq_lens=None, scale=None, workspace=None, o=None,
+                       lse=None, stream=None):
+    """As :func:`decode_local_compact_partial` over an 8-bit cache: q [B, Hq, D] over tokens
+    [t0, min(t1, seq_lens)) of each sequence -> (o [B, Hq, D] fp32, lse [B, Hq] fp32)."""
+    torch = _torch()
+    pp, fmt = _kv8(pool, scales)
+    o, lse = _decode_rows(q, pool, o, lse, torch.float32)
+    _decode_tables("block_tables", block_tables, seq_lens, q.shape[0], pool.device)
+    if not o.is_contiguous():
+        raise ValueError("o must be contiguous")
+    desc = decode_desc(q, pool, block_tables, t0, t1, scale)
+    if workspace is None:
+        need = lib().hcp_kv8_decode_workspace_size(ctypes.byref(desc), ctypes.byref(pp))
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+    with _on(pool.device):
+        _check(lib().hcp_kv8_decode_partial(ctypes.byref(desc), ctypes.byref(pp), scales.data_ptr(), fmt,
+                                            View(q.data_ptr(), q.stride(1), q.stride(0)), block_tables.data_ptr(),
+                                            _ptr(seq_lens), o.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
+                                            workspace.numel() * workspace.element_size(), _stream(stream)))
+    return o, lse
+
+
+def kv8_decode_ring_workspace_size(q, pool, shards) -> int:
+    """Workspace bytes of :func:`kv8_decode_ring_replay` for these shards."""
+    desc, (pp, _), arr = _ring_desc(q, pool), _kv8_shape(pool), _shards(shards)
+    return lib().hcp_kv8_decode_ring_workspace_size(ctypes.byref(desc), ctypes.byref(pp), len(shards), arr)
+
+
+def kv8_decode_ring_replay(q, pool, scales, shards, seed_domain, scale=None, out=None, lse_out=None, workspace=None,
+                           stream=None):
+    """As :func:`decode_ring_replay` over an 8-bit cache (shards as there)."""
+    torch = _torch()
+    pp, fmt = _kv8(pool, scales)
+    out, lse_out = _decode_rows(q, pool, out, lse_out, q.dtype)
+    for tables, lens, _ in shards:
+        _decode_tables("a shard's tables", tables, lens, q.shape[0], pool.device)
+    desc, arr, n = _ring_desc(q, pool, scale), _shards(shards), len(shards)
+    if workspace is None:
+        need = lib().hcp_kv8_decode_ring_workspace_size(ctypes.byref(desc), ctypes.byref(pp), n, arr)
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+    with _on(pool.device):
+        _check(lib().hcp_kv8_decode_ring_replay(ctypes.byref(desc), ctypes.byref(pp), scales.data_ptr(), fmt,
+                                                View(q.data_ptr(), q.stride(1), q.stride(0)), n, arr, seed_domain,
+                                                View(out.data_ptr(), out.stride(1), out.stride(0)), lse_out.data_ptr(),
+                                                workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                                                _stream(stream)))
+    return out, lse_out
 
 
 def kv8_ring_attention_replay_paged(q, pool, scales, block_table, chunks, causal=True, scale=None, out=None,

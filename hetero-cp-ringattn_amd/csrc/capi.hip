@@ -1878,6 +1878,101 @@ int hcp_kv8_gather(const hcp_paged_pool* pool, const float* scales, int32_t form
   });
 }
 
+}  // extern "C": internal helpers below have C++ linkage
+namespace {
+// What both decode entries ask of their arguments; the pool's description.
+Kv8Pool check_kv8_decode(const hcp_paged_decode_desc* d, const hcp_paged_pool* pool, const float* scales, int32_t format,
+                         const hcp_ring_view& q) {
+  require(d != nullptr, "null descriptor");
+  const Kv8Pool c = check_kv8(pool, scales, format);
+  require(d->dtype == HCP_DTYPE_BF16 || d->dtype == HCP_DTYPE_F16, "dtype must be BF16 or F16");
+  require(d->batch > 0, "batch must be positive");
+  require(d->num_q_heads > 0 && d->num_kv_heads == pool->num_kv_heads, "kv heads must match the pool");
+  require(d->num_q_heads % d->num_kv_heads == 0 && d->num_q_heads / d->num_kv_heads <= 16,
+          "num_q_heads must be a multiple of num_kv_heads, up to 16 times it");
+  require(d->head_dim == pool->head_dim, "head_dim must match the pool");
+  require(d->head_dim <= 128, "decode takes a head_dim up to 128");
+  require(pool->block_size % 16 == 0, "block_size must be a multiple of 16");
+  require(d->scale > 0.f, "scale must be positive");
+  check_view(q, "q", 1);
+  require(mfma_layout_ok(q), "q must be 16-byte aligned with strides multiple of 8");
+  return c;
+}
+size_t kv8_workspace(const hcp_paged_decode_desc* d, int n, const DecodeSpan* spans) {
+  require(d->num_kv_heads > 0 && d->num_q_heads > 0 && d->num_q_heads % d->num_kv_heads == 0 && d->head_dim > 0 && d->batch > 0,
+          "bad decode shape");
+  return kv8_decode_workspace_bytes(d->batch, d->num_q_heads, d->num_kv_heads, d->head_dim, n, spans);
+}
+}  // namespace
+extern "C" {
+
+size_t hcp_kv8_decode_workspace_size(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool) {
+  (void)pool;
+  try {
+    require(desc != nullptr, "null descriptor");
+    const DecodeSpan span{nullptr, 0, 0, nullptr, desc->t0, desc->t1};
+    return kv8_workspace(desc, 1, &span);
+  } catch (...) {
+    return 0;  // the entry point itself reports it
+  }
+}
+
+int hcp_kv8_decode_partial(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool, const float* scales,
+                           int32_t format, hcp_ring_view q, const int32_t* block_tables, const int32_t* seq_lens,
+                           float* o, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded(__func__, [&] {
+    const Kv8Pool c = check_kv8_decode(desc, pool, scales, format, q);
+    require(desc->t0 >= 0 && desc->t1 >= desc->t0, "need 0 <= t0 <= t1");
+    require(block_tables != nullptr && o != nullptr && lse != nullptr, "null pointer");
+    require(reinterpret_cast<uintptr_t>(o) % 16 == 0, "o must be 16-byte aligned");
+    require(desc->table_len >= 1 && desc->table_stride >= desc->table_len, "bad table shape");
+    if (desc->t1 > desc->t0) require((desc->t1 - 1) / pool->block_size < desc->table_len, "block table too short");
+    const bool any = desc->t1 > desc->t0;
+    const int64_t skip = any ? desc->t0 / pool->block_size : 0;  // whole blocks before t0
+    const int64_t off = skip * pool->block_size;
+    const DecodeSpan span{block_tables + skip, desc->table_stride, desc->table_len - skip, seq_lens,
+                          any ? desc->t0 - off : 0, any ? desc->t1 - off : 0, off};
+    launch_kv8_decode(c, desc->dtype, desc->batch, desc->num_q_heads, q.data, q.seq_stride, q.head_stride, 1, &span,
+                      desc->scale, kF32, o, desc->head_dim, lse, workspace, workspace_bytes, device_error_flags(),
+                      as_stream(stream));
+  });
+}
+
+size_t hcp_kv8_decode_ring_workspace_size(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool,
+                                          int32_t num_domains, const hcp_decode_shard* shards) {
+  (void)pool;
+  try {
+    const std::vector<DecodeSpan> spans = ring_spans(desc, num_domains, shards, 0);
+    return kv8_workspace(desc, num_domains, spans.data());
+  } catch (...) {
+    return 0;
+  }
+}
+
+int hcp_kv8_decode_ring_replay(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool, const float* scales,
+                               int32_t format, hcp_ring_view q, int32_t num_domains, const hcp_decode_shard* shards,
+                               int32_t seed_domain, hcp_ring_view out, float* lse_out, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  return guarded(__func__, [&] {
+    const Kv8Pool c = check_kv8_decode(desc, pool, scales, format, q);
+    require(num_domains < 1 || (seed_domain >= 0 && seed_domain < num_domains), "seed_domain out of range");
+    const std::vector<DecodeSpan> spans = ring_spans(desc, num_domains, shards, seed_domain);
+    check_view(out, "out", 1);
+    check_out_view(out, desc->dtype);
+    require(out.seq_stride == static_cast<int64_t>(desc->num_q_heads) * out.head_stride,
+            "out must hold the [batch, Hq] rows at one stride (seq_stride == Hq * head_stride)");
+    for (const DecodeSpan& sp : spans) {
+      if (sp.t1 == 0) continue;
+      require(sp.tables != nullptr, "null block table of a non-empty shard");
+      require(sp.table_len >= 1 && sp.table_stride >= sp.table_len, "bad shard table shape");
+      require((sp.t1 - 1) / pool->block_size < sp.table_len, "shard block table too short");
+    }
+    launch_kv8_decode(c, desc->dtype, desc->batch, desc->num_q_heads, q.data, q.seq_stride, q.head_stride, num_domains,
+                      spans.data(), desc->scale, desc->dtype, out.data, out.head_stride, lse_out, workspace,
+                      workspace_bytes, device_error_flags(), as_stream(stream));
+  });
+}
+
 int hcp_kv8_prefill_replay_paged(const hcp_ring_replay_desc* desc, hcp_ring_view q, const hcp_paged_pool* pool,
                                  const float* scales, int32_t format, const int32_t* block_table, int64_t table_len,
                                  hcp_ring_view out, float* lse_out, void* workspace, size_t workspace_bytes,

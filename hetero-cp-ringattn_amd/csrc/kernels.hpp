@@ -191,6 +191,13 @@ struct Kv8Gather {
 };
 void launch_kv8_gather(const Kv8Pool& pool, int dtype, int n, const PagedRangeDesc* ranges, int* err, hipStream_t stream);
 
+// Attention of one query per sequence over its n shards in an 8-bit cache, as
+// launch_paged_decode.
+size_t kv8_decode_workspace_bytes(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans);
+void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const void* q, int64_t q_bs, int64_t q_hs, int n,
+                       const DecodeSpan* spans, float scale, int out_dtype, void* out, int64_t out_rs, float* lse, void* ws,
+                       size_t ws_bytes, int* err, hipStream_t stream);
+
 // Scheduling strategies (strategy.rs:14-24) and their closed-form positions; see
 // positions.hip.
 enum Strategy : int32_t { kStrategyVanilla = 0, kStrategyStriped = 1, kStrategyZigZag = 2 };

@@ -746,6 +746,12 @@ int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, cons
  * scale NaN, and with it all that the block and head stand for, until it is started anew.
  * A block takes one run per call: of two, either may be lost.
  *
+ * hcp_kv8_decode_partial / hcp_kv8_decode_ring_replay: as hcp_paged_decode_partial and
+ * hcp_decode_ring_replay, straight over the codes (desc->dtype: the type of q and of the
+ * ring's out; the same limits on head_dim, heads and block_size).  Products of codes and q
+ * are exact, softmax weights carry 22 bits, sums and statistics 32.  Scales may be any
+ * finite values >= 0; o must be 16-byte aligned.  Workspaces are 256-byte aligned and cover
+ * every shorter context of the same batch and heads.
  * hcp_kv8_gather: as hcp_paged_kv_gather, out = scale * code rounded to dtype.
  * hcp_kv8_prefill_replay_paged: as hcp_ring_prefill_replay_paged, K/V staged that way
  * (workspace: hcp_ring_replay_workspace_size(desc, 1)).
@@ -759,6 +765,22 @@ int hcp_kv8_append(const hcp_paged_pool* pool, float* scales, int32_t format, in
 int hcp_kv8_gather(const hcp_paged_pool* pool, const float* scales, int32_t format, int32_t dtype,
                    const int32_t* block_table, int64_t table_len, int64_t table_seq_offset,
                    int64_t t0, int64_t t1, hcp_ring_view k_out, hcp_ring_view v_out, void* stream);
+
+size_t hcp_kv8_decode_workspace_size(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool);
+
+int hcp_kv8_decode_partial(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool,
+                           const float* scales, int32_t format, hcp_ring_view q,
+                           const int32_t* block_tables, const int32_t* seq_lens, float* o, float* lse,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+size_t hcp_kv8_decode_ring_workspace_size(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool,
+                                          int32_t num_domains, const hcp_decode_shard* shards);
+
+int hcp_kv8_decode_ring_replay(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool,
+                               const float* scales, int32_t format, hcp_ring_view q,
+                               int32_t num_domains, const hcp_decode_shard* shards,
+                               int32_t seed_domain, hcp_ring_view out, float* lse_out, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 int hcp_kv8_prefill_replay_paged(const hcp_ring_replay_desc* desc, hcp_ring_view q,
                                  const hcp_paged_pool* pool, const float* scales, int32_t format,
