@@ -126,6 +126,11 @@ struct DecodeSpan {
   int64_t t0, t1;
   int64_t len_off = 0;
 };
+// 16-token groups of the longest sequence that the spans allow; most parts of a decode plan
+// over them, and the bytes of `parts` partials of every (sequence, head): o, then lse.
+int64_t span_groups(int n, const DecodeSpan* spans);
+int most_parts(int batch, int hq, int d, int64_t groups);
+size_t parts_bytes(int parts, int batch, int hq, int d);
 // Workspace of launch_paged_decode for these shards, and for any shorter ones.
 size_t decode_workspace_bytes(int batch, int hq, int d, int n, const DecodeSpan* spans);
 // Attention of one query per sequence over its n shards, merged: out[row * out_rs + d] in
@@ -193,7 +198,7 @@ void launch_kv8_gather(const Kv8Pool& pool, int dtype, int n, const PagedRangeDe
 
 // Attention of one query per sequence over its n shards in an 8-bit cache, as
 // launch_paged_decode.
-size_t kv8_decode_workspace_bytes(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans);
+size_t kv8_decode_workspace_bytes(int batch, int hq, int d, int n, const DecodeSpan* spans);
 void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const void* q, int64_t q_bs, int64_t q_hs, int n,
                        const DecodeSpan* spans, float scale, int out_dtype, void* out, int64_t out_rs, float* lse, void* ws,
                        size_t ws_bytes, int* err, hipStream_t stream);

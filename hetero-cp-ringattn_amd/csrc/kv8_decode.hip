@@ -1,114 +1,542 @@
 // Single-query attention over the 8-bit paged cache (layout in kv8.hpp): per sequence and
 // query head S = scale * s_K (q . c_K) over its tokens, shard after shard; O = sum P s_V c_V,
 // lse = ln sum e^S; no token: O = 0, lse = -inf.
+//
+// HBM-bound: every code is read once, half the bytes of the 16-bit decode for the same
+// products, so the work beside the loads has to be half as large, too.  Both products run on
+// the matrix cores and no value passes through LDS on the way:
+//   * One launch covers all shards; a sequence's 16-token groups are dealt out in equal runs
+//     to parts x subs waves (grid (parts, batch, head groups), a workgroup holding `heads` kv
+//     heads x `subs` runs).  The subs of a part meet in LDS, parts in the LSE merge; a lone
+//     part writes the output itself.
+//   * A step is 32 tokens.  S^T = K Q^T (16x16x32, f16): A = 16 key rows, their codes converted
+//     in registers (exact: a code has at most 8 significant bits), B = the rep <= 16 query
+//     heads.  16-bit q times a power of two that brings its largest value to 2^14 is exact in
+//     f16, too (what falls below f16 is 2^-38 of the largest), so bf16 and fp16 share the
+//     kernel.  Scales are applied to S in fp32.
+//   * O^T = V^T P^T: lane (col, grp) of S^T holds the scores of query col and keys 4 grp + i of
+//     both groups, which is the B operand of keys {4 grp + i, 16 + 4 grp + i} as it stands.  A =
+//     V^T for the same keys: lane (m, grp) loads D/16 neighbouring dims of those 8 keys, so
+//     tile j of the product holds dims m D/16 + j and pairs of keys are put together by byte
+//     permutes.  O^T stays in the lane whose query it is: max, rescale and sum need two
+//     cross-lane steps each and no broadcast.
+//   * Weights w = p s_V 2^(14 + m - a) with `a` the running maximum of log2(p s_V), which is
+//     tracked like m: w <= 2^14 whatever the scales, and split into two f16 of 11 bits each, w
+//     = hi + lo, so P carries 22 bits (one f16 alone would put 2^-12 on every weight, against
+//     the fp32 weights of the 16-bit decode).  Sums and statistics are fp32.
+#include <algorithm>
+
 #include "kv8.hpp"
 
 namespace hcp {
 
 struct Kv8DecodeArgs {
-  const void* q;
-  int64_t q_bs, q_hs;
+  const uint16_t* q;
+  int64_t q_bs, q_hs;  // elements
   const uint8_t* pool;
   const float* scales;
+  int64_t plane_bytes, plane_scales;  // from K's to V's
   int64_t num_blocks;
-  int32_t bs, hkv, hq, d;
+  int32_t bs, hkv, hq, rep;
   DecodeSpan span[kMaxDomains];
-  int32_t n_spans, out_dtype;
-  float scale;
+  int32_t n_spans, heads, subs;
+  int32_t gpb, gpb_shift;  // 16-token groups per block, its log2 or -1
+  int32_t q_bf16, out_dtype, dn;
+  float scale_log2;
+  float *ws_o, *ws_lse;  // [parts][batch * hq][dn]; null: a lone part
   void* out;
   int64_t out_rs;
   float* lse;
+  int32_t batch;
   int* err;
 };
 static_assert(sizeof(Kv8DecodeArgs) <= 4096, "kernel arguments are limited to 4 KiB");
 
-// One wave per sequence and query head; lane l has dims 2l, 2l + 1.
-template <int F, int DT>
-__global__ __launch_bounds__(64) void kv8_decode_kernel(Kv8DecodeArgs a) {
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x, kvh = h / (a.hq / a.hkv);
-  const int c = lane * 2;
-  const bool in = c < a.d;
-  float q0 = 0.f, q1 = 0.f;
-  if (in) {
-    q0 = load_elem<DT>(a.q, b * a.q_bs + h * a.q_hs + c) * a.scale;
-    q1 = load_elem<DT>(a.q, b * a.q_bs + h * a.q_hs + c + 1) * a.scale;
+constexpr float kNoMax = -1.0e30f;
+constexpr int kKv8Waves = 8;  // most waves per workgroup
+
+// A word of codes to two pairs of f16: codes 0, 1 and 2, 3.  int8: u = code + 128 as the low
+// byte of 1024 + u, then - 1152.
+template <int F>
+__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (F == kE4M3) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+  } else {
+    const f16x2 bias = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+    auto f = [&](uint32_t sel) {
+      return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, sel)) + bias);
+    };
+    w ^= 0x80808080u;
+    lo = f(0x04010400u);
+    hi = f(0x04030402u);
   }
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  const int64_t row = static_cast<int64_t>(a.hkv) * a.d;
-  for (int s = 0; s < a.n_spans; ++s) {
-    const DecodeSpan& sp = a.span[s];
-    const int64_t end = sp.seq_lens == nullptr ? sp.t1 : min(sp.t1, static_cast<int64_t>(sp.seq_lens[b]) - sp.len_off);
-    const int32_t* table = sp.tables + b * sp.table_stride;
-    for (int64_t t = sp.t0; t < end; ++t) {
-      const int64_t entry = t / a.bs;
-      const int32_t blk = table[entry];
-      if (blk < 0 || blk >= a.num_blocks) {
-        if (lane == 0) atomicOr(a.err, 1);
-        continue;
-      }
-      const int64_t at = (static_cast<int64_t>(blk) * a.bs + (t - entry * a.bs)) * row + kvh * a.d + c;
-      const uint8_t* k = a.pool + at;
-      const uint8_t* v = k + a.num_blocks * a.bs * row;
-      float kx[4] = {}, vx[4] = {};
-      if (in) {
-        kv8_decode4<F>(*reinterpret_cast<const uint16_t*>(k), kx);
-        kv8_decode4<F>(*reinterpret_cast<const uint16_t*>(v), vx);
-      }
-      float sc = q0 * kx[0] + q1 * kx[1];
-      for (int off = 32; off > 0; off /= 2) sc += __shfl_xor(sc, off);
-      sc *= a.scales[static_cast<int64_t>(blk) * a.hkv + kvh];
-      const float vs = a.scales[(a.num_blocks + blk) * a.hkv + kvh];
-      const float mn = fmaxf(m, sc), f = m == -INFINITY ? 0.f : __expf(m - mn), p = __expf(sc - mn);
-      m = mn;
-      l = l * f + p;
-      o0 = o0 * f + p * vs * vx[0];
-      o1 = o1 * f + p * vs * vx[1];
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t r = static_cast<int64_t>(b) * a.hq + h;
-  if (in) {
-    store_elem_rt(a.out, a.out_dtype, r * a.out_rs + c, o0 * inv);
-    store_elem_rt(a.out, a.out_dtype, r * a.out_rs + c + 1, o1 * inv);
-  }
-  if (lane == 0 && a.lse != nullptr) a.lse[r] = l == 0.f ? -INFINITY : m + __logf(l);
 }
 
-size_t kv8_decode_workspace_bytes(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans) { return 0; }
+__device__ __forceinline__ f32x4 mma_f16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// The four lanes with the same lane & 15.
+template <typename Op>
+__device__ __forceinline__ float over_groups(float v, Op op) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2));
+}
+
+// N consecutive outputs (4 or 8) in the output type; rows start on 4-element boundaries.
+template <int N>
+__device__ __forceinline__ void store_out(void* out, int dtype, int64_t at, const float* x) {
+#pragma unroll
+  for (int e = 0; e < N; e += 4) {
+    if (dtype == kF32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(out) + at + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+    } else if (dtype == kBF16) {
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + at + e) =
+          u32x2{f32x2_to_bf16x2_bits(x[e], x[e + 1]), f32x2_to_bf16x2_bits(x[e + 2], x[e + 3])};
+    } else {
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + at + e) = u32x2{pack_f16(x[e], x[e + 1]), pack_f16(x[e + 2], x[e + 3])};
+    }
+  }
+}
+
+// PAD: head dim a.dn < D (a multiple of 8); 8-byte pieces past it are not loaded (zeros) nor
+// stored.
+template <int F, int D, bool PAD>
+__global__ __launch_bounds__(512) void kv8_decode_kernel(Kv8DecodeArgs a) {
+  const int dn = PAD ? a.dn : D;
+  constexpr int KL = D / 64;  // 16-byte loads of a key row per lane
+  constexpr int KS = D / 32;  // k-steps of S
+  constexpr int VB = D / 16;  // dims of V per lane, and tiles of O
+  constexpr int VW = VB / 4;
+  constexpr int OS = D + 4;   // LDS row of the meeting, 4 floats apart from a bank's multiple
+  extern __shared__ __attribute__((aligned(16))) float meet_lds[];  // subs > 1: [wave][rep][OS], then lse [wave][16]
+
+  const int b = blockIdx.y, part = blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int sub = wave / a.heads;
+  const int kvh = blockIdx.z * a.heads + wave - sub * a.heads;
+  const bool idle = kvh >= a.hkv;
+  if (idle && a.subs == 1) return;  // no workgroup barrier below
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+
+  auto span_end = [&](int s) __attribute__((always_inline)) -> int64_t {
+    const DecodeSpan& sp = a.span[s];
+    if (sp.seq_lens == nullptr) return sp.t1;
+    return min(sp.t1, static_cast<int64_t>(__builtin_amdgcn_readfirstlane(sp.seq_lens[b])) - sp.len_off);
+  };
+  auto span_groups = [&](int s, int64_t t_end) __attribute__((always_inline)) {
+    const int64_t t0 = a.span[s].t0;
+    return t_end > t0 ? static_cast<int>((t_end + 15) / 16 - t0 / 16) : 0;
+  };
+  int total = 0;
+  for (int s = 0; s < a.n_spans; ++s) total += span_groups(s, span_end(s));
+  const int runs = gridDim.x * a.subs;
+  const int run_len = (total + 2 * runs - 1) / (2 * runs) * 2;  // whole steps
+  const int g0 = idle ? total : static_cast<int>(min(static_cast<int64_t>(part * a.subs + sub) * run_len, static_cast<int64_t>(total)));
+  const int g1 = min(g0 + run_len, total);
+
+  // Q^T in f16, times a power of two that brings the row's largest value to 2^14 .. 2^15.
+  // k-step 2 h + e holds dims 16 grp + 64 h + 8 e + i, as the 16-byte loads of K bring them.
+  u32x4 qf[KS];
+  float c_log2;
+  {
+    float x[KS][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d0 = grp * 16 + 64 * (s / 2) + 8 * (s % 2);
+      u32x4 v = {0, 0, 0, 0};
+      if (!idle && col < a.rep && (!PAD || d0 < dn))
+        v = *reinterpret_cast<const u32x4*>(a.q + b * a.q_bs + (kvh * a.rep + col) * a.q_hs + d0);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        x[s][2 * w] = a.q_bf16 ? __uint_as_float(v[w] << 16) : f16_bits_to_f32(static_cast<uint16_t>(v[w] & 0xffffu));
+        x[s][2 * w + 1] = a.q_bf16 ? __uint_as_float(v[w] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(v[w] >> 16));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
+    }
+    // as floats the bits of |x| keep their order (NaN: dropped by the maximum, kept in x)
+    const float m = over_groups(__uint_as_float(top), [](float u, float v) { return fmaxf(u, v); });
+    const bool plain = m > 0.f && m < INFINITY;
+    const int k = plain ? max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100) : 14;
+    const float up = __uint_as_float(static_cast<uint32_t>(14 - k + 127) << 23);
+    c_log2 = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(k - 14 + 127) << 23);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) qf[s][w] = pack_f16(x[s][2 * w] * up, x[s][2 * w + 1] * up);
+  }
+
+  f32x4 acc[VB];
+#pragma unroll
+  for (int j = 0; j < VB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = kNoMax, a_run = kNoMax, l_run = 0.f;
+
+  const int64_t row = static_cast<int64_t>(a.hkv) * dn;  // bytes of a slot, all heads
+  struct Step {
+    u32x4 k[2][KL];
+    uint32_t v[2][4][VW];
+    float ks[2], vs[2];
+    int lo[2], hi[2];  // keys [lo, hi) of each group count
+  };
+  typedef __attribute__((address_space(4))) const float ConstF;  // uniform loads
+  // Cursor over the shards: groups [s_begin, s_end) of the sequence lie in shard s.
+  int s = -1, s_begin = 0, s_end = 0;
+  int64_t t_end = 0, t_beg = 0;
+  int g_first = 0;
+  const int32_t* table = nullptr;
+  int64_t table_len = 0;
+  // Block ids of the run's groups, 64 at a time: lane i holds that of group ids_base + i.
+  int ids = -1, ids_base = -64;
+  auto load_group = [&](int g, Step& S, int h) __attribute__((always_inline)) {
+    S.lo[h] = S.hi[h] = 0;
+    S.ks[h] = S.vs[h] = 0.f;
+    if (g >= g1) {
+#pragma unroll
+      for (int i = 0; i < KL; ++i) S.k[h][i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) S.v[h][j][w] = 0;
+      return;
+    }
+    if (g >= s_end) {
+      do {
+        ++s;
+        s_begin = s_end;
+        t_end = span_end(s);
+        s_end += span_groups(s, t_end);
+      } while (g >= s_end);
+      const DecodeSpan& sp = a.span[s];
+      t_beg = sp.t0;
+      g_first = static_cast<int>(t_beg / 16);
+      table = sp.tables + static_cast<int64_t>(b) * sp.table_stride;
+      table_len = sp.table_len;
+      ids_base = g - 64;
+    }
+    if (g - ids_base >= 64) {
+      ids_base = g;
+      const int gl = g_first + g - s_begin + lane;
+      const int e = a.gpb_shift >= 0 ? gl >> a.gpb_shift : gl / a.gpb;
+      ids = g + lane < min(g1, s_end) && e < table_len ? table[e] : -1;
+    }
+    const int32_t blk = __builtin_amdgcn_readlane(ids, g - ids_base);
+    const int gl = g_first + g - s_begin;
+    const int entry = a.gpb_shift >= 0 ? gl >> a.gpb_shift : gl / a.gpb;
+    const int64_t tok0 = static_cast<int64_t>(gl) * 16;
+    if (blk < 0 || blk >= a.num_blocks) {
+      if (lane == 0 && entry < table_len) atomicOr(a.err, 1);
+#pragma unroll
+      for (int i = 0; i < KL; ++i) S.k[h][i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) S.v[h][j][w] = 0;
+      return;
+    }
+    S.lo[h] = __builtin_amdgcn_readfirstlane(static_cast<int>(t_beg > tok0 ? t_beg - tok0 : 0));
+    S.hi[h] = __builtin_amdgcn_readfirstlane(static_cast<int>(min(t_end - tok0, static_cast<int64_t>(16))));
+    const float* sc = a.scales + static_cast<int64_t>(blk) * a.hkv + kvh;
+    S.ks[h] = *(ConstF*)(uintptr_t)sc;
+    S.vs[h] = *(ConstF*)(uintptr_t)(sc + a.plane_scales);
+    const uint8_t* slot = a.pool + (static_cast<int64_t>(blk) * a.bs + (gl - entry * a.gpb) * 16) * row + kvh * dn;
+    const uint8_t* kr = slot + col * row + grp * 16;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      if constexpr (PAD) {  // rows of 8-byte multiples
+        u32x2 x = {0, 0}, y = {0, 0};
+        if (grp * 16 + 64 * i < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kr + 64 * i));
+        if (grp * 16 + 64 * i + 8 < dn) y = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kr + 64 * i + 8));
+        S.k[h][i] = u32x4{x[0], x[1], y[0], y[1]};
+      } else {
+        S.k[h][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kr + 64 * i));
+      }
+    }
+    const uint8_t* vr = slot + a.plane_bytes + grp * 4 * row + col * VB;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (VW == 2) {
+        u32x2 x = {0, 0};
+        if (!PAD || col * VB < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(vr + j * row));
+        S.v[h][j][0] = x[0];
+        S.v[h][j][1] = x[1];
+      } else {
+        S.v[h][j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vr + j * row));
+      }
+    }
+  };
+  auto compute = [&](Step& S) __attribute__((always_inline)) {
+    // ---- scores, in the log2 domain: t[h][i] is key 4 grp + i of group h ----
+    float t[2][4];
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        u32x4 w;
+        uint32_t p, q;
+        to_f16<F>(S.k[h][k / 2][2 * (k % 2)], p, q);
+        w[0] = p; w[1] = q;
+        to_f16<F>(S.k[h][k / 2][2 * (k % 2) + 1], p, q);
+        w[2] = p; w[3] = q;
+        s4 = mma_f16(w, qf[k], s4);
+      }
+      const float c = c_log2 * S.ks[h];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[h][i] = s4[i] * c;
+      if (S.lo[h] > 0 || S.hi[h] < 16) {  // keys out of the range: no weight, whatever their bytes
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = grp * 4 + i;
+          const bool ok = key >= S.lo[h] && key < S.hi[h];
+          t[h][i] = ok ? t[h][i] : -INFINITY;
+#pragma unroll
+          for (int w = 0; w < VW; ++w) S.v[h][i][w] = ok ? S.v[h][i][w] : 0;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, t[h][i]);
+    }
+    tmax = over_groups(tmax, [](float u, float v) { return fmaxf(u, v); });
+    // ---- running maxima of the scores and of weight times scale ----
+    const float m_new = fmaxf(m_run, tmax);
+    const float top = fmaxf(fmaxf(fabsf(S.vs[0]), fabsf(S.vs[1])), 1.17549435e-38f);
+    const float a_new = fmaxf(a_run, tmax + __builtin_amdgcn_logf(top));
+    l_run *= __builtin_amdgcn_exp2f(m_run - m_new);
+    if (__any(a_new > a_run)) {
+      const float f = __builtin_amdgcn_exp2f(a_run - a_new);
+#pragma unroll
+      for (int j = 0; j < VB; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] *= f;
+    }
+    m_run = m_new;
+    a_run = a_new;
+    const float f = __builtin_amdgcn_exp2f(m_new - a_new + 14.f);
+    // ---- weights: hi + lo ----
+    u32x4 ph, pl;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float fv = f * S.vs[h];
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(t[h][i] - m_new);
+        l_run += p;
+        w[i] = p * fv;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t u = pack_f16(w[2 * i], w[2 * i + 1]);
+        const f16x2 x = __builtin_bit_cast(f16x2, u);
+        ph[2 * h + i] = u;
+        pl[2 * h + i] = pack_f16(w[2 * i] - static_cast<float>(x[0]), w[2 * i + 1] - static_cast<float>(x[1]));
+      }
+    }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      u32x4 va[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {  // keys 2 p, 2 p + 1 of the lane's eight
+        const uint32_t x = S.v[p / 2][2 * (p % 2)][w], y = S.v[p / 2][2 * (p % 2) + 1][w];
+        uint32_t u, v;
+        to_f16<F>(__builtin_amdgcn_perm(y, x, 0x05010400u), u, v);
+        va[0][p] = u; va[1][p] = v;
+        to_f16<F>(__builtin_amdgcn_perm(y, x, 0x07030602u), u, v);
+        va[2][p] = u; va[3][p] = v;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[4 * w + j] = mma_f16(va[j], ph, acc[4 * w + j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[4 * w + j] = mma_f16(va[j], pl, acc[4 * w + j]);
+    }
+  };
+
+  // Rolling double buffer: the next step is loading while one is computed.
+  Step sa, sb;
+  auto load = [&](int g, Step& S) __attribute__((always_inline)) {
+    load_group(g, S, 0);
+    load_group(g + 1, S, 1);
+  };
+  if (g0 < g1) load(g0, sa);
+  for (int g = g0; g < g1; g += 4) {
+    if (g + 2 < g1) load(g + 2, sb);
+    compute(sa);
+    if (g + 4 < g1) load(g + 4, sa);
+    if (g + 2 < g1) compute(sb);
+  }
+
+  // ---- epilogue: dims (4 grp + i) VB + j of query col are acc[j][i] ----
+  const float l = over_groups(l_run, [](float u, float v) { return u + v; });
+  const float inv = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(a_run - m_run - 14.f) / l;  // NaN stays
+  const float lse2 = l == 0.f ? -INFINITY : m_run + __log2f(l);
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.hq;
+  const int64_t row0 = static_cast<int64_t>(b) * a.hq + kvh * a.rep;
+  if (a.subs == 1) {
+    if (col >= a.rep) return;
+    const int64_t r = row0 + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d0 = (4 * grp + i) * VB;
+      float x[VB];
+#pragma unroll
+      for (int j = 0; j < VB; ++j) x[j] = acc[j][i] * inv;
+      if (PAD && d0 >= dn) continue;
+      if (a.ws_o != nullptr) store_out<VB>(a.ws_o, kF32, (part * rows + r) * dn + d0, x);
+      else store_out<VB>(a.out, a.out_dtype, r * a.out_rs + d0, x);
+    }
+    if (grp == 0) {
+      if (a.ws_o != nullptr) a.ws_lse[part * rows + r] = lse2 * kLn2;
+      else if (a.lse != nullptr) a.lse[r] = lse2 * kLn2;
+    }
+    return;
+  }
+  // The runs of a part meet in LDS; wave `sub` of a kv head finishes its query heads sub, sub + subs, ...
+  float* const o_lds = meet_lds;
+  float* const lse_lds = meet_lds + a.heads * a.subs * a.rep * OS;
+  if (col < a.rep) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < VB; j += 4)
+        *reinterpret_cast<float4*>(o_lds + (wave * a.rep + col) * OS + (4 * grp + i) * VB + j) =
+            make_float4(acc[j][i] * inv, acc[j + 1][i] * inv, acc[j + 2][i] * inv, acc[j + 3][i] * inv);
+    if (grp == 0) lse_lds[wave * 16 + col] = lse2;
+  }
+  __syncthreads();
+  if (idle) return;
+  const int w0 = wave - sub * a.heads;
+  for (int c = sub; c < a.rep; c += a.subs) {
+    float m = -INFINITY;
+    for (int i = 0; i < a.subs; ++i) m = fmaxf(m, lse_lds[(w0 + i * a.heads) * 16 + c]);
+    const float ref = m == -INFINITY ? 0.f : m;  // no finite one: 0, or NaN with a NaN one
+    float o[D / 64] = {}, den = 0.f;
+    for (int i = 0; i < a.subs; ++i) {
+      const int w = w0 + i * a.heads;
+      const float f = __builtin_amdgcn_exp2f(lse_lds[w * 16 + c] - ref);
+      den += f;
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) o[k] += f * o_lds[(w * a.rep + c) * OS + lane + 64 * k];
+    }
+    const float inv_den = den == 0.f ? 0.f : 1.f / den;
+    const int64_t r = row0 + c;
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) {
+      const int d0 = lane + 64 * k;
+      if (PAD && d0 >= dn) continue;
+      if (a.ws_o != nullptr) a.ws_o[(part * rows + r) * dn + d0] = o[k] * inv_den;
+      else store_elem_rt(a.out, a.out_dtype, r * a.out_rs + d0, o[k] * inv_den);
+    }
+    if (lane == 0) {
+      const float v = den == 0.f ? -INFINITY : (ref + __log2f(den)) * kLn2;
+      if (a.ws_o != nullptr) a.ws_lse[part * rows + r] = v;
+      else if (a.lse != nullptr) a.lse[r] = v;
+    }
+  }
+}
+
+struct Kv8Plan {
+  int parts, heads, subs;
+};
+
+static Kv8Plan plan_kv8(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans) {
+  const int64_t groups = span_groups(n, spans), steps = ceil_div(groups, 2);
+  const int heads = static_cast<int>(ceil_div(hkv, ceil_div(hkv, kKv8Waves)));
+  const int64_t want = std::max<int64_t>(1, int64_t(device_cus()) * 8 / (int64_t(batch) * hkv));
+  const int64_t runs = std::min(want, steps);
+  int subs = 1;
+  while (heads * subs * 2 <= kKv8Waves && subs * 2 <= runs) subs *= 2;
+  const int parts = static_cast<int>(std::min<int64_t>(ceil_div(runs, subs), most_parts(batch, hq, d, groups)));
+  return Kv8Plan{parts, heads, subs};
+}
+
+// Covers these spans and any shorter ones.
+size_t kv8_decode_workspace_bytes(int batch, int hq, int d, int n, const DecodeSpan* spans) {
+  return parts_bytes(most_parts(batch, hq, d, span_groups(n, spans)), batch, hq, d);
+}
+
+template <int F, int D, bool PAD>
+static void launch_kv8_typed(const Kv8DecodeArgs& a, dim3 grid, hipStream_t stream) {
+  const int waves = a.heads * a.subs;
+  const size_t lds = a.subs > 1 ? sizeof(float) * waves * (static_cast<size_t>(a.rep) * (D + 4) + 16) : 0;
+  kv8_decode_kernel<F, D, PAD><<<grid, 64 * waves, lds, stream>>>(a);
+}
 
 void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const void* q, int64_t q_bs, int64_t q_hs, int n,
                        const DecodeSpan* spans, float scale, int out_dtype, void* out, int64_t out_rs, float* lse, void* ws,
                        size_t ws_bytes, int* err, hipStream_t stream) {
-  (void)ws;
-  (void)ws_bytes;
+  const int hkv = pool.hkv, d = pool.d;
+  require(batch <= 65535, "kv8_decode: batch must be at most 65535");  // grid y
+  for (int i = 0; i < n; ++i) require(spans[i].t0 >= 0 && spans[i].t0 < pool.bs, "kv8_decode: a span starts in its first block");
+  const Kv8Plan p = plan_kv8(batch, hq, hkv, d, n, spans);
   Kv8DecodeArgs a;
-  a.q = q;
+  a.ws_o = a.ws_lse = nullptr;
+  const int64_t rows = static_cast<int64_t>(batch) * hq;
+  if (p.parts > 1) {
+    const size_t need = parts_bytes(p.parts, batch, hq, d);
+    require(ws != nullptr && ws_bytes >= need, "workspace too small: need " + std::to_string(need) + " bytes");
+    require(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "workspace must be 16-byte aligned");
+    a.ws_o = static_cast<float*>(ws);
+    a.ws_lse = a.ws_o + (static_cast<size_t>(p.parts) * rows * d + 63) / 64 * 64;
+  }
+  a.q = static_cast<const uint16_t*>(q);
   a.q_bs = q_bs;
   a.q_hs = q_hs;
   a.pool = pool.codes;
   a.scales = pool.scales;
+  a.plane_bytes = pool.num_blocks * pool.bs * hkv * static_cast<int64_t>(d);
+  a.plane_scales = pool.num_blocks * hkv;
   a.num_blocks = pool.num_blocks;
   a.bs = pool.bs;
-  a.hkv = pool.hkv;
+  a.hkv = hkv;
   a.hq = hq;
-  a.d = pool.d;
+  a.rep = hq / hkv;
   a.n_spans = n;
   for (int i = 0; i < n; ++i) a.span[i] = spans[i];
+  a.heads = p.heads;
+  a.subs = p.subs;
+  a.gpb = pool.bs / 16;
+  a.gpb_shift = (a.gpb & (a.gpb - 1)) == 0 ? __builtin_ctz(a.gpb) : -1;
+  a.q_bf16 = dtype == kBF16;
   a.out_dtype = out_dtype;
-  a.scale = scale;
+  a.dn = d;
+  a.scale_log2 = scale * kLog2e;
   a.out = out;
   a.out_rs = out_rs;
   a.lse = lse;
+  a.batch = batch;
   a.err = err;
-  const dim3 grid(hq, batch);
+  const dim3 grid(static_cast<unsigned>(p.parts), static_cast<unsigned>(batch), static_cast<unsigned>(ceil_div(hkv, p.heads)));
+  // head dim 64: its own kernel; other multiples of 8 up to 128: 128 with the dims past it zero
   if (pool.format == kE4M3) {
-    if (dtype == kBF16) kv8_decode_kernel<kE4M3, kBF16><<<grid, 64, 0, stream>>>(a);
-    else kv8_decode_kernel<kE4M3, kF16><<<grid, 64, 0, stream>>>(a);
+    if (d == 128) launch_kv8_typed<kE4M3, 128, false>(a, grid, stream);
+    else if (d == 64) launch_kv8_typed<kE4M3, 64, false>(a, grid, stream);
+    else launch_kv8_typed<kE4M3, 128, true>(a, grid, stream);
   } else {
-    if (dtype == kBF16) kv8_decode_kernel<kInt8, kBF16><<<grid, 64, 0, stream>>>(a);
-    else kv8_decode_kernel<kInt8, kF16><<<grid, 64, 0, stream>>>(a);
+    if (d == 128) launch_kv8_typed<kInt8, 128, false>(a, grid, stream);
+    else if (d == 64) launch_kv8_typed<kInt8, 64, false>(a, grid, stream);
+    else launch_kv8_typed<kInt8, 128, true>(a, grid, stream);
   }
   HCP_HIP(hipGetLastError());
+  if (p.parts == 1) return;
+  const float* o_parts[64];
+  const float* l_parts[64];
+  for (int i = 0; i < p.parts; ++i) {
+    o_parts[i] = a.ws_o + static_cast<size_t>(i) * rows * d;
+    l_parts[i] = a.ws_lse + static_cast<size_t>(i) * rows;
+  }
+  launch_lse_merge(p.parts, o_parts, l_parts, static_cast<int>(rows), 1, d, out_dtype, out, out_rs, out_rs, lse, 1, stream);
 }
 
 }  // namespace hcp
