@@ -25,6 +25,7 @@
 //     = hi + lo, so P carries 22 bits (one f16 alone would put 2^-12 on every weight, against
 //     the fp32 weights of the 16-bit decode).  Sums and statistics are fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8.hpp"
 
@@ -181,200 +182,216 @@ __global__ __launch_bounds__(512) void kv8_decode_kernel(Kv8DecodeArgs a) {
   for (int j = 0; j < VB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = kNoMax, a_run = kNoMax, l_run = 0.f;
 
-  const int64_t row = static_cast<int64_t>(a.hkv) * dn;  // bytes of a slot, all heads
-  struct Step {
-    u32x4 k[2][KL];
-    uint32_t v[2][4][VW];
-    float ks[2], vs[2];
-    int lo[2], hi[2];  // keys [lo, hi) of each group count
-  };
-  typedef __attribute__((address_space(4))) const float ConstF;  // uniform loads
-  // Cursor over the shards: groups [s_begin, s_end) of the sequence lie in shard s.
-  int s = -1, s_begin = 0, s_end = 0;
-  int64_t t_end = 0, t_beg = 0;
-  int g_first = 0;
-  const int32_t* table = nullptr;
-  int64_t table_len = 0;
-  // Block ids of the run's groups, 64 at a time: lane i holds that of group ids_base + i.
-  int ids = -1, ids_base = -64;
-  auto load_group = [&](int g, Step& S, int h) __attribute__((always_inline)) {
-    S.lo[h] = S.hi[h] = 0;
-    S.ks[h] = S.vs[h] = 0.f;
-    if (g >= g1) {
-#pragma unroll
-      for (int i = 0; i < KL; ++i) S.k[h][i] = u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) S.v[h][j][w] = 0;
-      return;
-    }
-    if (g >= s_end) {
-      do {
-        ++s;
-        s_begin = s_end;
-        t_end = span_end(s);
-        s_end += span_groups(s, t_end);
-      } while (g >= s_end);
-      const DecodeSpan& sp = a.span[s];
-      t_beg = sp.t0;
-      g_first = static_cast<int>(t_beg / 16);
-      table = sp.tables + static_cast<int64_t>(b) * sp.table_stride;
-      table_len = sp.table_len;
-      ids_base = g - 64;
-    }
-    if (g - ids_base >= 64) {
-      ids_base = g;
-      const int gl = g_first + g - s_begin + lane;
-      const int e = a.gpb_shift >= 0 ? gl >> a.gpb_shift : gl / a.gpb;
-      ids = g + lane < min(g1, s_end) && e < table_len ? table[e] : -1;
-    }
-    const int32_t blk = __builtin_amdgcn_readlane(ids, g - ids_base);
-    const int gl = g_first + g - s_begin;
-    const int entry = a.gpb_shift >= 0 ? gl >> a.gpb_shift : gl / a.gpb;
-    const int64_t tok0 = static_cast<int64_t>(gl) * 16;
-    if (blk < 0 || blk >= a.num_blocks) {
-      if (lane == 0 && entry < table_len) atomicOr(a.err, 1);
-#pragma unroll
-      for (int i = 0; i < KL; ++i) S.k[h][i] = u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) S.v[h][j][w] = 0;
-      return;
-    }
-    S.lo[h] = __builtin_amdgcn_readfirstlane(static_cast<int>(t_beg > tok0 ? t_beg - tok0 : 0));
-    S.hi[h] = __builtin_amdgcn_readfirstlane(static_cast<int>(min(t_end - tok0, static_cast<int64_t>(16))));
-    const float* sc = a.scales + static_cast<int64_t>(blk) * a.hkv + kvh;
-    S.ks[h] = *(ConstF*)(uintptr_t)sc;
-    S.vs[h] = *(ConstF*)(uintptr_t)(sc + a.plane_scales);
-    const uint8_t* slot = a.pool + (static_cast<int64_t>(blk) * a.bs + (gl - entry * a.gpb) * 16) * row + kvh * dn;
-    const uint8_t* kr = slot + col * row + grp * 16;
+  const uint32_t row = static_cast<uint32_t>(a.hkv) * dn;  // bytes of a slot, all heads
+  const int64_t block_bytes = static_cast<int64_t>(a.bs) * row;
+  const uint8_t* const k_head = a.pool + kvh * dn;
+  const uint8_t* const v_head = k_head + a.plane_bytes;
+  const uint32_t k_at = col * row + grp * 16, v_at = grp * 4 * row + col * VB;  // of a group's first row
+  u32x4 kx[2][KL];         // the step's codes
+  uint32_t vx[2][4][VW];
+  // Groups of the shard, 64 at a time: lane i holds the place in the pool and the scales of
+  // group `batch` + i (place 0 and scales 0 for one that is not there: always in the pool, of
+  // no weight), and the block id of group batch + 64 + i.
+  int batch = 0, next_id = -1;
+  int64_t place = 0;
+  float ks_l = 0.f, vs_l = 0.f;
+  uint64_t absent = 0;  // groups of the batch with a bad block id
+  auto load_k = [&](int h, int64_t at) __attribute__((always_inline)) {
+    const uint8_t* const p = k_head + at;
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
       if constexpr (PAD) {  // rows of 8-byte multiples
         u32x2 x = {0, 0}, y = {0, 0};
-        if (grp * 16 + 64 * i < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kr + 64 * i));
-        if (grp * 16 + 64 * i + 8 < dn) y = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kr + 64 * i + 8));
-        S.k[h][i] = u32x4{x[0], x[1], y[0], y[1]};
+        if (grp * 16 + 64 * i < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + k_at + 64 * i));
+        if (grp * 16 + 64 * i + 8 < dn) y = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + k_at + 64 * i + 8));
+        kx[h][i] = u32x4{x[0], x[1], y[0], y[1]};
       } else {
-        S.k[h][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kr + 64 * i));
+        kx[h][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + k_at + 64 * i));
       }
     }
-    const uint8_t* vr = slot + a.plane_bytes + grp * 4 * row + col * VB;
+  };
+  auto load_v = [&](int h, int64_t at) __attribute__((always_inline)) {
+    const uint8_t* const p = v_head + at;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (VW == 2) {
         u32x2 x = {0, 0};
-        if (!PAD || col * VB < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(vr + j * row));
-        S.v[h][j][0] = x[0];
-        S.v[h][j][1] = x[1];
+        if (!PAD || col * VB < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + v_at + j * row));
+        vx[h][j][0] = x[0];
+        vx[h][j][1] = x[1];
       } else {
-        S.v[h][j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vr + j * row));
+        vx[h][j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p + v_at + j * row));
       }
     }
   };
-  auto compute = [&](Step& S) __attribute__((always_inline)) {
-    // ---- scores, in the log2 domain: t[h][i] is key 4 grp + i of group h ----
-    float t[2][4];
-    float tmax = -INFINITY;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        u32x4 w;
-        uint32_t p, q;
-        to_f16<F>(S.k[h][k / 2][2 * (k % 2)], p, q);
-        w[0] = p; w[1] = q;
-        to_f16<F>(S.k[h][k / 2][2 * (k % 2) + 1], p, q);
-        w[2] = p; w[3] = q;
-        s4 = mma_f16(w, qf[k], s4);
-      }
-      const float c = c_log2 * S.ks[h];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t[h][i] = s4[i] * c;
-      if (S.lo[h] > 0 || S.hi[h] < 16) {  // keys out of the range: no weight, whatever their bytes
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = grp * 4 + i;
-          const bool ok = key >= S.lo[h] && key < S.hi[h];
-          t[h][i] = ok ? t[h][i] : -INFINITY;
-#pragma unroll
-          for (int w = 0; w < VW; ++w) S.v[h][i][w] = ok ? S.v[h][i][w] : 0;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, t[h][i]);
-    }
-    tmax = over_groups(tmax, [](float u, float v) { return fmaxf(u, v); });
-    // ---- running maxima of the scores and of weight times scale ----
-    const float m_new = fmaxf(m_run, tmax);
-    const float top = fmaxf(fmaxf(fabsf(S.vs[0]), fabsf(S.vs[1])), 1.17549435e-38f);
-    const float a_new = fmaxf(a_run, tmax + __builtin_amdgcn_logf(top));
-    l_run *= __builtin_amdgcn_exp2f(m_run - m_new);
-    if (__any(a_new > a_run)) {
-      const float f = __builtin_amdgcn_exp2f(a_run - a_new);
-#pragma unroll
-      for (int j = 0; j < VB; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] *= f;
-    }
-    m_run = m_new;
-    a_run = a_new;
-    const float f = __builtin_amdgcn_exp2f(m_new - a_new + 14.f);
-    // ---- weights: hi + lo ----
-    u32x4 ph, pl;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float fv = f * S.vs[h];
-      float w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(t[h][i] - m_new);
-        l_run += p;
-        w[i] = p * fv;
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t u = pack_f16(w[2 * i], w[2 * i + 1]);
-        const f16x2 x = __builtin_bit_cast(f16x2, u);
-        ph[2 * h + i] = u;
-        pl[2 * h + i] = pack_f16(w[2 * i] - static_cast<float>(x[0]), w[2 * i + 1] - static_cast<float>(x[1]));
-      }
-    }
-    // ---- O^T += V^T P^T ----
-#pragma unroll
-    for (int w = 0; w < VW; ++w) {
-      u32x4 va[4];
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {  // keys 2 p, 2 p + 1 of the lane's eight
-        const uint32_t x = S.v[p / 2][2 * (p % 2)][w], y = S.v[p / 2][2 * (p % 2) + 1][w];
-        uint32_t u, v;
-        to_f16<F>(__builtin_amdgcn_perm(y, x, 0x05010400u), u, v);
-        va[0][p] = u; va[1][p] = v;
-        to_f16<F>(__builtin_amdgcn_perm(y, x, 0x07030602u), u, v);
-        va[2][p] = u; va[3][p] = v;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[4 * w + j] = mma_f16(va[j], ph, acc[4 * w + j]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[4 * w + j] = mma_f16(va[j], pl, acc[4 * w + j]);
-    }
+  auto place_of = [&](int i) __attribute__((always_inline)) -> int64_t {
+    return static_cast<int64_t>(
+        static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place >> 32), i))) << 32 |
+        static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place), i)));
+  };
+  auto scale_of = [&](float v, int i) __attribute__((always_inline)) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
   };
 
-  // Rolling double buffer: the next step is loading while one is computed.
-  Step sa, sb;
-  auto load = [&](int g, Step& S) __attribute__((always_inline)) {
-    load_group(g, S, 0);
-    load_group(g + 1, S, 1);
-  };
-  if (g0 < g1) load(g0, sa);
-  for (int g = g0; g < g1; g += 4) {
-    if (g + 2 < g1) load(g + 2, sb);
-    compute(sa);
-    if (g + 4 < g1) load(g + 4, sa);
-    if (g + 2 < g1) compute(sb);
+  int before = 0;  // groups of the shards before
+  for (int s = 0; s < a.n_spans; ++s) {
+    const DecodeSpan& sp = a.span[s];
+    const int64_t t_beg = sp.t0, t_end = span_end(s);
+    const int here = span_groups(s, t_end), g_first = static_cast<int>(t_beg / 16);
+    // the run's groups of this shard, counted from the table's start
+    const int lo = max(g0 - before, 0) + g_first, end = min(g1 - before, here) + g_first;
+    before += here;
+    if (lo >= end) continue;
+    const int32_t* const table = sp.tables + static_cast<int64_t>(b) * sp.table_stride;
+    auto id_of = [&](int g) __attribute__((always_inline)) {
+      const int e = a.gpb_shift >= 0 ? g >> a.gpb_shift : g / a.gpb;
+      return g < end && e < sp.table_len ? table[e] : -1;
+    };
+    auto take_batch = [&](int first) __attribute__((always_inline)) {
+      batch = first;
+      const int g = first + lane, blk = next_id;
+      const bool in = g < end, ok = in && blk >= 0 && blk < a.num_blocks;
+      const int slot = 16 * (a.gpb_shift >= 0 ? g & (a.gpb - 1) : g % a.gpb);
+      place = ok ? blk * block_bytes + static_cast<int64_t>(slot) * row : 0;
+      ks_l = vs_l = 0.f;
+      if (ok) {
+        const float* const sc = a.scales + static_cast<int64_t>(blk) * a.hkv + kvh;
+        ks_l = sc[0];
+        vs_l = sc[a.plane_scales];
+      }
+      absent = __ballot(in && !ok);
+      if (in && !ok) atomicOr(a.err, 1);
+      next_id = id_of(g + 64);
+    };
+    const int full_lo = static_cast<int>((t_beg + 15) / 16), full_end = min(end, static_cast<int>(min(t_end / 16, static_cast<int64_t>(INT32_MAX))));
+
+    // 32 tokens: groups g, g + 1.  The next step's K takes the registers of this one's once S
+    // is known, its V those of this one's at the end: loads are always under way, and none
+    // stands in a branch (where it would make every wait one for all loads).
+    auto step = [&](int g, auto more) __attribute__((always_inline)) {
+      constexpr bool kMore = decltype(more)::value;
+      const int at = g - batch;
+      const float ks[2] = {scale_of(ks_l, at), scale_of(ks_l, at + 1)}, vs[2] = {scale_of(vs_l, at), scale_of(vs_l, at + 1)};
+      const bool full = g >= full_lo && g + 1 < full_end && (absent >> at & 3) == 0;
+      const uint64_t gone = absent >> at;
+      // ---- scores: s4[h][i] is key 4 grp + i of group h ----
+      f32x4 s4[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s4[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t w[4];
+          to_f16<F>(kx[h][k / 2][2 * (k % 2)], w[0], w[1]);
+          to_f16<F>(kx[h][k / 2][2 * (k % 2) + 1], w[2], w[3]);
+          s4[h] = mma_f16(u32x4{w[0], w[1], w[2], w[3]}, qf[k], s4[h]);
+        }
+      }
+      int64_t next[2] = {0, 0};
+      if constexpr (kMore) {
+        if (g + 2 - batch >= 64) take_batch(g + 2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          next[h] = place_of(g + 2 + h - batch);
+          load_k(h, next[h]);
+        }
+      }
+      // ---- log2 domain; keys outside the range and groups that are not there weigh nothing ----
+      bool ok[2][4];
+      float tmax = -INFINITY;
+      const float c[2] = {c_log2 * ks[0], c_log2 * ks[1]};
+      float t[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[h][i] = s4[h][i] * c[h];
+      if (!full) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int64_t tok = static_cast<int64_t>(g + h) * 16 + grp * 4 + i;
+            ok[h][i] = g + h < end && tok >= t_beg && tok < t_end && (gone >> h & 1) == 0;
+            t[h][i] = ok[h][i] ? t[h][i] : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, t[h][i]);
+      tmax = over_groups(tmax, [](float u, float v) { return fmaxf(u, v); });
+      // ---- running maxima of the scores and of weight times scale ----
+      const float m_new = fmaxf(m_run, tmax);
+      const float top = fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), 1.17549435e-38f);
+      const float a_new = fmaxf(a_run, tmax + __builtin_amdgcn_logf(top));
+      l_run *= __builtin_amdgcn_exp2f(m_run - m_new);
+      if (__any(a_new > a_run)) {
+        const float f = __builtin_amdgcn_exp2f(a_run - a_new);
+#pragma unroll
+        for (int j = 0; j < VB; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[j][i] *= f;
+      }
+      m_run = m_new;
+      a_run = a_new;
+      const float f = __builtin_amdgcn_exp2f(m_new - a_new + 14.f);
+      // ---- weights: hi + lo ----
+      u32x4 ph, pl;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float fv = f * vs[h];
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = __builtin_amdgcn_exp2f(t[h][i] - m_new);
+          l_run += p;
+          w[i] = p * fv;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t u = pack_f16(w[2 * i], w[2 * i + 1]);
+          const f16x2 x = __builtin_bit_cast(f16x2, u);
+          ph[2 * h + i] = u;
+          pl[2 * h + i] = pack_f16(w[2 * i] - static_cast<float>(x[0]), w[2 * i + 1] - static_cast<float>(x[1]));
+        }
+      }
+      // ---- O^T += V^T P^T ----
+      if (F == kE4M3 && !full) {  // a NaN code times a weight of 0
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vx[h][i][w] = ok[h][i] ? vx[h][i][w] : 0;
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        uint32_t va[4][4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {  // keys 2 p, 2 p + 1 of the lane's eight
+          const uint32_t x = vx[p / 2][2 * (p % 2)][w], y = vx[p / 2][2 * (p % 2) + 1][w];
+          to_f16<F>(__builtin_amdgcn_perm(y, x, 0x05010400u), va[0][p], va[1][p]);
+          to_f16<F>(__builtin_amdgcn_perm(y, x, 0x07030602u), va[2][p], va[3][p]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[4 * w + j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, ph, acc[4 * w + j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[4 * w + j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, pl, acc[4 * w + j]);
+      }
+      if constexpr (kMore) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_v(h, next[h]);
+      }
+    };
+    next_id = id_of(lo + lane);
+    take_batch(lo);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) load_k(h, place_of(h));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) load_v(h, place_of(h));
+    int g = lo;
+    for (; g + 2 < end; g += 2) step(g, std::true_type{});
+    step(g, std::false_type{});
   }
 
   // ---- epilogue: dims (4 grp + i) VB + j of query col are acc[j][i] ----
