@@ -170,7 +170,7 @@ struct Kv8Append {
   uint8_t* pool;
   float* scales;
   int64_t num_blocks;
-  int32_t bs, hkv, d, lanes_per_row;
+  int32_t bs, hkv, d, lanes_per_row, window;  // window: tokens whose runs a wave takes
   const void* src[2];  // k, v views [hkv, tokens, d]
   int64_t hs[2], ss[2];
   int64_t tokens;
@@ -181,7 +181,7 @@ void launch_kv8_append(int format, int dtype, Kv8Append p, hipStream_t stream);
 constexpr int kKv8Ranges = 16;
 struct Kv8Range {
   const int32_t* table;
-  int64_t at0;  // place in the table's blocks of the range's first token
+  int64_t entry0, at0, tokens;  // first table entry, place in the table's blocks of the first token
   void *k, *v;
   int64_t hs, ss;
 };
@@ -189,8 +189,8 @@ struct Kv8Gather {
   const uint8_t* pool;
   const float* scales;
   int64_t num_blocks;
-  int32_t bs, hkv, d, lanes_per_row, n;
-  int64_t tokens, begin[kKv8Ranges];  // tokens of all ranges; those before a range
+  int32_t bs, hkv, d, lanes_per_row, per_block, n;  // per_block: work items of a block
+  int32_t begin[kKv8Ranges + 1];                     // items before a range
   Kv8Range r[kKv8Ranges];
   int* err;
 };
