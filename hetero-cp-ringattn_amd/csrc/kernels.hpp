@@ -126,11 +126,8 @@ struct DecodeSpan {
   int64_t t0, t1;
   int64_t len_off = 0;
 };
-// 16-token groups of the longest sequence that the spans allow; most parts of a decode plan
-// over them, and the bytes of `parts` partials of every (sequence, head): o, then lse.
+// 16-token groups of the longest sequence that the spans allow.
 int64_t span_groups(int n, const DecodeSpan* spans);
-int most_parts(int batch, int hq, int d, int64_t groups);
-size_t parts_bytes(int parts, int batch, int hq, int d);
 // Workspace of launch_paged_decode for these shards, and for any shorter ones.
 size_t decode_workspace_bytes(int batch, int hq, int d, int n, const DecodeSpan* spans);
 // Attention of one query per sequence over its n shards, merged: out[row * out_rs + d] in

@@ -5,10 +5,13 @@
 // HBM-bound: every code is read once, half the bytes of the 16-bit decode for the same
 // products, so the work beside the loads has to be half as large, too.  Both products run on
 // the matrix cores and no value passes through LDS on the way:
-//   * One launch covers all shards; a sequence's 16-token groups are dealt out in equal runs
-//     to parts x subs waves (grid (parts, batch, head groups), a workgroup holding `heads` kv
-//     heads x `subs` runs).  The subs of a part meet in LDS, parts in the LSE merge; a lone
-//     part writes the output itself.
+//   * One launch covers all shards.  Where the sequences alone fill the chip, or are short, a
+//     workgroup has one of them (direct): `heads` kv heads x `subs` waves that share its
+//     tokens and meet in LDS.  Otherwise the 16-token groups of all sequences stand in one row
+//     and every worker takes the same length of it (balanced), so ragged lengths leave no
+//     CU behind: a worker that crosses a sequence's end writes one partial of each side, at
+//     place (worker + sequence) of the workspace -- a pair moves on in one or the other, so no
+//     two share a place -- and kv8_join_kernel merges a sequence's places, which are neighbours.
 //   * A step is 32 tokens.  S^T = K Q^T (16x16x32, f16): A = 16 key rows, their codes converted
 //     in registers (exact: a code has at most 8 significant bits), B = the rep <= 16 query
 //     heads.  16-bit q times a power of two that brings its largest value to 2^14 is exact in
@@ -44,7 +47,9 @@ struct Kv8DecodeArgs {
   int32_t gpb, gpb_shift;  // 16-token groups per block, its log2 or -1
   int32_t q_bf16, out_dtype, dn;
   float scale_log2;
-  float *ws_o, *ws_lse;  // [parts][batch * hq][dn]; null: a lone part
+  int32_t workers, min_len;  // balanced: workers per head group (0: direct), least groups of one
+  float *ws_o, *ws_lse;      // [workers + batch][hq][dn]
+  int2* range;               // [batch] first place and places of a sequence
   void* out;
   int64_t out_rs;
   float* lse;
@@ -54,7 +59,8 @@ struct Kv8DecodeArgs {
 static_assert(sizeof(Kv8DecodeArgs) <= 4096, "kernel arguments are limited to 4 KiB");
 
 constexpr float kNoMax = -1.0e30f;
-constexpr int kKv8Waves = 8;  // most waves per workgroup
+// Most waves per workgroup: four to a SIMD, which 128 registers allow; the padded form needs more.
+constexpr int kv8_waves(bool pad) { return pad ? 8 : 16; }
 
 // A word of codes to two pairs of f16: codes 0, 1 and 2, 3.  int8: u = code + 128 as the low
 // byte of 1024 + u, then - 1152.
@@ -111,7 +117,7 @@ __device__ __forceinline__ void store_out(void* out, int dtype, int64_t at, cons
 // PAD: head dim a.dn < D (a multiple of 8); 8-byte pieces past it are not loaded (zeros) nor
 // stored.
 template <int F, int D, bool PAD>
-__global__ __launch_bounds__(512) void kv8_decode_kernel(Kv8DecodeArgs a) {
+__global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8DecodeArgs a) {
   const int dn = PAD ? a.dn : D;
   constexpr int KL = D / 64;  // 16-byte loads of a key row per lane
   constexpr int KS = D / 32;  // k-steps of S
@@ -120,13 +126,13 @@ __global__ __launch_bounds__(512) void kv8_decode_kernel(Kv8DecodeArgs a) {
   constexpr int OS = D + 4;   // LDS row of the meeting, 4 floats apart from a bank's multiple
   extern __shared__ __attribute__((aligned(16))) float meet_lds[];  // subs > 1: [wave][rep][OS], then lse [wave][16]
 
-  const int b = blockIdx.y, part = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int sub = wave / a.heads;
   const int kvh = blockIdx.z * a.heads + wave - sub * a.heads;
   const bool idle = kvh >= a.hkv;
   if (idle && a.subs == 1) return;  // no workgroup barrier below
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  int b = blockIdx.y;
 
   auto span_end = [&](int s) __attribute__((always_inline)) -> int64_t {
     const DecodeSpan& sp = a.span[s];
@@ -137,12 +143,71 @@ __global__ __launch_bounds__(512) void kv8_decode_kernel(Kv8DecodeArgs a) {
     const int64_t t0 = a.span[s].t0;
     return t_end > t0 ? static_cast<int>((t_end + 15) / 16 - t0 / 16) : 0;
   };
-  int total = 0;
-  for (int s = 0; s < a.n_spans; ++s) total += span_groups(s, span_end(s));
-  const int runs = gridDim.x * a.subs;
-  const int run_len = (total + 2 * runs - 1) / (2 * runs) * 2;  // whole steps
-  const int g0 = idle ? total : static_cast<int>(min(static_cast<int64_t>(part * a.subs + sub) * run_len, static_cast<int64_t>(total)));
-  const int g1 = min(g0 + run_len, total);
+  auto seq_groups = [&]() __attribute__((always_inline)) {
+    int n = 0;
+    for (int s = 0; s < a.n_spans; ++s) n += span_groups(s, span_end(s));
+    return n;
+  };
+  int total, begin = 0, end_all;  // groups of sequence b; the workgroup's: [begin, end_all)
+  int left = 0;                   // groups of the worker after those
+  if (a.workers == 0) {
+    total = end_all = seq_groups();
+  } else {
+    // The row of all sequences' groups, each rounded to whole steps: lane i has sequence i of 64.
+    auto lane_groups = [&](int i) __attribute__((always_inline)) {
+      int n = 0;
+      if (i < a.batch)
+        for (int s = 0; s < a.n_spans; ++s) {
+          const DecodeSpan& sp = a.span[s];
+          const int64_t t_end = sp.seq_lens == nullptr ? sp.t1 : min(sp.t1, static_cast<int64_t>(sp.seq_lens[i]) - sp.len_off);
+          n += span_groups(s, t_end);
+        }
+      return (n + 1) & ~1;
+    };
+    auto scan = [&](int n) __attribute__((always_inline)) {  // inclusive, over the wave
+      for (int off = 1; off < 64; off *= 2) {
+        const int v = __shfl_up(n, off);
+        if (lane >= off) n += v;
+      }
+      return n;
+    };
+    int all = 0;
+    for (int i = 0; i < a.batch; i += 64) all += __builtin_amdgcn_readlane(scan(lane_groups(i + lane)), 63);
+    const int len = max((all + 2 * a.workers - 1) / (2 * a.workers) * 2, a.min_len);
+    const int w = blockIdx.x;
+    const int64_t from = static_cast<int64_t>(w) * len;
+    if (w == 0 && blockIdx.z == 0 && wave == 0) {  // where the join finds every sequence
+      int start = 0;
+      for (int i = 0; i < a.batch; i += 64) {
+        const int n = lane_groups(i + lane), sum = scan(n), at = start + sum - n;
+        if (i + lane < a.batch) a.range[i + lane] = n == 0 ? make_int2(0, 0) : make_int2(at / len + i + lane, (at + n - 1) / len - at / len + 1);
+        start += __builtin_amdgcn_readlane(sum, 63);
+      }
+    }
+    if (from >= all) return;  // the whole workgroup
+    int start = 0;
+    b = 0;
+    for (int i = 0; i < a.batch; i += 64) {
+      const int n = lane_groups(i + lane), sum = scan(n);
+      const uint64_t past = __ballot(start + sum > from);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        b = i + at;
+        begin = static_cast<int>(from) - (start + __builtin_amdgcn_readlane(sum - n, at));
+        break;
+      }
+      start += __builtin_amdgcn_readlane(sum, 63);
+    }
+    total = seq_groups();
+    const int mine = min(len, all - static_cast<int>(from));
+    end_all = min(begin + mine, (total + 1) & ~1);
+    left = mine - (end_all - begin);
+  }
+
+  for (;;) {  // one sequence's share
+  const int run_len = (end_all - begin + 2 * a.subs - 1) / (2 * a.subs) * 2;  // whole steps
+  const int g0 = idle ? total : min(begin + sub * run_len, total);
+  const int g1 = min(min(g0 + run_len, end_all), total);
 
   // Q^T in f16, times a power of two that brings the row's largest value to 2^14 .. 2^15.
   // k-step 2 h + e holds dims 16 grp + 64 h + 8 e + i, as the 16-byte loads of K bring them.
@@ -365,19 +430,20 @@ __global__ __launch_bounds__(512) void kv8_decode_kernel(Kv8DecodeArgs a) {
             for (int w = 0; w < VW; ++w) vx[h][i][w] = ok[h][i] ? vx[h][i][w] : 0;
       }
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        uint32_t va[4][4];
+      for (int w = 0; w < VW; ++w)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {  // keys 2 p, 2 p + 1 of the lane's eight
-          const uint32_t x = vx[p / 2][2 * (p % 2)][w], y = vx[p / 2][2 * (p % 2) + 1][w];
-          to_f16<F>(__builtin_amdgcn_perm(y, x, 0x05010400u), va[0][p], va[1][p]);
-          to_f16<F>(__builtin_amdgcn_perm(y, x, 0x07030602u), va[2][p], va[3][p]);
+        for (int half = 0; half < 2; ++half) {  // tiles 4 w + 2 half, + 1
+          uint32_t va[2][4];
+#pragma unroll
+          for (int p = 0; p < 4; ++p)  // keys 2 p, 2 p + 1 of the lane's eight
+            to_f16<F>(__builtin_amdgcn_perm(vx[p / 2][2 * (p % 2) + 1][w], vx[p / 2][2 * (p % 2)][w], half ? 0x07030602u : 0x05010400u),
+                      va[0][p], va[1][p]);
+          f32x4* const o = acc + 4 * w + 2 * half;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) o[j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, ph, o[j]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) o[j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, pl, o[j]);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[4 * w + j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, ph, acc[4 * w + j]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[4 * w + j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, pl, acc[4 * w + j]);
-      }
       if constexpr (kMore) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) load_v(h, next[h]);
@@ -398,89 +464,168 @@ __global__ __launch_bounds__(512) void kv8_decode_kernel(Kv8DecodeArgs a) {
   const float l = over_groups(l_run, [](float u, float v) { return u + v; });
   const float inv = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(a_run - m_run - 14.f) / l;  // NaN stays
   const float lse2 = l == 0.f ? -INFINITY : m_run + __log2f(l);
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.hq;
-  const int64_t row0 = static_cast<int64_t>(b) * a.hq + kvh * a.rep;
+  // Addresses below are made from a lane number of their own: hoisted out of the loop over
+  // sequences they would cost registers all the way through it.
+  int ln = lane;
+  asm volatile("" : "+v"(ln));
+  const int col = ln & 15, grp = ln >> 4;
+  // rows of the output, or of the workspace
+  const bool last = a.workers == 0;
+  const int64_t row0 = (last ? b : blockIdx.x + b) * static_cast<int64_t>(a.hq) + kvh * a.rep;
+  void* const o_to = last ? a.out : a.ws_o;
+  float* const lse_to = last ? a.lse : a.ws_lse;
+  const int64_t o_rs = last ? a.out_rs : dn;
+  const int o_dt = last ? a.out_dtype : kF32;
   if (a.subs == 1) {
-    if (col >= a.rep) return;
-    const int64_t r = row0 + col;
+    if (col < a.rep) {
+      const int64_t r = row0 + col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d0 = (4 * grp + i) * VB;
-      float x[VB];
+      for (int i = 0; i < 4; ++i) {
+        const int d0 = (4 * grp + i) * VB;
+        float x[VB];
 #pragma unroll
-      for (int j = 0; j < VB; ++j) x[j] = acc[j][i] * inv;
-      if (PAD && d0 >= dn) continue;
-      if (a.ws_o != nullptr) store_out<VB>(a.ws_o, kF32, (part * rows + r) * dn + d0, x);
-      else store_out<VB>(a.out, a.out_dtype, r * a.out_rs + d0, x);
+        for (int j = 0; j < VB; ++j) x[j] = acc[j][i] * inv;
+        if (!PAD || d0 < dn) store_out<VB>(o_to, o_dt, r * o_rs + d0, x);
+      }
+      if (grp == 0 && lse_to != nullptr) lse_to[r] = lse2 * kLn2;
     }
-    if (grp == 0) {
-      if (a.ws_o != nullptr) a.ws_lse[part * rows + r] = lse2 * kLn2;
-      else if (a.lse != nullptr) a.lse[r] = lse2 * kLn2;
+  } else {
+    // The waves of a kv head meet in LDS; wave `sub` finishes its query heads sub, sub + subs, ...
+    float* const o_lds = meet_lds;
+    float* const lse_lds = meet_lds + a.heads * a.subs * a.rep * OS;
+    if (col < a.rep) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < VB; j += 4)
+          *reinterpret_cast<float4*>(o_lds + (wave * a.rep + col) * OS + (4 * grp + i) * VB + j) =
+              make_float4(acc[j][i] * inv, acc[j + 1][i] * inv, acc[j + 2][i] * inv, acc[j + 3][i] * inv);
+      if (grp == 0) lse_lds[wave * 16 + col] = lse2;
     }
-    return;
+    __syncthreads();
+    const int w0 = wave - sub * a.heads;
+    for (int c = idle ? a.rep : sub; c < a.rep; c += a.subs) {
+      float m = -INFINITY;
+      for (int i = 0; i < a.subs; ++i) m = fmaxf(m, lse_lds[(w0 + i * a.heads) * 16 + c]);
+      const float ref = m == -INFINITY ? 0.f : m;  // no finite one: 0, or NaN with a NaN one
+      float o[D / 64] = {}, den = 0.f;
+      for (int i = 0; i < a.subs; ++i) {
+        const int w = w0 + i * a.heads;
+        const float f = __builtin_amdgcn_exp2f(lse_lds[w * 16 + c] - ref);
+        den += f;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) o[k] += f * o_lds[(w * a.rep + c) * OS + ln + 64 * k];
+      }
+      const float inv_den = den == 0.f ? 0.f : 1.f / den;
+      const int64_t r = row0 + c;
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) {
+        const int d0 = ln + 64 * k;
+        if (!PAD || d0 < dn) store_elem_rt(o_to, o_dt, r * o_rs + d0, o[k] * inv_den);
+      }
+      if (ln == 0 && lse_to != nullptr) lse_to[r] = den == 0.f ? -INFINITY : (ref + __log2f(den)) * kLn2;
+    }
   }
-  // The runs of a part meet in LDS; wave `sub` of a kv head finishes its query heads sub, sub + subs, ...
-  float* const o_lds = meet_lds;
-  float* const lse_lds = meet_lds + a.heads * a.subs * a.rep * OS;
-  if (col < a.rep) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < VB; j += 4)
-        *reinterpret_cast<float4*>(o_lds + (wave * a.rep + col) * OS + (4 * grp + i) * VB + j) =
-            make_float4(acc[j][i] * inv, acc[j + 1][i] * inv, acc[j + 2][i] * inv, acc[j + 3][i] * inv);
-    if (grp == 0) lse_lds[wave * 16 + col] = lse2;
-  }
-  __syncthreads();
-  if (idle) return;
-  const int w0 = wave - sub * a.heads;
-  for (int c = sub; c < a.rep; c += a.subs) {
-    float m = -INFINITY;
-    for (int i = 0; i < a.subs; ++i) m = fmaxf(m, lse_lds[(w0 + i * a.heads) * 16 + c]);
-    const float ref = m == -INFINITY ? 0.f : m;  // no finite one: 0, or NaN with a NaN one
-    float o[D / 64] = {}, den = 0.f;
-    for (int i = 0; i < a.subs; ++i) {
-      const int w = w0 + i * a.heads;
-      const float f = __builtin_amdgcn_exp2f(lse_lds[w * 16 + c] - ref);
-      den += f;
-#pragma unroll
-      for (int k = 0; k < D / 64; ++k) o[k] += f * o_lds[(w * a.rep + c) * OS + lane + 64 * k];
-    }
-    const float inv_den = den == 0.f ? 0.f : 1.f / den;
-    const int64_t r = row0 + c;
-#pragma unroll
-    for (int k = 0; k < D / 64; ++k) {
-      const int d0 = lane + 64 * k;
-      if (PAD && d0 >= dn) continue;
-      if (a.ws_o != nullptr) a.ws_o[(part * rows + r) * dn + d0] = o[k] * inv_den;
-      else store_elem_rt(a.out, a.out_dtype, r * a.out_rs + d0, o[k] * inv_den);
-    }
-    if (lane == 0) {
-      const float v = den == 0.f ? -INFINITY : (ref + __log2f(den)) * kLn2;
-      if (a.ws_o != nullptr) a.ws_lse[part * rows + r] = v;
-      else if (a.lse != nullptr) a.lse[r] = v;
-    }
+  if (left == 0) return;
+  if (a.subs > 1) __syncthreads();  // LDS is read
+  do {  // the next sequence that holds tokens
+    ++b;
+    total = seq_groups();
+  } while (total == 0);
+  begin = 0;
+  end_all = min(left, (total + 1) & ~1);
+  left -= end_all;
   }
 }
 
+// Merge of a sequence's neighbouring places, one (sequence, query head) per workgroup:
+// 256 / lpr slots take every so-manieth place with kU loads in flight each, and meet in LDS.
+template <int OUT_DT>
+__global__ __launch_bounds__(256) void kv8_join_kernel(const float* ws_o, const float* ws_lse, const int2* range, int hq, int dn,
+                                                       int lpr, void* out, int64_t out_rs, float* lse) {
+  constexpr int kU = 4;
+  __shared__ float4 acc_l[256];
+  __shared__ float m_l[256], den_l[256];
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int2 where = range[b];
+  const int slots = 256 / lpr, slot = threadIdx.x / lpr, c = threadIdx.x % lpr * 4;
+  const bool active = c < dn;
+  float m = -INFINITY, den = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = slot; base < where.y; base += kU * slots) {
+    float l[kU];
+    float4 v[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int i = base + u * slots;
+      const int64_t r = static_cast<int64_t>(where.x + i) * hq + h;
+      l[u] = i < where.y ? ws_lse[r] : -INFINITY;
+      v[u] = i < where.y && active ? *reinterpret_cast<const float4*>(ws_o + r * dn + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) mn = fmaxf(mn, l[u]);
+    const float ref = mn == -INFINITY ? 0.f : mn;  // all empty so far: they add 0, a NaN stays
+    const float sc = __expf(m - ref);
+    den *= sc;
+    acc.x *= sc; acc.y *= sc; acc.z *= sc; acc.w *= sc;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const float w = __expf(l[u] - ref);
+      den += w;
+      acc.x += w * v[u].x; acc.y += w * v[u].y; acc.z += w * v[u].z; acc.w += w * v[u].w;
+    }
+    m = mn;
+  }
+  acc_l[threadIdx.x] = acc;
+  m_l[threadIdx.x] = m;
+  den_l[threadIdx.x] = den;
+  __syncthreads();
+  if (slot != 0) return;
+  const int used = max(min(slots, where.y), 1);
+  float mt = -INFINITY;
+  for (int s = 0; s < used; ++s) mt = fmaxf(mt, m_l[threadIdx.x + s * lpr]);
+  const float ref = mt == -INFINITY ? 0.f : mt;
+  float dt = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < used; ++s) {
+    const float ms = m_l[threadIdx.x + s * lpr];
+    const float w = ms == -INFINITY ? 1.f : __expf(ms - ref);  // no finite place: its sum is 0 or NaN as it stands
+    const float4 x = acc_l[threadIdx.x + s * lpr];
+    dt += w * den_l[threadIdx.x + s * lpr];
+    o.x += w * x.x; o.y += w * x.y; o.z += w * x.z; o.w += w * x.w;
+  }
+  const float inv = dt == 0.f ? 0.f : 1.f / dt;
+  const float x[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  const int64_t r = static_cast<int64_t>(b) * hq + h;
+  if (active) store_out<4>(out, OUT_DT, r * out_rs + c, x);
+  if (lse != nullptr && threadIdx.x == 0) lse[r] = dt == 0.f ? -INFINITY : ref + __logf(dt);
+}
+
 struct Kv8Plan {
-  int parts, heads, subs;
+  int workers, heads, subs, min_len;  // workers 0: direct
 };
 
 static Kv8Plan plan_kv8(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans) {
   const int64_t groups = span_groups(n, spans), steps = ceil_div(groups, 2);
-  const int heads = static_cast<int>(ceil_div(hkv, ceil_div(hkv, kKv8Waves)));
-  const int64_t want = std::max<int64_t>(1, int64_t(device_cus()) * 8 / (int64_t(batch) * hkv));
-  const int64_t runs = std::min(want, steps);
-  int subs = 1;
-  while (heads * subs * 2 <= kKv8Waves && subs * 2 <= runs) subs *= 2;
-  const int parts = static_cast<int>(std::min<int64_t>(ceil_div(runs, subs), most_parts(batch, hq, d, groups)));
-  return Kv8Plan{parts, heads, subs};
+  const int most = kv8_waves(d != 128 && d != 64), cus = device_cus();
+  const int heads = std::min(hkv, 4), subs = most / 2 / 4;
+  const int64_t per_head_group = std::max<int64_t>(1, int64_t(cus) * 2 / ceil_div(hkv, heads));
+  if (steps <= 4 || batch > 1024) return Kv8Plan{0, 1, static_cast<int>(std::min<int64_t>(most, steps)), 0};
+  return Kv8Plan{static_cast<int>(std::min<int64_t>(per_head_group, batch * ceil_div(steps, subs))), heads, subs, 2 * subs};
+}
+
+constexpr int kMostWorkers = 1024;
+static size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+static size_t workers_bytes(int64_t workers, int batch, int hq, int d) {
+  const size_t rows = static_cast<size_t>(workers + batch) * hq;
+  return align256(rows * d * sizeof(float)) + align256(rows * sizeof(float)) + align256(sizeof(int2) * batch);
 }
 
 // Covers these spans and any shorter ones.
 size_t kv8_decode_workspace_bytes(int batch, int hq, int d, int n, const DecodeSpan* spans) {
-  return parts_bytes(most_parts(batch, hq, d, span_groups(n, spans)), batch, hq, d);
+  const int64_t steps = ceil_div(span_groups(n, spans), 2);
+  return workers_bytes(std::min<int64_t>(kMostWorkers, batch * steps), batch, hq, d);
 }
 
 template <int F, int D, bool PAD>
@@ -499,14 +644,21 @@ void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const 
   const Kv8Plan p = plan_kv8(batch, hq, hkv, d, n, spans);
   Kv8DecodeArgs a;
   a.ws_o = a.ws_lse = nullptr;
-  const int64_t rows = static_cast<int64_t>(batch) * hq;
-  if (p.parts > 1) {
-    const size_t need = parts_bytes(p.parts, batch, hq, d);
+  a.range = nullptr;
+  if (p.workers > 0) {
+    const size_t rows = static_cast<size_t>(p.workers + batch) * hq;
+    const size_t need = workers_bytes(p.workers, batch, hq, d);
     require(ws != nullptr && ws_bytes >= need, "workspace too small: need " + std::to_string(need) + " bytes");
     require(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "workspace must be 16-byte aligned");
-    a.ws_o = static_cast<float*>(ws);
-    a.ws_lse = a.ws_o + (static_cast<size_t>(p.parts) * rows * d + 63) / 64 * 64;
+    char* at = static_cast<char*>(ws);
+    a.ws_o = reinterpret_cast<float*>(at);
+    at += align256(rows * d * sizeof(float));
+    a.ws_lse = reinterpret_cast<float*>(at);
+    at += align256(rows * sizeof(float));
+    a.range = reinterpret_cast<int2*>(at);
   }
+  a.workers = p.workers;
+  a.min_len = p.min_len;
   a.q = static_cast<const uint16_t*>(q);
   a.q_bs = q_bs;
   a.q_hs = q_hs;
@@ -534,7 +686,7 @@ void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const 
   a.lse = lse;
   a.batch = batch;
   a.err = err;
-  const dim3 grid(static_cast<unsigned>(p.parts), static_cast<unsigned>(batch), static_cast<unsigned>(ceil_div(hkv, p.heads)));
+  const dim3 grid(std::max(p.workers, 1), p.workers > 0 ? 1 : batch, static_cast<unsigned>(ceil_div(hkv, p.heads)));
   // head dim 64: its own kernel; other multiples of 8 up to 128: 128 with the dims past it zero
   if (pool.format == kE4M3) {
     if (d == 128) launch_kv8_typed<kE4M3, 128, false>(a, grid, stream);
@@ -546,14 +698,16 @@ void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const 
     else launch_kv8_typed<kInt8, 128, true>(a, grid, stream);
   }
   HCP_HIP(hipGetLastError());
-  if (p.parts == 1) return;
-  const float* o_parts[64];
-  const float* l_parts[64];
-  for (int i = 0; i < p.parts; ++i) {
-    o_parts[i] = a.ws_o + static_cast<size_t>(i) * rows * d;
-    l_parts[i] = a.ws_lse + static_cast<size_t>(i) * rows;
+  if (p.workers == 0) return;
+  int lpr = 1;
+  while (lpr * 4 < d) lpr *= 2;
+  const dim3 rows(hq, batch);
+  switch (out_dtype) {
+    case kBF16: kv8_join_kernel<kBF16><<<rows, 256, 0, stream>>>(a.ws_o, a.ws_lse, a.range, hq, d, lpr, out, out_rs, lse); break;
+    case kF16: kv8_join_kernel<kF16><<<rows, 256, 0, stream>>>(a.ws_o, a.ws_lse, a.range, hq, d, lpr, out, out_rs, lse); break;
+    default: kv8_join_kernel<kF32><<<rows, 256, 0, stream>>>(a.ws_o, a.ws_lse, a.range, hq, d, lpr, out, out_rs, lse); break;
   }
-  launch_lse_merge(p.parts, o_parts, l_parts, static_cast<int>(rows), 1, d, out_dtype, out, out_rs, out_rs, lse, 1, stream);
+  HCP_HIP(hipGetLastError());
 }
 
 }  // namespace hcp
