@@ -1901,7 +1901,7 @@ Kv8Pool check_kv8_decode(const hcp_paged_decode_desc* d, const hcp_paged_pool* p
 size_t kv8_workspace(const hcp_paged_decode_desc* d, int n, const DecodeSpan* spans) {
   require(d->num_kv_heads > 0 && d->num_q_heads > 0 && d->num_q_heads % d->num_kv_heads == 0 && d->head_dim > 0 && d->batch > 0,
           "bad decode shape");
-  return kv8_decode_workspace_bytes(d->batch, d->num_q_heads, d->head_dim, n, spans);
+  return kv8_decode_workspace_bytes(d->batch, d->num_q_heads, d->num_kv_heads, d->head_dim, n, spans);
 }
 }  // namespace
 extern "C" {

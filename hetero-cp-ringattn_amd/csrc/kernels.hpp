@@ -195,7 +195,7 @@ void launch_kv8_gather(const Kv8Pool& pool, int dtype, int n, const PagedRangeDe
 
 // Attention of one query per sequence over its n shards in an 8-bit cache, as
 // launch_paged_decode.
-size_t kv8_decode_workspace_bytes(int batch, int hq, int d, int n, const DecodeSpan* spans);
+size_t kv8_decode_workspace_bytes(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans);
 void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const void* q, int64_t q_bs, int64_t q_hs, int n,
                        const DecodeSpan* spans, float scale, int out_dtype, void* out, int64_t out_rs, float* lse, void* ws,
                        size_t ws_bytes, int* err, hipStream_t stream);

@@ -205,336 +205,333 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
   }
 
   for (;;) {  // one sequence's share
-  const int run_len = (end_all - begin + 2 * a.subs - 1) / (2 * a.subs) * 2;  // whole steps
-  const int g0 = idle ? total : min(begin + sub * run_len, total);
-  const int g1 = min(min(g0 + run_len, end_all), total);
+    const int run_len = (end_all - begin + 2 * a.subs - 1) / (2 * a.subs) * 2;  // whole steps
+    const int g0 = idle ? total : min(begin + sub * run_len, total);
+    const int g1 = min(min(g0 + run_len, end_all), total);
 
-  // Q^T in f16, times a power of two that brings the row's largest value to 2^14 .. 2^15.
-  // k-step 2 h + e holds dims 16 grp + 64 h + 8 e + i, as the 16-byte loads of K bring them.
-  u32x4 qf[KS];
-  float c_log2;
-  {
-    float x[KS][8];
-    uint32_t top = 0;
+    // Q^T in f16, times a power of two that brings the row's largest value to 2^14 .. 2^15.
+    // k-step 2 h + e holds dims 16 grp + 64 h + 8 e + i, as the 16-byte loads of K bring them.
+    u32x4 qf[KS];
+    float c_log2;
+    {
+      float x[KS][8];
+      uint32_t top = 0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d0 = grp * 16 + 64 * (s / 2) + 8 * (s % 2);
-      u32x4 v = {0, 0, 0, 0};
-      if (!idle && col < a.rep && (!PAD || d0 < dn))
-        v = *reinterpret_cast<const u32x4*>(a.q + b * a.q_bs + (kvh * a.rep + col) * a.q_hs + d0);
+      for (int s = 0; s < KS; ++s) {
+        const int d0 = grp * 16 + 64 * (s / 2) + 8 * (s % 2);
+        u32x4 v = {0, 0, 0, 0};
+        if (!idle && col < a.rep && (!PAD || d0 < dn))
+          v = *reinterpret_cast<const u32x4*>(a.q + b * a.q_bs + (kvh * a.rep + col) * a.q_hs + d0);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        x[s][2 * w] = a.q_bf16 ? __uint_as_float(v[w] << 16) : f16_bits_to_f32(static_cast<uint16_t>(v[w] & 0xffffu));
-        x[s][2 * w + 1] = a.q_bf16 ? __uint_as_float(v[w] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(v[w] >> 16));
+        for (int w = 0; w < 4; ++w) {
+          x[s][2 * w] = a.q_bf16 ? __uint_as_float(v[w] << 16) : f16_bits_to_f32(static_cast<uint16_t>(v[w] & 0xffffu));
+          x[s][2 * w + 1] = a.q_bf16 ? __uint_as_float(v[w] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(v[w] >> 16));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
       }
+      // as floats the bits of |x| keep their order (NaN: dropped by the maximum, kept in x)
+      const float m = over_groups(__uint_as_float(top), [](float u, float v) { return fmaxf(u, v); });
+      const bool plain = m > 0.f && m < INFINITY;
+      const int k = plain ? max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100) : 14;
+      const float up = __uint_as_float(static_cast<uint32_t>(14 - k + 127) << 23);
+      c_log2 = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(k - 14 + 127) << 23);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) qf[s][w] = pack_f16(x[s][2 * w] * up, x[s][2 * w + 1] * up);
     }
-    // as floats the bits of |x| keep their order (NaN: dropped by the maximum, kept in x)
-    const float m = over_groups(__uint_as_float(top), [](float u, float v) { return fmaxf(u, v); });
-    const bool plain = m > 0.f && m < INFINITY;
-    const int k = plain ? max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100) : 14;
-    const float up = __uint_as_float(static_cast<uint32_t>(14 - k + 127) << 23);
-    c_log2 = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(k - 14 + 127) << 23);
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) qf[s][w] = pack_f16(x[s][2 * w] * up, x[s][2 * w + 1] * up);
-  }
 
-  f32x4 acc[VB];
+    f32x4 acc[VB];
 #pragma unroll
-  for (int j = 0; j < VB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = kNoMax, a_run = kNoMax, l_run = 0.f;
+    for (int j = 0; j < VB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run = kNoMax, a_run = kNoMax, l_run = 0.f;
 
-  const uint32_t row = static_cast<uint32_t>(a.hkv) * dn;  // bytes of a slot, all heads
-  const int64_t block_bytes = static_cast<int64_t>(a.bs) * row;
-  const uint8_t* const k_head = a.pool + kvh * dn;
-  const uint8_t* const v_head = k_head + a.plane_bytes;
-  const uint32_t k_at = col * row + grp * 16, v_at = grp * 4 * row + col * VB;  // of a group's first row
-  u32x4 kx[2][KL];         // the step's codes
-  uint32_t vx[2][4][VW];
-  // Groups of the shard, 64 at a time: lane i holds the place in the pool and the scales of
-  // group `batch` + i (place 0 and scales 0 for one that is not there: always in the pool, of
-  // no weight), and the block id of group batch + 64 + i.
-  int batch = 0, next_id = -1;
-  int64_t place = 0;
-  float ks_l = 0.f, vs_l = 0.f;
-  uint64_t absent = 0;  // groups of the batch with a bad block id
-  auto load_k = [&](int h, int64_t at) __attribute__((always_inline)) {
-    const uint8_t* const p = k_head + at;
+    const uint32_t row = static_cast<uint32_t>(a.hkv) * dn;  // bytes of a slot, all heads
+    const int64_t block_bytes = static_cast<int64_t>(a.bs) * row;
+    const uint8_t* const k_head = a.pool + kvh * dn;
+    const uint8_t* const v_head = k_head + a.plane_bytes;
+    const uint32_t k_at = col * row + grp * 16, v_at = grp * 4 * row + col * VB;  // of a group's first row
+    u32x4 kx[2][KL];         // the step's codes
+    uint32_t vx[2][4][VW];
+    // Groups of the shard, 64 at a time: lane i holds the place in the pool and the scales of
+    // group `batch` + i (place 0 and scales 0 for one that is not there: always in the pool, of
+    // no weight), and the block id of group batch + 64 + i.
+    int batch = 0, next_id = -1;
+    int64_t place = 0;
+    float ks_l = 0.f, vs_l = 0.f;
+    uint64_t absent = 0;  // groups of the batch with a bad block id
+    auto load_k = [&](int h, int64_t at) __attribute__((always_inline)) {
+      const uint8_t* const p = k_head + at;
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {
-      if constexpr (PAD) {  // rows of 8-byte multiples
-        u32x2 x = {0, 0}, y = {0, 0};
-        if (grp * 16 + 64 * i < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + k_at + 64 * i));
-        if (grp * 16 + 64 * i + 8 < dn) y = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + k_at + 64 * i + 8));
-        kx[h][i] = u32x4{x[0], x[1], y[0], y[1]};
-      } else {
-        kx[h][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + k_at + 64 * i));
-      }
-    }
-  };
-  auto load_v = [&](int h, int64_t at) __attribute__((always_inline)) {
-    const uint8_t* const p = v_head + at;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (VW == 2) {
-        u32x2 x = {0, 0};
-        if (!PAD || col * VB < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + v_at + j * row));
-        vx[h][j][0] = x[0];
-        vx[h][j][1] = x[1];
-      } else {
-        vx[h][j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p + v_at + j * row));
-      }
-    }
-  };
-  auto place_of = [&](int i) __attribute__((always_inline)) -> int64_t {
-    return static_cast<int64_t>(
-        static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place >> 32), i))) << 32 |
-        static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place), i)));
-  };
-  auto scale_of = [&](float v, int i) __attribute__((always_inline)) {
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
-  };
-
-  int before = 0;  // groups of the shards before
-  for (int s = 0; s < a.n_spans; ++s) {
-    const DecodeSpan& sp = a.span[s];
-    const int64_t t_beg = sp.t0, t_end = span_end(s);
-    const int here = span_groups(s, t_end), g_first = static_cast<int>(t_beg / 16);
-    // the run's groups of this shard, counted from the table's start
-    const int lo = max(g0 - before, 0) + g_first, end = min(g1 - before, here) + g_first;
-    before += here;
-    if (lo >= end) continue;
-    const int32_t* const table = sp.tables + static_cast<int64_t>(b) * sp.table_stride;
-    auto id_of = [&](int g) __attribute__((always_inline)) {
-      const int e = a.gpb_shift >= 0 ? g >> a.gpb_shift : g / a.gpb;
-      return g < end && e < sp.table_len ? table[e] : -1;
-    };
-    auto take_batch = [&](int first) __attribute__((always_inline)) {
-      batch = first;
-      const int g = first + lane, blk = next_id;
-      const bool in = g < end, ok = in && blk >= 0 && blk < a.num_blocks;
-      const int slot = 16 * (a.gpb_shift >= 0 ? g & (a.gpb - 1) : g % a.gpb);
-      place = ok ? blk * block_bytes + static_cast<int64_t>(slot) * row : 0;
-      ks_l = vs_l = 0.f;
-      if (ok) {
-        const float* const sc = a.scales + static_cast<int64_t>(blk) * a.hkv + kvh;
-        ks_l = sc[0];
-        vs_l = sc[a.plane_scales];
-      }
-      absent = __ballot(in && !ok);
-      if (in && !ok) atomicOr(a.err, 1);
-      next_id = id_of(g + 64);
-    };
-    const int full_lo = static_cast<int>((t_beg + 15) / 16), full_end = min(end, static_cast<int>(min(t_end / 16, static_cast<int64_t>(INT32_MAX))));
-
-    // 32 tokens: groups g, g + 1.  The next step's K takes the registers of this one's once S
-    // is known, its V those of this one's at the end: loads are always under way, and none
-    // stands in a branch (where it would make every wait one for all loads).
-    auto step = [&](int g, auto more) __attribute__((always_inline)) {
-      constexpr bool kMore = decltype(more)::value;
-      const int at = g - batch;
-      const float ks[2] = {scale_of(ks_l, at), scale_of(ks_l, at + 1)}, vs[2] = {scale_of(vs_l, at), scale_of(vs_l, at + 1)};
-      const bool full = g >= full_lo && g + 1 < full_end && (absent >> at & 3) == 0;
-      const uint64_t gone = absent >> at;
-      // ---- scores: s4[h][i] is key 4 grp + i of group h ----
-      f32x4 s4[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s4[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          uint32_t w[4];
-          to_f16<F>(kx[h][k / 2][2 * (k % 2)], w[0], w[1]);
-          to_f16<F>(kx[h][k / 2][2 * (k % 2) + 1], w[2], w[3]);
-          s4[h] = mma_f16(u32x4{w[0], w[1], w[2], w[3]}, qf[k], s4[h]);
+      for (int i = 0; i < KL; ++i) {
+        if constexpr (PAD) {  // rows of 8-byte multiples
+          u32x2 x = {0, 0}, y = {0, 0};
+          if (grp * 16 + 64 * i < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + k_at + 64 * i));
+          if (grp * 16 + 64 * i + 8 < dn) y = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + k_at + 64 * i + 8));
+          kx[h][i] = u32x4{x[0], x[1], y[0], y[1]};
+        } else {
+          kx[h][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + k_at + 64 * i));
         }
       }
-      int64_t next[2] = {0, 0};
-      if constexpr (kMore) {
-        if (g + 2 - batch >= 64) take_batch(g + 2);
+    };
+    auto load_v = [&](int h, int64_t at) __attribute__((always_inline)) {
+      const uint8_t* const p = v_head + at;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (VW == 2) {
+          u32x2 x = {0, 0};
+          if (!PAD || col * VB < dn) x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + v_at + j * row));
+          vx[h][j][0] = x[0];
+          vx[h][j][1] = x[1];
+        } else {
+          vx[h][j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p + v_at + j * row));
+        }
+      }
+    };
+    auto place_of = [&](int i) __attribute__((always_inline)) -> int64_t {
+      return static_cast<int64_t>(
+          static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place >> 32), i))) << 32 |
+          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place), i)));
+    };
+    auto scale_of = [&](float v, int i) __attribute__((always_inline)) {
+      return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+    };
+
+    int before = 0;  // groups of the shards before
+    for (int s = 0; s < a.n_spans; ++s) {
+      const DecodeSpan& sp = a.span[s];
+      const int64_t t_beg = sp.t0, t_end = span_end(s);
+      const int here = span_groups(s, t_end), g_first = static_cast<int>(t_beg / 16);
+      // the run's groups of this shard, counted from the table's start
+      const int lo = max(g0 - before, 0) + g_first, end = min(g1 - before, here) + g_first;
+      before += here;
+      if (lo >= end) continue;
+      const int32_t* const table = sp.tables + static_cast<int64_t>(b) * sp.table_stride;
+      auto id_of = [&](int g) __attribute__((always_inline)) {
+        const int e = a.gpb_shift >= 0 ? g >> a.gpb_shift : g / a.gpb;
+        return g < end && e < sp.table_len ? table[e] : -1;
+      };
+      auto take_batch = [&](int first) __attribute__((always_inline)) {
+        batch = first;
+        const int g = first + lane, blk = next_id;
+        const bool in = g < end, ok = in && blk >= 0 && blk < a.num_blocks;
+        const int slot = 16 * (a.gpb_shift >= 0 ? g & (a.gpb - 1) : g % a.gpb);
+        place = ok ? blk * block_bytes + static_cast<int64_t>(slot) * row : 0;
+        ks_l = vs_l = 0.f;
+        if (ok) {
+          const float* const sc = a.scales + static_cast<int64_t>(blk) * a.hkv + kvh;
+          ks_l = sc[0];
+          vs_l = sc[a.plane_scales];
+        }
+        absent = __ballot(in && !ok);
+        if (in && !ok) atomicOr(a.err, 1);
+        next_id = id_of(g + 64);
+      };
+      const int full_lo = static_cast<int>((t_beg + 15) / 16);
+      const int full_end = min(end, static_cast<int>(min(t_end / 16, static_cast<int64_t>(INT32_MAX))));
+
+      // 32 tokens: groups g, g + 1.  The next step's K takes the registers of this one's once S
+      // is known, its V those of this one's at the end: loads are always under way, and none
+      // stands in a branch (where it would make every wait one for all loads).
+      auto step = [&](int g, auto more) __attribute__((always_inline)) {
+        constexpr bool kMore = decltype(more)::value;
+        const int at = g - batch;
+        const float ks[2] = {scale_of(ks_l, at), scale_of(ks_l, at + 1)}, vs[2] = {scale_of(vs_l, at), scale_of(vs_l, at + 1)};
+        const bool full = g >= full_lo && g + 1 < full_end && (absent >> at & 3) == 0;
+        const uint64_t gone = absent >> at;
+        // ---- scores: s4[h][i] is key 4 grp + i of group h ----
+        f32x4 s4[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          next[h] = place_of(g + 2 + h - batch);
-          load_k(h, next[h]);
+          s4[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            uint32_t w[4];
+            to_f16<F>(kx[h][k / 2][2 * (k % 2)], w[0], w[1]);
+            to_f16<F>(kx[h][k / 2][2 * (k % 2) + 1], w[2], w[3]);
+            s4[h] = mma_f16(u32x4{w[0], w[1], w[2], w[3]}, qf[k], s4[h]);
+          }
         }
-      }
-      // ---- log2 domain; keys outside the range and groups that are not there weigh nothing ----
-      bool ok[2][4];
-      float tmax = -INFINITY;
-      const float c[2] = {c_log2 * ks[0], c_log2 * ks[1]};
-      float t[2][4];
+        int64_t next[2] = {0, 0};
+        if constexpr (kMore) {
+          if (g + 2 - batch >= 64) take_batch(g + 2);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) {
+            next[h] = place_of(g + 2 + h - batch);
+            load_k(h, next[h]);
+          }
+        }
+        // ---- log2 domain; keys outside the range and groups that are not there weigh nothing ----
+        bool ok[2][4];
+        float c[2] = {c_log2 * ks[0], c_log2 * ks[1]};  // >= 0: the maximum may come first
+        if (!full) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t[h][i] = s4[h][i] * c[h];
-      if (!full) {
+          for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int i = 0; i < 4; ++i) {
+              const int64_t tok = static_cast<int64_t>(g + h) * 16 + grp * 4 + i;
+              ok[h][i] = g + h < end && tok >= t_beg && tok < t_end && (gone >> h & 1) == 0;
+              s4[h][i] = ok[h][i] ? s4[h][i] * c[h] : -INFINITY;
+            }
+            c[h] = 1.f;
+          }
+        }
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) tmax = fmaxf(tmax, c[h] * fmaxf(fmaxf(s4[h][0], s4[h][1]), fmaxf(s4[h][2], s4[h][3])));
+        tmax = over_groups(tmax, [](float u, float v) { return fmaxf(u, v); });
+        // ---- running maxima of the scores and of weight times scale ----
+        const float m_new = fmaxf(m_run, tmax);
+        const float top = fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), 1.17549435e-38f);
+        const float a_new = fmaxf(a_run, tmax + __builtin_amdgcn_logf(top));
+        l_run *= __builtin_amdgcn_exp2f(m_run - m_new);
+        if (__any(a_new > a_run)) {
+          const float f = __builtin_amdgcn_exp2f(a_run - a_new);
+#pragma unroll
+          for (int j = 0; j < VB; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] *= f;
+        }
+        m_run = m_new;
+        a_run = a_new;
+        const float f = __builtin_amdgcn_exp2f(m_new - a_new + 14.f);
+        // ---- weights: hi + lo ----
+        u32x4 ph, pl;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float fv = f * vs[h];
+          float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int64_t tok = static_cast<int64_t>(g + h) * 16 + grp * 4 + i;
-            ok[h][i] = g + h < end && tok >= t_beg && tok < t_end && (gone >> h & 1) == 0;
-            t[h][i] = ok[h][i] ? t[h][i] : -INFINITY;
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s4[h][i], c[h], -m_new));
+            l_run += p;
+            w[i] = p * fv;
           }
-      }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t u = pack_f16(w[2 * i], w[2 * i + 1]);
+            const f16x2 x = __builtin_bit_cast(f16x2, u);
+            ph[2 * h + i] = u;
+            pl[2 * h + i] = pack_f16(__builtin_fmaf(static_cast<float>(x[0]), -1.f, w[2 * i]),
+                                     __builtin_fmaf(static_cast<float>(x[1]), -1.f, w[2 * i + 1]));
+          }
+        }
+        // ---- O^T += V^T P^T ----
+        if (F == kE4M3 && !full) {  // a NaN code times a weight of 0
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, t[h][i]);
-      tmax = over_groups(tmax, [](float u, float v) { return fmaxf(u, v); });
-      // ---- running maxima of the scores and of weight times scale ----
-      const float m_new = fmaxf(m_run, tmax);
-      const float top = fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), 1.17549435e-38f);
-      const float a_new = fmaxf(a_run, tmax + __builtin_amdgcn_logf(top));
-      l_run *= __builtin_amdgcn_exp2f(m_run - m_new);
-      if (__any(a_new > a_run)) {
-        const float f = __builtin_amdgcn_exp2f(a_run - a_new);
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < VB; ++j)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[j][i] *= f;
-      }
-      m_run = m_new;
-      a_run = a_new;
-      const float f = __builtin_amdgcn_exp2f(m_new - a_new + 14.f);
-      // ---- weights: hi + lo ----
-      u32x4 ph, pl;
+              for (int w = 0; w < VW; ++w) vx[h][i][w] = ok[h][i] ? vx[h][i][w] : 0;
+        }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float fv = f * vs[h];
-        float w[4];
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {  // tiles 4 w + 2 half, + 1
+            uint32_t va[2][4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p)  // keys 2 p, 2 p + 1 of the lane's eight
+              to_f16<F>(__builtin_amdgcn_perm(vx[p / 2][2 * (p % 2) + 1][w], vx[p / 2][2 * (p % 2)][w], half ? 0x07030602u : 0x05010400u),
+                        va[0][p], va[1][p]);
+            f32x4* const o = acc + 4 * w + 2 * half;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) o[j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, ph, o[j]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) o[j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, pl, o[j]);
+          }
+        if constexpr (kMore) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) load_v(h, next[h]);
+        }
+      };
+      next_id = id_of(lo + lane);
+      take_batch(lo);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) load_k(h, place_of(h));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) load_v(h, place_of(h));
+      int g = lo;
+      for (; g + 2 < end; g += 2) step(g, std::true_type{});
+      step(g, std::false_type{});
+    }
+
+    // ---- epilogue: dims (4 grp + i) VB + j of query col are acc[j][i] ----
+    const float l = over_groups(l_run, [](float u, float v) { return u + v; });
+    const float inv = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(a_run - m_run - 14.f) / l;  // NaN stays
+    const float lse2 = l == 0.f ? -INFINITY : m_run + __log2f(l);
+    // Addresses below are made from a lane number of their own: hoisted out of the loop over
+    // sequences they would cost registers all the way through it.
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int col = ln & 15, grp = ln >> 4;
+    // rows of the output, or of the workspace
+    const bool last = a.workers == 0;
+    const int64_t row0 = (last ? b : blockIdx.x + b) * static_cast<int64_t>(a.hq) + kvh * a.rep;
+    void* const o_to = last ? a.out : a.ws_o;
+    float* const lse_to = last ? a.lse : a.ws_lse;
+    const int64_t o_rs = last ? a.out_rs : dn;
+    const int o_dt = last ? a.out_dtype : kF32;
+    if (a.subs == 1) {
+      if (col < a.rep) {
+        const int64_t r = row0 + col;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(t[h][i] - m_new);
-          l_run += p;
-          w[i] = p * fv;
+          const int d0 = (4 * grp + i) * VB;
+          float x[VB];
+#pragma unroll
+          for (int j = 0; j < VB; ++j) x[j] = acc[j][i] * inv;
+          if (!PAD || d0 < dn) store_out<VB>(o_to, o_dt, r * o_rs + d0, x);
         }
+        if (grp == 0 && lse_to != nullptr) lse_to[r] = lse2 * kLn2;
+      }
+    } else {
+      // The waves of a kv head meet in LDS; wave `sub` finishes its query heads sub, sub + subs, ...
+      float* const o_lds = meet_lds;
+      float* const lse_lds = meet_lds + a.heads * a.subs * a.rep * OS;
+      if (col < a.rep) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t u = pack_f16(w[2 * i], w[2 * i + 1]);
-          const f16x2 x = __builtin_bit_cast(f16x2, u);
-          ph[2 * h + i] = u;
-          pl[2 * h + i] = pack_f16(w[2 * i] - static_cast<float>(x[0]), w[2 * i + 1] - static_cast<float>(x[1]));
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < VB; j += 4)
+            *reinterpret_cast<float4*>(o_lds + (wave * a.rep + col) * OS + (4 * grp + i) * VB + j) =
+                make_float4(acc[j][i] * inv, acc[j + 1][i] * inv, acc[j + 2][i] * inv, acc[j + 3][i] * inv);
+        if (grp == 0) lse_lds[wave * 16 + col] = lse2;
+      }
+      __syncthreads();
+      const int w0 = wave - sub * a.heads;
+      for (int c = idle ? a.rep : sub; c < a.rep; c += a.subs) {
+        float m = -INFINITY;
+        for (int i = 0; i < a.subs; ++i) m = fmaxf(m, lse_lds[(w0 + i * a.heads) * 16 + c]);
+        const float ref = m == -INFINITY ? 0.f : m;  // no finite one: 0, or NaN with a NaN one
+        float o[D / 64] = {}, den = 0.f;
+        for (int i = 0; i < a.subs; ++i) {
+          const int w = w0 + i * a.heads;
+          const float f = __builtin_amdgcn_exp2f(lse_lds[w * 16 + c] - ref);
+          den += f;
+#pragma unroll
+          for (int k = 0; k < D / 64; ++k) o[k] += f * o_lds[(w * a.rep + c) * OS + ln + 64 * k];
         }
-      }
-      // ---- O^T += V^T P^T ----
-      if (F == kE4M3 && !full) {  // a NaN code times a weight of 0
+        const float inv_den = den == 0.f ? 0.f : 1.f / den;
+        const int64_t r = row0 + c;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vx[h][i][w] = ok[h][i] ? vx[h][i][w] : 0;
-      }
-#pragma unroll
-      for (int w = 0; w < VW; ++w)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {  // tiles 4 w + 2 half, + 1
-          uint32_t va[2][4];
-#pragma unroll
-          for (int p = 0; p < 4; ++p)  // keys 2 p, 2 p + 1 of the lane's eight
-            to_f16<F>(__builtin_amdgcn_perm(vx[p / 2][2 * (p % 2) + 1][w], vx[p / 2][2 * (p % 2)][w], half ? 0x07030602u : 0x05010400u),
-                      va[0][p], va[1][p]);
-          f32x4* const o = acc + 4 * w + 2 * half;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) o[j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, ph, o[j]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) o[j] = mma_f16(u32x4{va[j][0], va[j][1], va[j][2], va[j][3]}, pl, o[j]);
+        for (int k = 0; k < D / 64; ++k) {
+          const int d0 = ln + 64 * k;
+          if (!PAD || d0 < dn) store_elem_rt(o_to, o_dt, r * o_rs + d0, o[k] * inv_den);
         }
-      if constexpr (kMore) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) load_v(h, next[h]);
+        if (ln == 0 && lse_to != nullptr) lse_to[r] = den == 0.f ? -INFINITY : (ref + __log2f(den)) * kLn2;
       }
-    };
-    next_id = id_of(lo + lane);
-    take_batch(lo);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) load_k(h, place_of(h));
-#pragma unroll
-    for (int h = 0; h < 2; ++h) load_v(h, place_of(h));
-    int g = lo;
-    for (; g + 2 < end; g += 2) step(g, std::true_type{});
-    step(g, std::false_type{});
-  }
-
-  // ---- epilogue: dims (4 grp + i) VB + j of query col are acc[j][i] ----
-  const float l = over_groups(l_run, [](float u, float v) { return u + v; });
-  const float inv = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(a_run - m_run - 14.f) / l;  // NaN stays
-  const float lse2 = l == 0.f ? -INFINITY : m_run + __log2f(l);
-  // Addresses below are made from a lane number of their own: hoisted out of the loop over
-  // sequences they would cost registers all the way through it.
-  int ln = lane;
-  asm volatile("" : "+v"(ln));
-  const int col = ln & 15, grp = ln >> 4;
-  // rows of the output, or of the workspace
-  const bool last = a.workers == 0;
-  const int64_t row0 = (last ? b : blockIdx.x + b) * static_cast<int64_t>(a.hq) + kvh * a.rep;
-  void* const o_to = last ? a.out : a.ws_o;
-  float* const lse_to = last ? a.lse : a.ws_lse;
-  const int64_t o_rs = last ? a.out_rs : dn;
-  const int o_dt = last ? a.out_dtype : kF32;
-  if (a.subs == 1) {
-    if (col < a.rep) {
-      const int64_t r = row0 + col;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d0 = (4 * grp + i) * VB;
-        float x[VB];
-#pragma unroll
-        for (int j = 0; j < VB; ++j) x[j] = acc[j][i] * inv;
-        if (!PAD || d0 < dn) store_out<VB>(o_to, o_dt, r * o_rs + d0, x);
-      }
-      if (grp == 0 && lse_to != nullptr) lse_to[r] = lse2 * kLn2;
     }
-  } else {
-    // The waves of a kv head meet in LDS; wave `sub` finishes its query heads sub, sub + subs, ...
-    float* const o_lds = meet_lds;
-    float* const lse_lds = meet_lds + a.heads * a.subs * a.rep * OS;
-    if (col < a.rep) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < VB; j += 4)
-          *reinterpret_cast<float4*>(o_lds + (wave * a.rep + col) * OS + (4 * grp + i) * VB + j) =
-              make_float4(acc[j][i] * inv, acc[j + 1][i] * inv, acc[j + 2][i] * inv, acc[j + 3][i] * inv);
-      if (grp == 0) lse_lds[wave * 16 + col] = lse2;
-    }
-    __syncthreads();
-    const int w0 = wave - sub * a.heads;
-    for (int c = idle ? a.rep : sub; c < a.rep; c += a.subs) {
-      float m = -INFINITY;
-      for (int i = 0; i < a.subs; ++i) m = fmaxf(m, lse_lds[(w0 + i * a.heads) * 16 + c]);
-      const float ref = m == -INFINITY ? 0.f : m;  // no finite one: 0, or NaN with a NaN one
-      float o[D / 64] = {}, den = 0.f;
-      for (int i = 0; i < a.subs; ++i) {
-        const int w = w0 + i * a.heads;
-        const float f = __builtin_amdgcn_exp2f(lse_lds[w * 16 + c] - ref);
-        den += f;
-#pragma unroll
-        for (int k = 0; k < D / 64; ++k) o[k] += f * o_lds[(w * a.rep + c) * OS + ln + 64 * k];
-      }
-      const float inv_den = den == 0.f ? 0.f : 1.f / den;
-      const int64_t r = row0 + c;
-#pragma unroll
-      for (int k = 0; k < D / 64; ++k) {
-        const int d0 = ln + 64 * k;
-        if (!PAD || d0 < dn) store_elem_rt(o_to, o_dt, r * o_rs + d0, o[k] * inv_den);
-      }
-      if (ln == 0 && lse_to != nullptr) lse_to[r] = den == 0.f ? -INFINITY : (ref + __log2f(den)) * kLn2;
-    }
-  }
-  if (left == 0) return;
-  if (a.subs > 1) __syncthreads();  // LDS is read
-  do {  // the next sequence that holds tokens
-    ++b;
-    total = seq_groups();
-  } while (total == 0);
-  begin = 0;
-  end_all = min(left, (total + 1) & ~1);
-  left -= end_all;
+    if (left == 0) return;
+    if (a.subs > 1) __syncthreads();  // LDS is read
+    do {  // the next sequence that holds tokens
+      if (++b >= a.batch) return;
+      total = seq_groups();
+    } while (total == 0);
+    begin = 0;
+    end_all = min(left, (total + 1) & ~1);
+    left -= end_all;
   }
 }
 
@@ -606,16 +603,56 @@ struct Kv8Plan {
   int workers, heads, subs, min_len;  // workers 0: direct
 };
 
-static Kv8Plan plan_kv8(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans) {
-  const int64_t groups = span_groups(n, spans), steps = ceil_div(groups, 2);
-  const int most = kv8_waves(d != 128 && d != 64), cus = device_cus();
-  const int heads = std::min(hkv, 4), subs = most / 2 / 4;
-  const int64_t per_head_group = std::max<int64_t>(1, int64_t(cus) * 2 / ceil_div(hkv, heads));
-  if (steps <= 4 || batch > 1024) return Kv8Plan{0, 1, static_cast<int>(std::min<int64_t>(most, steps)), 0};
-  return Kv8Plan{static_cast<int>(std::min<int64_t>(per_head_group, batch * ceil_div(steps, subs))), heads, subs, 2 * subs};
+// Waves that take a head's share alone, of all sequences: one for every step while that is at
+// most two a SIMD, so that no worker crosses a sequence's end (2.5-4 us each time: lengths,
+// table, q and the first codes one after another), else one a SIMD -- it reaches 6.1 TB/s, more
+// of them no more.
+static int64_t lone_workers(int batch, int hkv, int64_t steps) {
+  const int64_t cus = device_cus();
+  return batch * steps * hkv <= 8 * cus ? batch * steps : std::max<int64_t>(4 * cus / hkv, 1);
 }
 
-constexpr int kMostWorkers = 1024;
+// Direct or balanced, by modelled time (us, fitted on MI355X to 31 calls: 1-300 sequences of
+// 130-100000 tokens, 8, 2 and 1 kv heads of 128, 64 and 96 dims; within 10% of the fastest of 13
+// splits where the two are apart):
+//   direct:   6 + the longest sequence's steps over four waves, 0.95 each, times the workgroups a
+//             CU has, or the bytes at 6 TB/s -- of sequences as long as the longest, as long as a
+//             CU has no more than two; past that the lengths even out.
+//   balanced: 11 (the join is a launch of its own) + its waves' steps, or three quarters of those
+//             bytes (lengths between half the longest and the longest, as a serving batch's), +
+//             2.5 for every sequence that a worker meets.
+// e.g. 4 x 700 tokens, 32/8 heads: 10.1 direct, 10.7 balanced; 64 x 1000: 26.3 / 29.3; 64 x 2000:
+// 51.0 / 44.9; 64 x 16384: 363 / 267; 6 x 2085, 16/2 heads: 18.3 / 12.0; 200 x 500, 14/2 heads of 64
+// dims: 10.3 / 21.0.  A direct workgroup is one kv head and four waves, one a SIMD: eight take as
+// long (4 x 700: 10.7), two longer (14.0).
+static Kv8Plan plan_kv8(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans) {
+  const int64_t groups = span_groups(n, spans), steps = ceil_div(groups, 2);
+  const int most = kv8_waves(d != 128 && d != 64);
+  const Kv8Plan direct{0, 1, static_cast<int>(std::min<int64_t>(4, steps)), 0};
+  // the lanes that lay out the row count groups in 32 bits and take 64 sequences at a time
+  if (batch > 1024 || batch * (groups + 1) > INT32_MAX / 2 || steps <= 4) return direct;
+  const int64_t lone = lone_workers(batch, hkv, steps);
+  const double cus = device_cus(), all = static_cast<double>(batch) * hkv * steps;  // steps of a wave
+  const double bytes = all * 64 * d / 6e6, per_cu = batch * hkv / cus;
+  const double run = std::max(all / (static_cast<double>(lone) * hkv), all / (4 * cus));
+  const double t_direct = 6.0 + std::max(bytes * (0.75 + 0.25 * std::min(1.0, 2.0 / per_cu)), 0.95 * steps / 4 * std::max(1.0, per_cu));
+  const double t_balanced = 11.0 + std::max(0.75 * bytes, 0.95 * run) + (run > 1.0 ? 2.5 * (1.0 + static_cast<double>(batch) / lone) : 0.0);
+  if (t_direct <= t_balanced) return direct;
+  // Up to 100 places a sequence and head for the join, 200 where runs are long: else waves of a
+  // workgroup meet first, four at least (one sequence of 4096 tokens, 32/8 heads: 11.6 us as 32
+  // workers of four waves a head, 12.5 as 128 lone ones, 13.4 as 64 of two; of 100000: 46.8, 44.7;
+  // of 32000, 16/2 heads: 15.3 as four, 17.2 as 16).
+  // Lone waves of four heads share a workgroup (1% faster, they read whole rows), never those of
+  // two: workgroups of two waves leave half of the SIMDs without one (64 x 16384 tokens, 14/2
+  // heads of 64 dims: 62.8 us, single waves 52.7).
+  int subs = 1;
+  const int64_t places = (run < 16.0 ? 100 : 200) * static_cast<int64_t>(batch);
+  if (lone > places)
+    for (subs = 4; subs < most && lone > places * subs;) subs *= 2;
+  const int heads = subs == 1 && hkv % 4 == 0 ? 4 : 1;
+  return Kv8Plan{static_cast<int>(ceil_div(lone, subs)), heads, subs, 2 * subs};
+}
+
 static size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 static size_t workers_bytes(int64_t workers, int batch, int hq, int d) {
   const size_t rows = static_cast<size_t>(workers + batch) * hq;
@@ -623,9 +660,9 @@ static size_t workers_bytes(int64_t workers, int batch, int hq, int d) {
 }
 
 // Covers these spans and any shorter ones.
-size_t kv8_decode_workspace_bytes(int batch, int hq, int d, int n, const DecodeSpan* spans) {
-  const int64_t steps = ceil_div(span_groups(n, spans), 2);
-  return workers_bytes(std::min<int64_t>(kMostWorkers, batch * steps), batch, hq, d);
+size_t kv8_decode_workspace_bytes(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans) {
+  const int64_t steps = ceil_div(span_groups(n, spans), 2), cus = device_cus();
+  return workers_bytes(std::min<int64_t>(batch * steps, std::max<int64_t>(8 * cus / hkv, 1)), batch, hq, d);
 }
 
 template <int F, int D, bool PAD>
@@ -640,6 +677,7 @@ void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const 
                        size_t ws_bytes, int* err, hipStream_t stream) {
   const int hkv = pool.hkv, d = pool.d;
   require(batch <= 65535, "kv8_decode: batch must be at most 65535");  // grid y
+  require(16ll * hkv * d < (1ll << 31), "kv8_decode: too many heads");   // 32-bit offsets in a group
   for (int i = 0; i < n; ++i) require(spans[i].t0 >= 0 && spans[i].t0 < pool.bs, "kv8_decode: a span starts in its first block");
   const Kv8Plan p = plan_kv8(batch, hq, hkv, d, n, spans);
   Kv8DecodeArgs a;
