@@ -27,7 +27,6 @@ ABI status code and the library's message.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 import os
@@ -345,14 +344,25 @@ def last_error() -> str:
 # ---------------------------------------------------------------------------------
 # torch plumbing
 # ---------------------------------------------------------------------------------
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
+
+
+_dtype_codes = {}
 
 
 def dtype_code(t) -> int:
-    torch = _torch()
-    return {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}[t]
+    if not _dtype_codes:
+        torch = _torch()
+        _dtype_codes.update({torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32})
+    return _dtype_codes[t]
 
 
 def _stream(stream=None):
@@ -360,9 +370,14 @@ def _stream(stream=None):
     raw handle (0: the default stream)."""
     if isinstance(stream, int):
         return ctypes.c_void_p(stream)
-    torch = _torch()
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return ctypes.c_void_p(s.cuda_stream)
+    if stream is None:
+        torch = _torch()
+        # the handle itself where torch hands it out (0.2 us; the stream object takes 2.8)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        if raw is not None:
+            return ctypes.c_void_p(raw(torch.cuda.current_device()))
+        stream = torch.cuda.current_stream()
+    return ctypes.c_void_p(stream.cuda_stream)
 
 
 def view(t) -> View:
@@ -473,10 +488,10 @@ def lse_merge(o_parts, lse_parts, out_dtype=None, out=None, lse_out=None, stream
 # ---------------------------------------------------------------------------------
 def paged_pool(pool) -> PagedPool:
     """pool tensor [2, num_blocks, block_size, Hkv, D] -> hcp_paged_pool."""
-    if pool.dim() != 5 or pool.shape[0] != 2 or not pool.is_contiguous():
+    shape = pool.shape
+    if len(shape) != 5 or shape[0] != 2 or not pool.is_contiguous():
         raise ValueError("pool must be a contiguous [2, num_blocks, block_size, Hkv, D] tensor")
-    return PagedPool(pool.data_ptr(), pool.shape[1], pool.shape[2], pool.shape[3], pool.shape[4],
-                     pool.element_size())
+    return PagedPool(pool.data_ptr(), shape[1], shape[2], shape[3], shape[4], pool.element_size())
 
 
 def paged_kv_gather(pool, block_table, table_seq_offset, t0, t1, k_out=None, v_out=None,
@@ -630,21 +645,36 @@ def decode_ring_replay(q, pool, shards, seed_domain, scale=None, out=None, lse_o
 # ---------------------------------------------------------------------------------
 # (9) step plan of a paged cache
 # ---------------------------------------------------------------------------------
-def _want(name, t, dtype, shape, device):
-    """Refuses a tensor that a kernel could not read as ``dtype`` [shape] on ``device``."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+def _want(name, t, dtype, shape, dev):
+    """Refuses a tensor that a kernel could not read as ``dtype`` [shape] on GPU ``dev``."""
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {_place(dev)}")
 
 
-def _on(device):
-    """Context in which ``device`` is the current one (kernels and error flags go by it)."""
+def _place(dev):
+    return f"GPU {dev}" if dev >= 0 else "the CPU"
+
+
+def _launch(fn, dev, stream, *args):
+    """fn(*args, stream) with GPU ``dev`` current (kernels and error flags go by it)."""
     torch = _torch()
-    if device.type != "cuda":
-        raise ValueError(f"tensors must be on a GPU, not on {device}")
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    if dev < 0:
+        raise ValueError("tensors must be on a GPU")
+    if dev == torch.cuda.current_device():
+        _check(fn(*args, _stream(stream)))
+    else:
+        with torch.cuda.device(dev):
+            _check(fn(*args, _stream(stream)))
 
 
-_HERE = contextlib.nullcontext()
+def _workspace(ws, need, dev):
+    """(tensor that keeps the memory, address, bytes) of a workspace, made where None."""
+    torch = _torch()
+    if ws is None:
+        ws = torch.empty(max(need(), 1), dtype=torch.uint8, device=torch.device("cuda", dev) if dev >= 0 else "cpu")
+    elif ws.get_device() != dev or not ws.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {_place(dev)}")
+    return ws, ws.data_ptr(), ws.numel() * ws.element_size()
 
 
 def kv_plan_workspace_size(batch: int) -> int:
@@ -665,38 +695,34 @@ def kv_plan_step(seq_lens, new_lens, block_tables, free_blocks, free_count, bloc
     few free blocks, a full table, a token past ``capacity``) keeps its length, and its
     tokens get slot -1, as the places past the last token do."""
     torch = _torch()
-    b, dev = seq_lens.shape[0], seq_lens.device
+    b, dev = seq_lens.shape[0], seq_lens.get_device()
     if slots is not None:
         capacity = slots.shape[0]
     elif capacity is None:
         raise ValueError("kv_plan_step needs a capacity or slots")
     i32, i64 = torch.int32, torch.int64
-    new = lambda n, dt: torch.empty(n, dtype=dt, device=dev)  # noqa: E731
+    new = lambda n, dt: torch.empty(n, dtype=dt, device=seq_lens.device)  # noqa: E731
     slots = new(capacity, i64) if slots is None else slots
     positions = new(capacity, i64) if positions is None else positions
     token_starts = new(b + 1, i32) if token_starts is None else token_starts
     seq_lens_out = new(b, i32) if seq_lens_out is None else seq_lens_out
     free_count_out = new(1, i32) if free_count_out is None else free_count_out
-    for name, t, dt, n in (("seq_lens", seq_lens, i32, b), ("new_lens", new_lens, i32, b),
-                           ("free_blocks", free_blocks, i32, free_blocks.numel()), ("free_count", free_count, i32, 1),
-                           ("slots", slots, i64, capacity), ("positions", positions, i64, capacity),
-                           ("token_starts", token_starts, i32, b + 1), ("seq_lens_out", seq_lens_out, i32, b),
-                           ("free_count_out", free_count_out, i32, 1)):
-        _want(name, t, dt, (n,), dev)
-    if block_tables.dtype != i32 or block_tables.dim() != 2 or block_tables.shape[0] != b or block_tables.device != dev \
-            or (block_tables.stride(1) != 1 and block_tables.shape[1] > 1):
-        raise ValueError(f"block_tables must be an int32 tensor of {b} contiguous rows on {dev}")
-    if workspace is None:
-        workspace = torch.empty(max(kv_plan_workspace_size(b), 1), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev:
-        raise ValueError(f"workspace must be on {dev}")
-    with _on(dev):
-        _check(lib().hcp_kv_plan_step(b, block_size, free_blocks.numel(), seq_lens.data_ptr(), new_lens.data_ptr(),
-                                      block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
-                                      free_blocks.data_ptr(), free_count.data_ptr(), capacity, token_starts.data_ptr(),
-                                      slots.data_ptr(), positions.data_ptr(), seq_lens_out.data_ptr(),
-                                      free_count_out.data_ptr(), workspace.data_ptr(),
-                                      workspace.numel() * workspace.element_size(), _stream(stream)))
+    rows, one, places = (b,), (1,), (capacity,)
+    _want("seq_lens", seq_lens, i32, rows, dev)
+    _want("new_lens", new_lens, i32, rows, dev)
+    _want("free_blocks", free_blocks, i32, (free_blocks.numel(),), dev)
+    _want("free_count", free_count, i32, one, dev)
+    _want("slots", slots, i64, places, dev)
+    _want("positions", positions, i64, places, dev)
+    _want("token_starts", token_starts, i32, (b + 1,), dev)
+    _want("seq_lens_out", seq_lens_out, i32, rows, dev)
+    _want("free_count_out", free_count_out, i32, one, dev)
+    _decode_tables("block_tables", block_tables, None, b, dev)
+    _ws, ws, ws_bytes = _workspace(workspace, lambda: kv_plan_workspace_size(b), dev)
+    _launch(lib().hcp_kv_plan_step, dev, stream, b, block_size, free_blocks.shape[0], seq_lens.data_ptr(),
+            new_lens.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
+            free_blocks.data_ptr(), free_count.data_ptr(), capacity, token_starts.data_ptr(), slots.data_ptr(),
+            positions.data_ptr(), seq_lens_out.data_ptr(), free_count_out.data_ptr(), ws, ws_bytes)
     return slots, positions, token_starts, seq_lens_out, free_count_out
 
 
@@ -786,24 +812,30 @@ def kv8_pool(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
             torch.zeros(2, num_blocks, num_kv_heads, dtype=torch.float32, device=device))
 
 
+_kv8_formats = {}
+
+
 def _kv8(pool, scales):
-    """(hcp_paged_pool, HCP_KV8_* of the pool's type), the scales checked against it."""
+    """(hcp_paged_pool, HCP_KV8_* of the pool's type, its GPU), pool and scales checked."""
     pp, fmt = _kv8_shape(pool)
-    _want("scales", scales, _torch().float32, (2, pool.shape[1], pool.shape[3]), pool.device)
-    return pp, fmt
+    dev = pool.get_device()
+    _want("scales", scales, _torch().float32, (2, pp.num_blocks, pp.num_kv_heads), dev)
+    return pp, fmt, dev
 
 
 def _kv8_shape(pool):
-    torch = _torch()
-    fmt = {torch.float8_e4m3fn: KV8_E4M3, torch.int8: KV8_INT8}.get(pool.dtype)
+    if not _kv8_formats:
+        torch = _torch()
+        _kv8_formats.update({torch.float8_e4m3fn: KV8_E4M3, torch.int8: KV8_INT8})
+    fmt = _kv8_formats.get(pool.dtype)
     if fmt is None:
         raise ValueError("an 8-bit pool is float8_e4m3fn or int8")
     return paged_pool(pool), fmt
 
 
-def _rows_of(name, t, shape, pool, dtype=None):
-    if tuple(t.shape) != tuple(shape) or t.device != pool.device or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{name} must be [{', '.join(str(n) for n in shape)}] on {pool.device}"
+def _rows_of(name, t, shape, dev, dtype=None):
+    if t.shape != shape or t.get_device() != dev or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name} must be [{', '.join(str(n) for n in shape)}] on {_place(dev)}"
                          + (f" in {dtype}" if dtype is not None else ""))
 
 
@@ -811,59 +843,57 @@ def kv8_append(pool, scales, k, v, slots, stream=None):
     """Quantise the rows of k / v [Hkv, T, D] into the slots [T] int64 of an 8-bit cache
     (:func:`kv_plan_step`; negative: skipped).  A block's scale is a power of two that only
     grows while the block fills; rows held already are rounded to the new one."""
-    torch = _torch()
-    pp, fmt = _kv8(pool, scales)
+    pp, fmt, dev = _kv8(pool, scales)
     tokens = slots.shape[0]
-    shape = (pool.shape[3], tokens, pool.shape[4])
-    _rows_of("k", k, shape, pool)
-    _rows_of("v", v, shape, pool, k.dtype)
-    _want("slots", slots, torch.int64, (tokens,), pool.device)
-    with _on(pool.device):
-        _check(lib().hcp_kv8_append(ctypes.byref(pp), scales.data_ptr(), fmt, dtype_code(k.dtype), view(k), view(v),
-                                    tokens, slots.data_ptr(), _stream(stream)))
+    shape = (pp.num_kv_heads, tokens, pp.head_dim)
+    _rows_of("k", k, shape, dev)
+    _rows_of("v", v, shape, dev, k.dtype)
+    _want("slots", slots, _torch().int64, (tokens,), dev)
+    _launch(lib().hcp_kv8_append, dev, stream, ctypes.byref(pp), scales.data_ptr(), fmt, dtype_code(k.dtype), view(k),
+            view(v), tokens, slots.data_ptr())
 
 
 def kv8_gather(pool, scales, block_table, table_seq_offset, t0, t1, dtype=None, k_out=None, v_out=None, stream=None):
     """As :func:`paged_kv_gather` from an 8-bit cache: scale * code rounded to ``dtype``
     (default bfloat16) -> k, v [Hkv, t1 - t0, D]."""
     torch = _torch()
-    pp, fmt = _kv8(pool, scales)
-    shape = (pool.shape[3], t1 - t0, pool.shape[4])
+    pp, fmt, dev = _kv8(pool, scales)
+    shape = (pp.num_kv_heads, t1 - t0, pp.head_dim)
     if k_out is None:
         k_out = torch.empty(shape, dtype=dtype or torch.bfloat16, device=pool.device)
     if v_out is None:
         v_out = torch.empty(shape, dtype=k_out.dtype, device=pool.device)
-    _rows_of("k_out", k_out, shape, pool, dtype)
-    _rows_of("v_out", v_out, shape, pool, k_out.dtype)
-    _want("block_table", block_table, torch.int32, (block_table.numel(),), pool.device)
-    with _on(pool.device):
-        _check(lib().hcp_kv8_gather(ctypes.byref(pp), scales.data_ptr(), fmt, dtype_code(k_out.dtype),
-                                    block_table.data_ptr(), block_table.numel(), table_seq_offset, t0, t1, view(k_out),
-                                    view(v_out), _stream(stream)))
+    _rows_of("k_out", k_out, shape, dev, dtype)
+    _rows_of("v_out", v_out, shape, dev, k_out.dtype)
+    n = block_table.numel()
+    _want("block_table", block_table, torch.int32, (n,), dev)
+    _launch(lib().hcp_kv8_gather, dev, stream, ctypes.byref(pp), scales.data_ptr(), fmt, dtype_code(k_out.dtype),
+            block_table.data_ptr(), n, table_seq_offset, t0, t1, view(k_out), view(v_out))
     return k_out, v_out
 
 
-def _decode_tables(name, tables, lens, b, device):
+def _decode_tables(name, tables, lens, b, dev):
     torch = _torch()
     if tables is not None and (tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != b
-                               or tables.device != device or (tables.stride(1) != 1 and tables.shape[1] > 1)):
-        raise ValueError(f"{name} must be an int32 tensor of {b} contiguous rows on {device}")
+                               or tables.get_device() != dev or (tables.stride(1) != 1 and tables.shape[1] > 1)):
+        raise ValueError(f"{name} must be an int32 tensor of {b} contiguous rows on {_place(dev)}")
     if lens is not None:
-        _want("seq_lens", lens, torch.int32, (b,), device)
+        _want("seq_lens", lens, torch.int32, (b,), dev)
 
 
-def _decode_rows(q, pool, o, lse, o_dtype):
+def _decode_rows(q, pp, dev, o, lse, o_dtype):
     """Outputs [B, Hq, D] and [B, Hq] (made where None), and q checked against the pool."""
     torch = _torch()
-    b, hq, d = q.shape
-    if d != pool.shape[4] or q.device != pool.device or (q.stride(2) != 1 and d > 1):
-        raise ValueError(f"q must be [B, Hq, {pool.shape[4]}] with contiguous rows on {pool.device}")
+    shape = q.shape
+    b, hq, d = shape
+    if d != pp.head_dim or q.get_device() != dev or (q.stride(2) != 1 and d > 1):
+        raise ValueError(f"q must be [B, Hq, {pp.head_dim}] with contiguous rows on {_place(dev)}")
     if o is None:
-        o = torch.empty((b, hq, d), dtype=o_dtype, device=q.device)
+        o = torch.empty(shape, dtype=o_dtype, device=q.device)
     if lse is None:
         lse = torch.empty((b, hq), dtype=torch.float32, device=q.device)
-    _rows_of("o", o, (b, hq, d), pool, o_dtype)
-    _want("lse", lse, torch.float32, (b, hq), pool.device)
+    _rows_of("o", o, shape, dev, o_dtype)
+    _want("lse", lse, torch.float32, (b, hq), dev)
     return o, lse
 
 
@@ -877,21 +907,18 @@ def kv8_decode_partial(q, pool, scales, block_tables, t0, t1, seq_lens=None, sca
                        lse=None, stream=None):
     """As :func:`decode_local_compact_partial` over an 8-bit cache: q [B, Hq, D] over tokens
     [t0, min(t1, seq_lens)) of each sequence -> (o [B, Hq, D] fp32, lse [B, Hq] fp32)."""
-    torch = _torch()
-    pp, fmt = _kv8(pool, scales)
-    o, lse = _decode_rows(q, pool, o, lse, torch.float32)
-    _decode_tables("block_tables", block_tables, seq_lens, q.shape[0], pool.device)
+    pp, fmt, dev = _kv8(pool, scales)
+    o, lse = _decode_rows(q, pp, dev, o, lse, _torch().float32)
+    _decode_tables("block_tables", block_tables, seq_lens, q.shape[0], dev)
     if not o.is_contiguous():
         raise ValueError("o must be contiguous")
     desc = decode_desc(q, pool, block_tables, t0, t1, scale)
-    if workspace is None:
-        need = lib().hcp_kv8_decode_workspace_size(ctypes.byref(desc), ctypes.byref(pp))
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
-    with _on(pool.device):
-        _check(lib().hcp_kv8_decode_partial(ctypes.byref(desc), ctypes.byref(pp), scales.data_ptr(), fmt,
-                                            View(q.data_ptr(), q.stride(1), q.stride(0)), block_tables.data_ptr(),
-                                            _ptr(seq_lens), o.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
-                                            workspace.numel() * workspace.element_size(), _stream(stream)))
+    fns = lib()
+    _ws, ws, ws_bytes = _workspace(workspace, lambda: fns.hcp_kv8_decode_workspace_size(ctypes.byref(desc), ctypes.byref(pp)),
+                                   dev)
+    _launch(fns.hcp_kv8_decode_partial, dev, stream, ctypes.byref(desc), ctypes.byref(pp), scales.data_ptr(), fmt,
+            View(q.data_ptr(), q.stride(1), q.stride(0)), block_tables.data_ptr(),
+            None if seq_lens is None else seq_lens.data_ptr(), o.data_ptr(), lse.data_ptr(), ws, ws_bytes)
     return o, lse
 
 
@@ -904,21 +931,16 @@ def kv8_decode_ring_workspace_size(q, pool, shards) -> int:
 def kv8_decode_ring_replay(q, pool, scales, shards, seed_domain, scale=None, out=None, lse_out=None, workspace=None,
                            stream=None):
     """As :func:`decode_ring_replay` over an 8-bit cache (shards as there)."""
-    torch = _torch()
-    pp, fmt = _kv8(pool, scales)
-    out, lse_out = _decode_rows(q, pool, out, lse_out, q.dtype)
+    pp, fmt, dev = _kv8(pool, scales)
+    out, lse_out = _decode_rows(q, pp, dev, out, lse_out, q.dtype)
     for tables, lens, _ in shards:
-        _decode_tables("a shard's tables", tables, lens, q.shape[0], pool.device)
-    desc, arr, n = _ring_desc(q, pool, scale), _shards(shards), len(shards)
-    if workspace is None:
-        need = lib().hcp_kv8_decode_ring_workspace_size(ctypes.byref(desc), ctypes.byref(pp), n, arr)
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
-    with _on(pool.device):
-        _check(lib().hcp_kv8_decode_ring_replay(ctypes.byref(desc), ctypes.byref(pp), scales.data_ptr(), fmt,
-                                                View(q.data_ptr(), q.stride(1), q.stride(0)), n, arr, seed_domain,
-                                                View(out.data_ptr(), out.stride(1), out.stride(0)), lse_out.data_ptr(),
-                                                workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                                                _stream(stream)))
+        _decode_tables("a shard's tables", tables, lens, q.shape[0], dev)
+    desc, arr, n, fns = _ring_desc(q, pool, scale), _shards(shards), len(shards), lib()
+    _ws, ws, ws_bytes = _workspace(
+        workspace, lambda: fns.hcp_kv8_decode_ring_workspace_size(ctypes.byref(desc), ctypes.byref(pp), n, arr), dev)
+    _launch(fns.hcp_kv8_decode_ring_replay, dev, stream, ctypes.byref(desc), ctypes.byref(pp), scales.data_ptr(), fmt,
+            View(q.data_ptr(), q.stride(1), q.stride(0)), n, arr, seed_domain,
+            View(out.data_ptr(), out.stride(1), out.stride(0)), lse_out.data_ptr(), ws, ws_bytes)
     return out, lse_out
 
 
@@ -926,28 +948,23 @@ def kv8_ring_attention_replay_paged(q, pool, scales, block_table, chunks, causal
                                     lse_out=None, workspace=None, stream=None, strategy="vanilla", schedule="auto"):
     """As :func:`ring_attention_replay_paged`, K/V staged from an 8-bit cache in q's type."""
     torch = _torch()
-    pp, fmt = _kv8(pool, scales)
+    pp, fmt, dev = _kv8(pool, scales)
     hq, s, d = q.shape
-    hkv = pool.shape[3]
-    desc, arr = replay_desc(q.dtype, hq, hkv, d, chunks, causal, scale, strategy, schedule)
-    _want("block_table", block_table, torch.int32, (block_table.numel(),), pool.device)
     if s != sum(chunks):
         raise ValueError(f"invalid chunk sum: actual {sum(chunks)}, expected {s}")
-    if workspace is None:
-        need = lib().hcp_ring_replay_workspace_size(ctypes.byref(desc), 1)
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+    desc, arr = replay_desc(q.dtype, hq, pp.num_kv_heads, d, chunks, causal, scale, strategy, schedule)
+    n, fns = block_table.numel(), lib()
+    _want("block_table", block_table, torch.int32, (n,), dev)
     if out is None:
         out = torch.empty((hq, s, d), dtype=q.dtype, device=q.device)
     if lse_out is None:
         lse_out = torch.empty((hq, s), dtype=torch.float32, device=q.device)
-    _rows_of("q", q, (hq, s, d), pool)
-    _rows_of("out", out, (hq, s, d), pool, q.dtype)
-    _want("lse_out", lse_out, torch.float32, (hq, s), pool.device)
-    with _on(pool.device):
-        _check(lib().hcp_kv8_prefill_replay_paged(ctypes.byref(desc), view(q), ctypes.byref(pp), scales.data_ptr(), fmt,
-                                                  block_table.data_ptr(), block_table.numel(), view(out),
-                                                  lse_out.data_ptr(), workspace.data_ptr(),
-                                                  workspace.numel() * workspace.element_size(), _stream(stream)))
+    _rows_of("q", q, (hq, s, d), dev)
+    _rows_of("out", out, (hq, s, d), dev, q.dtype)
+    _want("lse_out", lse_out, torch.float32, (hq, s), dev)
+    _ws, ws, ws_bytes = _workspace(workspace, lambda: fns.hcp_ring_replay_workspace_size(ctypes.byref(desc), 1), dev)
+    _launch(fns.hcp_kv8_prefill_replay_paged, dev, stream, ctypes.byref(desc), view(q), ctypes.byref(pp),
+            scales.data_ptr(), fmt, block_table.data_ptr(), n, view(out), lse_out.data_ptr(), ws, ws_bytes)
     del arr
     return out, lse_out
 

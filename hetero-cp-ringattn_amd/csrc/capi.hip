@@ -1802,7 +1802,8 @@ int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, cons
     const size_t need = kv_plan_workspace_bytes(batch);
     require(workspace != nullptr && workspace_bytes >= need, "workspace too small: need " + std::to_string(need) + " bytes");
     require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
-    launch_kv_plan(KvPlan{batch, block_size, num_blocks, seq_lens, new_lens, block_tables, table_stride, table_len,
+    const int shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
+    launch_kv_plan(KvPlan{batch, block_size, shift, num_blocks, seq_lens, new_lens, block_tables, table_stride, table_len,
                           free_blocks, free_count, capacity, token_starts, seq_lens_out, free_count_out, slots, positions,
                           device_error_flags()},
                    workspace, as_stream(stream));

@@ -140,7 +140,7 @@ void launch_paged_decode(int dtype, int batch, int hq, int hkv, int d, const voi
 // The plan of one step of a paged cache (kv_plan.hip); pointers and their meaning as in
 // hcp_kv_plan_step.
 struct KvPlan {
-  int32_t batch, bs;
+  int32_t batch, bs, bs_shift;  // bs_shift: log2 of bs, or -1
   int64_t num_blocks;
   const int32_t *seq_lens, *new_lens;
   int32_t* block_tables;

@@ -14,7 +14,9 @@
 // the entries that are read (below the old count) and written (from it on) never meet.
 //
 // Bound by latency: a batch of 256 reads and writes some 20 KB.  The running sums need all
-// sequences, so one workgroup takes them (scan), then the whole grid fills (fill).
+// sequences, so one workgroup takes them; where it can hold them in LDS and the tokens are few
+// it fills everything, too, in one launch (kv_plan_one_kernel), else the whole grid fills in a
+// second one (kv_plan_fill_kernel).
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -38,12 +40,20 @@ struct PlanArgs {
   int32_t* back_end;  // [batch] blocks given back by sequences 0 .. b
 };
 
-constexpr int kScan = 1024;  // threads of the scan's workgroup
+// What the scan leaves for the filling, in LDS or in the workspace.
+struct PlanSums {
+  const PlanInfo* info;
+  const int32_t *starts, *back_end;  // starts as token_starts
+  PlanHead head;
+};
 
-// Inclusive sums over the workgroup of two counts per thread, and their totals.
+constexpr int kScan = 1024;  // threads of the scan's workgroup, and most sequences of the one-launch form
+
+// Inclusive sums over the T threads of the workgroup of two counts each, and their totals.
 struct Pair {
   int64_t x, y;
 };
+template <int T>
 __device__ Pair scan_pair(Pair v, Pair* part, Pair& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int off = 1; off < 64; off *= 2) {
@@ -58,7 +68,8 @@ __device__ Pair scan_pair(Pair v, Pair* part, Pair& total) {
   __syncthreads();
   Pair before{0, 0};
   total = Pair{0, 0};
-  for (int w = 0; w < kScan / 64; ++w) {
+#pragma unroll
+  for (int w = 0; w < T / 64; ++w) {
     if (w == wave) before = total;
     total.x += part[w].x;
     total.y += part[w].y;
@@ -68,117 +79,85 @@ __device__ Pair scan_pair(Pair v, Pair* part, Pair& total) {
 
 __device__ __forceinline__ int32_t sat32(int64_t v) { return static_cast<int32_t>(min(v, static_cast<int64_t>(INT32_MAX))); }
 
-__device__ void plan_scan(const PlanArgs& a) {
-  __shared__ Pair part[kScan / 64];
-  const KvPlan& p = a.p;
-  int flags = 0;
-  int64_t count = *p.free_count;
+// x / bs: by a shift where bs is a power of two (a 64-bit division takes some 150 instructions).
+__device__ __forceinline__ uint32_t plan_div(const KvPlan& p, uint32_t x) { return p.bs_shift >= 0 ? x >> p.bs_shift : x / p.bs; }
+__device__ __forceinline__ uint32_t plan_ceil(const KvPlan& p, uint32_t x) {
+  const uint32_t q = plan_div(p, x);
+  return q + (q * p.bs != x);
+}
+
+// One sequence's lengths and what they ask for.
+struct PlanSeq {
+  int64_t len, add, used;
+  bool sane, ended;
+};
+__device__ __forceinline__ PlanSeq plan_seq(const KvPlan& p, int b) {
+  PlanSeq s;
+  s.len = p.seq_lens[b];
+  s.add = p.new_lens[b];
+  s.used = plan_ceil(p, max(p.seq_lens[b], 0));
+  s.sane = s.len >= 0 && s.used <= p.table_len;
+  s.ended = s.sane && s.add < 0;
+  return s;
+}
+// New blocks of a sequence with room for them, its tokens ending at `end`; -1 without.
+__device__ __forceinline__ int64_t plan_need(const KvPlan& p, const PlanSeq& s, int32_t end) {
+  const int64_t blocks = plan_ceil(p, static_cast<uint32_t>(max(s.len, static_cast<int64_t>(0)) + max(s.add, static_cast<int64_t>(0))));
+  const bool fits = s.sane && s.add >= 0 && blocks <= p.table_len && s.len + s.add <= INT32_MAX && end <= p.capacity;
+  return fits ? blocks - s.used : -1;
+}
+// What happens to it: `end` is the running sum of the needs, its own included.
+__device__ __forceinline__ PlanInfo plan_info(const PlanSeq& s, int64_t need, int64_t end, int64_t top, int32_t back_end) {
+  const bool served = need == 0 || (need > 0 && end <= top);
+  return PlanInfo{static_cast<int32_t>(s.len), s.ended ? kEnded : served ? kServed : kIdle,
+                  sat32(s.ended ? back_end - s.used : end - max(need, static_cast<int64_t>(0))),
+                  static_cast<int32_t>(s.ended ? s.used : served ? need : 0)};
+}
+__device__ __forceinline__ int32_t plan_len_out(const PlanSeq& s, const PlanInfo& i) {
+  return static_cast<int32_t>(i.state == kEnded ? 0 : i.state == kServed ? s.len + s.add : s.len);
+}
+// Height of the stack, and with the ended sequences' blocks on it; flags of what is wrong with them.
+__device__ __forceinline__ int64_t plan_count(const KvPlan& p, int& flags) {
+  const int64_t count = *p.free_count;
   if (count < 0 || count > p.num_blocks) flags |= 8;
-  count = min(max(count, static_cast<int64_t>(0)), p.num_blocks);
-  // tokens and blocks given back first: the stack's height decides who is served
-  Pair sum{0, 0}, total;
-  for (int base = 0; base < p.batch; base += kScan) {
-    const int b = base + threadIdx.x;
-    Pair v{0, 0};
-    if (b < p.batch) {
-      const int64_t len = p.seq_lens[b], add = p.new_lens[b];
-      const int64_t used = (max(len, static_cast<int64_t>(0)) + p.bs - 1) / p.bs;
-      const bool sane = len >= 0 && used <= p.table_len;
-      if (!sane) flags |= 8;
-      v.x = max(add, static_cast<int64_t>(0));
-      v.y = sane && add < 0 ? used : 0;
-    }
-    const Pair inc = scan_pair(v, part, total);
-    if (b < p.batch) {
-      p.token_starts[b + 1] = sat32(sum.x + inc.x);
-      a.back_end[b] = sat32(sum.y + inc.y);
-    }
-    sum.x += total.x;
-    sum.y += total.y;
-  }
-  int64_t top = count + sum.y;
-  if (top > p.num_blocks) {  // blocks given back twice: what has no place is dropped
-    flags |= 8;
-    top = p.num_blocks;
-  }
-  Pair taken{0, 0};  // needs of all, and of the served
-  int64_t tokens = 0;
-  for (int base = 0; base < p.batch; base += kScan) {
-    const int b = base + threadIdx.x;
-    Pair v{0, 0};
-    int64_t len = 0, add = 0, used = 0;
-    bool fits = false, ended = false;
-    if (b < p.batch) {
-      len = p.seq_lens[b];
-      add = p.new_lens[b];
-      used = (max(len, static_cast<int64_t>(0)) + p.bs - 1) / p.bs;
-      const bool sane = len >= 0 && used <= p.table_len;
-      ended = sane && add < 0;
-      const int64_t blocks = (len + max(add, static_cast<int64_t>(0)) + p.bs - 1) / p.bs;
-      fits = sane && add >= 0 && blocks <= p.table_len && len + add <= INT32_MAX &&
-             p.token_starts[b + 1] <= p.capacity;
-      if (fits) v.x = blocks - used;
-    }
-    const Pair inc = scan_pair(v, part, total);
-    const int64_t end = taken.x + inc.x;
-    const bool served = fits && (v.x == 0 || end <= top);
-    if (b < p.batch) {
-      PlanInfo i;
-      i.len = static_cast<int32_t>(len);
-      i.state = ended ? kEnded : served ? kServed : kIdle;
-      i.first = sat32(ended ? a.back_end[b] - used : end - v.x);
-      i.need = static_cast<int32_t>(ended ? used : served ? v.x : 0);
-      a.info[b] = i;
-      p.seq_lens_out[b] = static_cast<int32_t>(ended ? 0 : served ? len + add : len);
-    }
-    // the served ones that need blocks are a prefix of those that ask: the last one's end is
-    // what is taken
-    const Pair most = Pair{0, served ? v.x : 0};
-    taken.x += total.x;
-    scan_pair(most, part, total);
-    tokens += total.y;
-  }
-  if (threadIdx.x == 0) {
-    p.token_starts[0] = 0;
-    *a.head = PlanHead{static_cast<int32_t>(count), static_cast<int32_t>(top), static_cast<int32_t>(top - tokens), 0};
-    *p.free_count_out = static_cast<int32_t>(top - tokens);
-  }
-  if (flags != 0) atomicOr(p.err, flags);
+  return min(max(count, static_cast<int64_t>(0)), p.num_blocks);
+}
+__device__ __forceinline__ int64_t plan_top(const KvPlan& p, int64_t count, int64_t back, int& flags) {
+  if (count + back > p.num_blocks) flags |= 8;  // given back twice: what has no place is dropped
+  return min(count + back, p.num_blocks);
 }
 
 // Place `at` of the stack with the ended sequences' blocks on it.
-__device__ __forceinline__ int32_t stack_block(const PlanArgs& a, const PlanHead& h, int64_t at) {
-  if (at < h.count) return a.p.free_blocks[at];
-  const int32_t i = static_cast<int32_t>(at) - h.count;
-  int lo = 0, hi = a.p.batch - 1;  // first sequence whose running sum is past i
+__device__ __forceinline__ int32_t stack_block(const KvPlan& p, const PlanSums& s, int64_t at) {
+  if (at < s.head.count) return p.free_blocks[at];
+  const int32_t i = static_cast<int32_t>(at) - s.head.count;
+  int lo = 0, hi = p.batch - 1;  // first sequence whose running sum is past i
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
-    if (a.back_end[mid] > i) hi = mid;
+    if (s.back_end[mid] > i) hi = mid;
     else lo = mid + 1;
   }
-  return a.p.block_tables[lo * a.p.table_stride + i - a.info[lo].first];
+  return p.block_tables[lo * p.table_stride + i - s.info[lo].first];
 }
 
-__device__ void plan_fill(const PlanArgs& a, int64_t thread, int64_t threads) {
-  const KvPlan& p = a.p;
-  const PlanHead h = *a.head;
-  const int64_t total = p.token_starts[p.batch];
+__device__ __forceinline__ void plan_tokens(const KvPlan& p, const PlanSums& s, int64_t thread, int64_t threads) {
+  const int64_t total = s.starts[p.batch];
   for (int64_t i = thread; i < p.capacity; i += threads) {
     int64_t slot = -1, pos = 0;
     if (i < total) {
       int lo = 0, hi = p.batch - 1;  // the sequence of token i
       while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (p.token_starts[mid + 1] > i) hi = mid;
+        if (s.starts[mid + 1] > i) hi = mid;
         else lo = mid + 1;
       }
-      const PlanInfo s = a.info[lo];
-      pos = s.len < 0 ? 0 : static_cast<int64_t>(s.len) + i - p.token_starts[lo];
-      if (s.state == kServed) {
-        const int64_t entry = pos / p.bs, used = (s.len + p.bs - 1) / p.bs;
+      const PlanInfo q = s.info[lo];
+      pos = q.len < 0 ? 0 : static_cast<int64_t>(q.len) + i - s.starts[lo];
+      if (q.state == kServed) {
+        const int32_t entry = plan_div(p, static_cast<uint32_t>(pos)), used = plan_ceil(p, q.len);
         const int32_t blk = entry < used ? p.block_tables[lo * p.table_stride + entry]
-                                         : stack_block(a, h, h.top - 1 - (s.first + entry - used));
-        if (blk >= 0 && blk < p.num_blocks) slot = static_cast<int64_t>(blk) * p.bs + (pos - entry * p.bs);
+                                         : stack_block(p, s, s.head.top - 1 - (static_cast<int64_t>(q.first) + entry - used));
+        if (blk >= 0 && blk < p.num_blocks) slot = static_cast<int64_t>(blk) * p.bs + (pos - static_cast<int64_t>(entry) * p.bs);
         else atomicOr(p.err, 1);
       }
     }
@@ -187,31 +166,124 @@ __device__ void plan_fill(const PlanArgs& a, int64_t thread, int64_t threads) {
   }
 }
 
-// Entries that a sequence gets or gives back, by one wave.
-__device__ void plan_blocks(const PlanArgs& a, int64_t wave, int64_t waves) {
-  const KvPlan& p = a.p;
-  const PlanHead h = *a.head;
-  for (int64_t b = wave; b < p.batch; b += waves) {
-    const PlanInfo s = a.info[b];
-    int32_t* const row = p.block_tables + b * p.table_stride;
-    if (s.state == kServed) {
-      const int32_t used = (s.len + p.bs - 1) / p.bs;
-      for (int32_t i = threadIdx.x & 63; i < s.need; i += 64) row[used + i] = stack_block(a, h, h.top - 1 - (int64_t(s.first) + i));
-    } else if (s.state == kEnded) {
-      for (int32_t i = threadIdx.x & 63; i < s.need; i += 64) {
-        const int64_t at = int64_t(h.count) + s.first + i;
-        if (at < h.left) p.free_blocks[at] = row[i];
-      }
+// Entries from .. , from + step, ... that sequence b gets or gives back.
+__device__ __forceinline__ void plan_blocks(const KvPlan& p, const PlanSums& s, int64_t b, int from, int to, int step) {
+  const PlanInfo q = s.info[b];
+  int32_t* const row = p.block_tables + b * p.table_stride;
+  if (q.state == kServed) {
+    const int32_t used = plan_ceil(p, q.len);
+    for (int32_t i = from; i < min(q.need, to); i += step)
+      row[used + i] = stack_block(p, s, s.head.top - 1 - (static_cast<int64_t>(q.first) + i));
+  } else if (q.state == kEnded) {
+    for (int32_t i = from; i < min(q.need, to); i += step) {
+      const int64_t at = static_cast<int64_t>(s.head.count) + q.first + i;
+      if (at < s.head.left) p.free_blocks[at] = row[i];
     }
   }
 }
 
-__global__ __launch_bounds__(kScan) void kv_plan_scan_kernel(PlanArgs a) { plan_scan(a); }
+// Up to T sequences, one a thread.
+template <int T>
+__global__ __launch_bounds__(T) void kv_plan_one_kernel(KvPlan p) {
+  __shared__ Pair part[T / 64];
+  __shared__ PlanInfo info[T];
+  __shared__ int32_t starts[T + 1], back_end[T], many[T];
+  __shared__ int32_t taken, n_many;
+  const int b = threadIdx.x;
+  int flags = 0;
+  PlanSeq s{0, 0, 0, true, false};
+  if (b < p.batch) s = plan_seq(p, b);
+  if (!s.sane) flags |= 8;
+  const int64_t count = plan_count(p, flags);
+  if (b == 0) taken = n_many = 0;
+  Pair total;
+  const Pair sum = scan_pair<T>(Pair{max(s.add, static_cast<int64_t>(0)), s.ended ? s.used : 0}, part, total);
+  const int64_t top = plan_top(p, count, total.y, flags);
+  starts[b + 1] = sat32(sum.x);
+  if (b == 0) starts[0] = 0;
+  back_end[b] = sat32(sum.y);
+  const int64_t need = b < p.batch ? plan_need(p, s, starts[b + 1]) : -1;
+  const int64_t end = scan_pair<T>(Pair{max(need, static_cast<int64_t>(0)), 0}, part, total).x;
+  const PlanInfo mine = plan_info(s, need, end, top, back_end[b]);
+  info[b] = mine;
+  // the served ones that need blocks come before those that get none: the last one's end is what is taken
+  if (mine.state == kServed && mine.need > 0) atomicMax(&taken, static_cast<int32_t>(end));
+  if (flags != 0) atomicOr(p.err, flags);
+  __syncthreads();
+  const PlanSums sums{info, starts, back_end,
+                      PlanHead{static_cast<int32_t>(count), static_cast<int32_t>(top), static_cast<int32_t>(top - taken), 0}};
+  plan_tokens(p, sums, b, T);
+  if (b < p.batch) {
+    p.seq_lens_out[b] = plan_len_out(s, mine);
+    p.token_starts[b + 1] = starts[b + 1];
+    plan_blocks(p, sums, b, 0, 2, 1);  // a decode step's sequence gets one at most
+  }
+  if (b == 0) {
+    p.token_starts[0] = 0;
+    *p.free_count_out = sums.head.left;
+  }
+  // long rows (a prompt's, an ended sequence's): one a wave, from a list whose order is of no matter
+  if (mine.need > 2) many[atomicAdd(&n_many, 1)] = b;
+  __syncthreads();
+  for (int w = b >> 6; w < n_many; w += T / 64) plan_blocks(p, sums, many[w], 2 + (b & 63), INT32_MAX, 64);
+}
+
+__global__ __launch_bounds__(kScan) void kv_plan_scan_kernel(PlanArgs a) {
+  __shared__ Pair part[kScan / 64];
+  __shared__ int32_t taken;
+  const KvPlan& p = a.p;
+  int flags = 0;
+  const int64_t count = plan_count(p, flags);
+  if (threadIdx.x == 0) taken = 0;
+  // tokens and blocks given back first: the stack's height decides who is served
+  Pair sum{0, 0}, total;
+  for (int base = 0; base < p.batch; base += kScan) {
+    const int b = base + threadIdx.x;
+    PlanSeq s{0, 0, 0, true, false};
+    if (b < p.batch) s = plan_seq(p, b);
+    if (!s.sane) flags |= 8;
+    const Pair inc = scan_pair<kScan>(Pair{max(s.add, static_cast<int64_t>(0)), s.ended ? s.used : 0}, part, total);
+    if (b < p.batch) {
+      p.token_starts[b + 1] = sat32(sum.x + inc.x);
+      a.back_end[b] = sat32(sum.y + inc.y);
+    }
+    sum.x += total.x;
+    sum.y += total.y;
+  }
+  const int64_t top = plan_top(p, count, sum.y, flags);
+  int64_t asked = 0;
+  for (int base = 0; base < p.batch; base += kScan) {
+    const int b = base + threadIdx.x;
+    PlanSeq s{0, 0, 0, true, false};
+    int64_t need = -1;
+    if (b < p.batch) {
+      s = plan_seq(p, b);
+      need = plan_need(p, s, p.token_starts[b + 1]);
+    }
+    const int64_t end = asked + scan_pair<kScan>(Pair{max(need, static_cast<int64_t>(0)), 0}, part, total).x;
+    asked += total.x;
+    if (b < p.batch) {
+      const PlanInfo mine = plan_info(s, need, end, top, a.back_end[b]);
+      a.info[b] = mine;
+      if (mine.state == kServed && mine.need > 0) atomicMax(&taken, static_cast<int32_t>(end));
+      p.seq_lens_out[b] = plan_len_out(s, mine);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    p.token_starts[0] = 0;
+    const int32_t left = static_cast<int32_t>(top) - taken;
+    *a.head = PlanHead{static_cast<int32_t>(count), static_cast<int32_t>(top), left, 0};
+    *p.free_count_out = left;
+  }
+  if (flags != 0) atomicOr(p.err, flags);
+}
 
 __global__ __launch_bounds__(256) void kv_plan_fill_kernel(PlanArgs a) {
-  const int64_t thread = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  plan_fill(a, thread, static_cast<int64_t>(gridDim.x) * 256);
-  plan_blocks(a, thread >> 6, static_cast<int64_t>(gridDim.x) * 4);
+  const int64_t thread = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, threads = static_cast<int64_t>(gridDim.x) * 256;
+  const PlanSums sums{a.info, a.p.token_starts, a.back_end, *a.head};
+  plan_tokens(a.p, sums, thread, threads);
+  for (int64_t b = thread >> 6; b < a.p.batch; b += threads >> 6) plan_blocks(a.p, sums, b, threadIdx.x & 63, INT32_MAX, 64);
 }
 
 static size_t plan_align(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
@@ -221,6 +293,12 @@ size_t kv_plan_workspace_bytes(int batch) {
 }
 
 void launch_kv_plan(const KvPlan& p, void* ws, hipStream_t stream) {
+  if (p.batch <= kScan && p.capacity <= 4 * kScan) {
+    if (p.batch <= 256 && p.capacity <= 1024) kv_plan_one_kernel<256><<<1, 256, 0, stream>>>(p);
+    else kv_plan_one_kernel<kScan><<<1, kScan, 0, stream>>>(p);
+    HCP_HIP(hipGetLastError());
+    return;
+  }
   PlanArgs a;
   a.p = p;
   char* at = static_cast<char*>(ws);
