@@ -47,7 +47,10 @@ struct PlanSums {
   PlanHead head;
 };
 
-constexpr int kScan = 1024;  // threads of the scan's workgroup, and most sequences of the one-launch form
+constexpr int kScan = 1024;       // threads of the scan's workgroup, and most sequences of the one-launch form
+// Most tokens of the one-launch form: 4000 of 1000 sequences take it 12.4 us, two launches 12.6;
+// 1500 of 256 8.2 and 11.0; 60000 of 1000 (three loads in line for each token on one CU) 14.4 in two.
+constexpr int kOneTokens = 4096;
 
 // Inclusive sums over the T threads of the workgroup of two counts each, and their totals.
 struct Pair {
@@ -140,30 +143,33 @@ __device__ __forceinline__ int32_t stack_block(const KvPlan& p, const PlanSums& 
   return p.block_tables[lo * p.table_stride + i - s.info[lo].first];
 }
 
-__device__ __forceinline__ void plan_tokens(const KvPlan& p, const PlanSums& s, int64_t thread, int64_t threads) {
-  const int64_t total = s.starts[p.batch];
-  for (int64_t i = thread; i < p.capacity; i += threads) {
-    int64_t slot = -1, pos = 0;
-    if (i < total) {
-      int lo = 0, hi = p.batch - 1;  // the sequence of token i
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (s.starts[mid + 1] > i) hi = mid;
-        else lo = mid + 1;
-      }
-      const PlanInfo q = s.info[lo];
-      pos = q.len < 0 ? 0 : static_cast<int64_t>(q.len) + i - s.starts[lo];
-      if (q.state == kServed) {
-        const int32_t entry = plan_div(p, static_cast<uint32_t>(pos)), used = plan_ceil(p, q.len);
-        const int32_t blk = entry < used ? p.block_tables[lo * p.table_stride + entry]
-                                         : stack_block(p, s, s.head.top - 1 - (static_cast<int64_t>(q.first) + entry - used));
-        if (blk >= 0 && blk < p.num_blocks) slot = static_cast<int64_t>(blk) * p.bs + (pos - static_cast<int64_t>(entry) * p.bs);
-        else atomicOr(p.err, 1);
-      }
-    }
-    p.slots[i] = slot;
-    p.positions[i] = pos;
+// The sequence of token i among lo .. hi: the first that ends past it.
+__device__ __forceinline__ int plan_seq_of(const int32_t* starts, int lo, int hi, int64_t i) {
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (starts[mid + 1] > i) hi = mid;
+    else lo = mid + 1;
   }
+  return lo;
+}
+
+// Slot and position of token i, which is one of sequences lo .. hi's or lies past all tokens.
+__device__ __forceinline__ void plan_token(const KvPlan& p, const PlanSums& s, int64_t i, int lo, int hi) {
+  int64_t slot = -1, pos = 0;
+  if (i < s.starts[p.batch]) {
+    const int b = plan_seq_of(s.starts, lo, hi, i);
+    const PlanInfo q = s.info[b];
+    pos = q.len < 0 ? 0 : static_cast<int64_t>(q.len) + i - s.starts[b];
+    if (q.state == kServed) {
+      const int32_t entry = plan_div(p, static_cast<uint32_t>(pos)), used = plan_ceil(p, q.len);
+      const int32_t blk = entry < used ? p.block_tables[b * p.table_stride + entry]
+                                       : stack_block(p, s, s.head.top - 1 - (static_cast<int64_t>(q.first) + entry - used));
+      if (blk >= 0 && blk < p.num_blocks) slot = static_cast<int64_t>(blk) * p.bs + (pos - static_cast<int64_t>(entry) * p.bs);
+      else atomicOr(p.err, 1);
+    }
+  }
+  p.slots[i] = slot;
+  p.positions[i] = pos;
 }
 
 // Entries from .. , from + step, ... that sequence b gets or gives back.
@@ -182,9 +188,11 @@ __device__ __forceinline__ void plan_blocks(const KvPlan& p, const PlanSums& s, 
   }
 }
 
-// Up to T sequences, one a thread.
-template <int T>
-__global__ __launch_bounds__(T) void kv_plan_one_kernel(KvPlan p) {
+// Up to T sequences, one a thread, their sums in registers and LDS.  kFill: tokens and blocks,
+// too; else the sums go to the workspace for the fill kernel.
+template <int T, bool kFill>
+__global__ __launch_bounds__(T) void kv_plan_one_kernel(PlanArgs a) {
+  const KvPlan& p = a.p;
   __shared__ Pair part[T / 64];
   __shared__ PlanInfo info[T];
   __shared__ int32_t starts[T + 1], back_end[T], many[T];
@@ -212,22 +220,31 @@ __global__ __launch_bounds__(T) void kv_plan_one_kernel(KvPlan p) {
   __syncthreads();
   const PlanSums sums{info, starts, back_end,
                       PlanHead{static_cast<int32_t>(count), static_cast<int32_t>(top), static_cast<int32_t>(top - taken), 0}};
-  plan_tokens(p, sums, b, T);
   if (b < p.batch) {
     p.seq_lens_out[b] = plan_len_out(s, mine);
     p.token_starts[b + 1] = starts[b + 1];
-    plan_blocks(p, sums, b, 0, 2, 1);  // a decode step's sequence gets one at most
   }
   if (b == 0) {
     p.token_starts[0] = 0;
     *p.free_count_out = sums.head.left;
   }
+  if constexpr (!kFill) {
+    if (b < p.batch) {
+      a.info[b] = mine;
+      a.back_end[b] = back_end[b];
+    }
+    if (b == 0) *a.head = sums.head;
+    return;
+  }
+  for (int64_t i = b; i < p.capacity; i += T) plan_token(p, sums, i, 0, p.batch - 1);
+  if (b < p.batch) plan_blocks(p, sums, b, 0, 2, 1);  // a decode step's sequence gets one at most
   // long rows (a prompt's, an ended sequence's): one a wave, from a list whose order is of no matter
   if (mine.need > 2) many[atomicAdd(&n_many, 1)] = b;
   __syncthreads();
   for (int w = b >> 6; w < n_many; w += T / 64) plan_blocks(p, sums, many[w], 2 + (b & 63), INT32_MAX, 64);
 }
 
+// Any number of sequences.
 __global__ __launch_bounds__(kScan) void kv_plan_scan_kernel(PlanArgs a) {
   __shared__ Pair part[kScan / 64];
   __shared__ int32_t taken;
@@ -279,11 +296,21 @@ __global__ __launch_bounds__(kScan) void kv_plan_scan_kernel(PlanArgs a) {
   if (flags != 0) atomicOr(p.err, flags);
 }
 
+// 256 tokens a workgroup, whose sequences lie between its first and its last token's (two of
+// the searches over all sequences instead of 256), and a sequence's blocks a wave.
 __global__ __launch_bounds__(256) void kv_plan_fill_kernel(PlanArgs a) {
-  const int64_t thread = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, threads = static_cast<int64_t>(gridDim.x) * 256;
-  const PlanSums sums{a.info, a.p.token_starts, a.back_end, *a.head};
-  plan_tokens(a.p, sums, thread, threads);
-  for (int64_t b = thread >> 6; b < a.p.batch; b += threads >> 6) plan_blocks(a.p, sums, b, threadIdx.x & 63, INT32_MAX, 64);
+  __shared__ int ends[2];
+  const KvPlan& p = a.p;
+  const PlanSums sums{a.info, p.token_starts, a.back_end, *a.head};
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256;
+  if (first < p.capacity) {
+    if (threadIdx.x < 128 && (threadIdx.x & 63) == 0)
+      ends[threadIdx.x >> 6] = plan_seq_of(sums.starts, 0, p.batch - 1, threadIdx.x == 0 ? first : first + 255);
+    __syncthreads();
+    if (first + threadIdx.x < p.capacity) plan_token(p, sums, first + threadIdx.x, ends[0], ends[1]);
+  }
+  const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (b < p.batch) plan_blocks(p, sums, b, threadIdx.x & 63, INT32_MAX, 64);
 }
 
 static size_t plan_align(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
@@ -293,12 +320,6 @@ size_t kv_plan_workspace_bytes(int batch) {
 }
 
 void launch_kv_plan(const KvPlan& p, void* ws, hipStream_t stream) {
-  if (p.batch <= kScan && p.capacity <= 4 * kScan) {
-    if (p.batch <= 256 && p.capacity <= 1024) kv_plan_one_kernel<256><<<1, 256, 0, stream>>>(p);
-    else kv_plan_one_kernel<kScan><<<1, kScan, 0, stream>>>(p);
-    HCP_HIP(hipGetLastError());
-    return;
-  }
   PlanArgs a;
   a.p = p;
   char* at = static_cast<char*>(ws);
@@ -307,11 +328,19 @@ void launch_kv_plan(const KvPlan& p, void* ws, hipStream_t stream) {
   a.info = reinterpret_cast<PlanInfo*>(at);
   at += plan_align(sizeof(PlanInfo) * p.batch);
   a.back_end = reinterpret_cast<int32_t*>(at);
-  kv_plan_scan_kernel<<<1, kScan, 0, stream>>>(a);
+  if (p.batch <= kScan && p.capacity <= kOneTokens) {
+    // four waves for a decode step (256 tokens 4.8 us); 1024 tokens 8.3 us with four, 7.1 with sixteen
+    if (p.batch <= 256 && p.capacity <= 512) kv_plan_one_kernel<256, true><<<1, 256, 0, stream>>>(a);
+    else kv_plan_one_kernel<kScan, true><<<1, kScan, 0, stream>>>(a);
+    HCP_HIP(hipGetLastError());
+    return;
+  }
+  const int64_t grid = std::max<int64_t>(ceil_div(p.capacity, 256), ceil_div(p.batch, 4));
+  require(grid < (1 << 24), "kv_plan: too many tokens or sequences");  // threads of a launch: 2^32
+  if (p.batch <= kScan) kv_plan_one_kernel<kScan, false><<<1, kScan, 0, stream>>>(a);
+  else kv_plan_scan_kernel<<<1, kScan, 0, stream>>>(a);
   HCP_HIP(hipGetLastError());
-  const int64_t items = std::max<int64_t>(p.capacity, static_cast<int64_t>(p.batch) * 64);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(items, 256), 1), 2048));
-  kv_plan_fill_kernel<<<grid, 256, 0, stream>>>(a);
+  kv_plan_fill_kernel<<<static_cast<unsigned>(grid), 256, 0, stream>>>(a);
   HCP_HIP(hipGetLastError());
 }
 
