@@ -167,7 +167,7 @@ struct Kv8Append {
   uint8_t* pool;
   float* scales;
   int64_t num_blocks;
-  int32_t bs, hkv, d, lanes_per_row, window;  // window: tokens whose runs a wave takes
+  int32_t bs, bs_shift, hkv, d, lanes_per_row, window;  // bs_shift: log2 or -1; window: tokens whose runs a wave takes
   const void* src[2];  // k, v views [hkv, tokens, d]
   int64_t hs[2], ss[2];
   int64_t tokens;

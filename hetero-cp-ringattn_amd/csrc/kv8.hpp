@@ -49,38 +49,65 @@ __device__ __forceinline__ void kv8_decode4(uint32_t w, float* x) {
   }
 }
 
-// Eight consecutive values of a row in DT, as fp32 and back.  VEC: 16-byte accesses.
+// Eight consecutive values of a row in DT as they are stored, to fp32 and back.  VEC: 16-byte
+// accesses.
 template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void* p, int64_t at, float* x) {
-  if constexpr (VEC && DT == kF32) {
-    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-    const float4 lo = q[0], hi = q[1];
-    x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w; x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
-  } else if constexpr (VEC) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = DT == kBF16 ? __uint_as_float(w[i] << 16) : f16_bits_to_f32(static_cast<uint16_t>(w[i] & 0xffffu));
-      x[2 * i + 1] = DT == kBF16 ? __uint_as_float(w[i] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(w[i] >> 16));
-    }
-  } else {
+struct Row8 {
+  float x[8];
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = load_elem<DT>(p, at + i);
   }
-}
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  }
+  __device__ __forceinline__ void get(float* y) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
+  }
+};
+template <>
+struct Row8<kF32, true> {
+  float4 lo, hi;
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    lo = q[0];
+    hi = q[1];
+  }
+  __device__ __forceinline__ void clear() { lo = hi = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float* y) const {
+    y[0] = lo.x; y[1] = lo.y; y[2] = lo.z; y[3] = lo.w; y[4] = hi.x; y[5] = hi.y; y[6] = hi.z; y[7] = hi.w;
+  }
+};
+template <int DT>
+struct Row8<DT, true> {
+  u32x4 w;
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+    w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
+  }
+  __device__ __forceinline__ void clear() { w = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void get(float* y) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[2 * i] = DT == kBF16 ? __uint_as_float(w[i] << 16) : f16_bits_to_f32(static_cast<uint16_t>(w[i] & 0xffffu));
+      y[2 * i + 1] = DT == kBF16 ? __uint_as_float(w[i] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(w[i] >> 16));
+    }
+  }
+};
 template <int DT, bool VEC>
 __device__ __forceinline__ void store8(void* p, int64_t at, const float* x) {
   if constexpr (VEC && DT == kF32) {
-    float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
-    q[0] = make_float4(x[0], x[1], x[2], x[3]);
-    q[1] = make_float4(x[4], x[5], x[6], x[7]);
+    float* const q = static_cast<float*>(p) + at;
+    store16_nt_sc1(q, __builtin_bit_cast(u32x4, make_float4(x[0], x[1], x[2], x[3])));
+    store16_nt_sc1(q + 4, __builtin_bit_cast(u32x4, make_float4(x[4], x[5], x[6], x[7])));
   } else if constexpr (VEC) {
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       w[i] = DT == kBF16 ? f32x2_to_bf16x2_bits(x[2 * i], x[2 * i + 1])
                          : static_cast<uint32_t>(f32_to_f16_bits(x[2 * i])) | static_cast<uint32_t>(f32_to_f16_bits(x[2 * i + 1])) << 16;
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + at) = w;
+    store16_nt_sc1(static_cast<uint16_t*>(p) + at, w);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) store_elem<DT>(p, at + i, x[i]);

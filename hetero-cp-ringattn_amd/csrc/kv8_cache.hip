@@ -20,18 +20,48 @@
 
 namespace hcp {
 
-// Largest magnitude over the wave, as the bits of |x| (NaN above infinity above finite).
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-  for (int off = 32; off > 0; off /= 2) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), off)));
+// Largest magnitude over the n lanes of a group, as the bits of |x| (NaN above infinity above finite).
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v, int n) {
+  for (int off = n / 2; off > 0; off /= 2) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), off)));
   return v;
 }
+__device__ __forceinline__ uint32_t top_of(const float* x, uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  return top;
+}
 
-// One run of n tokens (rows tok0 .. of the view) into slots a .. a + n of block blk.  A pass
-// is 64 chunks of 8 values; kKeep passes stay in registers from the maximum to the codes
-// (a block of 16 tokens of 128 dims: 4), later ones are read again, from the L2.
-constexpr int kKeep = 4;
-template <int F, int DT, bool VEC>
-__device__ void append_run(const Kv8Append& p, int plane, int head, int64_t blk, int a, int n, int64_t tok0) {
+// A block's scale after a run whose largest magnitude is `top` (bits), `old` held rows' (0: none).
+struct BlockScale {
+  float s;   // what divides
+  bool bad;  // a value that is not finite: the scale is NaN, codes 0
+};
+template <int F>
+__device__ __forceinline__ BlockScale block_scale(uint32_t top, float old) {
+  const bool bad = top >= 0x7f800000u || !(old >= 0.f && old < INFINITY);
+  return BlockScale{fmaxf(old, kv8_scale<F>(__uint_as_float(bad ? 0u : top))), bad};
+}
+template <int F>
+__device__ __forceinline__ void put_codes(uint8_t* at, const float* x, float inv, bool bad) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = bad ? 0.f : x[i] * inv;
+  *reinterpret_cast<u32x2*>(at) = u32x2{kv8_encode4<F>(y[0], y[1], y[2], y[3]), kv8_encode4<F>(y[4], y[5], y[6], y[7])};
+}
+template <int F>
+__device__ __forceinline__ void scale_codes(uint8_t* at, float f) {
+  const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+  float y[8];
+  kv8_decode4<F>(w[0], y);
+  kv8_decode4<F>(w[1], y + 4);
+  put_codes<F>(at, y, f, false);
+}
+
+// One run of n tokens (rows tok0 .. of the view) into slots a .. a + n of block blk, by a wave.
+// A pass is 64 chunks of 8 values; KEEP passes stay in registers from the maximum to the codes
+// (4: a block of 16 tokens of 128 dims; 16: of 64), later ones are read again, from the L2.
+template <int F, int DT, bool VEC, int KEEP>
+__device__ __forceinline__ void append_run(const Kv8Append& p, int plane, int head, int64_t blk, int a, int n, int64_t tok0) {
   const int lane = threadIdx.x & 63;
   const int lpr = p.lanes_per_row, rpp = 64 / lpr;  // lanes per row, rows per pass
   const int c = lane % lpr * 8, r0 = lane / lpr;
@@ -43,66 +73,81 @@ __device__ void append_run(const Kv8Append& p, int plane, int head, int64_t blk,
   uint8_t* const dst = p.pool + ((plane * p.num_blocks + blk) * p.bs * p.hkv + head) * p.d + c;
   const int64_t row = static_cast<int64_t>(p.hkv) * p.d;
   uint32_t top = 0;
-  float x[kKeep][8];
+  Row8<DT, VEC> x[KEEP];
 #pragma unroll
-  for (int k = 0; k < kKeep; ++k) {
+  for (int k = 0; k < KEEP; ++k) {
     const int r = r0 + k * rpp;
-    if (in && r < n) load8<DT, VEC>(src, src0 + r * ss, x[k]);
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[k][i] = 0.f;
+    if (in && r < n) x[k].load(src, src0 + r * ss);
+    else x[k].clear();
   }
+  float y[8];
 #pragma unroll
-  for (int k = 0; k < kKeep; ++k)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[k][i]) & 0x7fffffffu);
-  for (int r = r0 + kKeep * rpp; r < n; r += rpp)
+  for (int k = 0; k < KEEP; ++k) {
+    x[k].get(y);
+    top = top_of(y, top);
+  }
+  for (int r = r0 + KEEP * rpp; r < n; r += rpp)
     if (in) {
-      float y[8];
-      load8<DT, VEC>(src, src0 + r * ss, y);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+      Row8<DT, VEC> z;
+      z.load(src, src0 + r * ss);
+      z.get(y);
+      top = top_of(y, top);
     }
-  top = wave_max(top);
-  const bool bad = top >= 0x7f800000u || !(old >= 0.f && old < INFINITY);
-  const float need = kv8_scale<F>(__uint_as_float(bad ? 0u : top));
-  const float s = fmaxf(old, need);
-  if (lane == 0) *scale_at = bad ? __uint_as_float(0x7fc00000u) : s;
-  const float inv = 1.f / s;
-  auto put = [&](int r, const float* v) __attribute__((always_inline)) {
-    float y[8];
+  const BlockScale b = block_scale<F>(lanes_max(top, 64), old);
+  if (lane == 0) *scale_at = b.bad ? __uint_as_float(0x7fc00000u) : b.s;
+  const float inv = 1.f / b.s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = bad ? 0.f : v[i] * inv;
-    *reinterpret_cast<u32x2*>(dst + (a + r) * row) = u32x2{kv8_encode4<F>(y[0], y[1], y[2], y[3]), kv8_encode4<F>(y[4], y[5], y[6], y[7])};
-  };
-#pragma unroll
-  for (int k = 0; k < kKeep; ++k)
-    if (in && r0 + k * rpp < n) put(r0 + k * rpp, x[k]);
-  for (int r = r0 + kKeep * rpp; r < n; r += rpp)
+  for (int k = 0; k < KEEP; ++k)
+    if (in && r0 + k * rpp < n) {
+      x[k].get(y);
+      put_codes<F>(dst + (a + r0 + k * rpp) * row, y, inv, b.bad);
+    }
+  for (int r = r0 + KEEP * rpp; r < n; r += rpp)
     if (in) {
-      float y[8];
-      load8<DT, VEC>(src, src0 + r * ss, y);
-      put(r, y);
+      Row8<DT, VEC> z;
+      z.load(src, src0 + r * ss);
+      z.get(y);
+      put_codes<F>(dst + (a + r) * row, y, inv, b.bad);
     }
-  if (bad || s == old || a == 0) return;
-  const float f = old / s;
+  if (b.bad || b.s == old || a == 0) return;
   for (int r = r0; r < a; r += rpp)
-    if (in) {
-      u32x2* const at = reinterpret_cast<u32x2*>(dst + r * row);
-      const u32x2 w = *at;
-      float y[8];
-      kv8_decode4<F>(w[0], y);
-      kv8_decode4<F>(w[1], y + 4);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= f;
-      *at = u32x2{kv8_encode4<F>(y[0], y[1], y[2], y[3]), kv8_encode4<F>(y[4], y[5], y[6], y[7])};
-    }
+    if (in) scale_codes<F>(dst + r * row, old / b.s);
 }
 
-// One wave per window of tokens, head and plane; it has the runs that begin in the window.
+// A run of one token (a decode step's), by the lanes_per_row lanes of a group: 64 / lpr heads and
+// planes a wave, where a wave for each would have most of its lanes idle.
 template <int F, int DT, bool VEC>
+__device__ __forceinline__ void append_one(const Kv8Append& p, int plane, int head, int64_t blk, int a, int64_t tok) {
+  const int lpr = p.lanes_per_row, c = (threadIdx.x & 63) % lpr * 8;
+  const bool in = c < p.d;
+  float* const scale_at = p.scales + (plane * p.num_blocks + blk) * p.hkv + head;
+  uint8_t* const dst = p.pool + ((plane * p.num_blocks + blk) * p.bs * p.hkv + head) * p.d + c;
+  const int64_t row = static_cast<int64_t>(p.hkv) * p.d;
+  const float old = a > 0 ? *scale_at : 0.f;
+  Row8<DT, VEC> x;
+  if (in) x.load(p.src[plane], head * p.hs[plane] + tok * p.ss[plane] + c);
+  else x.clear();
+  float y[8];
+  x.get(y);
+  const BlockScale b = block_scale<F>(lanes_max(top_of(y, 0), lpr), old);
+  if (c == 0) *scale_at = b.bad ? __uint_as_float(0x7fc00000u) : b.s;
+  if (!in) return;
+  put_codes<F>(dst + a * row, y, 1.f / b.s, b.bad);
+  if (b.bad || b.s == old || a == 0) return;
+  for (int r = 0; r < a; ++r) scale_codes<F>(dst + r * row, old / b.s);
+}
+
+// Block of a slot: a shift where bs is a power of two (a 64-bit division takes some 150
+// instructions: 1000 decode tokens, 32/8 heads, 11.7 us with three of them a wave).
+__device__ __forceinline__ int64_t block_of(const Kv8Append& p, int64_t slot) {
+  return p.bs_shift >= 0 ? slot >> p.bs_shift : slot / p.bs;
+}
+
+// One wave per window of tokens, head and plane; it has the runs that begin in the window.  In
+// windows of one token the first wave of a workgroup takes runs of one token for all four.
+template <int F, int DT, bool VEC, int KEEP>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append p) {
-  const int task = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), task = blockIdx.y * 4 + wave;
   if (task >= 2 * p.hkv) return;
   const int plane = task / p.hkv, head = task - plane * p.hkv;
   const int lane = threadIdx.x & 63;
@@ -112,11 +157,11 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append p) {
   const int64_t t = first + lane;
   if (lane < p.window && t < p.tokens) {
     const int64_t slot = p.slots[t];
-    begins = slot >= 0 && (slot % p.bs == 0 || t == 0 || p.slots[t - 1] != slot - 1);
+    begins = slot >= 0 && (t == 0 || p.slots[t - 1] != slot - 1 || block_of(p, slot) * p.bs == slot);
   }
   for (uint64_t todo = __ballot(begins); todo != 0; todo &= todo - 1) {
     const int64_t t0 = first + __builtin_ctzll(todo), slot = p.slots[t0];
-    const int64_t blk = slot / p.bs;
+    const int64_t blk = block_of(p, slot);
     if (blk >= p.num_blocks) {
       if (lane == 0 && task == 0) atomicOr(p.err, 1);
       continue;
@@ -130,15 +175,26 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append p) {
       n += stop == 0 ? 64 : __builtin_ctzll(stop);
       if (stop != 0) break;
     }
-    append_run<F, DT, VEC>(p, plane, head, blk, a, n, t0);
+    if (n == 1 && p.window == 1) {
+      const int groups = 64 / p.lanes_per_row;  // heads and planes a wave
+      if (wave % min(groups, 4) != 0) return;
+      for (int g = lane / p.lanes_per_row; g < min(groups, 4); g += groups) {
+        const int mine = task + g;
+        if (mine < 2 * p.hkv) append_one<F, DT, VEC>(p, mine / p.hkv, mine % p.hkv, blk, a, t0);
+      }
+      return;
+    }
+    append_run<F, DT, VEC, KEEP>(p, plane, head, blk, a, n, t0);
   }
 }
 
 template <int F, int DT>
 static void append_typed(const Kv8Append& p, bool vec, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(ceil_div(p.tokens, p.window)), static_cast<unsigned>(ceil_div(2 * p.hkv, 4)));
-  if (vec) kv8_append_kernel<F, DT, true><<<grid, 256, 0, stream>>>(p);
-  else kv8_append_kernel<F, DT, false><<<grid, 256, 0, stream>>>(p);
+  const bool large = static_cast<int64_t>(p.bs) * p.lanes_per_row > 4 * 64;  // a block is more than four passes
+  if (vec && large) kv8_append_kernel<F, DT, true, 16><<<grid, 256, 0, stream>>>(p);
+  else if (vec) kv8_append_kernel<F, DT, true, 4><<<grid, 256, 0, stream>>>(p);
+  else kv8_append_kernel<F, DT, false, 4><<<grid, 256, 0, stream>>>(p);
 }
 
 // 8-element chunks of every row start on a 16-byte boundary.
@@ -158,6 +214,7 @@ void launch_kv8_append(int format, int dtype, Kv8Append p, hipStream_t stream) {
   const int es = dtype == kF32 ? 4 : 2;
   const bool vec = rows_aligned(p.src[0], p.hs[0], p.ss[0], es) && rows_aligned(p.src[1], p.hs[1], p.ss[1], es);
   p.lanes_per_row = lanes_for(p.d);
+  p.bs_shift = (p.bs & (p.bs - 1)) == 0 ? __builtin_ctz(p.bs) : -1;
   p.window = p.tokens > 2048 ? 16 : 1;
   auto typed = [&](auto f) {
     constexpr int F = decltype(f)::value;
