@@ -114,77 +114,112 @@ __device__ __forceinline__ void append_run(const Kv8Append& p, int plane, int he
     if (in) scale_codes<F>(dst + r * row, old / b.s);
 }
 
-// A run of one token (a decode step's), by the lanes_per_row lanes of a group: 64 / lpr heads and
-// planes a wave, where a wave for each would have most of its lanes idle.
-template <int F, int DT, bool VEC>
-__device__ __forceinline__ void append_one(const Kv8Append& p, int plane, int head, int64_t blk, int a, int64_t tok) {
-  const int lpr = p.lanes_per_row, c = (threadIdx.x & 63) % lpr * 8;
-  const bool in = c < p.d;
-  float* const scale_at = p.scales + (plane * p.num_blocks + blk) * p.hkv + head;
-  uint8_t* const dst = p.pool + ((plane * p.num_blocks + blk) * p.bs * p.hkv + head) * p.d + c;
-  const int64_t row = static_cast<int64_t>(p.hkv) * p.d;
-  const float old = a > 0 ? *scale_at : 0.f;
-  Row8<DT, VEC> x;
-  if (in) x.load(p.src[plane], head * p.hs[plane] + tok * p.ss[plane] + c);
-  else x.clear();
-  float y[8];
-  x.get(y);
-  const BlockScale b = block_scale<F>(lanes_max(top_of(y, 0), lpr), old);
-  if (c == 0) *scale_at = b.bad ? __uint_as_float(0x7fc00000u) : b.s;
-  if (!in) return;
-  put_codes<F>(dst + a * row, y, 1.f / b.s, b.bad);
-  if (b.bad || b.s == old || a == 0) return;
-  for (int r = 0; r < a; ++r) scale_codes<F>(dst + r * row, old / b.s);
-}
-
 // Block of a slot: a shift where bs is a power of two (a 64-bit division takes some 150
 // instructions: 1000 decode tokens, 32/8 heads, 11.7 us with three of them a wave).
 __device__ __forceinline__ int64_t block_of(const Kv8Append& p, int64_t slot) {
   return p.bs_shift >= 0 ? slot >> p.bs_shift : slot / p.bs;
 }
 
-// One wave per window of tokens, head and plane; it has the runs that begin in the window.  In
-// windows of one token the first wave of a workgroup takes runs of one token for all four.
+// N runs of one token (a decode step's), by the lanes_per_row lanes of a group: 64 / lpr
+// heads and planes a wave, where a wave for each would have most of its lanes idle, and the N
+// runs' rows and scales under way together.  slot[u] < 0: none.
+template <int F, int DT, bool VEC, int N>
+__device__ __forceinline__ void append_singles(const Kv8Append& p, int plane, int head, const int64_t* slot, const int64_t* tok) {
+  const int lpr = p.lanes_per_row, c = (threadIdx.x & 63) % lpr * 8;
+  const int64_t row = static_cast<int64_t>(p.hkv) * p.d;
+  Row8<DT, VEC> x[N];
+  float old[N];
+  float* scale_at[N];
+  uint8_t* block[N];
+  int a[N];
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const int64_t blk = slot[u] < 0 ? 0 : block_of(p, slot[u]);
+    a[u] = slot[u] < 0 ? -1 : static_cast<int>(slot[u] - blk * p.bs);
+    scale_at[u] = p.scales + (plane * p.num_blocks + blk) * p.hkv + head;
+    block[u] = p.pool + ((plane * p.num_blocks + blk) * p.bs * p.hkv + head) * p.d + c;
+    old[u] = a[u] > 0 ? *scale_at[u] : 0.f;
+    if (c < p.d && a[u] >= 0) x[u].load(p.src[plane], head * p.hs[plane] + tok[u] * p.ss[plane] + c);
+    else x[u].clear();
+  }
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    float y[8];
+    x[u].get(y);
+    const BlockScale b = block_scale<F>(lanes_max(top_of(y, 0), lpr), old[u]);
+    if (a[u] < 0) continue;
+    if (c == 0) *scale_at[u] = b.bad ? __uint_as_float(0x7fc00000u) : b.s;
+    if (c >= p.d) continue;
+    put_codes<F>(block[u] + a[u] * row, y, 1.f / b.s, b.bad);
+    if (b.bad || b.s == old[u]) continue;
+    for (int r = 0; r < a[u]; ++r) scale_codes<F>(block[u] + r * row, old[u] / b.s);
+  }
+}
+
+// One wave per window of tokens, head and plane; it has the runs that begin in the window, those of
+// one token for as many heads and planes of its workgroup as it has groups of lanes.
 template <int F, int DT, bool VEC, int KEEP>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), task = blockIdx.y * 4 + wave;
   if (task >= 2 * p.hkv) return;
-  const int plane = task / p.hkv, head = task - plane * p.hkv;
   const int lane = threadIdx.x & 63;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.window;
-  // lane i: does token first + i begin a run?
-  bool begins = false;
+  // lane i: does token first + i begin a run, and of more than itself?
+  bool begins = false, longer = false;
   const int64_t t = first + lane;
+  int64_t slot = -1;
   if (lane < p.window && t < p.tokens) {
-    const int64_t slot = p.slots[t];
-    begins = slot >= 0 && (t == 0 || p.slots[t - 1] != slot - 1 || block_of(p, slot) * p.bs == slot);
-  }
-  for (uint64_t todo = __ballot(begins); todo != 0; todo &= todo - 1) {
-    const int64_t t0 = first + __builtin_ctzll(todo), slot = p.slots[t0];
+    slot = p.slots[t];
+    const int64_t before = t > 0 ? p.slots[t - 1] : -2, after = t + 1 < p.tokens ? p.slots[t + 1] : -2;
     const int64_t blk = block_of(p, slot);
-    if (blk >= p.num_blocks) {
-      if (lane == 0 && task == 0) atomicOr(p.err, 1);
-      continue;
+    begins = slot >= 0 && (before != slot - 1 || blk * p.bs == slot);
+    longer = after == slot + 1 && after != (blk + 1) * p.bs;
+    if (begins && blk >= p.num_blocks) {
+      begins = false;
+      if (task == 0) atomicOr(p.err, 1);
     }
-    const int a = static_cast<int>(slot - blk * p.bs);
+  }
+  auto slot_at = [&](int i) __attribute__((always_inline)) {
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(slot >> 32), i))) << 32 |
+                                static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(slot), i)));
+  };
+  uint64_t singles = __ballot(begins && !longer), runs = __ballot(begins && longer);
+  const int groups = min(64 / p.lanes_per_row, 4), mine = task + lane / p.lanes_per_row;
+  const bool lanes_used = lane / p.lanes_per_row < groups && mine < 2 * p.hkv;
+  if (wave % groups != 0) singles = 0;
+  if (singles != 0 && (singles & (singles - 1)) == 0) {
+    const int i = __builtin_ctzll(singles);
+    const int64_t at[1] = {slot_at(i)}, tok[1] = {first + i};
+    if (lanes_used) append_singles<F, DT, VEC, 1>(p, mine / p.hkv, mine % p.hkv, at, tok);
+    singles = 0;
+  }
+  while (singles != 0) {
+    int64_t at[4], tok[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      at[u] = -1;
+      tok[u] = 0;
+      if (singles == 0) continue;
+      const int i = __builtin_ctzll(singles);
+      singles &= singles - 1;
+      at[u] = slot_at(i);
+      tok[u] = first + i;
+    }
+    if (lanes_used) append_singles<F, DT, VEC, 4>(p, mine / p.hkv, mine % p.hkv, at, tok);
+  }
+  for (; runs != 0; runs &= runs - 1) {
+    const int i0 = __builtin_ctzll(runs);
+    const int64_t t0 = first + i0, s0 = slot_at(i0), blk = block_of(p, s0);
+    const int a = static_cast<int>(s0 - blk * p.bs);
     int n = 1;
     for (;;) {  // 64 followers at a time
       const int64_t i = t0 + n + lane;
-      const bool follows = a + n + lane < p.bs && i < p.tokens && p.slots[i] == slot + n + lane;
+      const bool follows = a + n + lane < p.bs && i < p.tokens && p.slots[i] == s0 + n + lane;
       const uint64_t stop = __ballot(!follows);
       n += stop == 0 ? 64 : __builtin_ctzll(stop);
       if (stop != 0) break;
     }
-    if (n == 1 && p.window == 1) {
-      const int groups = 64 / p.lanes_per_row;  // heads and planes a wave
-      if (wave % min(groups, 4) != 0) return;
-      for (int g = lane / p.lanes_per_row; g < min(groups, 4); g += groups) {
-        const int mine = task + g;
-        if (mine < 2 * p.hkv) append_one<F, DT, VEC>(p, mine / p.hkv, mine % p.hkv, blk, a, t0);
-      }
-      return;
-    }
-    append_run<F, DT, VEC, KEEP>(p, plane, head, blk, a, n, t0);
+    append_run<F, DT, VEC, KEEP>(p, task / p.hkv, task % p.hkv, blk, a, n, t0);
   }
 }
 
@@ -215,7 +250,12 @@ void launch_kv8_append(int format, int dtype, Kv8Append p, hipStream_t stream) {
   const bool vec = rows_aligned(p.src[0], p.hs[0], p.ss[0], es) && rows_aligned(p.src[1], p.hs[1], p.ss[1], es);
   p.lanes_per_row = lanes_for(p.d);
   p.bs_shift = (p.bs & (p.bs - 1)) == 0 ? __builtin_ctz(p.bs) : -1;
-  p.window = p.tokens > 2048 ? 16 : 1;
+  // The smallest window that leaves at most 4096 waves, 16 at most: most waves of a prompt find that
+  // no run begins at their token, and a wave goes through its window's runs in turn.  bf16, 8 heads of
+  // 128, us at a window of 1 / 4 / 16: a prompt of 500 tokens 7.6 / 4.8 / 5.5, of 1000 16.6 / 5.9 / 5.7,
+  // of 4000 63 / 21 / 8.6; tokens of 64 sequences 4.3 / 6.5 / 17, of 1000 9.2 / 7.6 / 17.
+  p.window = 1;
+  while (p.window < 16 && p.tokens * 2 * p.hkv > 4096ll * p.window) p.window *= 2;
   auto typed = [&](auto f) {
     constexpr int F = decltype(f)::value;
     if (dtype == kBF16) append_typed<F, kBF16>(p, vec, stream);
