@@ -107,6 +107,45 @@ def test_decode_partial(gpu, case, q_layout):
     assert H.fetch_device_errors() == 0
 
 
+SPLIT = [
+    # seed, batch, Hq, Hkv, D, block size, format, longest, sequences that hold more than a block
+    (31, 1, 16, 1, 128, 16, "e4m3", 30000, 1),  # 16 waves of a head meet in LDS: 133 KB of it
+    (32, 1, 16, 1, 64, 16, "int8", 30000, 1),
+    (33, 1, 16, 1, 96, 16, "e4m3", 30000, 1),   # 8 waves
+    (34, 2, 8, 8, 128, 64, "e4m3", 9000, 2),
+    (35, 70, 8, 2, 64, 16, "int8", 4000, 5),    # more than 64 sequences in one row
+    (36, 65, 16, 8, 128, 16, "e4m3", 3000, 65),
+    (37, 200, 10, 5, 40, 32, "e4m3", 2500, 9),
+    (38, 1024, 4, 4, 8, 16, "int8", 4000, 12),
+    (39, 1025, 4, 4, 8, 16, "e4m3", 4000, 3),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SPLIT, ids=[str(c[0]) for c in SPLIT])
+def test_decode_of_few_long_and_many_short_sequences(gpu, case):
+    """Lengths from none to the longest in one call, the empty ones also first, last and in a row;
+    sequences share blocks, and a table names a block twice.  A wave sums at most a few thousand
+    weights here and the waves' sums are joined in 32 bits, so `tolerance` holds as it stands."""
+    seed, b, hq, hkv, d, bs, fmt, longest, long_ones = case
+    r = np.random.default_rng(seed)
+    lens = r.integers(0, bs + 1, b)
+    lens[r.permutation(b)[:long_ones]] = r.integers(1, longest + 1, long_ones)
+    if b > 8:
+        lens[[0, b // 2, b // 2 + 1, b - 1]] = 0
+    lens[b // 3] = longest
+    codes, scales = R.random_cache(r, 60, bs, hkv, d, fmt, 3)
+    table = r.integers(0, 60, (b, -(-longest // bs))).astype(np.int32)
+    qt = torch.from_numpy(r.normal(size=(b, hq, d)) * 0.5).to(torch.bfloat16)
+    pool, sc = R.to_device(codes, scales, fmt)
+    H.fetch_device_errors()
+    o, lse = H.kv8_decode_partial(qt.cuda(), pool, sc, torch.from_numpy(table).cuda(), 0, longest,
+                                  seq_lens=torch.from_numpy(lens.astype(np.int32)).cuda())
+    want, want_lse = reference(qt.double().numpy(), codes, scales, fmt, [table], [lens])
+    compare(o, lse, want, want_lse, R.LARGEST[fmt] * scales.max())
+    assert H.fetch_device_errors() == 0
+
+
 RING = [
     # seed, batch, Hq, Hkv, D, block size, dtype, format, tokens, domains, seed domain
     (21, 2, 32, 8, 128, 16, "bf16", "e4m3", 200, 3, 1),
