@@ -744,7 +744,7 @@ int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, cons
  * starts the block anew); where it grows the held codes are rounded to it.  New codes are
  * the nearest to x / scale, ties to even.  A run with a value that is not finite makes the
  * scale NaN, and with it all that the block and head stand for, until it is started anew.
- * A block takes one run per call: of two, either may be lost.
+ * A block takes one run per call: of two, what the block and its scale hold is undefined.
  *
  * hcp_kv8_decode_partial / hcp_kv8_decode_ring_replay: as hcp_paged_decode_partial and
  * hcp_decode_ring_replay, straight over the codes (desc->dtype: the type of q and of the
