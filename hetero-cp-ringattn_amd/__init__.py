@@ -667,11 +667,23 @@ def _launch(fn, dev, stream, *args):
             _check(fn(*args, _stream(stream)))
 
 
-def _workspace(ws, need, dev):
+def _empty(shape, dtype, device, stream):
+    """A new tensor in memory of ``stream``: what the current stream still does to the memory
+    it had last, or does to it once the caller lets go of it, would meet that stream's kernels."""
+    torch = _torch()
+    if stream is None or device.type != "cuda":
+        return torch.empty(shape, dtype=dtype, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _workspace(ws, need, dev, stream):
     """(tensor that keeps the memory, address, bytes) of a workspace, made where None."""
     torch = _torch()
     if ws is None:
-        ws = torch.empty(max(need(), 1), dtype=torch.uint8, device=torch.device("cuda", dev) if dev >= 0 else "cpu")
+        ws = _empty(max(need(), 1), torch.uint8, torch.device("cuda", dev) if dev >= 0 else torch.device("cpu"), stream)
     elif ws.get_device() != dev or not ws.is_contiguous():
         raise ValueError(f"workspace must be contiguous on {_place(dev)}")
     return ws, ws.data_ptr(), ws.numel() * ws.element_size()
@@ -701,7 +713,7 @@ def kv_plan_step(seq_lens, new_lens, block_tables, free_blocks, free_count, bloc
     elif capacity is None:
         raise ValueError("kv_plan_step needs a capacity or slots")
     i32, i64 = torch.int32, torch.int64
-    new = lambda n, dt: torch.empty(n, dtype=dt, device=seq_lens.device)  # noqa: E731
+    new = lambda n, dt: _empty(n, dt, seq_lens.device, stream)  # noqa: E731
     slots = new(capacity, i64) if slots is None else slots
     positions = new(capacity, i64) if positions is None else positions
     token_starts = new(b + 1, i32) if token_starts is None else token_starts
@@ -718,7 +730,7 @@ def kv_plan_step(seq_lens, new_lens, block_tables, free_blocks, free_count, bloc
     _want("seq_lens_out", seq_lens_out, i32, rows, dev)
     _want("free_count_out", free_count_out, i32, one, dev)
     _decode_tables("block_tables", block_tables, None, b, dev)
-    _ws, ws, ws_bytes = _workspace(workspace, lambda: kv_plan_workspace_size(b), dev)
+    _ws, ws, ws_bytes = _workspace(workspace, lambda: kv_plan_workspace_size(b), dev, stream)
     _launch(lib().hcp_kv_plan_step, dev, stream, b, block_size, free_blocks.shape[0], seq_lens.data_ptr(),
             new_lens.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
             free_blocks.data_ptr(), free_count.data_ptr(), capacity, token_starts.data_ptr(), slots.data_ptr(),
@@ -860,9 +872,9 @@ def kv8_gather(pool, scales, block_table, table_seq_offset, t0, t1, dtype=None, 
     pp, fmt, dev = _kv8(pool, scales)
     shape = (pp.num_kv_heads, t1 - t0, pp.head_dim)
     if k_out is None:
-        k_out = torch.empty(shape, dtype=dtype or torch.bfloat16, device=pool.device)
+        k_out = _empty(shape, dtype or torch.bfloat16, pool.device, stream)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=k_out.dtype, device=pool.device)
+        v_out = _empty(shape, k_out.dtype, pool.device, stream)
     _rows_of("k_out", k_out, shape, dev, dtype)
     _rows_of("v_out", v_out, shape, dev, k_out.dtype)
     n = block_table.numel()
@@ -881,7 +893,7 @@ def _decode_tables(name, tables, lens, b, dev):
         _want("seq_lens", lens, torch.int32, (b,), dev)
 
 
-def _decode_rows(q, pp, dev, o, lse, o_dtype):
+def _decode_rows(q, pp, dev, o, lse, o_dtype, stream):
     """Outputs [B, Hq, D] and [B, Hq] (made where None), and q checked against the pool."""
     torch = _torch()
     shape = q.shape
@@ -889,9 +901,9 @@ def _decode_rows(q, pp, dev, o, lse, o_dtype):
     if d != pp.head_dim or q.get_device() != dev or (q.stride(2) != 1 and d > 1):
         raise ValueError(f"q must be [B, Hq, {pp.head_dim}] with contiguous rows on {_place(dev)}")
     if o is None:
-        o = torch.empty(shape, dtype=o_dtype, device=q.device)
+        o = _empty(shape, o_dtype, q.device, stream)
     if lse is None:
-        lse = torch.empty((b, hq), dtype=torch.float32, device=q.device)
+        lse = _empty((b, hq), torch.float32, q.device, stream)
     _rows_of("o", o, shape, dev, o_dtype)
     _want("lse", lse, torch.float32, (b, hq), dev)
     return o, lse
@@ -908,14 +920,14 @@ def kv8_decode_partial(q, pool, scales, block_tables, t0, t1, seq_lens=None, sca
     """As :func:`decode_local_compact_partial` over an 8-bit cache: q [B, Hq, D] over tokens
     [t0, min(t1, seq_lens)) of each sequence -> (o [B, Hq, D] fp32, lse [B, Hq] fp32)."""
     pp, fmt, dev = _kv8(pool, scales)
-    o, lse = _decode_rows(q, pp, dev, o, lse, _torch().float32)
+    o, lse = _decode_rows(q, pp, dev, o, lse, _torch().float32, stream)
     _decode_tables("block_tables", block_tables, seq_lens, q.shape[0], dev)
     if not o.is_contiguous():
         raise ValueError("o must be contiguous")
     desc = decode_desc(q, pool, block_tables, t0, t1, scale)
     fns = lib()
     _ws, ws, ws_bytes = _workspace(workspace, lambda: fns.hcp_kv8_decode_workspace_size(ctypes.byref(desc), ctypes.byref(pp)),
-                                   dev)
+                                   dev, stream)
     _launch(fns.hcp_kv8_decode_partial, dev, stream, ctypes.byref(desc), ctypes.byref(pp), scales.data_ptr(), fmt,
             View(q.data_ptr(), q.stride(1), q.stride(0)), block_tables.data_ptr(),
             None if seq_lens is None else seq_lens.data_ptr(), o.data_ptr(), lse.data_ptr(), ws, ws_bytes)
@@ -932,12 +944,12 @@ def kv8_decode_ring_replay(q, pool, scales, shards, seed_domain, scale=None, out
                            stream=None):
     """As :func:`decode_ring_replay` over an 8-bit cache (shards as there)."""
     pp, fmt, dev = _kv8(pool, scales)
-    out, lse_out = _decode_rows(q, pp, dev, out, lse_out, q.dtype)
+    out, lse_out = _decode_rows(q, pp, dev, out, lse_out, q.dtype, stream)
     for tables, lens, _ in shards:
         _decode_tables("a shard's tables", tables, lens, q.shape[0], dev)
     desc, arr, n, fns = _ring_desc(q, pool, scale), _shards(shards), len(shards), lib()
     _ws, ws, ws_bytes = _workspace(
-        workspace, lambda: fns.hcp_kv8_decode_ring_workspace_size(ctypes.byref(desc), ctypes.byref(pp), n, arr), dev)
+        workspace, lambda: fns.hcp_kv8_decode_ring_workspace_size(ctypes.byref(desc), ctypes.byref(pp), n, arr), dev, stream)
     _launch(fns.hcp_kv8_decode_ring_replay, dev, stream, ctypes.byref(desc), ctypes.byref(pp), scales.data_ptr(), fmt,
             View(q.data_ptr(), q.stride(1), q.stride(0)), n, arr, seed_domain,
             View(out.data_ptr(), out.stride(1), out.stride(0)), lse_out.data_ptr(), ws, ws_bytes)
@@ -956,13 +968,13 @@ def kv8_ring_attention_replay_paged(q, pool, scales, block_table, chunks, causal
     n, fns = block_table.numel(), lib()
     _want("block_table", block_table, torch.int32, (n,), dev)
     if out is None:
-        out = torch.empty((hq, s, d), dtype=q.dtype, device=q.device)
+        out = _empty((hq, s, d), q.dtype, q.device, stream)
     if lse_out is None:
-        lse_out = torch.empty((hq, s), dtype=torch.float32, device=q.device)
+        lse_out = _empty((hq, s), torch.float32, q.device, stream)
     _rows_of("q", q, (hq, s, d), dev)
     _rows_of("out", out, (hq, s, d), dev, q.dtype)
     _want("lse_out", lse_out, torch.float32, (hq, s), dev)
-    _ws, ws, ws_bytes = _workspace(workspace, lambda: fns.hcp_ring_replay_workspace_size(ctypes.byref(desc), 1), dev)
+    _ws, ws, ws_bytes = _workspace(workspace, lambda: fns.hcp_ring_replay_workspace_size(ctypes.byref(desc), 1), dev, stream)
     _launch(fns.hcp_kv8_prefill_replay_paged, dev, stream, ctypes.byref(desc), view(q), ctypes.byref(pp),
             scales.data_ptr(), fmt, block_table.data_ptr(), n, view(out), lse_out.data_ptr(), ws, ws_bytes)
     del arr

@@ -679,6 +679,7 @@ void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const 
   require(batch <= 65535, "kv8_decode: batch must be at most 65535");  // grid y
   require(16ll * hkv * d < (1ll << 31), "kv8_decode: too many heads");   // 32-bit offsets in a group
   for (int i = 0; i < n; ++i) require(spans[i].t0 >= 0 && spans[i].t0 < pool.bs, "kv8_decode: a span starts in its first block");
+  require(span_groups(n, spans) <= INT32_MAX / 4, "kv8_decode: too many tokens");  // a sequence's groups are counted in 32 bits
   const Kv8Plan p = plan_kv8(batch, hq, hkv, d, n, spans);
   Kv8DecodeArgs a;
   a.ws_o = a.ws_lse = nullptr;

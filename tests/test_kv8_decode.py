@@ -423,6 +423,42 @@ def test_decode_on_another_stream(gpu):
     assert torch.equal(o, want[0]) and torch.equal(l, want[1])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("as_handle", [False, True])
+def test_memory_made_by_a_call_is_its_streams(gpu, monkeypatch, as_handle):
+    """Outputs and workspaces that a call makes come from the memory of the stream it is given."""
+    pool, sc = H.kv8_pool(20, 16, 2, 64)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table, lens, one = torch.arange(20, **i32).view(2, 10), torch.full((2,), 100, **i32), torch.ones(2, **i32)
+    q, rows = torch.randn(2, 8, 64, device="cuda", dtype=torch.bfloat16), torch.randn(8, 100, 64, device="cuda", dtype=torch.bfloat16)
+    sc.fill_(1)
+    s = torch.cuda.Stream()
+    handle = s.cuda_stream if as_handle else s
+    calls = [lambda st: H.kv_plan_step(lens, one, table.clone(), torch.zeros(20, **i32), torch.zeros(1, **i32), 16, capacity=2, stream=st),
+             lambda st: H.kv8_gather(pool, sc, table[0], 0, 0, 100, stream=st),
+             lambda st: H.kv8_decode_partial(q, pool, sc, table, 0, 100, seq_lens=lens, stream=st),
+             lambda st: H.kv8_decode_ring_replay(q, pool, sc, [(table, lens, 100)], 0, stream=st),
+             lambda st: H.kv8_ring_attention_replay_paged(rows, pool, sc, table[0], [60, 40], stream=st)]
+    empty, seen = torch.empty, []
+
+    def watched(*args, **kw):
+        seen.append(torch.cuda.current_stream().cuda_stream)
+        return empty(*args, **kw)
+
+    torch.cuda.synchronize()
+    for call in calls:
+        want = call(None)
+        torch.cuda.synchronize()
+        monkeypatch.setattr(torch, "empty", watched)
+        seen.clear()
+        got = call(handle)
+        monkeypatch.setattr(torch, "empty", empty)
+        assert len(seen) >= 2 and set(seen) == {s.cuda_stream}
+        s.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
 # ---- refusals (no GPU) ----
 P = 256  # a pointer that is never followed: every call below is refused on the host
 
