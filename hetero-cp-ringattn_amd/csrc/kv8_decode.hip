@@ -27,6 +27,13 @@
 //     tracked like m: w <= 2^14 whatever the scales, and split into two f16 of 11 bits each, w
 //     = hi + lo, so P carries 22 bits (one f16 alone would put 2^-12 on every weight, against
 //     the fp32 weights of the 16-bit decode).  Sums and statistics are fp32.
+//
+// Measured, 32/8 heads of 128, e4m3, blocks of 16: 64 sequences of 8-16k tokens 267 us (1.63 GB at
+// 6.1 TB/s, each byte fetched once; the 16-bit decode of 64 x 16k 635 us for 4.3 GB), 6 x 2085 of
+// 16/2 heads 12.4 us, one sequence of 130 tokens 6.7 us.  What bounds the short ones is the chain of
+// lengths, table, q and codes, one latency each (2.5-4 us), then 0.95 us a step of a lone wave, whose
+// instructions no other wave hides.  Two steps of codes under way instead of one cost more in
+// registers and instructions than they hid (64 sequences 270 us, one of 130 tokens 8.3).
 #include <algorithm>
 #include <type_traits>
 

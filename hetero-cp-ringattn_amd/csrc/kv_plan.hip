@@ -16,7 +16,8 @@
 // Bound by latency: a batch of 256 reads and writes some 20 KB.  The running sums need all
 // sequences, so one workgroup takes them; where it can hold them in LDS and the tokens are few
 // it fills everything, too, in one launch (kv_plan_one_kernel), else the whole grid fills in a
-// second one (kv_plan_fill_kernel).
+// second one (kv_plan_fill_kernel).  Decode steps of 16 sequences 3.5 us, of 256 with five that
+// ended 7.4 (4.8 without: their 800 blocks go on the stack); 1000 sequences, 60000 places 14.4.
 #include <algorithm>
 
 #include "kernels.hpp"
