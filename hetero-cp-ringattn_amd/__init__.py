@@ -365,9 +365,9 @@ def dtype_code(t) -> int:
     return _dtype_codes[t]
 
 
-def _stream(stream=None):
-    """hipStream_t of a torch stream (default: the current one); an int is taken as the
-    raw handle (0: the default stream)."""
+def _stream(stream=None, dev=None):
+    """hipStream_t of a torch stream (default: the current one, of GPU ``dev`` where the caller
+    knows which is current); an int is taken as the raw handle (0: the default stream)."""
     if isinstance(stream, int):
         return ctypes.c_void_p(stream)
     if stream is None:
@@ -375,18 +375,19 @@ def _stream(stream=None):
         # the handle itself where torch hands it out (0.2 us; the stream object takes 2.8)
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         if raw is not None:
-            return ctypes.c_void_p(raw(torch.cuda.current_device()))
+            return ctypes.c_void_p(raw(torch.cuda.current_device() if dev is None else dev))
         stream = torch.cuda.current_stream()
     return ctypes.c_void_p(stream.cuda_stream)
 
 
 def view(t) -> View:
     """[heads, tokens, head_dim] tensor (last dim contiguous) -> hcp_ring_view."""
-    if t.dim() != 3:
+    strides = t.stride()
+    if len(strides) != 3:
         raise ValueError("expected a [heads, tokens, head_dim] tensor")
-    if t.stride(2) != 1 and t.shape[2] > 1:
+    if strides[2] != 1 and t.shape[2] > 1:
         raise ValueError("head_dim must be the contiguous dimension")
-    return View(t.data_ptr(), t.stride(0), t.stride(1))
+    return View(t.data_ptr(), strides[0], strides[1])
 
 
 def _ptr(t) -> ctypes.c_void_p:
@@ -661,7 +662,9 @@ def _launch(fn, dev, stream, *args):
     if dev < 0:
         raise ValueError("tensors must be on a GPU")
     if dev == torch.cuda.current_device():
-        _check(fn(*args, _stream(stream)))
+        rc = fn(*args, _stream(stream, dev))
+        if rc != 0:
+            _check(rc)
     else:
         with torch.cuda.device(dev):
             _check(fn(*args, _stream(stream)))
