@@ -423,6 +423,84 @@ def test_decode_on_another_stream(gpu):
     assert torch.equal(o, want[0]) and torch.equal(l, want[1])
 
 
+def _two_decodes():
+    """Two calls that split sequences over workers: (q, pool, scales, table, tokens, lens) and what they give."""
+    calls = []
+    for seed, heads in ((38, (8, 2, 128)), (39, (8, 8, 64))):
+        _, lens, codes, scales, tables, qt, _ = inputs(seed, 3, *heads, 16, "bf16", "e4m3", 4000)
+        pool, sc = R.to_device(codes, scales, "e4m3")
+        calls.append((qt, pool, sc, torch.from_numpy(tables[0]).cuda(), 4000, torch.from_numpy(lens[0].astype(np.int32)).cuda()))
+    want = [H.kv8_decode_partial(q, p, sc, t, 0, n, seq_lens=l) for q, p, sc, t, n, l in calls]
+    torch.cuda.synchronize()
+    return calls, want
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once(gpu):
+    calls, want = _two_decodes()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        got = [H.kv8_decode_partial(q, p, sc, t, 0, n, seq_lens=l, stream=s) for s, (q, p, sc, t, n, l) in zip(streams, calls)]
+        torch.cuda.synchronize()
+        for (o, l), (wo, wl) in zip(got, want):
+            assert torch.equal(o, wo) and torch.equal(l, wl)
+
+
+@pytest.mark.gpu
+def test_two_graphs_share_a_workspace(gpu):
+    calls, want = _two_decodes()
+    size = max(H.kv8_decode_workspace_size(q, p, t, 0, n) for q, p, _, t, n, _ in calls)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")  # NaN
+    graphs, outs = [], []
+    for q, p, sc, t, n, l in calls:
+        o, lse = torch.empty(q.shape, device="cuda"), torch.empty(q.shape[:2], device="cuda")
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            H.kv8_decode_partial(q, p, sc, t, 0, n, seq_lens=l, workspace=ws, o=o, lse=lse)
+        graphs.append(g)
+        outs.append((o, lse))
+    for k in (0, 1, 1, 0, 1):
+        outs[k][0].fill_(7)
+        graphs[k].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[k][0], want[k][0]) and torch.equal(outs[k][1], want[k][1])
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(gpu):
+    """A cache of two planes of 4.3e9 codes, its last blocks in use, rows 2^28 elements apart: bit
+    for bit as the same blocks in a small cache with packed rows."""
+    hkv, d, bs, tokens = 8, 128, 16, 40
+    nb = (1 << 32) // (bs * hkv * d) + 64
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB of device memory")
+    pool = torch.empty(2, nb, bs, hkv, d, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scales = torch.zeros(2, nb, hkv, device="cuda")
+    small, small_scales = H.kv8_pool(64, bs, hkv, d)
+    ids = torch.tensor([nb - 1, 3, nb - 64], dtype=torch.int32, device="cuda")
+    near = torch.tensor([63, 3, 0], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(9)
+    k, v = (torch.randn(hkv, tokens, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    big = torch.empty(((tokens - 1) << 28) + hkv * d, dtype=torch.bfloat16, device="cuda")
+    far = big.as_strided((hkv, tokens, d), (d, 1 << 28, 1))
+    far.copy_(k)
+    slot = lambda t: (t.long()[:, None] * bs + torch.arange(bs, device="cuda")).flatten()[:tokens]  # noqa: E731
+    H.kv8_append(pool, scales, far, v, slot(ids))
+    H.kv8_append(small, small_scales, k, v, slot(near))
+    out = far.zero_()
+    gk, gv = H.kv8_gather(small, small_scales, near, 0, 0, tokens)
+    rows = torch.empty_like(big).as_strided(out.shape, out.stride())
+    H.kv8_gather(pool, scales, ids, 0, 0, tokens, k_out=out, v_out=rows)
+    assert torch.equal(out, gk) and torch.equal(rows, gv)
+    q = torch.randn(2, 32, d, generator=g, device="cuda").bfloat16()
+    tables, near_tables = (torch.stack([t, t.flip(0)]) for t in (ids, near))
+    lens = torch.tensor([tokens, 17], dtype=torch.int32, device="cuda")
+    got = H.kv8_decode_partial(q, pool, scales, tables, 0, tokens, seq_lens=lens)
+    want = H.kv8_decode_partial(q, small, small_scales, near_tables, 0, tokens, seq_lens=lens)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert H.fetch_device_errors() == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("as_handle", [False, True])
 def test_memory_made_by_a_call_is_its_streams(gpu, monkeypatch, as_handle):
