@@ -17,7 +17,7 @@
 // sequences, so one workgroup takes them; where it can hold them in LDS and the tokens are few
 // it fills everything, too, in one launch (kv_plan_one_kernel), else the whole grid fills in a
 // second one (kv_plan_fill_kernel).  Decode steps of 16 sequences 3.5 us, of 256 with five that
-// ended 7.4 (4.8 without: their 800 blocks go on the stack); 1000 sequences, 60000 places 14.4.
+// ended 7.4 (4.8 without: their 800 blocks go on the stack); 1000 sequences, 60000 places 12.
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -49,9 +49,9 @@ struct PlanSums {
 };
 
 constexpr int kScan = 1024;       // threads of the scan's workgroup, and most sequences of the one-launch form
-// Most tokens of the one-launch form: 4000 of 1000 sequences take it 12.4 us, two launches 12.6;
-// 1500 of 256 8.2 and 11.0; 60000 of 1000 (three loads in line for each token on one CU) 14.4 in two.
-constexpr int kOneTokens = 4096;
+// Most tokens of the one-launch form, where each token's three loads in line are one CU's: 2000 tokens
+// of 1000 sequences take it 9.3 us, two launches 10.4, of 16 8.1 and 8.9; 4000 of 1000 12.5 and 10.9.
+constexpr int kOneTokens = 2048;
 
 // Inclusive sums over the T threads of the workgroup of two counts each, and their totals.
 struct Pair {
@@ -297,21 +297,58 @@ __global__ __launch_bounds__(kScan) void kv_plan_scan_kernel(PlanArgs a) {
   if (flags != 0) atomicOr(p.err, flags);
 }
 
-// 256 tokens a workgroup, whose sequences lie between its first and its last token's (two of
-// the searches over all sequences instead of 256), and a sequence's blocks a wave.
-__global__ __launch_bounds__(256) void kv_plan_fill_kernel(PlanArgs a) {
+// As plan_seq_of by a whole wave: 64 probes at a time (1000 sequences: two loads in line, not ten).
+__device__ __forceinline__ int plan_seq_of_wave(const int32_t* starts, int lo, int hi, int64_t i) {
+  const int lane = threadIdx.x & 63;
+  while (lo < hi) {
+    const int step = (hi - lo + 63) / 64;
+    const int64_t mid = static_cast<int64_t>(lo) + (lane + 1ll) * step - 1;
+    const uint64_t past = __ballot(mid >= hi || starts[mid + 1] > i);
+    if (past == 0) return hi;
+    const int f = __builtin_ctzll(past);
+    hi = static_cast<int>(min(static_cast<int64_t>(lo) + (f + 1ll) * step - 1, static_cast<int64_t>(hi)));
+    lo = lo + f * step;
+  }
+  return lo;
+}
+
+// The first workgroups: 256 tokens each, whose sequences lie between its first and its last token's;
+// where those are few their starts are searched in LDS.  The others: a sequence's blocks a wave.
+constexpr int kStarts = 512;
+__global__ __launch_bounds__(256) void kv_plan_fill_kernel(PlanArgs a, int token_groups) {
   __shared__ int ends[2];
+  __shared__ int32_t near[kStarts + 1];
   const KvPlan& p = a.p;
   const PlanSums sums{a.info, p.token_starts, a.back_end, *a.head};
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256;
-  if (first < p.capacity) {
-    if (threadIdx.x < 128 && (threadIdx.x & 63) == 0)
-      ends[threadIdx.x >> 6] = plan_seq_of(sums.starts, 0, p.batch - 1, threadIdx.x == 0 ? first : first + 255);
-    __syncthreads();
-    if (first + threadIdx.x < p.capacity) plan_token(p, sums, first + threadIdx.x, ends[0], ends[1]);
+  if (static_cast<int>(blockIdx.x) >= token_groups) {
+    const int64_t b = static_cast<int64_t>(blockIdx.x - token_groups) * 4 + (threadIdx.x >> 6);
+    if (b < p.batch) plan_blocks(p, sums, b, threadIdx.x & 63, INT32_MAX, 64);
+    return;
   }
-  const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (b < p.batch) plan_blocks(p, sums, b, threadIdx.x & 63, INT32_MAX, 64);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256, i = first + threadIdx.x;
+  const int32_t all = p.token_starts[p.batch];
+  if (first >= all) {  // past all tokens
+    if (i < p.capacity) {
+      p.slots[i] = -1;
+      p.positions[i] = 0;
+    }
+    return;
+  }
+  if (threadIdx.x < 128) {
+    const int e = plan_seq_of_wave(p.token_starts, 0, p.batch - 1, threadIdx.x < 64 ? first : first + 255);
+    if ((threadIdx.x & 63) == 0) ends[threadIdx.x >> 6] = e;
+  }
+  __syncthreads();
+  const int lo = ends[0], n = ends[1] - lo + 1;
+  int b = lo;
+  if (n <= kStarts) {
+    for (int k = threadIdx.x; k <= n; k += 256) near[k] = p.token_starts[lo + k];
+    __syncthreads();
+    b = lo + plan_seq_of(near, 0, n - 1, i);
+  } else {
+    b = plan_seq_of(p.token_starts, lo, ends[1], i);
+  }
+  if (i < p.capacity) plan_token(p, sums, i, b, b);
 }
 
 static size_t plan_align(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
@@ -336,12 +373,12 @@ void launch_kv_plan(const KvPlan& p, void* ws, hipStream_t stream) {
     HCP_HIP(hipGetLastError());
     return;
   }
-  const int64_t grid = std::max<int64_t>(ceil_div(p.capacity, 256), ceil_div(p.batch, 4));
+  const int64_t token_groups = ceil_div(p.capacity, 256), grid = token_groups + ceil_div(p.batch, 4);
   require(grid < (1 << 24), "kv_plan: too many tokens or sequences");  // threads of a launch: 2^32
   if (p.batch <= kScan) kv_plan_one_kernel<kScan, false><<<1, kScan, 0, stream>>>(a);
   else kv_plan_scan_kernel<<<1, kScan, 0, stream>>>(a);
   HCP_HIP(hipGetLastError());
-  kv_plan_fill_kernel<<<static_cast<unsigned>(grid), 256, 0, stream>>>(a);
+  kv_plan_fill_kernel<<<static_cast<unsigned>(grid), 256, 0, stream>>>(a, static_cast<int>(token_groups));
   HCP_HIP(hipGetLastError());
 }
 
