@@ -119,6 +119,18 @@ def test_plan_matches_the_host(gpu, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,every,more", [(700, 97, 3000), (1024, 1024, 2100), (3000, 601, 0), (4000, 3, 500), (70000, 9000, 1)])
+def test_plan_of_mostly_idle_sequences(gpu, batch, every, more):
+    # many sequences between two tokens that are neighbours, and at either end; tokens end inside,
+    # at and before the capacity
+    args = list(plan_inputs(30, batch, 16, 60, 300, [0]))
+    args[1][::every] = np.resize([5, 300, 1], len(args[1][::every]))
+    args[1][batch // 2] = 17
+    check(args, 16, int(args[1].sum()) + more)
+    check(args, 16, int(args[1].sum()) - 20, in_place=True)
+
+
+@pytest.mark.gpu
 def test_plan_refuses_what_does_not_fit(gpu):
     # too few places in the token list, and rows too short for the new tokens: those
     # sequences keep their length and row, the others are served
