@@ -108,8 +108,8 @@ int elem_size(int dtype) {
 
 void check_view(const hcp_ring_view& v, const char* name, int64_t len) {
   if (len == 0) return;
-  require(v.data != nullptr, std::string(name) + ": null data pointer");
-  require(v.head_stride >= 0 && v.seq_stride > 0, std::string(name) + ": strides must be positive");
+  require(v.data != nullptr, name, ": null data pointer");
+  require(v.head_stride >= 0 && v.seq_stride > 0, name, ": strides must be positive");
 }
 
 void check_block_desc(const hcp_ring_block_desc* d) {
@@ -1800,7 +1800,7 @@ int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, cons
             "null pointer");
     require(capacity == 0 || (slots != nullptr && positions != nullptr), "null slots or positions");
     const size_t need = kv_plan_workspace_bytes(batch);
-    require(workspace != nullptr && workspace_bytes >= need, "workspace too small: need " + std::to_string(need) + " bytes");
+    if (workspace == nullptr || workspace_bytes < need) throw Error(-6, "workspace too small: need " + std::to_string(need) + " bytes");
     require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
     const int shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
     launch_kv_plan(KvPlan{batch, block_size, shift, num_blocks, seq_lens, new_lens, block_tables, table_stride, table_len,
@@ -1830,7 +1830,7 @@ Kv8Pool check_kv8(const hcp_paged_pool* pool, const float* scales, int32_t forma
 // Element accesses of a view: its rows start on element boundaries.
 void check_rows(const hcp_ring_view& v, const char* name, int64_t len, int dtype) {
   check_view(v, name, len);
-  require(reinterpret_cast<uintptr_t>(v.data) % elem_size(dtype) == 0, std::string(name) + ": not aligned to its elements");
+  require(reinterpret_cast<uintptr_t>(v.data) % elem_size(dtype) == 0, name, ": not aligned to its elements");
 }
 }  // namespace
 extern "C" {

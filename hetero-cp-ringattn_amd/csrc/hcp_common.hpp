@@ -37,6 +37,13 @@ inline void hip_check(hipError_t e, const char* what) {
 inline void require(bool ok, const std::string& msg) {
   if (!ok) throw Error(-6, msg);
 }
+// A call makes some 25 checks; a string is made for a refusal only.
+inline void require(bool ok, const char* msg) {
+  if (__builtin_expect(!ok, 0)) throw Error(-6, msg);
+}
+inline void require(bool ok, const char* name, const char* msg) {
+  if (__builtin_expect(!ok, 0)) throw Error(-6, std::string(name) + msg);
+}
 
 // Sticky device-side error flags (bit 0: paged block id out of range; bit 1: key
 // positions not non-decreasing).

@@ -694,7 +694,7 @@ void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const 
   if (p.workers > 0) {
     const size_t rows = static_cast<size_t>(p.workers + batch) * hq;
     const size_t need = workers_bytes(p.workers, batch, hq, d);
-    require(ws != nullptr && ws_bytes >= need, "workspace too small: need " + std::to_string(need) + " bytes");
+    if (ws == nullptr || ws_bytes < need) throw Error(-6, "workspace too small: need " + std::to_string(need) + " bytes");
     require(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "workspace must be 16-byte aligned");
     char* at = static_cast<char*>(ws);
     a.ws_o = reinterpret_cast<float*>(at);
