@@ -14,8 +14,8 @@ The operator names mirror the reference's ring-attention backend
 * :func:`kv_plan_step`  block tables, slots and positions of a step from request lengths ->
   ``hcp_kv_plan_step`` (no reference counterpart)
 * :func:`kv8_append` / :func:`kv8_decode_partial` / :func:`kv8_decode_ring_replay` /
-  :func:`kv8_gather` / :func:`kv8_ring_attention_replay_paged`  a paged K/V cache in 8 bits with a scale per block and head -> ``hcp_kv8_*`` (no reference
-  counterpart)
+  :func:`kv8_gather` / :func:`kv8_ring_attention_replay_paged`  a paged K/V cache in 8 bits
+  with a scale per block and head -> ``hcp_kv8_*`` (no reference counterpart)
 * :func:`ring_attention_replay`             ring.rs:861-1398 for every domain on one GPU ->
   ``hcp_ring_prefill_replay`` (``_paged`` variant stages K/V from a block pool)
 
