@@ -66,6 +66,10 @@ struct Kv8DecodeArgs {
 static_assert(sizeof(Kv8DecodeArgs) <= 4096, "kernel arguments are limited to 4 KiB");
 
 constexpr float kNoMax = -1.0e30f;
+// V scales count as 2^-110 at least in the running maximum a (not in the product): a >= m - 110, so
+// 2^(m - a + 14) and the 2^(a - m - 14) that takes it out again are normal numbers, for scales of 0,
+// too.  The weights of smaller scales are below 2^14 by their distance; of 2^-126 they keep 22 bits.
+constexpr float kLeastVScale = 0x1p-110f;
 // Most waves per workgroup: four to a SIMD, which 128 registers allow; the padded form needs more.
 constexpr int kv8_waves(bool pad) { return pad ? 8 : 16; }
 
@@ -390,7 +394,7 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
         tmax = over_groups(tmax, [](float u, float v) { return fmaxf(u, v); });
         // ---- running maxima of the scores and of weight times scale ----
         const float m_new = fmaxf(m_run, tmax);
-        const float top = fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), 1.17549435e-38f);
+        const float top = fmaxf(fmaxf(vs[0], vs[1]), kLeastVScale);
         const float a_new = fmaxf(a_run, tmax + __builtin_amdgcn_logf(top));
         l_run *= __builtin_amdgcn_exp2f(m_run - m_new);
         if (__any(a_new > a_run)) {
@@ -466,7 +470,8 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
 
     // ---- epilogue: dims (4 grp + i) VB + j of query col are acc[j][i] ----
     const float l = over_groups(l_run, [](float u, float v) { return u + v; });
-    const float inv = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(a_run - m_run - 14.f) / l;  // NaN stays
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays
+    const float down = __builtin_amdgcn_exp2f(a_run - m_run - 14.f);  // applied last: it may be 2^-124
     const float lse2 = l == 0.f ? -INFINITY : m_run + __log2f(l);
     // Addresses below are made from a lane number of their own: hoisted out of the loop over
     // sequences they would cost registers all the way through it.
@@ -488,7 +493,7 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
           const int d0 = (4 * grp + i) * VB;
           float x[VB];
 #pragma unroll
-          for (int j = 0; j < VB; ++j) x[j] = acc[j][i] * inv;
+          for (int j = 0; j < VB; ++j) x[j] = acc[j][i] * inv * down;
           if (!PAD || d0 < dn) store_out<VB>(o_to, o_dt, r * o_rs + d0, x);
         }
         if (grp == 0 && lse_to != nullptr) lse_to[r] = lse2 * kLn2;
@@ -503,7 +508,7 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
 #pragma unroll
           for (int j = 0; j < VB; j += 4)
             *reinterpret_cast<float4*>(o_lds + (wave * a.rep + col) * OS + (4 * grp + i) * VB + j) =
-                make_float4(acc[j][i] * inv, acc[j + 1][i] * inv, acc[j + 2][i] * inv, acc[j + 3][i] * inv);
+                make_float4(acc[j][i] * inv * down, acc[j + 1][i] * inv * down, acc[j + 2][i] * inv * down, acc[j + 3][i] * inv * down);
         if (grp == 0) lse_lds[wave * 16 + col] = lse2;
       }
       __syncthreads();
