@@ -388,14 +388,17 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
             c[h] = 1.f;
           }
         }
-        float tmax = -INFINITY;
+        // ---- running maxima of the scores and of weight times scale, the latter from each group's own ----
+        float tmax = -INFINITY, atop = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) tmax = fmaxf(tmax, c[h] * fmaxf(fmaxf(s4[h][0], s4[h][1]), fmaxf(s4[h][2], s4[h][3])));
+        for (int h = 0; h < 2; ++h) {
+          const float t = c[h] * fmaxf(fmaxf(s4[h][0], s4[h][1]), fmaxf(s4[h][2], s4[h][3]));
+          tmax = fmaxf(tmax, t);
+          atop = fmaxf(atop, t + __builtin_amdgcn_logf(fmaxf(vs[h], kLeastVScale)));
+        }
         tmax = over_groups(tmax, [](float u, float v) { return fmaxf(u, v); });
-        // ---- running maxima of the scores and of weight times scale ----
-        const float m_new = fmaxf(m_run, tmax);
-        const float top = fmaxf(fmaxf(vs[0], vs[1]), kLeastVScale);
-        const float a_new = fmaxf(a_run, tmax + __builtin_amdgcn_logf(top));
+        atop = over_groups(atop, [](float u, float v) { return fmaxf(u, v); });
+        const float m_new = fmaxf(m_run, tmax), a_new = fmaxf(a_run, atop);
         l_run *= __builtin_amdgcn_exp2f(m_run - m_new);
         if (__any(a_new > a_run)) {
           const float f = __builtin_amdgcn_exp2f(a_run - a_new);
@@ -411,13 +414,12 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
         u32x4 ph, pl;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float fv = f * vs[h];
           float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s4[h][i], c[h], -m_new));
             l_run += p;
-            w[i] = p * fv;
+            w[i] = p * f * vs[h];  // f * vs alone may overflow
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {

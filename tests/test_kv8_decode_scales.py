@@ -110,3 +110,39 @@ def test_fresh_pool(gpu, tokens, fmt):
         assert torch.equal(torch.isneginf(lse), n.expand(2, 8) == 0)
         fin = torch.isfinite(want)
         assert (lse.double()[fin] - want[fin]).abs().max() <= 2.0 ** -16
+
+
+FAR = [  # log2 of the weight and of the V scale, of the tokens of even blocks and of odd ones
+    (25, -20, -35, 20),
+    (-35, 20, 25, -20),
+    (0, -100, -110, 100),  # the small weights carry the row
+    (-118, 100, 0, -100),  # so that 2^14 over their sum is past fp32 with their scale
+    (0, -100, -300, 60),   # and here they are nothing
+    (0, 0, -200, 120),
+    (0, -126, -60, 0),
+    (0, 60, 3, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("tokens", [32, 100, 3000])
+@pytest.mark.parametrize("far", FAR, ids=str)
+def test_neighbouring_blocks_of_very_different_scales(gpu, far, tokens, fmt):
+    # two blocks of one step: what a token weighs is its own softmax weight times its own scale
+    b, bs, d = 2, 16, 128
+    _, lens, codes, scales, tables, qt, q = inputs(53, b, 4, 1, d, bs, "bf16", fmt, tokens)
+    lens[0][:] = [tokens, tokens - 16]
+    one = 0x38 if fmt == "e4m3" else 1  # K rows of one value: a score is its sign times the scale
+    for e in range(tables[0].shape[1]):
+        s, v = far[2 * (e % 2): 2 * (e % 2) + 2]
+        codes[0, tables[0][:, e]] = one if s >= 0 else (one | 0x80 if fmt == "e4m3" else 0xff)
+        scales[0, tables[0][:, e]] = abs(s) * math.log(2.0) / math.sqrt(d)
+        scales[1, tables[0][:, e]] = 2.0 ** v
+    want, want_lse = reference(np.ones_like(q), codes, scales, fmt, tables, lens)
+    o, lse = decode(lens, codes, scales, fmt, tables, torch.ones_like(qt))
+    err = np.abs(o.double().cpu().numpy() - want).max(axis=(1, 2))
+    # |S| <= 300 ln 2 is rounded to 2^-24 of it by scale and product and by each of 128 sums at most:
+    # 2^-24 * 208 * (2 * 136) < 2^-8 at the very worst, 2^-12.4 with sqrt(136); against a row's own largest
+    assert (err <= np.abs(want).max(axis=(1, 2)) * 2.0 ** -12 + 2.0 ** -126).all(), err / np.abs(want).max(axis=(1, 2))
+    assert np.abs(lse.double().cpu().numpy() - want_lse).max() <= 2.0 ** -12
