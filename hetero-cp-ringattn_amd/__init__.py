@@ -908,6 +908,8 @@ def _decode_rows(q, pp, dev, o, lse, o_dtype, stream):
     if lse is None:
         lse = _empty((b, hq), torch.float32, q.device, stream)
     _rows_of("o", o, shape, dev, o_dtype)
+    if o.stride(2) != 1 and d > 1:
+        raise ValueError("the output must have contiguous rows")
     _want("lse", lse, torch.float32, (b, hq), dev)
     return o, lse
 

@@ -620,3 +620,14 @@ def test_decode_workspace_covers_every_shorter_context(heads, batch):
         rings.append(H.lib().hcp_kv8_decode_ring_workspace_size(ctypes.byref(desc), ctypes.byref(pool), 3, shards))
     for s in (sizes, rings):
         assert all(a <= b for a, b in zip(s, s[1:])), (batch, heads)
+
+
+def test_decode_ring_refuses_an_out_of_strided_rows():
+    # strides of rows and heads that fit each other, but two elements from one dim to the next
+    pool, sc = H.kv8_pool(4, 16, 2, 64, device="cpu")
+    q, table = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 2, dtype=torch.int32)
+    for out in (torch.zeros(3, 4, 64, 2, dtype=q.dtype)[..., 0], torch.zeros(3, 64, 4, dtype=q.dtype).transpose(1, 2)):
+        with pytest.raises(ValueError, match="contiguous rows"):
+            H.kv8_decode_ring_replay(q, pool, sc, [(table, None, 20)], 0, out=out)
+    with pytest.raises(ValueError, match="GPU"):  # a wider row's slice is taken
+        H.kv8_decode_ring_replay(q, pool, sc, [(table, None, 20)], 0, out=torch.zeros(3, 4, 72, dtype=q.dtype)[..., :64])
