@@ -182,10 +182,15 @@ __device__ __forceinline__ void plan_blocks(const KvPlan& p, const PlanSums& s, 
     for (int32_t i = from; i < min(q.need, to); i += step)
       row[used + i] = stack_block(p, s, s.head.top - 1 - (static_cast<int64_t>(q.first) + i));
   } else if (q.state == kEnded) {
+    uint32_t most = 0;  // a negative id is past every block, too
     for (int32_t i = from; i < min(q.need, to); i += step) {
       const int64_t at = static_cast<int64_t>(s.head.count) + q.first + i;
-      if (at < s.head.left) p.free_blocks[at] = row[i];
+      if (at >= s.head.left) continue;  // taken again in this step, and looked at by its token
+      const int32_t blk = row[i];
+      most = max(most, static_cast<uint32_t>(blk));
+      p.free_blocks[at] = blk;
     }
+    if (most >= p.num_blocks) atomicOr(p.err, 1);
   }
 }
 

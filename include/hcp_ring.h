@@ -709,8 +709,8 @@ int hcp_block_wire_bytes(const hcp_block_agent* agent, uint64_t* sent, uint64_t*
  * height and below the new one.  Nothing else of the two is touched.
  * A negative length, one beyond its table, a free_count outside [0, num_blocks] or more
  * blocks than free_blocks holds set device error bit 3 (such a sequence is not served, what
- * does not fit the stack is dropped); a table or stack entry outside [0, num_blocks) sets
- * bit 0 and its tokens get slot -1.  All arrays are DEVICE memory; nothing is read on the
+ * does not fit the stack is dropped); a table or stack entry outside [0, num_blocks) that
+ * receives a token or is given back sets bit 0, and its tokens get slot -1.  All arrays are DEVICE memory; nothing is read on the
  * host, so a captured graph follows the lengths.  No two sequences may hold a block in
  * common.  Workspace: hcp_kv_plan_workspace_size(batch) bytes, 256-byte aligned.
  * ------------------------------------------------------------------------------- */

@@ -261,3 +261,29 @@ def test_plan_python_refusals():
         H.kv_plan_step(z(2), z(2), z((3, 2)).t(), z(8), z(1), 16, 4)
     with pytest.raises(ValueError, match="GPU"):
         H.kv_plan_step(z(2), z(2), z((2, 3)), z(8), z(1), 16, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [3, 1100])
+@pytest.mark.parametrize("bad", [-1, 40, 1 << 30])
+def test_plan_flags_a_bad_entry_that_an_ended_sequence_gives_back(gpu, batch, bad):
+    # one of many blocks that go on the stack, first, second or far along a row; taken again at once, too
+    for at in (0, 1, 7):
+        lens, new = np.zeros(batch, np.int64), np.zeros(batch, np.int64)
+        tables = np.full((batch, 10), -1)
+        tables[1] = np.arange(10, 20)
+        lens[1], new[1] = 150, -1
+        tables[1, at] = bad
+        args = (lens, new, tables, np.concatenate([np.arange(10), np.full(30, -1)]), 10)
+        H.fetch_device_errors()
+        got = call(*args, 16, 1)
+        assert H.fetch_device_errors() == 1
+        for name, g, w in zip(NAMES, got, plan_reference(*args, 16, 1)):
+            assert np.array_equal(g, w), name
+        tables[1, at] = 10 + at
+        call(*args[:2], tables, *args[3:], 16, 1)
+        assert H.fetch_device_errors() == 0
+    lens[2], new[2] = 0, 16 * 3  # takes the stack's top: places 9, 8 and 7 of the ended row
+    tables[1, 8] = bad
+    got = call(lens, new, tables, *args[3:], 16, 48)
+    assert H.fetch_device_errors() == 1 and (got[0][16:32] == -1).all() and (got[0][:16] >= 0).all()
