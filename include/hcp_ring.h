@@ -742,7 +742,9 @@ int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, cons
  * scale becomes the least power of two (2^-100 at least) under which the run's largest
  * magnitude fits the format, or stays if it is larger and rows are held (a run from place 0
  * starts the block anew); where it grows the held codes are rounded to it.  New codes are
- * the nearest to x / scale, ties to even.  A run with a value that is not finite makes the
+ * the nearest to x / scale, ties to even; under a held scale that is no power of two (from
+ * elsewhere: append writes none) the nearest to x / scale as fp32 has it within 2^-23, new and
+ * held ones alike.  A run with a value that is not finite makes the
  * scale NaN, and with it all that the block and head stand for, until it is started anew.
  * A block takes one run per call: of two, what the block and its scale hold is undefined.
  *

@@ -323,3 +323,66 @@ def test_python_refusals():
         H.kv8_gather(pool, sc, torch.zeros(2, dtype=torch.int32), 0, 0, 20, k_out=torch.zeros(2, 19, 64))
     with pytest.raises(ValueError):
         H.kv8_ring_attention_replay_paged(torch.zeros(4, 20, 64), pool, sc, torch.zeros(2, dtype=torch.int32), [10, 9])
+
+
+def _ties(fmt):
+    """Values halfway between two codes, and the codes' own values (positive, above the smallest)."""
+    v = R.E4M3[8:127] if fmt == "e4m3" else np.arange(1.0, 128.0)
+    return (v[:-1] + v[1:]) / 2, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_append_to_blocks_of_any_scale(gpu, dtype, fmt):
+    # held rows under scales that are no powers of two (quantised elsewhere): one token and three.
+    # Values on and next to a tie of x / scale, where the scale stays; held codes next to a tie of
+    # code * old / new, where it grows.  A code is the nearest to an fp32 product that two roundings
+    # (1 / scale and the product) leave within 2 * 2^-24 (1 + 2^-24) of x / scale: where that lies
+    # next to a tie the code may be the one across it, else it is equal
+    r = np.random.default_rng(14)
+    bs, heads, d, nb = 16, 64, 64, 4
+    ties, own = _ties(fmt)
+    slots = np.array([9, bs + 5, bs + 6, bs + 7, 2 * bs + 1, 3 * bs + 3, 3 * bs + 4])
+    for case in ("some grow", "grow", "stay"):
+        grow = case == "grow"
+        if case == "stay":  # at most half of the format's range: the least power of two is not past the scale
+            ties = ties[ties < R.LARGEST[fmt] / 2]
+        codes, scales = R.random_cache(r, nb, bs, heads, d, fmt)
+        scales[:] = np.float32(r.uniform(0.5, 1.0, scales.shape) * 2.0 ** r.integers(-6, 3, scales.shape))
+        if grow:  # scale = tie / code: the code times it is a tie, but for the scale's own rounding
+            c = r.integers(0, len(own), scales.shape)
+            t = r.integers(0, len(ties), scales.shape)
+            down = 2.0 ** np.ceil(np.log2(ties[t] / own[c]))
+            scales[:] = np.float32(ties[t] / down / own[c])  # in (1/2, 1]
+            one = R.encode(own[c].ravel(), fmt).reshape(c.shape)
+            codes[..., ::3] = one[:, :, None, :, None]
+        rows = []
+        for plane in range(2):
+            x = np.empty((heads, len(slots), d), np.float32)
+            for i, s in enumerate(slots):
+                size = scales[plane, s // bs][:, None].astype(np.float64)
+                near = np.float32(r.choice(ties, (heads, d)) * size) * r.choice([-1, 1], (heads, d))
+                x[:, i] = near * np.float32(0.9) if r.random() < 0.2 else near
+                if grow:
+                    x[:, i, 0] = R.LARGEST[fmt]  # the scale becomes 1 where it was not more
+                    x[:, i, 1:] = np.clip(x[:, i, 1:], -R.LARGEST[fmt], R.LARGEST[fmt])
+            rows.append(torch.from_numpy(x).to(DT[dtype]))
+        pool, sc = R.to_device(codes, scales, fmt)
+        held, old = R.values(codes, fmt), scales.astype(np.float64)
+        H.kv8_append(pool, sc, rows[0].cuda(), rows[1].cuda(), torch.from_numpy(slots).cuda())
+        before = scales.copy()
+        R.append(codes, scales, rows[0].double().numpy(), rows[1].double().numpy(), slots, fmt)
+        assert case != "stay" or np.array_equal(scales, before)
+        got_codes, got_scales = R.to_host(pool, sc)
+        assert np.array_equal(got_scales, scales)
+        got, want = R.values(got_codes, fmt), R.values(codes, fmt)
+        exact = held * (old / scales)[:, :, None, :, None]
+        for plane in range(2):
+            at = exact[plane].reshape(nb * bs, heads, d)
+            at[slots] = rows[plane].double().numpy().transpose(1, 0, 2) / scales[plane].astype(np.float64)[slots // bs][:, :, None]
+        # y within e of the value v, `got` the nearest code to y: |got - v| <= |got - y| + e <= |want - y| + e <= |want - v| + 2 e
+        off = np.abs(got - exact) - np.abs(want - exact)
+        assert (off <= 2 * np.abs(exact) * 2.0 ** -23 * (1 + 2.0 ** -20)).all(), off.max()
+        whole = (np.log2(scales) % 1 == 0) & (np.log2(old) % 1 == 0)
+        assert np.array_equal(got[whole[:, :, None, :].repeat(bs, 2)], want[whole[:, :, None, :].repeat(bs, 2)])
