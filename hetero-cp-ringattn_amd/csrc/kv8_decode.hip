@@ -140,8 +140,6 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int sub = wave / a.heads;
   const int kvh = blockIdx.z * a.heads + wave - sub * a.heads;
-  const bool idle = kvh >= a.hkv;
-  if (idle && a.subs == 1) return;  // no workgroup barrier below
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   int b = blockIdx.y;
 
@@ -217,7 +215,7 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
 
   for (;;) {  // one sequence's share
     const int run_len = (end_all - begin + 2 * a.subs - 1) / (2 * a.subs) * 2;  // whole steps
-    const int g0 = idle ? total : min(begin + sub * run_len, total);
+    const int g0 = min(begin + sub * run_len, total);
     const int g1 = min(min(g0 + run_len, end_all), total);
 
     // Q^T in f16, times a power of two that brings the row's largest value to 2^14 .. 2^15.
@@ -231,7 +229,7 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
       for (int s = 0; s < KS; ++s) {
         const int d0 = grp * 16 + 64 * (s / 2) + 8 * (s % 2);
         u32x4 v = {0, 0, 0, 0};
-        if (!idle && col < a.rep && (!PAD || d0 < dn))
+        if (col < a.rep && (!PAD || d0 < dn))
           v = *reinterpret_cast<const u32x4*>(a.q + b * a.q_bs + (kvh * a.rep + col) * a.q_hs + d0);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -515,7 +513,7 @@ __global__ __launch_bounds__(64 * kv8_waves(PAD)) void kv8_decode_kernel(Kv8Deco
       }
       __syncthreads();
       const int w0 = wave - sub * a.heads;
-      for (int c = idle ? a.rep : sub; c < a.rep; c += a.subs) {
+      for (int c = sub; c < a.rep; c += a.subs) {
         float m = -INFINITY;
         for (int i = 0; i < a.subs; ++i) m = fmaxf(m, lse_lds[(w0 + i * a.heads) * 16 + c]);
         const float ref = m == -INFINITY ? 0.f : m;  // no finite one: 0, or NaN with a NaN one
@@ -695,6 +693,7 @@ void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const 
   for (int i = 0; i < n; ++i) require(spans[i].t0 >= 0 && spans[i].t0 < pool.bs, "kv8_decode: a span starts in its first block");
   require(span_groups(n, spans) <= INT32_MAX / 4, "kv8_decode: too many tokens");  // a sequence's groups are counted in 32 bits
   const Kv8Plan p = plan_kv8(batch, hq, hkv, d, n, spans);
+  require(hkv % p.heads == 0, "kv8_decode: a workgroup's heads divide the kv heads");
   Kv8DecodeArgs a;
   a.ws_o = a.ws_lse = nullptr;
   a.range = nullptr;
@@ -739,7 +738,7 @@ void launch_kv8_decode(const Kv8Pool& pool, int dtype, int batch, int hq, const 
   a.lse = lse;
   a.batch = batch;
   a.err = err;
-  const dim3 grid(std::max(p.workers, 1), p.workers > 0 ? 1 : batch, static_cast<unsigned>(ceil_div(hkv, p.heads)));
+  const dim3 grid(std::max(p.workers, 1), p.workers > 0 ? 1 : batch, static_cast<unsigned>(hkv / p.heads));
   // head dim 64: its own kernel; other multiples of 8 up to 128: 128 with the dims past it zero
   if (pool.format == kE4M3) {
     if (d == 128) launch_kv8_typed<kE4M3, 128, false>(a, grid, stream);
