@@ -752,9 +752,10 @@ int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, cons
  * hcp_decode_ring_replay, straight over the codes (desc->dtype: the type of q and of the
  * ring's out; the same limits on head_dim, heads and block_size).  Products of codes and q
  * are exact, softmax weights carry 22 bits beside their scales (one below 2^-126 of its row's
- * largest is 0), sums and statistics 32.  Scales may be any finite values >= 0; o must be
- * 16-byte aligned.  Workspaces are 256-byte aligned and cover
- * every shorter context of the same batch and heads.
+ * largest is 0), sums and statistics 32.  Scales may be any finite values >= 0 that
+ * leave scores within 2^24 of 0 (past that fp32 scores are steps of 2 apart, and weights
+ * undefined); o must be 16-byte aligned.  Workspaces are 256-byte aligned and cover every
+ * shorter context of the same batch and heads.
  * hcp_kv8_gather: as hcp_paged_kv_gather, out = scale * code rounded to dtype.
  * hcp_kv8_prefill_replay_paged: as hcp_ring_prefill_replay_paged, K/V staged that way
  * (workspace: hcp_ring_replay_workspace_size(desc, 1)).

@@ -146,3 +146,30 @@ def test_neighbouring_blocks_of_very_different_scales(gpu, far, tokens, fmt):
     # 2^-24 * 208 * (2 * 136) < 2^-8 at the very worst, 2^-12.4 with sqrt(136); against a row's own largest
     assert (err <= np.abs(want).max(axis=(1, 2)) * 2.0 ** -12 + 2.0 ** -126).all(), err / np.abs(want).max(axis=(1, 2))
     assert np.abs(lse.double().cpu().numpy() - want_lse).max() <= 2.0 ** -12
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("split", SPLITS)
+def test_scores_of_the_largest_size(gpu, split, sign, fmt):
+    # K scales of 2^20 and scores all negative or all positive, to 2^23.5: one token of each sequence has all the weight
+    r, lens, codes, scales, tables, qt, q = setup(54, split, 16, fmt)
+    scales[0] = 2.0 ** 20
+    one = (0x38 if sign > 0 else 0xb8) if fmt == "e4m3" else (1 if sign > 0 else 0xff)
+    codes[0] = one if sign < 0 else 0  # a score is the scale times sum(code) / sqrt(D)
+    b, hq, hkv, d, tokens = SPLITS[split]
+    for i in range(b):
+        if lens[0][i]:
+            best = int(r.integers(lens[0][i]))
+            codes[0, tables[0][i, best // 16], best % 16, :, ::2] = one if sign > 0 else 0
+    want, want_lse = reference(np.ones_like(q), codes, scales, fmt, tables, lens)
+    o, lse = decode(lens, codes, scales, fmt, tables, torch.ones_like(qt))
+    err = np.abs(o.double().cpu().numpy() - want).max()
+    assert err <= tolerance(R.LARGEST[fmt] * scales[1].max(), torch.float32)
+    got = lse.double().cpu().numpy()
+    assert np.array_equal(np.isneginf(got), np.isneginf(want_lse))
+    fin = np.isfinite(want_lse)
+    # whole products and sums; scale, its log2 e, ln 2 and the products with them round, and the largest score
+    # against its own fp32 maximum: 8 roundings
+    assert (np.abs(got - want_lse)[fin] <= np.abs(want_lse[fin]) * 8 * 2.0 ** -24).all()
