@@ -1793,7 +1793,7 @@ int hcp_kv_plan_step(int32_t batch, int32_t block_size, int64_t num_blocks, cons
     require(batch > 0, "batch must be positive");
     require(block_size > 0, "block_size must be positive");
     require(num_blocks > 0 && num_blocks <= INT32_MAX, "num_blocks must be in [1, 2^31)");
-    require(capacity >= 0 && capacity <= INT32_MAX, "capacity must be in [0, 2^31)");
+    require(capacity >= 0 && capacity < INT32_MAX, "capacity must be in [0, 2^31 - 1)");  // token sums stop at 2^31 - 1
     require(table_len >= 1 && table_stride >= table_len, "bad table shape");
     require(seq_lens != nullptr && new_lens != nullptr && block_tables != nullptr && free_blocks != nullptr &&
                 free_count != nullptr && token_starts != nullptr && seq_lens_out != nullptr && free_count_out != nullptr,

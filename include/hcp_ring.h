@@ -700,7 +700,8 @@ int hcp_block_wire_bytes(const hcp_block_agent* agent, uint64_t* sent, uint64_t*
  *      or the needs up to and including it fit the stack.  One that is not served keeps its
  *      length and its row.
  * Written: token_starts [batch + 1] (token i of the step belongs to the b with
- * token_starts[b] <= i < token_starts[b + 1], served or not); for i < capacity slots[i] =
+ * token_starts[b] <= i < token_starts[b + 1], served or not; sums stop at 2^31 - 1, and
+ * capacity has to be less); for i < capacity slots[i] =
  * block * block_size + (position mod block_size), -1 for a token that was not served and
  * from token_starts[batch] on; positions[i] = the token's position in its sequence (0 from
  * token_starts[batch] on); seq_lens_out [batch] (0 for an ended sequence) and

@@ -287,3 +287,29 @@ def test_plan_flags_a_bad_entry_that_an_ended_sequence_gives_back(gpu, batch, ba
     tables[1, 8] = bad
     got = call(lens, new, tables, *args[3:], 16, 48)
     assert H.fetch_device_errors() == 1 and (got[0][16:32] == -1).all() and (got[0][:16] >= 0).all()
+
+
+def test_plan_refuses_a_capacity_that_sums_stop_at():
+    # token offsets are whole numbers of 32 bits that stop at 2^31 - 1: of a list that long none would be past the end
+    p = 256
+    args = lambda cap: (2, 16, 8, p, p, p, 4, 4, p, p, cap, p, p, p, p, p, p, 10, None)  # noqa: E731
+    assert H.lib().hcp_kv_plan_step(*args((1 << 31) - 1)) == -6 and "capacity" in H.last_error()
+    assert H.lib().hcp_kv_plan_step(*args((1 << 31) - 2)) == -6 and "workspace" in H.last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [3, 1100])
+def test_plan_of_more_tokens_than_32_bits_hold(gpu, batch):
+    # lengths whose sum passes 2^31 and 2^32: who lies past the capacity is not served, the others are
+    lens, new = np.zeros(batch, np.int64), np.zeros(batch, np.int64)
+    tables = np.full((batch, 4), -1)
+    new[:3] = [20, (1 << 31) - 1, 1]
+    if batch > 3:
+        new[3:6] = (1 << 31) - 1
+        new[batch - 1] = 1
+    out = call(lens, new, tables, np.arange(10), 10, 16, 100)
+    slots, pos, starts, out_lens, left, got_tables, _ = out
+    assert slots[:20].tolist() == [9 * 16 + i for i in range(16)] + [8 * 16 + i for i in range(4)]
+    assert (slots[20:] == -1).all() and pos[20:].tolist() == list(range(80))
+    assert out_lens[0] == 20 and not out_lens[1:].any() and left == 8 and (got_tables[1:] == -1).all()
+    assert starts.tolist() == np.minimum(np.concatenate([[0], np.cumsum(new)]), (1 << 31) - 1).tolist()
