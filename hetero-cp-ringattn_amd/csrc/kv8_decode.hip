@@ -24,16 +24,17 @@
 //     permutes.  O^T stays in the lane whose query it is: max, rescale and sum need two
 //     cross-lane steps each and no broadcast.
 //   * Weights w = p s_V 2^(14 + m - a) with `a` the running maximum of log2(p s_V), which is
-//     tracked like m: w <= 2^14 whatever the scales, and split into two f16 of 11 bits each, w
-//     = hi + lo, so P carries 22 bits (one f16 alone would put 2^-12 on every weight, against
-//     the fp32 weights of the 16-bit decode).  Sums and statistics are fp32.
+//     tracked like m, over each 16-token group's own scores and scale: w <= 2^14 whatever the
+//     scales, and split into two f16 of 11 bits each, w = hi + lo, so P carries 22 bits (one f16
+//     alone would put 2^-12 on every weight, against the fp32 weights of the 16-bit decode).
+//     Sums and statistics are fp32.
 //
 // Measured, 32/8 heads of 128, e4m3, blocks of 16: 64 sequences of 8-16k tokens 267 us (1.63 GB at
 // 6.1 TB/s, each byte fetched once; the 16-bit decode of 64 x 16k 635 us for 4.3 GB), 6 x 2085 of
-// 16/2 heads 12.4 us, one sequence of 130 tokens 6.7 us.  What bounds the short ones is the chain of
+// 16/2 heads 12.0 us, one sequence of 130 tokens 6.6 us.  What bounds the short ones is the chain of
 // lengths, table, q and codes, one latency each (2.5-4 us), then 0.95 us a step of a lone wave, whose
 // instructions no other wave hides.  Two steps of codes under way instead of one cost more in
-// registers and instructions than they hid (64 sequences 270 us, one of 130 tokens 8.3).
+// registers and instructions than they hid (64 sequences 263 -> 270 us, one of 130 tokens 6.6 -> 8.3).
 #include <algorithm>
 #include <type_traits>
 
@@ -624,19 +625,19 @@ static int64_t lone_workers(int batch, int hkv, int64_t steps) {
   return batch * steps * hkv <= 8 * cus ? batch * steps : std::max<int64_t>(4 * cus / hkv, 1);
 }
 
-// Direct or balanced, by modelled time (us, fitted on MI355X to 31 calls: 1-300 sequences of
-// 130-100000 tokens, 8, 2 and 1 kv heads of 128, 64 and 96 dims; within 10% of the fastest of 13
-// splits where the two are apart):
+// Direct or balanced, by modelled time (us, fitted on MI355X).  Over 38 calls (1-2000 sequences of
+// 64-100000 tokens, 1 to 12 kv heads of 128, 64 and 96 dims) what it takes is 1.4% in the mean behind
+// the fastest of up to 75 splits tried, 16% at most (one sequence of 32000 tokens, 16/2 heads, below):
 //   direct:   6 + the longest sequence's steps over four waves, 0.95 each, times the workgroups a
 //             CU has, or the bytes at 6 TB/s -- of sequences as long as the longest, as long as a
 //             CU has no more than two; past that the lengths even out.
 //   balanced: 11 (the join is a launch of its own) + its waves' steps, or three quarters of those
 //             bytes (lengths between half the longest and the longest, as a serving batch's), +
 //             2.5 for every sequence that a worker meets.
-// e.g. 4 x 700 tokens, 32/8 heads: 10.1 direct, 10.7 balanced; 64 x 1000: 26.3 / 29.3; 64 x 2000:
-// 51.0 / 44.9; 64 x 16384: 363 / 267; 6 x 2085, 16/2 heads: 18.3 / 12.0; 200 x 500, 14/2 heads of 64
-// dims: 10.3 / 21.0.  A direct workgroup is one kv head and four waves, one a SIMD: eight take as
-// long (4 x 700: 10.7), two longer (14.0).
+// e.g. 4 x 700 tokens, 32/8 heads: 9.9 direct, 10.7 balanced; 64 x 1000: 26.3 / 29.1; 64 x 2000:
+// 50.0 / 45.2; 64 x 16384: 362 / 267; 6 x 2085, 16/2 heads: 19.2 / 12.0; 200 x 500, 14/2 heads of 64
+// dims: 10.1 / 21.0.  A direct workgroup is one kv head and four waves, one a SIMD: eight take as
+// long (4 x 700: 10.3), two longer (14.4).
 static Kv8Plan plan_kv8(int batch, int hq, int hkv, int d, int n, const DecodeSpan* spans) {
   const int64_t groups = span_groups(n, spans), steps = ceil_div(groups, 2);
   const int most = kv8_waves(d != 128 && d != 64);
@@ -651,12 +652,13 @@ static Kv8Plan plan_kv8(int batch, int hq, int hkv, int d, int n, const DecodeSp
   const double t_balanced = 11.0 + std::max(0.75 * bytes, 0.95 * run) + (run > 1.0 ? 2.5 * (1.0 + static_cast<double>(batch) / lone) : 0.0);
   if (t_direct <= t_balanced) return direct;
   // Up to 100 places a sequence and head for the join, 200 where runs are long: else waves of a
-  // workgroup meet first, four at least (one sequence of 4096 tokens, 32/8 heads: 11.6 us as 32
-  // workers of four waves a head, 12.5 as 128 lone ones, 13.4 as 64 of two; of 100000: 46.8, 44.7;
-  // of 32000, 16/2 heads: 15.3 as four, 17.2 as 16).
+  // workgroup meet first, four at least (one sequence of 4096 tokens, 32/8 heads: 11.3 us as 32
+  // workers of four waves a head, 13.3 as 128 lone ones or as 64 of two; of 100000: 53.3 as 32 of
+  // four, 44.4 lone).  Where the rule loses: 32000 tokens, 16/2 heads, 17.4 us as 63 workers of 16
+  // waves, 15.1 as 128 of four; it is as fast at 16000 (13.6, 14.2).
   // Lone waves of four heads share a workgroup (1% faster, they read whole rows), never those of
   // two: workgroups of two waves leave half of the SIMDs without one (64 x 16384 tokens, 14/2
-  // heads of 64 dims: 62.8 us, single waves 52.7).
+  // heads of 64 dims: 63.4 us, single waves 52.5).
   int subs = 1;
   const int64_t places = (run < 16.0 ? 100 : 200) * static_cast<int64_t>(batch);
   if (lone > places)
