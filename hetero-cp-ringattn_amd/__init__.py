@@ -16,6 +16,8 @@ The operator names mirror the reference's ring-attention backend
 * :func:`kv8_append` / :func:`kv8_decode_partial` / :func:`kv8_decode_ring_replay` /
   :func:`kv8_gather` / :func:`kv8_ring_attention_replay_paged`  a paged K/V cache in 8 bits
   with a scale per block and head -> ``hcp_kv8_*`` (no reference counterpart)
+* :func:`qk_norm_rope` / :func:`qk_norm_rope_append`  norms of q and k heads with the rotation,
+  dense or into the paged cache -> ``hcp_qk_norm_rope*`` (no reference counterpart)
 * :func:`ring_attention_replay`             ring.rs:861-1398 for every domain on one GPU ->
   ``hcp_ring_prefill_replay`` (``_paged`` variant stages K/V from a block pool)
 
@@ -303,6 +305,9 @@ def lib() -> ctypes.CDLL:
                                        ctypes.c_int),
         "hcp_kv8_prefill_replay_paged": ([ctypes.POINTER(ReplayDesc), View, ctypes.POINTER(PagedPool), vp, i32, vp,
                                           i64, View, vp, vp, ctypes.c_size_t, vp], ctypes.c_int),
+        "hcp_qk_norm_rope": ([ctypes.POINTER(QkvDesc), i32, f32, View, View, vp, vp, vp, vp, View, View, vp], ctypes.c_int),
+        "hcp_qk_norm_rope_append": ([ctypes.POINTER(QkvDesc), i32, f32, View, View, View, vp, vp, vp, vp, View,
+                                     ctypes.POINTER(PagedPool), vp, vp], ctypes.c_int),
         "hcp_ring_trace_attach": ([vp, ctypes.c_size_t], ctypes.c_int),
         "hcp_ring_trace_record_bytes": ([ctypes.POINTER(ReplayDesc)], ctypes.c_size_t),
         "hcp_ring_trace_read": ([vp, ctypes.POINTER(TraceDomain), i32, ctypes.POINTER(i32),
@@ -984,6 +989,67 @@ def kv8_ring_attention_replay_paged(q, pool, scales, block_table, chunks, causal
             scales.data_ptr(), fmt, block_table.data_ptr(), n, view(out), lse_out.data_ptr(), ws, ws_bytes)
     del arr
     return out, lse_out
+
+
+# ---------------------------------------------------------------------------------
+# (11) norms of q and k with the rotation
+# ---------------------------------------------------------------------------------
+def _qk_norm(q, k, q_weight, k_weight, positions, table, eps, pairs, q_out, stream):
+    """(GPU, q_out, arguments up to k, arguments from the weights to q_out), the tensors checked."""
+    torch = _torch()
+    dev = q.get_device()
+    hq, tokens, d = q.shape
+    hkv = k.shape[0]
+    _rows_of("k", k, (hkv, tokens, d), dev, q.dtype)
+    if q_out is None:
+        q_out = _empty((hq, tokens, d), q.dtype, q.device, stream)
+    else:
+        _rows_of("q_out", q_out, (hq, tokens, d), dev, q.dtype)
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _want(name, w, q.dtype, (d,), dev)
+    rows = rot = 0
+    if table is not None:
+        if table.dim() != 3 or table.shape[0] != 2 or positions is None:
+            raise ValueError("the rotation needs positions and a table [2, rows, rope_dims / 2]")
+        rows, rot = table.shape[1], 2 * table.shape[2]
+        _want("table", table, torch.float32, (2, rows, rot // 2), dev)
+        _want("positions", positions, torch.int64, (tokens,), dev)
+    desc = QkvDesc(dtype_code(q.dtype), 0, hq, hkv, d, (2 if pairs else 1) if rot else 0, tokens, rows)
+    args = (ctypes.byref(desc), rot, eps, view(q), view(k))
+    more = (None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+            positions.data_ptr() if rot else None, table.data_ptr() if rot else None, view(q_out))
+    return dev, q_out, args, more
+
+
+def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, table=None, eps=1e-6, pairs=False, q_out=None,
+                 k_out=None, stream=None):
+    """q [Hq, T, D] and k [Hkv, T, D] normed row by row (x / sqrt(mean(x^2) + eps) * weight) and
+    turned at ``positions`` [T] int64 by the ``table`` of :func:`rope_table` (its rope_dims may be
+    less than D; None: no rotation; ``pairs``: planes of neighbouring dims instead of halves)
+    -> (q_out, k_out), which may be q and k themselves."""
+    dev, q_out, args, more = _qk_norm(q, k, q_weight, k_weight, positions, table, eps, pairs, q_out, stream)
+    if k_out is None:
+        k_out = _empty(k.shape, k.dtype, k.device, stream)
+    else:
+        _rows_of("k_out", k_out, k.shape, dev, k.dtype)
+    _launch(lib().hcp_qk_norm_rope, dev, stream, *args, *more, view(k_out))
+    return q_out, k_out
+
+
+def qk_norm_rope_append(q, k, v, q_weight, k_weight, pool, slots, positions=None, table=None, eps=1e-6, pairs=False,
+                        q_out=None, stream=None):
+    """As :func:`qk_norm_rope`, with the K rows and v [Hkv, T, D] as it is appended to the paged
+    ``pool`` [2, num_blocks, block_size, Hkv, D] at ``slots`` [T] int64 (:func:`kv_plan_step`;
+    negative: skipped) -> q_out."""
+    dev, q_out, args, more = _qk_norm(q, k, q_weight, k_weight, positions, table, eps, pairs, q_out, stream)
+    pp = paged_pool(pool)
+    _rows_of("v", v, k.shape, dev, k.dtype)
+    if pool.dtype != q.dtype or pool.get_device() != dev:
+        raise ValueError(f"pool must be {q.dtype} on {_place(dev)}")
+    _want("slots", slots, _torch().int64, (q.shape[1],), dev)
+    _launch(lib().hcp_qk_norm_rope_append, dev, stream, *args, view(v), *more, ctypes.byref(pp), slots.data_ptr())
+    return q_out
 
 
 # ---------------------------------------------------------------------------------

@@ -7,6 +7,7 @@
 // counterpart of HcpRingAttentionBackend::ring_attention, ring.rs:861-1398) lives here
 // too; it only enqueues kernels.
 #include <algorithm>
+#include <cfloat>
 #include <chrono>
 #include <cstdio>
 #include <cstdlib>
@@ -1983,6 +1984,88 @@ int hcp_kv8_prefill_replay_paged(const hcp_ring_replay_desc* desc, hcp_ring_view
     hcp_ring_view none{nullptr, 0, 1};
     run_replay(desc, q, none, none, pool, block_table, table_len, out, lse_out, workspace, workspace_bytes,
                as_stream(stream), &c);
+  });
+}
+
+// ---- (11) norms of q and k with the rotation ----
+}  // extern "C": internal helpers below have C++ linkage
+namespace {
+QkNorm make_qk_norm(const hcp_qkv_desc* d, int32_t rope_dims, float eps, const hcp_ring_view& q, const hcp_ring_view& k,
+                    const void* q_weight, const void* k_weight, const int64_t* positions, const float* table,
+                    const hcp_ring_view& q_out) {
+  require(d != nullptr, "null descriptor");
+  const int es = elem_size(d->dtype);
+  require(d->num_q_heads > 0 && d->num_kv_heads > 0, "head counts must be positive");
+  require(static_cast<int64_t>(d->num_q_heads) + 2 * static_cast<int64_t>(d->num_kv_heads) <= (1 << 20), "too many heads");
+  require(d->head_dim > 0 && d->head_dim <= 256 && d->head_dim % 8 == 0, "head_dim must be a multiple of 8 up to 256");
+  require(d->rope >= 0 && d->rope <= 2, "rope must be 0, 1 (halves) or 2 (pairs)");
+  const int32_t rot = d->rope != 0 ? rope_dims : 0;
+  if (d->rope != 0)
+    require(rot > 0 && rot <= d->head_dim && rot % 8 == 0, "rope_dims must be a multiple of 8 up to head_dim");
+  require(d->tokens >= 0 && d->tokens <= INT32_MAX, "tokens must be in [0, 2^31)");
+  require(eps > 0.f && eps <= FLT_MAX, "eps must be positive and finite");
+  QkNorm a{};
+  a.tokens = d->tokens;
+  if (a.tokens == 0) return a;
+  check_rows(q, "q", d->tokens, d->dtype);
+  check_rows(k, "k", d->tokens, d->dtype);
+  check_rows(q_out, "q_out", d->tokens, d->dtype);
+  for (const void* w : {q_weight, k_weight}) require(aligned(w, es), "weights must be aligned to their elements");
+  if (rot > 0)
+    require(positions != nullptr && table != nullptr && d->rope_rows > 0, "the rotation needs positions and a table");
+  require(aligned(positions, 8) && aligned(table, 4), "positions or table not aligned to their elements");
+  a.src[0] = q.data; a.src[1] = k.data;
+  a.hs[0] = q.head_stride; a.hs[1] = k.head_stride;
+  a.ss[0] = q.seq_stride; a.ss[1] = k.seq_stride;
+  a.w[0] = q_weight; a.w[1] = k_weight;
+  a.pos = positions;
+  a.rope_cos = table;
+  a.rope_sin = rot > 0 ? table + d->rope_rows * (rot / 2) : nullptr;
+  a.rope_rows = d->rope_rows;
+  a.hq = d->num_q_heads; a.hkv = d->num_kv_heads; a.d = d->head_dim; a.rot = rot;
+  a.eps = eps;
+  a.inv_d = 1.f / static_cast<float>(d->head_dim);
+  a.out[0] = q_out.data; a.out_hs[0] = q_out.head_stride; a.out_ss[0] = q_out.seq_stride;
+  return a;
+}
+}  // namespace
+extern "C" {
+
+int hcp_qk_norm_rope(const hcp_qkv_desc* desc, int32_t rope_dims, float eps, hcp_ring_view q, hcp_ring_view k,
+                     const void* q_weight, const void* k_weight, const int64_t* positions, const float* rope_table,
+                     hcp_ring_view q_out, hcp_ring_view k_out, void* stream) {
+  return guarded(__func__, [&] {
+    QkNorm a = make_qk_norm(desc, rope_dims, eps, q, k, q_weight, k_weight, positions, rope_table, q_out);
+    if (a.tokens == 0) return;
+    check_rows(k_out, "k_out", desc->tokens, desc->dtype);
+    a.out[1] = k_out.data; a.out_hs[1] = k_out.head_stride; a.out_ss[1] = k_out.seq_stride;
+    a.err = device_error_flags();
+    launch_qk_norm(desc->dtype, desc->rope == 2, a, as_stream(stream));
+  });
+}
+
+int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float eps, hcp_ring_view q, hcp_ring_view k,
+                            hcp_ring_view v, const void* q_weight, const void* k_weight, const int64_t* positions,
+                            const float* rope_table, hcp_ring_view q_out, const hcp_paged_pool* pool, const int64_t* slots,
+                            void* stream) {
+  return guarded(__func__, [&] {
+    QkNorm a = make_qk_norm(desc, rope_dims, eps, q, k, q_weight, k_weight, positions, rope_table, q_out);
+    check_pool(pool);
+    require(pool->num_kv_heads == desc->num_kv_heads && pool->head_dim == desc->head_dim &&
+                pool->elem_bytes == elem_size(desc->dtype),
+            "pool does not match the descriptor");
+    require(pool->num_blocks <= INT32_MAX, "num_blocks must be in [1, 2^31)");
+    require(aligned(pool->data, pool->elem_bytes), "pool: not aligned to its elements");
+    if (a.tokens == 0) return;
+    check_rows(v, "v", desc->tokens, desc->dtype);
+    require(slots != nullptr && aligned(slots, 8), "null or unaligned slots");
+    a.src[2] = v.data; a.hs[2] = v.head_stride; a.ss[2] = v.seq_stride;
+    a.pool = pool->data;
+    a.pool_slots = pool->num_blocks * pool->block_size;
+    a.plane_elems = a.pool_slots * pool->num_kv_heads * static_cast<int64_t>(pool->head_dim);
+    a.slots = slots;
+    a.err = device_error_flags();
+    launch_qk_norm(desc->dtype, desc->rope == 2, a, as_stream(stream));
   });
 }
 

@@ -320,6 +320,26 @@ void launch_qkv_rope(int dtype, int d, QkvArgs& a, hipStream_t stream);
 // cos / sin tables [rows, d/2] of RotaryEmbedding (rotary.rs:64-97).
 void launch_rope_table(int d, int64_t rows, double base, float* cos, float* sin, hipStream_t stream);
 
+// Norms of q and k heads with the rotation, dense or into the paged cache (qk_norm.hip).
+struct QkNorm {
+  const void* src[3];           // q, k and (append) v views [heads, tokens, d]
+  int64_t hs[3], ss[3];
+  const void* w[2];             // weights [d] of the q and k norms, or null (ones)
+  const int64_t* pos;           // [tokens], read where rot > 0
+  const float *rope_cos, *rope_sin;  // [rope_rows, rot / 2]
+  int64_t rope_rows, tokens;
+  int32_t hq, hkv, d, rot;      // rot: leading dims that turn
+  float eps, inv_d;
+  void* out[2];                 // q and (dense) k views
+  int64_t out_hs[2], out_ss[2];
+  void* pool;                   // append: K / V rows go to pool[plane][slots[t]]
+  int64_t plane_elems, pool_slots;
+  const int64_t* slots;
+  int* err;
+  int32_t lanes, lanes_log2, groups, splits;  // set by the launcher
+};
+void launch_qk_norm(int dtype, bool pairs, QkNorm a, hipStream_t stream);
+
 void launch_synth_normals(uint64_t seed, int64_t offset, int64_t count, int dtype, void* out,
                           hipStream_t stream);
 

@@ -794,6 +794,39 @@ int hcp_kv8_prefill_replay_paged(const hcp_ring_replay_desc* desc, hcp_ring_view
                                  void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * (11) Norms of the queries and keys of each head, with the position rotation in the same
+ * pass (no reference counterpart; its models have no such norms).
+ *
+ * A head's row x of a token becomes y = x / sqrt(mean(x^2) + eps) * weight (q_weight or
+ * k_weight, [head_dim] in dtype; NULL: ones).  With desc->rope = 1 or 2, of the first
+ * rope_dims dims every plane (i, j) is turned by the angle of the token's position: (y_i cos -
+ * y_j sin, y_j cos + y_i sin), with (i, j) = (p, p + rope_dims / 2), the halves of (7), for
+ * rope = 1 and the pairs (2p, 2p + 1) for 2, p < rope_dims / 2.  cos and sin come from
+ * rope_table, laid out as hcp_rope_table(rope_dims, rope_rows, ...) writes it.  The descriptor
+ * is that of (7); its hidden is not read.  Computed in fp32, rounded once.
+ * q / q_out [Hq, tokens, D] and k / k_out [Hkv, tokens, D] are views of any strides and
+ * alignment (16-byte chunks are read and written faster); an output may be its own input,
+ * but not overlap one otherwise.
+ *
+ * hcp_qk_norm_rope_append writes K rows (normed, turned) and V rows (as they are) to
+ * slots[t] = block * block_size + place of the paged pool of (3) (DEVICE int64 [tokens], e.g.
+ * of hcp_kv_plan_step) instead of k_out.  A negative slot is skipped (its q row is written),
+ * one past the pool sets device error bit 0.  Of two tokens with one slot, either's elements
+ * are kept.
+ * A position outside the table sets bit 2, and its rows are normed but not turned.
+ * dtype BF16, F16 or F32 (the pool's elements have its size); head_dim and rope_dims
+ * multiples of 8, head_dim up to 256; eps > 0.
+ * ------------------------------------------------------------------------------- */
+int hcp_qk_norm_rope(const hcp_qkv_desc* desc, int32_t rope_dims, float eps, hcp_ring_view q, hcp_ring_view k,
+                     const void* q_weight, const void* k_weight, const int64_t* positions,
+                     const float* rope_table, hcp_ring_view q_out, hcp_ring_view k_out, void* stream);
+
+int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float eps, hcp_ring_view q,
+                            hcp_ring_view k, hcp_ring_view v, const void* q_weight, const void* k_weight,
+                            const int64_t* positions, const float* rope_table, hcp_ring_view q_out,
+                            const hcp_paged_pool* pool, const int64_t* slots, void* stream);
+
+/* ---------------------------------------------------------------------------------
  * Replay kernel timing (no reference counterpart; benchmark instrumentation; the
  * reference logs wall-clock compute per phase to HCP_PERF_LOG, ring.rs:820-844).
  *
