@@ -18,6 +18,8 @@ The operator names mirror the reference's ring-attention backend
   with a scale per block and head -> ``hcp_kv8_*`` (no reference counterpart)
 * :func:`qk_norm_rope` / :func:`qk_norm_rope_append`  norms of q and k heads with the rotation,
   dense or into the paged cache -> ``hcp_qk_norm_rope*`` (no reference counterpart)
+* :func:`step_attn_plan` / :func:`step_attn`  attention of a serving step over the paged cache,
+  shared prefixes read once -> ``hcp_step_attn*`` (no reference counterpart)
 * :func:`ring_attention_replay`             ring.rs:861-1398 for every domain on one GPU ->
   ``hcp_ring_prefill_replay`` (``_paged`` variant stages K/V from a block pool)
 
@@ -308,6 +310,13 @@ def lib() -> ctypes.CDLL:
         "hcp_qk_norm_rope": ([ctypes.POINTER(QkvDesc), i32, f32, View, View, vp, vp, vp, vp, View, View, vp], ctypes.c_int),
         "hcp_qk_norm_rope_append": ([ctypes.POINTER(QkvDesc), i32, f32, View, View, View, vp, vp, vp, vp, View,
                                      ctypes.POINTER(PagedPool), vp, vp], ctypes.c_int),
+        "hcp_step_attn_plan_size": ([ctypes.POINTER(DecodeDesc), i64, i32], ctypes.c_size_t),
+        "hcp_step_attn_workspace_size": ([ctypes.POINTER(DecodeDesc), i64, i32], ctypes.c_size_t),
+        "hcp_step_attn_plan": ([ctypes.POINTER(DecodeDesc), ctypes.POINTER(PagedPool), i64, i32, vp, vp, i32,
+                                ctypes.POINTER(DecodeShard), vp, vp, ctypes.c_size_t, vp], ctypes.c_int),
+        "hcp_step_attn": ([ctypes.POINTER(DecodeDesc), ctypes.POINTER(PagedPool), i64, i32, View, vp, i32,
+                           ctypes.POINTER(DecodeShard), vp, ctypes.c_size_t, i32, View, vp, vp, ctypes.c_size_t, vp],
+                          ctypes.c_int),
         "hcp_ring_trace_attach": ([vp, ctypes.c_size_t], ctypes.c_int),
         "hcp_ring_trace_record_bytes": ([ctypes.POINTER(ReplayDesc)], ctypes.c_size_t),
         "hcp_ring_trace_read": ([vp, ctypes.POINTER(TraceDomain), i32, ctypes.POINTER(i32),
@@ -1050,6 +1059,102 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, pool, slots, positions=None
     _want("slots", slots, _torch().int64, (q.shape[1],), dev)
     _launch(lib().hcp_qk_norm_rope_append, dev, stream, *args, view(v), *more, ctypes.byref(pp), slots.data_ptr())
     return q_out
+
+
+# ---------------------------------------------------------------------------------
+# (12) attention of a serving step
+# ---------------------------------------------------------------------------------
+def _step_args(q, pool, block_tables, prefix_tables, prefix_lens=None, scale=None):
+    """(descriptor, pool, number of prefixes, hcp_decode_shard of them or None, GPU), checked."""
+    pp = paged_pool(pool)
+    dev = pool.get_device()
+    hq, _, d = q.shape
+    if q.dtype != pool.dtype or q.get_device() != dev:
+        raise ValueError(f"q must be {pool.dtype} on {_place(dev)}")
+    b = block_tables.shape[0]
+    _decode_tables("block_tables", block_tables, None, b, dev)
+    n = 0 if prefix_tables is None else prefix_tables.shape[0]
+    shard = None
+    if n:
+        _decode_tables("prefix_tables", prefix_tables, None, n, dev)
+        if prefix_lens is not None:
+            _want("prefix_lens", prefix_lens, _torch().int32, (n,), dev)
+        shard = DecodeShard(prefix_tables.data_ptr(), max(prefix_tables.stride(0), prefix_tables.shape[1]), prefix_tables.shape[1],
+                            None if prefix_lens is None else prefix_lens.data_ptr(), 0)
+    desc = DecodeDesc(dtype_code(q.dtype), b, hq, pp.num_kv_heads, d, 0, 0, 0,
+                      max(block_tables.stride(0), block_tables.shape[1]), block_tables.shape[1],
+                      scale if scale is not None else 1.0 / math.sqrt(d))
+    return desc, pp, n, shard, dev
+
+
+def _size(n):
+    if n == 0:
+        raise HcpRingError(-6, last_error())
+    return n
+
+
+def step_attn_plan_size(q, pool, block_tables, prefix_tables=None) -> int:
+    """Bytes of a plan of :func:`step_attn_plan`."""
+    desc, _, n, _, _ = _step_args(q, pool, block_tables, prefix_tables)
+    return _size(lib().hcp_step_attn_plan_size(ctypes.byref(desc), q.shape[1], n))
+
+
+def step_attn_workspace_size(q, pool, block_tables, prefix_tables=None) -> int:
+    """Workspace bytes of :func:`step_attn`."""
+    desc, _, n, _, _ = _step_args(q, pool, block_tables, prefix_tables)
+    return _size(lib().hcp_step_attn_workspace_size(ctypes.byref(desc), q.shape[1], n))
+
+
+def step_attn_plan(q, pool, block_tables, token_starts, seq_lens, prefix_tables=None, prefix_ids=None, prefix_lens=None,
+                   causal=True, plan=None, stream=None):
+    """The plan of a step's attention, made once for the :func:`step_attn` calls of all layers.
+
+    Sequence b has the new tokens token_starts[b] .. token_starts[b + 1] - 1 ([B + 1] int32, of
+    :func:`kv_plan_step`) among the rows of q [Hq, T, D] (only its shape and type count) and,
+    with them, seq_lens[b] tokens of its own in row b of block_tables [B, n] int32.  With
+    prefix_tables [P, m] int32 it stands behind the first prefix_lens[p] tokens of row
+    p = prefix_ids[b] ([B] int32, -1: none).  causal: new token i of n sees its own tokens up to
+    seq_lens[b] - n + i, else all.  Lengths are read on the GPU -> plan (uint8 tensor)."""
+    torch = _torch()
+    i32 = torch.int32
+    desc, pp, n, shard, dev = _step_args(q, pool, block_tables, prefix_tables, prefix_lens)
+    _want("token_starts", token_starts, i32, (desc.batch + 1,), dev)
+    _want("seq_lens", seq_lens, i32, (desc.batch,), dev)
+    if n:
+        if prefix_ids is None or prefix_lens is None:
+            raise ValueError("prefix_tables come with prefix_ids and prefix_lens")
+        _want("prefix_ids", prefix_ids, i32, (desc.batch,), dev)
+    tokens, fns = q.shape[1], lib()
+    plan, at, size = _workspace(plan, lambda: _size(fns.hcp_step_attn_plan_size(ctypes.byref(desc), tokens, n)), dev, stream)
+    _launch(fns.hcp_step_attn_plan, dev, stream, ctypes.byref(desc), ctypes.byref(pp), tokens, 1 if causal else 0,
+            token_starts.data_ptr(), seq_lens.data_ptr(), n, None if shard is None else ctypes.byref(shard),
+            prefix_ids.data_ptr() if n else None, at, size)
+    return plan
+
+
+def step_attn(q, pool, block_tables, plan, prefix_tables=None, causal=True, scale=None, out=None, lse=None, workspace=None,
+              stream=None):
+    """Attention of a step's new tokens q [Hq, T, D] over the paged cache, by a plan of
+    :func:`step_attn_plan` for the same shapes -> (out [Hq, T, D] in q's type, or fp32 if an fp32
+    ``out`` is given, lse [Hq, T] fp32).  Rows of no sequence are left as they are."""
+    desc, pp, n, shard, dev = _step_args(q, pool, block_tables, prefix_tables, None, scale)
+    torch = _torch()
+    hq, tokens, d = shape = q.shape
+    if out is None:
+        out = _empty(shape, q.dtype, q.device, stream)
+    _rows_of("out", out, shape, dev)
+    if lse is None:
+        lse = _empty((hq, tokens), torch.float32, q.device, stream)
+    _want("lse", lse, torch.float32, (hq, tokens), dev)
+    if plan.get_device() != dev or not plan.is_contiguous():
+        raise ValueError(f"plan must be contiguous on {_place(dev)}")
+    fns = lib()
+    _ws, ws, ws_bytes = _workspace(workspace, lambda: _size(fns.hcp_step_attn_workspace_size(ctypes.byref(desc), tokens, n)),
+                                   dev, stream)
+    _launch(fns.hcp_step_attn, dev, stream, ctypes.byref(desc), ctypes.byref(pp), tokens, 1 if causal else 0, view(q),
+            block_tables.data_ptr(), n, None if shard is None else ctypes.byref(shard), plan.data_ptr(),
+            plan.numel() * plan.element_size(), dtype_code(out.dtype), view(out), lse.data_ptr(), ws, ws_bytes)
+    return out, lse
 
 
 # ---------------------------------------------------------------------------------

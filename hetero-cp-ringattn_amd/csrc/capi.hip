@@ -2069,6 +2069,121 @@ int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float e
   });
 }
 
+// ---- (12) attention of a serving step ----
+}  // extern "C": internal helpers below have C++ linkage
+namespace {
+// What the size queries and both calls ask of a step's shape; block_size 16 stands in where
+// there is no pool (sizes do not go by it).
+StepShape step_shape(const hcp_paged_decode_desc* d, int64_t tokens, int32_t causal, int32_t num_prefixes,
+                     const hcp_decode_shard* prefixes, int32_t bs) {
+  require(d != nullptr, "null descriptor");
+  require(d->dtype == kBF16 || d->dtype == kF16, "dtype must be BF16 or F16");
+  require(d->batch > 0 && d->batch <= kStepMaxBatch, "batch must be in [1, 4096]");
+  require(d->num_q_heads > 0 && d->num_kv_heads > 0 && d->num_q_heads % d->num_kv_heads == 0 &&
+              d->num_q_heads / d->num_kv_heads <= 256,
+          "num_q_heads must be a multiple of num_kv_heads, up to 256 times it");
+  require(d->num_q_heads <= (1 << 16), "too many heads");
+  require(d->head_dim > 0 && d->head_dim <= 128 && d->head_dim % 8 == 0, "head_dim must be a multiple of 8 up to 128");
+  require(static_cast<int64_t>(d->num_kv_heads) * d->head_dim * 32 < (int64_t(1) << 31), "a token's K rows are too long");
+  require(causal == 0 || causal == 1, "causal must be 0 or 1");
+  require(tokens >= 0 && tokens * (d->num_q_heads / d->num_kv_heads) < (int64_t(1) << 30) && tokens <= (1 << 30), "too many tokens");
+  require(d->table_len >= 1 && d->table_stride >= d->table_len, "bad table shape");
+  require(d->table_len <= (int64_t(1) << 30) / bs, "tables of more than 2^30 tokens");
+  require(num_prefixes >= 0 && num_prefixes <= kStepMaxPrefixes, "num_prefixes must be in [0, 1024]");
+  StepShape s{d->batch, d->num_q_heads, d->num_kv_heads, d->head_dim, bs, causal, num_prefixes, tokens, d->table_len * bs, 0};
+  if (num_prefixes > 0) {
+    require(prefixes != nullptr, "null prefixes");
+    require(prefixes->table_len >= 1 && prefixes->table_stride >= prefixes->table_len, "bad prefix table shape");
+    require(prefixes->table_len <= (int64_t(1) << 30) / bs, "prefix tables of more than 2^30 tokens");
+    s.max_prefix = prefixes->table_len * bs;
+  }
+  // a plan counts (tile, kv head) units in 32 bits: a tile a 256 rows, up to three a sequence
+  require((tokens * (s.hq / s.hkv) / 128 + 4 * static_cast<int64_t>(s.batch)) * s.hkv < (int64_t(1) << 30), "too many rows for one step");
+  return s;
+}
+StepShape step_call(const hcp_paged_decode_desc* d, const hcp_paged_pool* pool, int64_t tokens, int32_t causal,
+                    int32_t num_prefixes, const hcp_decode_shard* prefixes, const void* plan, size_t plan_bytes) {
+  check_pool(pool);
+  require(pool->block_size % 16 == 0 && pool->block_size <= (1 << 20), "block_size must be a multiple of 16 up to 2^20");
+  const StepShape s = step_shape(d, tokens, causal, num_prefixes, prefixes, pool->block_size);
+  require(d->num_kv_heads == pool->num_kv_heads && d->head_dim == pool->head_dim && pool->elem_bytes == 2,
+          "pool does not match the descriptor");
+  require(pool->num_blocks <= INT32_MAX, "num_blocks must be in [1, 2^31)");
+  require(aligned(pool->data, 16), "the pool must be 16-byte aligned");
+  const size_t need = step_plan_bytes(s);
+  if (plan == nullptr || plan_bytes < need) throw Error(-6, "plan too small: need " + std::to_string(need) + " bytes");
+  require(aligned(plan, 256), "the plan must be 256-byte aligned");
+  return s;
+}
+}  // namespace
+extern "C" {
+
+size_t hcp_step_attn_plan_size(const hcp_paged_decode_desc* desc, int64_t tokens, int32_t num_prefixes) {
+  size_t n = 0;
+  const hcp_decode_shard any{nullptr, 1, 1, nullptr, 0};
+  if (guarded(__func__, [&] { n = step_plan_bytes(step_shape(desc, tokens, 1, num_prefixes, &any, 16)); }) != HCP_RING_OK) return 0;
+  return n;
+}
+
+size_t hcp_step_attn_workspace_size(const hcp_paged_decode_desc* desc, int64_t tokens, int32_t num_prefixes) {
+  size_t n = 0;
+  const hcp_decode_shard any{nullptr, 1, 1, nullptr, 0};
+  if (guarded(__func__, [&] { n = step_work_bytes(step_shape(desc, tokens, 1, num_prefixes, &any, 16)); }) != HCP_RING_OK) return 0;
+  return n;
+}
+
+int hcp_step_attn_plan(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool, int64_t tokens, int32_t causal,
+                       const int32_t* token_starts, const int32_t* seq_lens, int32_t num_prefixes,
+                       const hcp_decode_shard* prefixes, const int32_t* prefix_ids, void* plan, size_t plan_bytes,
+                       void* stream) {
+  return guarded(__func__, [&] {
+    const StepShape s = step_call(desc, pool, tokens, causal, num_prefixes, prefixes, plan, plan_bytes);
+    require(token_starts != nullptr && seq_lens != nullptr, "null token_starts or seq_lens");
+    if (num_prefixes > 0) require(prefixes->seq_lens != nullptr && prefix_ids != nullptr, "null prefix lengths or ids");
+    launch_step_plan(s, token_starts, seq_lens, num_prefixes > 0 ? prefix_ids : nullptr,
+                     num_prefixes > 0 ? prefixes->seq_lens : nullptr, plan, device_error_flags(), as_stream(stream));
+  });
+}
+
+int hcp_step_attn(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool, int64_t tokens, int32_t causal,
+                  hcp_ring_view q, const int32_t* block_tables, int32_t num_prefixes, const hcp_decode_shard* prefixes,
+                  const void* plan, size_t plan_bytes, int32_t out_dtype, hcp_ring_view out, float* lse, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  return guarded(__func__, [&] {
+    const StepShape s = step_call(desc, pool, tokens, causal, num_prefixes, prefixes, plan, plan_bytes);
+    require(desc->scale > 0.f && desc->scale <= FLT_MAX, "scale must be positive");
+    require(out_dtype == desc->dtype || out_dtype == kF32, "out_dtype must be dtype or F32");
+    require(block_tables != nullptr && (num_prefixes == 0 || prefixes->block_tables != nullptr), "null block tables");
+    const size_t need = step_work_bytes(s);
+    if (workspace == nullptr || workspace_bytes < need) throw Error(-6, "workspace too small: need " + std::to_string(need) + " bytes");
+    require(aligned(workspace, 256), "the workspace must be 256-byte aligned");
+    if (tokens == 0) return;
+    check_view(q, "q", tokens);
+    check_view(out, "out", tokens);
+    require(mfma_layout_ok(q), "q must be 16-byte aligned with strides multiple of 8");
+    const int per16 = out_dtype == kF32 ? 4 : 8;
+    require(aligned(out.data, 16) && out.head_stride % per16 == 0 && out.seq_stride % per16 == 0,
+            "out must be 16-byte aligned with strides of whole 16 bytes");
+    require(aligned(lse, 4), "lse not aligned to its elements");
+    StepLaunch L{};
+    L.s = s;
+    L.dtype = desc->dtype;
+    L.plan = plan;
+    L.q = q.data; L.q_hs = q.head_stride; L.q_ss = q.seq_stride;
+    L.pool = pool->data; L.num_blocks = pool->num_blocks;
+    L.tables = block_tables; L.table_stride = desc->table_stride;
+    L.prefix_tables = num_prefixes > 0 ? prefixes->block_tables : nullptr;
+    L.prefix_stride = num_prefixes > 0 ? prefixes->table_stride : 0;
+    L.scale = desc->scale;
+    L.out_dtype = out_dtype;
+    L.out = out.data; L.out_hs = out.head_stride; L.out_ss = out.seq_stride;
+    L.lse = lse;
+    L.ws = workspace;
+    L.err = device_error_flags();
+    launch_step_attn(L, as_stream(stream));
+  });
+}
+
 int hcp_ring_replay_timing(int32_t enable) {
   return guarded(__func__, [&] {
     ReplayTiming& t = timing();

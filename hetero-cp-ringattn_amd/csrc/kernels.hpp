@@ -340,6 +340,38 @@ struct QkNorm {
 };
 void launch_qk_norm(int dtype, bool pairs, QkNorm a, hipStream_t stream);
 
+// Attention of a serving step over the paged cache (step_attn.hip).
+constexpr int kStepMaxBatch = 4096, kStepMaxPrefixes = 1024, kStepMaxWorkers = 512;
+struct StepShape {
+  int32_t batch, hq, hkv, d, bs, causal, prefixes;
+  int64_t tokens;                // rows of the query
+  int64_t max_own, max_prefix;   // tokens that a table row holds
+};
+int step_workers();              // workgroups of the attention: one a CU
+size_t step_plan_bytes(const StepShape& s);
+size_t step_work_bytes(const StepShape& s);
+void launch_step_plan(const StepShape& s, const int32_t* token_starts, const int32_t* seq_lens, const int32_t* prefix_ids,
+                      const int32_t* prefix_lens, void* plan, int* err, hipStream_t stream);
+struct StepLaunch {
+  StepShape s;
+  int dtype;
+  const void* plan;
+  const void* q;
+  int64_t q_hs, q_ss;
+  const void* pool;
+  int64_t num_blocks;
+  const int32_t *tables, *prefix_tables;
+  int64_t table_stride, prefix_stride;
+  float scale;
+  int out_dtype;
+  void* out;
+  int64_t out_hs, out_ss;
+  float* lse;                    // [hq, tokens] or null
+  void* ws;
+  int* err;
+};
+void launch_step_attn(const StepLaunch& L, hipStream_t stream);
+
 void launch_synth_normals(uint64_t seed, int64_t offset, int64_t count, int dtype, void* out,
                           hipStream_t stream);
 

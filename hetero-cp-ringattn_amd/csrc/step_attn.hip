@@ -1,0 +1,1277 @@
+// Attention of one serving step over the paged cache: a batch of sequences with one or many
+// new tokens each, behind what the cache holds of each and behind prefixes that several share.
+//
+//   o = softmax(q K^T scale) V over a sequence's prefix keys and those of its own keys that a
+//   token sees; a prefix's K and V are read once for all of the step's tokens behind it.
+//
+// Rows.  The query heads of a kv head are packed token-major: row r of a source is token
+// r / rep, head r % rep of the group.  A source of more than 32 rows (a prompt chunk, or the
+// tokens behind one prefix) is cut into wide tiles of 256 rows, 32 a wave, whose K and V
+// tiles of 128 keys are shared through LDS (the ping-pong of the ring kernels, with the rows of
+// a tile fetched block by block).  One of up to 32 rows (a decoding sequence) is a narrow
+// tile: 8 waves hold the same rows and take 32 keys each in turn, out of LDS of their own,
+// with no barrier until their results meet.
+//
+// Work.  All (tile, kv head) units are laid end to end on an axis of modelled time, the wide
+// ones by kv head first (workgroups of one XCD then read one head's K and V), and dealt in
+// equal parts to one workgroup a CU: a unit that falls to several is joined afterwards
+// (step_join_kernel), as is a row's part behind a shared prefix with its own part.  The plan
+// (step_plan_kernel) lays the axis out once a step for the calls of all layers.
+#include <algorithm>
+
+#include "kernels.hpp"
+#include "lds_dma.hpp"
+#include "attn_tile.hpp"
+
+namespace hcp {
+
+namespace {
+
+constexpr int kStepWaves = 8;
+constexpr int kStepThreads = 64 * kStepWaves;
+constexpr int kWideRows = 32 * kStepWaves;  // rows of a wide tile
+constexpr int kWideKeys = 128;              // keys of its steps
+constexpr int kNarrowRows = 32;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanMagic = 0x53544550;
+
+// Modelled time in 0.1 us: of a unit beside its steps, and of a step of 128 (wide) or up to
+// 8 x 32 keys (narrow).
+constexpr int kWideFixed = 60, kWideStep = 22;
+constexpr int kNarrowFixed = 30, kNarrowStep = 45;
+
+// Where a unit's rows go when it is not cut.
+enum { kToOut = 0, kToOwn = 1, kToPrefix = 2 };
+
+struct StepTile {
+  int32_t tok0;        // query token of row 0 of the source, or its first list entry (list)
+  int32_t row0, rows;  // rows of the source in this tile
+  int32_t p_row, p_len;     // prefix table's row and keys (0: none)
+  int32_t s_row, s_len;     // own table's row and the keys that some row of the tile sees
+  int32_t vis0, vis_step;   // token i of the source sees own keys j < vis0 + i * vis_step
+  int32_t steps;
+  int32_t dest, list0;      // kTo*, list entry of token 0 of the source
+  int32_t list;             // tokens through the list
+  int32_t pad[3];
+};
+static_assert(sizeof(StepTile) == 64, "a tile is a cache line");
+
+// A token behind a shared prefix: its own narrow tile, and its rows in the prefix's tiles.
+struct StepShared {
+  int32_t token;
+  int32_t own_tile, own_row;           // narrow tile (counted from 0), row of its first head
+  int32_t pre_tile, pre_row, pre_wide; // the prefix's first tile (wide or narrow), row of its first head
+  int32_t pad[2];
+};
+
+struct StepHead {
+  int32_t magic, batch, tokens, hq, hkv, d, bs, causal, prefixes, max_own, max_prefix, workers;
+  int32_t n_wide, n_narrow, n_shared, n_cut, cut_rows, pad[3];
+};
+// Whether the plan was made for this shape and number of workers.
+template <typename P>
+__device__ bool plan_fits(P head, const StepShape& s, int workers) {
+  const int want[12] = {kPlanMagic, s.batch, static_cast<int>(s.tokens), s.hq, s.hkv, s.d, s.bs, s.causal, s.prefixes,
+                        static_cast<int>(s.max_own), static_cast<int>(s.max_prefix), workers};
+  bool ok = true;
+#pragma unroll
+  for (int i = 0; i < 12; ++i) ok = ok && head[i] == want[i];
+  return ok;
+}
+
+// Offsets of the plan's arrays, from host-known bounds alone.
+struct PlanLayout {
+  int64_t max_wide, max_narrow, max_shared, max_units;
+  size_t tiles, cum_wide, cum_narrow, shared, starts, cuts, cut_units, cut_row0, bytes;
+};
+
+size_t up256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+PlanLayout plan_layout(const StepShape& s) {
+  const int64_t rep = s.hq / s.hkv, live = std::min<int64_t>(s.batch, s.tokens);
+  PlanLayout l;
+  l.max_shared = s.prefixes > 0 ? std::min<int64_t>(s.tokens, live * std::max<int64_t>(1, kNarrowRows / rep)) : 0;
+  l.max_wide = s.tokens * rep / kWideRows + live + (s.prefixes > 0 ? l.max_shared * rep / kWideRows + std::min<int64_t>(s.prefixes, live) : 0);
+  l.max_narrow = live + std::min<int64_t>(s.prefixes, live);
+  l.max_units = (l.max_wide + l.max_narrow) * s.hkv;
+  size_t at = up256(sizeof(StepHead));
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += up256(bytes);
+    return here;
+  };
+  l.tiles = take((l.max_wide + l.max_narrow) * sizeof(StepTile));
+  l.cum_wide = take((l.max_wide + 1) * sizeof(int64_t));
+  l.cum_narrow = take((l.max_narrow + 1) * sizeof(int64_t));
+  l.shared = take(l.max_shared * sizeof(StepShared));
+  l.starts = take((kStepMaxWorkers + 1) * 2 * sizeof(int32_t));
+  l.cuts = take(l.max_units * sizeof(int32_t));
+  l.cut_units = take(kStepMaxWorkers * sizeof(int32_t));
+  l.cut_row0 = take((kStepMaxWorkers + 1) * sizeof(int32_t));
+  l.bytes = at;
+  return l;
+}
+
+// The workspace: two slots of partial rows a worker (its first and its last unit, where cut),
+// then the rows of tokens behind shared prefixes, their own part and the prefix's.
+struct WorkLayout {
+  int32_t slot_rows;
+  size_t slot_o, slot_lse, own_o, own_lse, pre_o, pre_lse, bytes;
+};
+WorkLayout work_layout(const StepShape& s, int workers) {
+  const int64_t rep = s.hq / s.hkv;
+  WorkLayout w;
+  w.slot_rows = static_cast<int32_t>(std::min<int64_t>(kWideRows, (s.tokens * rep + 31) / 32 * 32));
+  size_t at = 0;
+  auto take = [&](size_t floats) {
+    const size_t here = at;
+    at += up256(floats * sizeof(float));
+    return here;
+  };
+  const size_t slots = 2 * static_cast<size_t>(workers) * w.slot_rows;
+  const size_t rows = static_cast<size_t>(plan_layout(s).max_shared) * s.hq;
+  w.slot_o = take(slots * s.d);
+  w.slot_lse = take(slots);
+  w.own_o = take(rows * s.d);
+  w.own_lse = take(rows);
+  w.pre_o = take(rows * s.d);
+  w.pre_lse = take(rows);
+  w.bytes = at;
+  return w;
+}
+
+}  // namespace
+
+size_t step_plan_bytes(const StepShape& s) { return plan_layout(s).bytes; }
+size_t step_work_bytes(const StepShape& s) { return work_layout(s, step_workers()).bytes; }
+int step_workers() { return std::min(device_cus(), kStepMaxWorkers); }
+
+// ----------------------------------------------------------------------------------
+// Plan: one workgroup.
+// ----------------------------------------------------------------------------------
+struct PlanKernelArgs {
+  StepShape s;
+  int32_t workers;
+  const int32_t *token_starts, *seq_lens, *prefix_ids, *prefix_lens;
+  char* plan;
+  PlanLayout l;
+  int* err;
+};
+
+namespace {
+
+// Exclusive running sum of a[0 .. n) in LDS in place, by the whole workgroup; the total.
+__device__ int scan_lds(int* a, int n, int* tmp) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (n + kPlanThreads - 1) / kPlanThreads, b = min(tid * per, n), e = min(b + per, n);
+  int sum = 0;
+  for (int i = b; i < e; ++i) sum += a[i];
+  int x = sum;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(x, off);
+    if (lane >= off) x += y;
+  }
+  if (lane == 63) tmp[wave] = x;
+  __syncthreads();
+  int before = x - sum, total = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w < wave) before += tmp[w];
+    total += tmp[w];
+  }
+  for (int i = b; i < e; ++i) {
+    const int v = a[i];
+    a[i] = before;
+    before += v;
+  }
+  __syncthreads();
+  return total;
+}
+
+// cum[0 .. n] = running sums of cost(i), by the whole workgroup.
+template <typename F>
+__device__ int64_t scan_costs(int64_t* cum, int n, F&& cost, int64_t* tmp) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t base = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    const int64_t c = i < n ? cost(i) : 0;
+    int64_t x = c;
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t y = __shfl_up(x, off);
+      if (lane >= off) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) tmp[wave] = x;
+    __syncthreads();
+    int64_t before = base + x - c, total = 0;
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+      if (w < wave) before += tmp[w];
+      total += tmp[w];
+    }
+    if (i < n) cum[i] = before;
+    base += total;
+  }
+  if (tid == 0) cum[n] = base;
+  __syncthreads();
+  return base;
+}
+
+// The last i of a[0 .. n) (non-decreasing, a[0] <= x) with a[i] <= x.
+template <typename T>
+__device__ int last_at_most(const T* a, int n, T x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a[mid] <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+}  // namespace
+
+__global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs a) {
+  __shared__ int s_tok[kStepMaxBatch], s_n[kStepMaxBatch], s_vis[kStepMaxBatch], s_len[kStepMaxBatch];
+  __shared__ int s_pid[kStepMaxBatch], s_wide[kStepMaxBatch], s_nar[kStepMaxBatch];
+  __shared__ int g_seq[kStepMaxPrefixes], g_tok[kStepMaxPrefixes], g_list[kStepMaxPrefixes], g_wide[kStepMaxPrefixes],
+      g_nar[kStepMaxPrefixes];
+  __shared__ int64_t tmp64[kPlanThreads / 64];
+  __shared__ int tmp[kPlanThreads / 64];
+  __shared__ int st_unit[kStepMaxWorkers + 1], st_step[kStepMaxWorkers + 1];
+  __shared__ int n_cut;
+
+  const int tid = threadIdx.x;
+  const int B = a.s.batch, NP = a.s.prefixes, rep = a.s.hq / a.s.hkv, hkv = a.s.hkv;
+  const int tokens = static_cast<int>(a.s.tokens);
+  StepHead* head = reinterpret_cast<StepHead*>(a.plan);
+  StepTile* tiles = reinterpret_cast<StepTile*>(a.plan + a.l.tiles);
+  int64_t* cum_w = reinterpret_cast<int64_t*>(a.plan + a.l.cum_wide);
+  int64_t* cum_n = reinterpret_cast<int64_t*>(a.plan + a.l.cum_narrow);
+  StepShared* shared = reinterpret_cast<StepShared*>(a.plan + a.l.shared);
+  int32_t* starts = reinterpret_cast<int32_t*>(a.plan + a.l.starts);
+  int32_t* cuts = reinterpret_cast<int32_t*>(a.plan + a.l.cuts);
+  int32_t* cut_units = reinterpret_cast<int32_t*>(a.plan + a.l.cut_units);
+  int32_t* cut_row0 = reinterpret_cast<int32_t*>(a.plan + a.l.cut_row0);
+  auto flag = [&] { atomicOr(a.err, 8); };
+  auto prefix_len = [&](int p) {  // of prefix p, within its table
+    const int64_t n = a.prefix_lens[p];
+    return static_cast<int>(n < 0 ? 0 : n > a.s.max_prefix ? a.s.max_prefix : n);
+  };
+
+  // ---- sequences: tokens within the query, lengths within their tables ----
+  for (int p = tid; p < NP; p += kPlanThreads) {
+    g_seq[p] = g_tok[p] = 0;
+    const int n = a.prefix_lens[p];
+    if (n < 0 || n > a.s.max_prefix) flag();
+  }
+  if (tid == 0) n_cut = 0;
+  __syncthreads();
+  for (int b = tid; b < B; b += kPlanThreads) {
+    int t0 = a.token_starts[b], t1 = a.token_starts[b + 1];
+    if (t0 < 0 || t1 < t0) {
+      flag();
+      t0 = t1 = 0;
+    }
+    int64_t len = a.seq_lens[b];
+    if (len < 0 || len > a.s.max_own) {
+      flag();
+      len = len < 0 ? 0 : a.s.max_own;
+    }
+    const int n = min(t1, tokens) - min(t0, tokens);
+    int pid = NP > 0 && a.prefix_ids != nullptr ? a.prefix_ids[b] : -1;
+    if (pid < -1 || pid >= NP) {
+      flag();
+      pid = -1;
+    }
+    if (pid >= 0 && prefix_len(pid) == 0) pid = -1;
+    s_tok[b] = min(t0, tokens);
+    s_n[b] = n;
+    s_len[b] = static_cast<int>(len);
+    // own keys that the sequence's first token sees (its last one sees all)
+    s_vis[b] = a.s.causal ? static_cast<int>(max(len - (static_cast<int64_t>(t1) - t0) + 1, static_cast<int64_t>(INT32_MIN / 2)))
+                          : static_cast<int>(len);
+    s_pid[b] = pid;
+    const bool narrow = n > 0 && static_cast<int64_t>(n) * rep <= kNarrowRows;
+    if (narrow && pid >= 0) {
+      atomicAdd(&g_seq[pid], 1);
+      atomicAdd(&g_tok[pid], n);
+    }
+  }
+  __syncthreads();
+  // ---- prefixes with tokens of several sequences behind them: list places and tiles ----
+  for (int p = tid; p < NP; p += kPlanThreads) {
+    const bool on = g_seq[p] >= 2;
+    const int rows = on ? g_tok[p] * rep : 0;
+    if (!on) g_seq[p] = 0;
+    g_list[p] = on ? g_tok[p] : 0;
+    g_wide[p] = rows > kNarrowRows ? (rows + kWideRows - 1) / kWideRows : 0;
+    g_nar[p] = rows > 0 && rows <= kNarrowRows ? 1 : 0;
+  }
+  __syncthreads();
+  const int n_shared = NP > 0 ? scan_lds(g_list, NP, tmp) : 0;
+  const int pre_wide = NP > 0 ? scan_lds(g_wide, NP, tmp) : 0;
+  const int pre_nar = NP > 0 ? scan_lds(g_nar, NP, tmp) : 0;
+  for (int b = tid; b < B; b += kPlanThreads) {
+    const int64_t rows = static_cast<int64_t>(s_n[b]) * rep;
+    s_wide[b] = rows > kNarrowRows ? static_cast<int>((rows + kWideRows - 1) / kWideRows) : 0;
+    s_nar[b] = rows > 0 && rows <= kNarrowRows ? 1 : 0;
+  }
+  __syncthreads();
+  const int n_wide = pre_wide + scan_lds(s_wide, B, tmp);
+  const int n_nar = pre_nar + scan_lds(s_nar, B, tmp);
+
+  // ---- the list of tokens behind shared prefixes, and the narrow tiles of sequences ----
+  for (int b = tid; b < B; b += kPlanThreads) {
+    const int n = s_n[b], rows = n * rep;
+    if (n == 0 || static_cast<int64_t>(n) * rep > kNarrowRows) continue;
+    const int p = s_pid[b];
+    const bool on = p >= 0 && g_seq[p] > 0;
+    const int own = pre_nar + s_nar[b];
+    int at = 0;
+    if (on) {
+      // place behind the earlier sequences of the same prefix
+      at = g_list[p];
+      for (int c = 0; c < b; ++c)
+        if (s_pid[c] == p && static_cast<int64_t>(s_n[c]) * rep <= kNarrowRows) at += s_n[c];
+      const int wide = g_tok[p] * rep > kNarrowRows;
+      for (int i = 0; i < n; ++i)
+        shared[at + i] = StepShared{s_tok[b] + i, own, i * rep, wide ? g_wide[p] : g_nar[p], (at + i - g_list[p]) * rep, wide, {0, 0}};
+    }
+    const int vstep = a.s.causal ? 1 : 0;
+    StepTile t{};
+    t.tok0 = s_tok[b];
+    t.rows = rows;
+    t.p_row = max(p, 0);
+    t.p_len = p >= 0 && !on ? prefix_len(p) : 0;
+    t.s_row = b;
+    t.s_len = max(0, min(s_len[b], s_vis[b] + (n - 1) * vstep));
+    t.vis0 = s_vis[b];
+    t.vis_step = vstep;
+    t.steps = max(1, ((t.p_len + 31) / 32 + (t.s_len + 31) / 32 + kStepWaves - 1) / kStepWaves);
+    t.dest = on ? kToOwn : kToOut;
+    t.list0 = at;
+    tiles[n_wide + own] = t;
+  }
+  // ---- narrow tiles of prefixes ----
+  for (int p = tid; p < NP; p += kPlanThreads) {
+    const int rows = g_seq[p] > 0 ? g_tok[p] * rep : 0;
+    if (rows == 0 || rows > kNarrowRows) continue;
+    StepTile t{};
+    t.tok0 = g_list[p];
+    t.rows = rows;
+    t.p_row = p;
+    t.p_len = prefix_len(p);
+    t.steps = max(1, ((t.p_len + 31) / 32 + kStepWaves - 1) / kStepWaves);
+    t.dest = kToPrefix;
+    t.list0 = g_list[p];
+    t.list = 1;
+    tiles[n_wide + g_nar[p]] = t;
+  }
+  // ---- wide tiles, one a thread ----
+  for (int i = tid; i < n_wide; i += kPlanThreads) {
+    StepTile t{};
+    if (i < pre_wide) {
+      const int p = last_at_most(g_wide, NP, i);
+      t.tok0 = t.list0 = g_list[p];
+      t.list = 1;
+      t.row0 = (i - g_wide[p]) * kWideRows;
+      t.rows = min(kWideRows, g_tok[p] * rep - t.row0);
+      t.p_row = p;
+      t.p_len = prefix_len(p);
+      t.dest = kToPrefix;
+    } else {
+      const int b = last_at_most(s_wide, B, i - pre_wide), vstep = a.s.causal ? 1 : 0;
+      t.tok0 = s_tok[b];
+      t.row0 = (i - pre_wide - s_wide[b]) * kWideRows;
+      t.rows = min(kWideRows, s_n[b] * rep - t.row0);
+      t.p_row = max(s_pid[b], 0);
+      t.p_len = s_pid[b] >= 0 ? prefix_len(s_pid[b]) : 0;
+      t.s_row = b;
+      t.s_len = max(0, min(s_len[b], s_vis[b] + (t.row0 + t.rows - 1) / rep * vstep));
+      t.vis0 = s_vis[b];
+      t.vis_step = vstep;
+      t.dest = kToOut;
+    }
+    t.steps = max(1, (t.p_len + kWideKeys - 1) / kWideKeys + (t.s_len + kWideKeys - 1) / kWideKeys);
+    tiles[i] = t;
+  }
+  const int units_w = n_wide * hkv, units = units_w + n_nar * hkv;
+  for (int i = tid; i < units; i += kPlanThreads) cuts[i] = 0;
+  __syncthreads();
+
+  // ---- the axis, and every worker's start on it ----
+  const int64_t all_w = scan_costs(cum_w, n_wide, [&](int i) { return static_cast<int64_t>(kWideFixed + tiles[i].steps * kWideStep); }, tmp64);
+  const int64_t all_n = scan_costs(cum_n, n_nar, [&](int i) { return static_cast<int64_t>(kNarrowFixed + tiles[n_wide + i].steps * kNarrowStep); }, tmp64);
+  const int64_t total = (all_w + all_n) * hkv;
+  const int W = a.workers;
+  for (int w = tid; w <= W; w += kPlanThreads) {
+    int unit = units, step = 0;
+    if (w < W && total > 0) {
+      const int64_t x = total / W * w + total % W * w / W;
+      int t, fixed, each;
+      int64_t off;
+      if (x < all_w * hkv) {
+        const int kvh = static_cast<int>(x / all_w);
+        const int64_t y = x - kvh * all_w;
+        t = last_at_most(cum_w, n_wide, y);
+        off = y - cum_w[t];
+        unit = kvh * n_wide + t;
+        fixed = kWideFixed;
+        each = kWideStep;
+      } else {
+        const int64_t y = x - all_w * hkv;
+        const int i = last_at_most(cum_n, n_nar, y / hkv);
+        const int64_t cost = cum_n[i + 1] - cum_n[i], z = y - cum_n[i] * hkv;
+        const int kvh = static_cast<int>(z / cost);
+        t = n_wide + i;
+        off = z - kvh * cost;
+        unit = units_w + i * hkv + kvh;
+        fixed = kNarrowFixed;
+        each = kNarrowStep;
+      }
+      step = off <= fixed ? 0 : static_cast<int>((off - fixed + each / 2) / each);
+      if (step >= tiles[t].steps) {
+        ++unit;
+        step = 0;
+      }
+    }
+    st_unit[w] = unit;
+    st_step[w] = step;
+    starts[2 * w] = unit;
+    starts[2 * w + 1] = step;
+  }
+  __syncthreads();
+  // ---- units that several workers share: the first of them and their number ----
+  auto tile_of = [&](int unit) { return unit < units_w ? unit % n_wide : n_wide + (unit - units_w) / hkv; };
+  for (int w = 1 + tid; w < W; w += kPlanThreads) {
+    const int unit = st_unit[w];
+    if (st_step[w] == 0 || (st_unit[w - 1] == unit && st_step[w - 1] > 0)) continue;
+    int k = w + 1;
+    while (k < W && st_unit[k] == unit) ++k;
+    cuts[unit] = w | (k - w + 1) << 16;  // first worker + 1, workers
+    if (tiles[tile_of(unit)].dest == kToOut) cut_units[atomicAdd(&n_cut, 1)] = unit;
+  }
+  __syncthreads();
+  for (int i = tid; i < n_cut; i += kPlanThreads) st_step[i] = tiles[tile_of(cut_units[i])].rows;
+  __syncthreads();
+  const int rows = scan_lds(st_step, n_cut, tmp);
+  for (int i = tid; i < n_cut; i += kPlanThreads) cut_row0[i] = st_step[i];
+  if (tid == 0) {
+    cut_row0[n_cut] = rows;
+    *head = StepHead{kPlanMagic, B, tokens, a.s.hq, hkv, a.s.d, a.s.bs, a.s.causal, NP, static_cast<int>(a.s.max_own),
+                     static_cast<int>(a.s.max_prefix), W, n_wide, n_nar, n_shared, n_cut, rows, {0, 0, 0}};
+  }
+}
+
+void launch_step_plan(const StepShape& s, const int32_t* token_starts, const int32_t* seq_lens, const int32_t* prefix_ids,
+                      const int32_t* prefix_lens, void* plan, int* err, hipStream_t stream) {
+  const PlanKernelArgs a{s, step_workers(), token_starts, seq_lens, prefix_ids, prefix_lens, static_cast<char*>(plan), plan_layout(s), err};
+  step_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+  HCP_HIP(hipGetLastError());
+}
+
+// ----------------------------------------------------------------------------------
+// Attention
+// ----------------------------------------------------------------------------------
+struct StepArgs {
+  const char* plan;
+  size_t p_tiles, p_shared, p_starts, p_cuts, p_cut_units, p_cut_row0;
+  StepShape s;
+  int32_t workers;
+  const uint16_t* q;
+  int64_t q_hs, q_ss;
+  const uint16_t* pool;
+  int64_t plane_bytes, num_blocks;
+  int32_t rep, gpb, gpb_shift;  // 16-token groups of a block, its log2 or -1
+  const int32_t *tables, *prefix_tables;
+  int64_t table_stride, prefix_stride;
+  float scale_log2;
+  void* out;
+  int64_t out_hs, out_ss;
+  int32_t out_dtype;
+  float* lse;  // [hq, tokens] or null
+  float *slot_o, *slot_lse, *own_o, *own_lse, *pre_o, *pre_lse;
+  int32_t slot_rows;
+  int* err;
+};
+
+namespace {
+
+// Wave-uniform reads through scalar loads: they wait on a counter of their own, not on the
+// K / V loads in flight.
+typedef const __attribute__((address_space(4))) int32_t* scalar_i32;
+__device__ __forceinline__ scalar_i32 scalar_ptr(const void* p) {
+  return (scalar_i32)(reinterpret_cast<uintptr_t>(p));
+}
+
+__device__ __forceinline__ void wait_dma(int left) {  // at most `left` (0 or one K or V part) still in flight
+  if (left == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  else if (left == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+  else if (left == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// Bytes of LDS: the wide tiles' rings (2 K + 3 V of 128 rows); the narrow tiles' 8 x 64 rows,
+// then their 8 results of 32 rows, fit within.
+template <int DW>
+constexpr int kStepLds = 5 * kWideKeys * DW * 2;
+
+// A 16-key group of the paged cache for one kv head: address of its first K row and how many
+// of its rows count; one with a bad block id counts none (its bit is set), so reads of its
+// rows give zeros.
+struct KeyGroup {
+  uint64_t addr;
+  int rows;
+};
+
+template <int DT, int DW>
+struct StepCtx {
+  const StepArgs& a;
+  scalar_i32 p_tab, s_tab;  // table rows of the tile
+  int kvh, d, row_bytes;
+  __device__ __forceinline__ int entry(int key0) const {
+    const int g = key0 >> 4;
+    return a.gpb_shift >= 0 ? g >> a.gpb_shift : g / a.gpb;
+  }
+  // block id of the group at key0 (end: keys of the span), -1 past the end
+  __device__ __forceinline__ int block(scalar_i32 tab, int key0, int end) const {
+    return key0 < end ? tab[entry(key0)] : -1;
+  }
+  __device__ __forceinline__ KeyGroup group(int blk, int key0, int end) const {
+    int rows = min(max(end - key0, 0), 16);
+    if (rows > 0 && (blk < 0 || blk >= a.num_blocks)) {
+      if ((threadIdx.x & 63) == 0) atomicOr(a.err, 1);
+      rows = 0;
+    }
+    const int slot = key0 - entry(key0) * (a.gpb << 4);
+    const int64_t row = rows > 0 ? static_cast<int64_t>(blk) * (a.gpb << 4) + slot : 0;
+    return {reinterpret_cast<uint64_t>(a.pool) + static_cast<uint64_t>(row) * row_bytes + static_cast<uint64_t>(kvh) * d * 2, rows};
+  }
+  __device__ __forceinline__ u32x4 srd(const KeyGroup& g, bool v) const {
+    const uint64_t at = g.addr + (v ? a.plane_bytes : 0);
+    u32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+    r[1] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32) & 0xffffu);
+    r[2] = __builtin_amdgcn_readfirstlane(g.rows > 0 ? static_cast<uint32_t>((g.rows - 1) * row_bytes + d * 2) : 0u);
+    r[3] = 0x00020000u;
+    return r;
+  }
+};
+
+// Destination of row r of a unit: element offsets of its output row and its LSE.
+struct RowDest {
+  void* o;
+  int dtype;
+  int64_t o_off;
+  float* lse;
+};
+__device__ __forceinline__ RowDest row_dest(const StepArgs& a, const StepTile& t, int kvh, int slot, int row, int token, int i, int h) {
+  const int head = kvh * a.rep + h;
+  if (slot >= 0) {
+    const int64_t at = static_cast<int64_t>(slot) * a.slot_rows + row;
+    return {a.slot_o, kF32, at * a.s.d, a.slot_lse + at};
+  }
+  if (t.dest == kToOut)
+    return {a.out, a.out_dtype, head * a.out_hs + token * a.out_ss, a.lse != nullptr ? a.lse + head * a.s.tokens + token : nullptr};
+  const int64_t at = static_cast<int64_t>(t.list0 + i) * a.s.hq + head;
+  return t.dest == kToOwn ? RowDest{a.own_o, kF32, at * a.s.d, a.own_lse + at} : RowDest{a.pre_o, kF32, at * a.s.d, a.pre_lse + at};
+}
+
+template <int DT>
+__device__ __forceinline__ float frag_value(typename MfmaOps<DT>::frag f, int i) {
+  return static_cast<float>(f[i]);
+}
+
+}  // namespace
+
+// TN, TW: terms of 16 bits in which a softmax weight enters the product with V, in narrow and
+// wide tiles.
+template <int DT, int DW, int TN, int TW>
+__global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs a) {
+  using Ops = MfmaOps<DT>;
+  using frag = typename Ops::frag;
+  constexpr int KS = DW / 16, DB = DW / 32;
+  constexpr int PW = DW * 2, CPR = PW / 16, RPI = 1024 / PW;
+  constexpr int NJ = 16 / RPI;  // DMA instructions of a 16-key group
+  __shared__ __attribute__((aligned(1024))) char lds[kStepLds<DW>];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lcol = lane & 31, lhalf = lane >> 5;
+  const scalar_i32 head = scalar_ptr(a.plan);
+  if (!plan_fits(head, a.s, a.workers)) {
+    if (blockIdx.x == 0 && tid == 0) atomicOr(a.err, 8);
+    return;
+  }
+  const int n_wide = head[12], units_w = n_wide * a.s.hkv;
+  const int worker = xcd_remap(blockIdx.x, gridDim.x);
+  const scalar_i32 starts = scalar_ptr(a.plan + a.p_starts) + 2 * worker;
+  const int end_unit = starts[2], end_step = starts[3];
+
+  // Swizzles and fragment addresses as in the ring kernels (rows of 256 or 128 bytes).
+  auto swz_k = [](int r) __attribute__((always_inline)) { return PW == 256 ? (r & 15) : ((r >> 1) & 7); };
+  auto swz_v = [](int r) __attribute__((always_inline)) { return PW == 256 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
+  const int dn = a.s.d, row_bytes = a.s.hkv * dn * 2;
+  uint32_t k_voff[NJ], v_voff[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int r = j * RPI + lane / CPR, p = lane % CPR, kc = p ^ swz_k(r), vc = p ^ swz_v(r);
+    k_voff[j] = kc * 8 < dn ? static_cast<uint32_t>(r * row_bytes + (kc << 4)) : 0x80000000u;
+    v_voff[j] = vc * 8 < dn ? static_cast<uint32_t>(r * row_bytes + (vc << 4)) : 0x80000000u;
+  }
+  const int krow = kperm(lcol);
+  const uint32_t k_rd = krow * PW + ((lhalf ^ swz_k(krow)) << 4);
+  const int g16 = lane >> 4, sl = lane & 15;
+  uint32_t v_rd[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b) {
+    const int vs = PW == 256 ? (sl >> 2) : ((sl >> 3) & 1);
+    v_rd[b] = (8 * (g16 >> 1) + (sl >> 2)) * PW + ((4 * (b ^ vs) + 2 * (g16 & 1) + ((sl & 3) >> 1)) << 4) + 8 * (sl & 1);
+  }
+  const uint32_t lds0 = lds_offset(lds);
+  const float c = a.scale_log2;
+
+  for (int unit = starts[0], s0 = starts[1]; unit < end_unit || (unit == end_unit && s0 < end_step); ++unit, s0 = 0) {
+    const bool wide = unit < units_w;
+    int ti, kvh;
+    if (wide) {
+      kvh = unit / n_wide;
+      ti = unit - kvh * n_wide;
+    } else {
+      ti = (unit - units_w) / a.s.hkv;
+      kvh = unit - units_w - ti * a.s.hkv;
+      ti += n_wide;
+    }
+    StepTile t;
+    {
+      const scalar_i32 tp = scalar_ptr(a.plan + a.p_tiles) + ti * 16;
+      t.tok0 = tp[0]; t.row0 = tp[1]; t.rows = tp[2]; t.p_row = tp[3]; t.p_len = tp[4]; t.s_row = tp[5]; t.s_len = tp[6];
+      t.vis0 = tp[7]; t.vis_step = tp[8]; t.steps = tp[9]; t.dest = tp[10]; t.list0 = tp[11]; t.list = tp[12];
+    }
+    const int s1 = unit == end_unit ? min(end_step, t.steps) : t.steps;
+    const int slot = s0 > 0 ? 2 * worker : s1 < t.steps ? 2 * worker + 1 : -1;
+    StepCtx<DT, DW> ctx{a, scalar_ptr(a.prefix_tables + t.p_row * a.prefix_stride), scalar_ptr(a.tables + t.s_row * a.table_stride),
+                        kvh, dn, row_bytes};
+
+    // this lane's row of the unit
+    const int row = (wide ? wave * 32 : 0) + lcol;
+    const bool has_row = row < t.rows;
+    const int src_row = t.row0 + min(row, t.rows - 1);
+    const int li = src_row / a.rep, lh = src_row - li * a.rep;  // token of the source, head of the group
+    int token = t.tok0 + li;
+    if (t.list) token = reinterpret_cast<const StepShared*>(a.plan + a.p_shared)[token].token;
+    frag qf[KS];
+    {
+      const uint16_t* qrow = a.q + (kvh * a.rep + lh) * a.q_hs + token * a.q_ss;
+      u32x4 x[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int at = 16 * s + 8 * lhalf;
+        x[s] = *reinterpret_cast<const u32x4*>(qrow + (at < dn ? at : 0));
+      }
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qf[s] = as_frag<frag>(16 * s + 8 * lhalf < dn ? x[s] : u32x4{0u, 0u, 0u, 0u});
+    }
+    const int vis = min(max(t.vis0 + li * t.vis_step, 0), t.s_len);                      // own keys this row sees
+    const int first_i = (t.row0 + (wide ? min(wave * 32, t.rows - 1) : 0)) / a.rep;
+    const int vis_min = min(max(t.vis0 + first_i * t.vis_step, 0), t.s_len);             // the wave's fewest
+
+    f32x16 oacc[DB];
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) oacc[b][r] = 0.f;
+    float m_run = kInitMax, l_run = 0.f;
+    __syncthreads();  // the previous unit's reads of LDS are over
+
+    if (!wide) {
+      // ---- narrow: this wave's groups of 32 keys, s0 * 8 + wave, + 8, ... ----
+      const int np = (t.p_len + 31) >> 5, ng = min(np + ((t.s_len + 31) >> 5), s1 * kStepWaves);
+      const uint32_t kbuf = lds0 + wave * (64 * PW), vbuf = kbuf + 32 * PW;
+      constexpr int kDma = 2 * NJ;
+      KeyGroup g0, g1;     // the two 16-key groups being loaded
+      int id0, id1;        // block ids of the ones after them
+      auto span = [&](int g, scalar_i32& tab, int& key0, int& end) __attribute__((always_inline)) {
+        const bool pre = g < np;
+        tab = pre ? ctx.p_tab : ctx.s_tab;
+        key0 = 32 * (pre ? g : g - np);
+        end = g >= ng ? 0 : pre ? t.p_len : t.s_len;
+      };
+      auto fetch = [&](int g) __attribute__((always_inline)) {
+        scalar_i32 tab;
+        int key0, end;
+        span(g, tab, key0, end);
+        id0 = ctx.block(tab, key0, end);
+        id1 = ctx.block(tab, key0 + 16, end);
+      };
+      auto locate = [&](int g) __attribute__((always_inline)) {
+        scalar_i32 tab;
+        int key0, end;
+        span(g, tab, key0, end);
+        g0 = ctx.group(id0, key0, end);
+        g1 = ctx.group(id1, key0 + 16, end);
+      };
+      auto load_k = [&] __attribute__((always_inline)) {
+        const u32x4 a0 = ctx.srd(g0, false), a1 = ctx.srd(g1, false);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) dma16(a0, k_voff[j], kbuf + j * 1024);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) dma16(a1, k_voff[j], kbuf + (NJ + j) * 1024);
+      };
+      auto load_v = [&] __attribute__((always_inline)) {
+        const u32x4 a0 = ctx.srd(g0, true), a1 = ctx.srd(g1, true);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) dma16(a0, v_voff[j], vbuf + j * 1024);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) dma16(a1, v_voff[j], vbuf + (NJ + j) * 1024);
+      };
+      int g = s0 * kStepWaves + wave;
+      bool first = true;
+      if (g < ng) {
+        fetch(g);
+        locate(g);
+        load_k();
+        load_v();
+        fetch(g + kStepWaves);
+      }
+      for (; g < ng; g += kStepWaves) {
+        const bool more = g + kStepWaves < ng;
+        scalar_i32 tab;
+        int key0, end;
+        span(g, tab, key0, end);
+        wait_dma(kDma);  // K is there, V may still be on its way
+        f32x16 sacc;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sacc[r] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const frag kf = as_frag<frag>(*reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
+              static_cast<uintptr_t>((kbuf + k_rd) ^ static_cast<uint32_t>(s << 5))));
+          sacc = Ops::mma(kf, qf[s], sacc);
+        }
+        pin(sacc);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's last reads are done
+        if (more) {
+          locate(g + kStepWaves);
+          load_k();
+          fetch(g + 2 * kStepWaves);
+        }
+        const bool own = g >= np;
+        if (end - key0 < 32 || (own && vis_min < key0 + 32)) {
+          const int lim = min(end - key0, own ? vis - key0 : 32) - 1 - 8 * lhalf;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sacc[r] = 16 * (r >> 3) + 4 * ((r >> 2) & 1) + (r & 3) <= lim ? sacc[r] : -INFINITY;
+        }
+        float p[16];
+        auto weigh = [&] __attribute__((always_inline)) {
+          float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[r], c, -m_run));
+            l4[r & 3] += p[r];
+          }
+          return (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        };
+        float lsum = 0.f;
+        bool redo = first;
+        if (!redo) {
+          lsum = weigh();
+          redo = __any(!(lsum <= kGrowSum));
+        }
+        if (redo) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, sacc[r]);
+          const float m_new = fmaxf(m_run, max_xor32(top) * c);
+          const float alpha = exp2f(m_run - m_new);
+          l_run *= alpha;
+#pragma unroll
+          for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) oacc[b][r] *= alpha;
+          m_run = m_new;
+          lsum = weigh();
+        }
+        l_run += lsum;
+        first = false;
+        wait_dma(more ? kDma : 0);  // V is there
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          frag pf[TN];
+          float rest[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) rest[i] = p[8 * s + i];
+#pragma unroll
+          for (int k = 0; k < TN; ++k) {
+            pf[k] = Ops::pack(rest);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rest[i] -= frag_value<DT>(pf[k], i);
+          }
+#pragma unroll
+          for (int b = 0; b < DB; ++b) {
+            const char* p0 = lds + (vbuf - lds0) + v_rd[b] + s * 16 * PW;
+            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0));
+            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0 + 4 * PW));
+            const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
+            const frag vf = as_frag<frag>(u32x4{lo2[0], lo2[1], hi2[0], hi2[1]});
+#pragma unroll
+            for (int k = 0; k < TN; ++k) oacc[b] = Ops::mma(vf, pf[k], oacc[b]);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < DB; ++b) pin(oacc[b]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) load_v();
+      }
+      // ---- the waves' results meet in LDS: [wave][row][DW + 4] and m, l of every row ----
+      constexpr int OS = DW + 4;
+      float* const os = reinterpret_cast<float*>(lds);
+      float* const ml = os + kStepWaves * kNarrowRows * OS;
+      static_assert((kStepWaves * kNarrowRows * (OS + 2)) * 4 <= kStepLds<DW>, "results fit");
+      const float l_tot = sum_xor32(l_run);
+      __syncthreads();
+      if (has_row) {
+        if (lhalf == 0) {
+          ml[(wave * kNarrowRows + row) * 2] = m_run;
+          ml[(wave * kNarrowRows + row) * 2 + 1] = l_tot;
+        }
+        if (l_tot != 0.f) {
+#pragma unroll
+          for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<f32x4*>(os + (wave * kNarrowRows + row) * OS + 32 * b + 8 * j + 4 * lhalf) =
+                  f32x4{oacc[b][4 * j], oacc[b][4 * j + 1], oacc[b][4 * j + 2], oacc[b][4 * j + 3]};
+        }
+      }
+      __syncthreads();
+      const int d4 = dn / 4;
+      for (int i = tid; i < t.rows * (DW / 4); i += kStepThreads) {
+        const int r = i / (DW / 4), d = (i - r * (DW / 4));
+        if (d >= d4) continue;
+        float m = kInitMax;
+#pragma unroll
+        for (int w = 0; w < kStepWaves; ++w) m = fmaxf(m, ml[(w * kNarrowRows + r) * 2]);
+        float den = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kStepWaves; ++w) {
+          const float lw = ml[(w * kNarrowRows + r) * 2 + 1];
+          if (lw == 0.f) continue;  // took no key
+          const float f = exp2f(ml[(w * kNarrowRows + r) * 2] - m);
+          den += f * lw;
+          const f32x4 o = *reinterpret_cast<const f32x4*>(os + (w * kNarrowRows + r) * OS + 4 * d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] += f * o[e];
+        }
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        const int sr = t.row0 + r, ri = sr / a.rep, rh = sr - ri * a.rep;
+        int tok = t.tok0 + ri;
+        if (t.list) tok = reinterpret_cast<const StepShared*>(a.plan + a.p_shared)[tok].token;
+        const RowDest dst = row_dest(a, t, kvh, slot, r, tok, ri, rh);
+        store4(dst.o, dst.dtype, dst.o_off + 4 * d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        if (d == 0 && dst.lse != nullptr) *dst.lse = den == 0.f ? -INFINITY : (m + __log2f(den)) * kLn2;
+      }
+      continue;
+    }
+
+    // ---- wide: tiles of 128 keys, [0, np) of the prefix, then the sequence's own ----
+    constexpr int BK = kWideKeys, NKB = BK / 32, NPS = BK / 16;
+    constexpr int kTile = BK * PW, NBK = 2, NBV = 3;
+    const int np = (t.p_len + BK - 1) / BK;
+    const int n_tiles = s1 - s0;
+    const uint32_t k_lds0 = lds0, v_lds0 = lds0 + NBK * kTile;
+    const char* v_lds_c = lds + NBK * kTile;
+    int* const simd_of = reinterpret_cast<int*>(lds + (NBK + NBV - 1) * kTile);  // in the last V buffer, first written in super-step 1
+    auto span = [&](int u, scalar_i32& tab, int& key0, int& end) __attribute__((always_inline)) {
+      const int at = s0 + u;
+      const bool pre = at < np;
+      tab = pre ? ctx.p_tab : ctx.s_tab;
+      key0 = BK * (pre ? at : at - np);
+      end = pre ? t.p_len : t.s_len;
+    };
+    int next_id;
+    auto fetch = [&](int u) __attribute__((always_inline)) {
+      if (u >= n_tiles) return;
+      scalar_i32 tab;
+      int key0, end;
+      span(u, tab, key0, end);
+      next_id = ctx.block(tab, key0 + 16 * wave, end);
+    };
+    // wave w loads rows 16 w .. 16 w + 15 of the tile: one 16-key group
+    auto issue_tile = [&](int u) __attribute__((always_inline)) {
+      scalar_i32 tab;
+      int key0, end;
+      span(u, tab, key0, end);
+      const KeyGroup g = ctx.group(next_id, key0 + 16 * wave, end);
+      const u32x4 ks = ctx.srd(g, false), vs = ctx.srd(g, true);
+      const uint32_t kb = k_lds0 + (u % NBK) * kTile + wave * 16 * PW, vb = v_lds0 + (u % NBV) * kTile + wave * 16 * PW;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) dma16(ks, k_voff[j], kb + j * 1024);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) dma16(vs, v_voff[j], vb + j * 1024);
+      fetch(u + 1);
+    };
+    fetch(0);
+    issue_tile(0);
+    if (lane == 0) simd_of[wave] = simd_id();
+    f32x16 sacc[NKB];
+    frag pf[TW == 1 ? NPS : 1];
+
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    bool lead = true;
+    {
+      const int mine = simd_of[wave];
+#pragma unroll
+      for (int w = 0; w < kStepWaves; ++w) lead = lead && !(w < wave && simd_of[w] == mine);
+    }
+    lead = __builtin_amdgcn_readfirstlane(static_cast<int>(lead)) != 0;
+    // last tile with a key that some row of this wave sees
+    int last_live = -1;
+    if (wave * 32 < t.rows) {
+      const int last_i = (t.row0 + min(wave * 32 + 31, t.rows - 1)) / a.rep;
+      const int most = min(max(t.vis0 + last_i * t.vis_step, 0), t.s_len);
+      last_live = min(n_tiles, np + (most + BK - 1) / BK - s0) - 1;
+    }
+    auto live = [&](int u) __attribute__((always_inline)) { return u >= 0 && u <= last_live; };
+
+    auto pv_part = [&](int vb) __attribute__((always_inline)) {
+      const char* vl = v_lds_c + vb * kTile;
+#pragma unroll
+      for (int s = 0; s < NPS; ++s) {
+        frag pk[TW];
+        if constexpr (TW == 1) {
+          pk[0] = pf[s];
+        } else {
+          float rest[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) rest[i] = sacc[s >> 1][8 * (s & 1) + i];
+#pragma unroll
+          for (int k = 0; k < TW; ++k) {
+            pk[k] = Ops::pack(rest);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rest[i] -= frag_value<DT>(pk[k], i);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          const char* p0 = vl + v_rd[b] + s * 16 * PW;
+          const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0));
+          const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0 + 4 * PW));
+          const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
+          const frag vf = as_frag<frag>(u32x4{lo2[0], lo2[1], hi2[0], hi2[1]});
+#pragma unroll
+          for (int k = 0; k < TW; ++k) oacc[b] = Ops::mma(vf, pk[k], oacc[b]);
+        }
+      }
+    };
+    auto s_part = [&](int kb) __attribute__((always_inline)) {
+      const uint32_t kl = k_lds0 + kb * kTile + k_rd;
+#pragma unroll
+      for (int b = 0; b < NKB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sacc[b][r] = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const uint32_t ks = kl ^ static_cast<uint32_t>(s << 5);
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) {
+          const frag kf = as_frag<frag>(*reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
+              static_cast<uintptr_t>(ks + b * 32 * PW)));
+          sacc[b] = Ops::mma(kf, qf[s], sacc[b]);
+        }
+      }
+    };
+    auto m_full = [&](int kb, int vb) __attribute__((always_inline)) {
+      __builtin_amdgcn_s_setprio(1);
+      pv_part(vb);
+      s_part(kb);
+      if constexpr (TW == 1) {
+        constexpr int A = 8, NPV = NPS * DB, NS = NKB * KS;
+        __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
+#pragma unroll
+        for (int i = 0; i < NPV - A / 2; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, A / 2, 0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+      for (int b = 0; b < DB; ++b) pin(oacc[b]);
+#pragma unroll
+      for (int b = 0; b < NKB; ++b) pin(sacc[b]);
+    };
+    auto xphase = [&](int u) __attribute__((always_inline)) {
+      scalar_i32 tab;
+      int key0, end;
+      span(u, tab, key0, end);
+      const bool own = s0 + u >= np;
+      if (end - key0 < BK || (own && vis_min < key0 + BK)) {
+        const int lim = min(min(end - key0, BK), own ? vis - key0 : BK) - 1 - 8 * lhalf;
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            sacc[b][r] = 32 * b + 16 * (r >> 3) + 4 * ((r >> 2) & 1) + (r & 3) <= lim ? sacc[b][r] : -INFINITY;
+      }
+      float lsum = 0.f;
+      // P = 2^(s c - m); the terms for several of them are made from s later, so it stays in place
+      auto weigh = [&](bool keep) __attribute__((always_inline)) {
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) {
+          float p[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[b][r], c, -m_run));
+            ls[r & 3] += p[r];
+          }
+          if constexpr (TW == 1) {
+            pf[2 * b] = Ops::pack(p);
+            pf[2 * b + 1] = Ops::pack(p + 8);
+          } else if (keep) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sacc[b][r] = p[r];
+          }
+        }
+        lsum = (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      };
+      bool redo = u == 0;
+      if (!redo) {
+        weigh(false);
+        redo = __any(!(lsum <= kGrowSum));
+      }
+      if (redo) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, sacc[b][r]);
+        const float m_new = fmaxf(m_run, max_xor32(top) * c);
+        const float alpha = exp2f(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) oacc[b][r] *= alpha;
+        m_run = m_new;
+      }
+      if (redo || TW > 1) weigh(true);
+      l_run += lsum;
+      if constexpr (TW == 1) {
+#pragma unroll
+        for (int s = 0; s < NPS; ++s) pin(pf[s]);
+      } else {
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) pin(sacc[b]);
+      }
+      pin(l_run);
+    };
+    auto issue = [&](int u) __attribute__((always_inline)) {
+      if (u + 1 < n_tiles) issue_tile(u + 1);
+    };
+    auto settle = [&](int u) __attribute__((always_inline)) {
+      if (u < n_tiles) {
+        // K_{u+1} and V_u have to be there; V_{u+1}, issued after K_{u+1}, may be on its way
+        wait_dma(u + 1 < n_tiles ? NJ : 0);
+        __syncthreads();
+      }
+    };
+    const int hot = max(last_live, 0);
+    auto next = [](int r, int nb) __attribute__((always_inline)) { return r + 1 == nb ? 0 : r + 1; };
+    if (lead) {
+      if (live(0)) s_part(0);
+      issue(0);
+      if (live(0)) xphase(0);
+      settle(0);
+    } else {
+      issue(0);
+      if (live(0)) s_part(0);
+      settle(0);
+      issue(1);
+      if (live(0)) xphase(0);
+    }
+    const int lag = lead ? 0 : 1;
+    int u = 1, rk = 1 % NBK, rv = 0;
+    for (; u <= hot; ++u, rk = next(rk, NBK), rv = next(rv, NBV)) {
+      m_full(rk, rv);
+      if (!lead) settle(u);
+      issue(u + lag);
+      xphase(u);
+      if (lead) settle(u);
+    }
+    for (; u <= n_tiles; ++u, rv = next(rv, NBV)) {
+      if (live(u - 1)) pv_part(rv);
+      if (lead) issue(u);
+      settle(u);
+      if (!lead) issue(u + 1);
+    }
+    if (has_row) {
+      const RowDest dst = row_dest(a, t, kvh, slot, row, token, li, lh);
+      write_final_row<DW>(dst.o, dst.dtype, dst.o_off, dst.lse, lhalf, oacc, m_run, sum_xor32(l_run), dn);
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------
+// Join: a wave a row.  The rows of tokens behind shared prefixes (own part and prefix part),
+// then those of cut units; a part is a unit's rows as one worker left them.
+// ----------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
+  const int32_t* head = reinterpret_cast<const int32_t*>(a.plan);
+  if (!plan_fits(head, a.s, a.workers)) return;  // the attention kernel has said so
+  const int n_wide = head[12], n_shared = head[14], n_cut = head[15], cut_rows = head[16];
+  const int units_w = n_wide * a.s.hkv, hkv = a.s.hkv, hq = a.s.hq, d = a.s.d;
+  const StepTile* tiles = reinterpret_cast<const StepTile*>(a.plan + a.p_tiles);
+  const StepShared* shared = reinterpret_cast<const StepShared*>(a.plan + a.p_shared);
+  const int32_t* starts = reinterpret_cast<const int32_t*>(a.plan + a.p_starts);
+  const int32_t* cuts = reinterpret_cast<const int32_t*>(a.plan + a.p_cuts);
+  const int32_t* cut_units = reinterpret_cast<const int32_t*>(a.plan + a.p_cut_units);
+  const int32_t* cut_row0 = reinterpret_cast<const int32_t*>(a.plan + a.p_cut_row0);
+  const int lane = threadIdx.x & 63;
+  const int64_t shared_rows = static_cast<int64_t>(n_shared) * hq, rows = shared_rows + cut_rows;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); i < rows; i += static_cast<int64_t>(gridDim.x) * 4) {
+    // up to two sources of parts: a cut unit's slots or one row
+    const float *o1 = nullptr, *l1 = nullptr;  // an uncut row
+    const float *o2 = nullptr, *l2 = nullptr;
+    int c1 = 0, r1 = 0, c2 = 0, r2 = 0;        // cuts entry and row in the slots
+    int token, hd;
+    if (i < shared_rows) {
+      const int li = static_cast<int>(i / hq);
+      hd = static_cast<int>(i - static_cast<int64_t>(li) * hq);
+      const StepShared s = shared[li];
+      token = s.token;
+      const int kvh = hd / a.rep, h = hd - kvh * a.rep;
+      c1 = cuts[units_w + s.own_tile * hkv + kvh];
+      r1 = s.own_row + h;
+      o1 = a.own_o + i * d;
+      l1 = a.own_lse + i;
+      const int pr = s.pre_row + h;
+      c2 = s.pre_wide ? cuts[kvh * n_wide + s.pre_tile + pr / kWideRows] : cuts[units_w + s.pre_tile * hkv + kvh];
+      r2 = s.pre_wide ? pr % kWideRows : pr;
+      o2 = a.pre_o + i * d;
+      l2 = a.pre_lse + i;
+    } else {
+      const int x = static_cast<int>(i - shared_rows);
+      const int e = last_at_most(cut_row0, n_cut, x), unit = cut_units[e];
+      const int ti = unit < units_w ? unit % n_wide : n_wide + (unit - units_w) / hkv;
+      const int kvh = unit < units_w ? unit / n_wide : (unit - units_w) % hkv;
+      r1 = x - cut_row0[e];
+      c1 = cuts[unit];
+      const int sr = tiles[ti].row0 + r1, ri = sr / a.rep;
+      token = tiles[ti].tok0 + ri;
+      hd = kvh * a.rep + sr - ri * a.rep;
+    }
+    const int w1 = (c1 & 0xffff) - 1, w2 = (c2 & 0xffff) - 1;
+    const int n1 = c1 != 0 ? c1 >> 16 : 1, n2 = o2 == nullptr ? 0 : c2 != 0 ? c2 >> 16 : 1, n = n1 + n2;
+    // part k: its LSE's and its row's address; a worker without steps left nothing
+    auto at = [&](int k, const float*& o) -> const float* {
+      const bool one = k < n1;
+      const int w = one ? w1 : w2, j = one ? k : k - n1;
+      if ((one ? c1 : c2) == 0) {
+        o = one ? o1 : o2;
+        return one ? l1 : l2;
+      }
+      const int worker = w + j;
+      if (starts[2 * worker] == starts[2 * worker + 2] && starts[2 * worker + 1] == starts[2 * worker + 3]) return nullptr;
+      const int64_t row = static_cast<int64_t>(2 * worker + (j == 0 ? 1 : 0)) * a.slot_rows + (one ? r1 : r2);
+      o = a.slot_o + row * d;
+      return a.slot_lse + row;
+    };
+    float m = -INFINITY, den = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int k0 = 0; k0 < n; k0 += 64) {
+      const float* o = nullptr;
+      const float* lp = k0 + lane < n ? at(k0 + lane, o) : nullptr;
+      const float l = lp != nullptr ? *lp : -INFINITY;
+      float top = l;
+      for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+      const float m_new = fmaxf(m, top);
+      const float keep = m == -INFINITY ? 0.f : __expf(m - m_new);
+      // a NaN part (a NaN key) stays one
+      const float f = l == -INFINITY ? 0.f : __expf(l - m_new);
+      m = m_new;
+      float fs = f;
+      for (int off = 32; off >= 1; off >>= 1) fs += __shfl_xor(fs, off);
+      den = den * keep + fs;
+      x0 *= keep;
+      x1 *= keep;
+      const uint64_t ptr = reinterpret_cast<uint64_t>(o);
+      for (int k = 0; k < min(64, n - k0); ++k) {
+        const float fk = __shfl(f, k);
+        const uint64_t pk = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr), k)) |
+                            static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr >> 32), k)) << 32;
+        if (fk == 0.f) continue;
+        const float* ok = reinterpret_cast<const float*>(pk);
+        if (2 * lane < d) {
+          const float2 v = *reinterpret_cast<const float2*>(ok + 2 * lane);
+          x0 += fk * v.x;
+          x1 += fk * v.y;
+        }
+      }
+    }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    if (2 * lane < d) {
+      const int64_t off = hd * a.out_hs + token * a.out_ss + 2 * lane;
+      if (a.out_dtype == kF32) *reinterpret_cast<float2*>(static_cast<float*>(a.out) + off) = make_float2(x0 * inv, x1 * inv);
+      else
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + off) =
+            a.out_dtype == kBF16 ? f32x2_to_bf16x2_bits(x0 * inv, x1 * inv)
+                                 : static_cast<uint32_t>(f32_to_f16_bits(x0 * inv)) | static_cast<uint32_t>(f32_to_f16_bits(x1 * inv)) << 16;
+    }
+    if (lane == 0 && a.lse != nullptr) a.lse[hd * a.s.tokens + token] = den == 0.f ? -INFINITY : m + __logf(den);
+  }
+}
+
+template <int DT, int DW>
+static void launch_step_d(const StepArgs& a, hipStream_t stream) {
+  if (a.out_dtype == kF32) step_attn_kernel<DT, DW, DT == kBF16 ? 3 : 2, DT == kBF16 ? 3 : 2><<<a.workers, kStepThreads, 0, stream>>>(a);
+  else step_attn_kernel<DT, DW, 2, 1><<<a.workers, kStepThreads, 0, stream>>>(a);
+}
+
+void launch_step_attn(const StepLaunch& L, hipStream_t stream) {
+  const PlanLayout l = plan_layout(L.s);
+  const int workers = step_workers();
+  const WorkLayout w = work_layout(L.s, workers);
+  StepArgs a;
+  a.plan = static_cast<const char*>(L.plan);
+  a.p_tiles = l.tiles; a.p_shared = l.shared; a.p_starts = l.starts; a.p_cuts = l.cuts; a.p_cut_units = l.cut_units; a.p_cut_row0 = l.cut_row0;
+  a.s = L.s;
+  a.workers = workers;
+  a.q = static_cast<const uint16_t*>(L.q);
+  a.q_hs = L.q_hs; a.q_ss = L.q_ss;
+  a.pool = static_cast<const uint16_t*>(L.pool);
+  a.num_blocks = L.num_blocks;
+  a.plane_bytes = L.num_blocks * L.s.bs * L.s.hkv * static_cast<int64_t>(L.s.d) * 2;
+  a.rep = L.s.hq / L.s.hkv;
+  a.gpb = L.s.bs / 16;
+  a.gpb_shift = (a.gpb & (a.gpb - 1)) == 0 ? __builtin_ctz(a.gpb) : -1;
+  a.tables = L.tables; a.prefix_tables = L.prefix_tables;
+  a.table_stride = L.table_stride; a.prefix_stride = L.prefix_stride;
+  a.scale_log2 = L.scale * kLog2e;
+  a.out = L.out; a.out_hs = L.out_hs; a.out_ss = L.out_ss; a.out_dtype = L.out_dtype;
+  a.lse = L.lse;
+  char* ws = static_cast<char*>(L.ws);
+  auto f = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
+  a.slot_o = f(w.slot_o); a.slot_lse = f(w.slot_lse); a.own_o = f(w.own_o); a.own_lse = f(w.own_lse);
+  a.pre_o = f(w.pre_o); a.pre_lse = f(w.pre_lse);
+  a.slot_rows = w.slot_rows;
+  a.err = L.err;
+  if (L.dtype == kBF16) {
+    if (L.s.d <= 64) launch_step_d<kBF16, 64>(a, stream);
+    else launch_step_d<kBF16, 128>(a, stream);
+  } else {
+    if (L.s.d <= 64) launch_step_d<kF16, 64>(a, stream);
+    else launch_step_d<kF16, 128>(a, stream);
+  }
+  HCP_HIP(hipGetLastError());
+  step_join_kernel<<<2 * workers, 256, 0, stream>>>(a);
+  HCP_HIP(hipGetLastError());
+}
+
+}  // namespace hcp

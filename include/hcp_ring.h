@@ -110,7 +110,8 @@ int hcp_ring_last_key_parts(void);
  *        consistency check; hcp_ring_block_partial_positioned takes keys in any order
  *        and never sets it);
  * bit 2: a RoPE position outside the cos / sin table;
- * bit 3: lengths or a free-block count that hcp_kv_plan_step cannot follow).
+ * bit 3: lengths or a free-block count that hcp_kv_plan_step cannot follow, lengths or ids that
+ *        hcp_step_attn_plan cannot, or a plan that is not for the hcp_step_attn it came to).
  * Synchronises `stream`.
  */
 int hcp_ring_fetch_device_errors(void* stream, int* flags);
@@ -825,6 +826,51 @@ int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float e
                             hcp_ring_view k, hcp_ring_view v, const void* q_weight, const void* k_weight,
                             const int64_t* positions, const float* rope_table, hcp_ring_view q_out,
                             const hcp_paged_pool* pool, const int64_t* slots, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * (12) Attention of a serving step over the paged cache (no reference counterpart: it attends
+ * one sequence at a time, and reads a prefix that several share for each of them).
+ *
+ * The step's new tokens are the rows of q [Hq, tokens, D]: those of sequence b are
+ * token_starts[b] <= i < token_starts[b + 1] (as hcp_kv_plan_step writes them; what lies past
+ * `tokens` is left out).  Sequence b holds seq_lens[b] tokens of its own, the new ones
+ * included, in row b of block_tables, and behind them all of prefix prefix_ids[b] (-1: none):
+ * the first prefixes->seq_lens[p] tokens of row p of prefixes->block_tables.  Its i-th of n new
+ * tokens sees the whole prefix and its own tokens j with j <= seq_lens[b] - n + i (causal = 1)
+ * or all of them (0, a peer domain's shard).  out [Hq, tokens, D] (out_dtype: dtype, or F32 for
+ * a partial) gets softmax(q k^T scale) v and lse [Hq, tokens] fp32 (may be NULL) the natural
+ * log-sum-exp: 0 and -inf where nothing is seen.  Rows of no sequence are left as they are.
+ *
+ * A prefix is read once for all the tokens behind it of sequences with up to 32 / (Hq / Hkv)
+ * new tokens; longer runs of tokens read it for themselves.
+ *
+ * hcp_step_attn_plan lays the step's work out over the GPU from the lengths (DEVICE memory,
+ * nothing is read on the host: a captured graph follows them); hcp_step_attn then takes the
+ * plan, for every layer of the step, with any q, pool, tables and outputs of the same shape
+ * (descriptor, tokens, causal, table lengths, num_prefixes; desc->t0 / t1 are ignored, as is
+ * prefixes->max_len).  A plan of another shape sets device error bit 3 and writes nothing.
+ * Lengths outside their tables, decreasing token_starts and prefix ids outside
+ * [-1, num_prefixes) set bit 3 too and are cut to what fits (an id: none).  A block id outside
+ * [0, num_blocks) sets bit 0, and its tokens count as rows of zeros.
+ * dtype BF16 or F16; head_dim a multiple of 8 up to 128; block_size a multiple of 16; up to
+ * 4096 sequences and 1024 prefixes; Hq / Hkv up to 256.  q and out 16-byte aligned with strides
+ * of whole 16 bytes.  plan and workspace: DEVICE memory, 256-byte aligned, of the bytes that
+ * the size queries report (0 for a bad shape); the workspace is scratch of one call, the plan
+ * is only read.
+ * ------------------------------------------------------------------------------- */
+size_t hcp_step_attn_plan_size(const hcp_paged_decode_desc* desc, int64_t tokens, int32_t num_prefixes);
+
+size_t hcp_step_attn_workspace_size(const hcp_paged_decode_desc* desc, int64_t tokens, int32_t num_prefixes);
+
+int hcp_step_attn_plan(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool, int64_t tokens, int32_t causal,
+                       const int32_t* token_starts, const int32_t* seq_lens, int32_t num_prefixes,
+                       const hcp_decode_shard* prefixes, const int32_t* prefix_ids, void* plan,
+                       size_t plan_bytes, void* stream);
+
+int hcp_step_attn(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool, int64_t tokens, int32_t causal,
+                  hcp_ring_view q, const int32_t* block_tables, int32_t num_prefixes,
+                  const hcp_decode_shard* prefixes, const void* plan, size_t plan_bytes, int32_t out_dtype,
+                  hcp_ring_view out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * Replay kernel timing (no reference counterpart; benchmark instrumentation; the
