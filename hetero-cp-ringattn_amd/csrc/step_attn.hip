@@ -12,11 +12,12 @@
 // tile: 8 waves hold the same rows and take 32 keys each in turn, out of LDS of their own,
 // with no barrier until their results meet.
 //
-// Work.  All (tile, kv head) units are laid end to end on an axis of modelled time, the wide
-// ones by kv head first (workgroups of one XCD then read one head's K and V), and dealt in
-// equal parts to one workgroup a CU: a unit that falls to several is joined afterwards
-// (step_join_kernel), as is a row's part behind a shared prefix with its own part.  The plan
-// (step_plan_kernel) lays the axis out once a step for the calls of all layers.
+// Work.  The (tile, kv head) units of each kind are laid end to end on an axis of modelled time,
+// the wide ones by kv head first (workgroups of one XCD then read one head's K and V), and
+// dealt in equal parts to one workgroup a CU: a unit that falls to several is joined afterwards
+// (step_join_kernel), as is a row's part behind a shared prefix with its own part.  One launch
+// holds the wide workers and, behind them, the narrow ones.  The plan (step_plan_kernel) lays
+// both axes out once a step for the calls of all layers.
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -104,15 +105,15 @@ PlanLayout plan_layout(const StepShape& s) {
   l.cum_wide = take((l.max_wide + 1) * sizeof(int64_t));
   l.cum_narrow = take((l.max_narrow + 1) * sizeof(int64_t));
   l.shared = take(l.max_shared * sizeof(StepShared));
-  l.starts = take((kStepMaxWorkers + 1) * 2 * sizeof(int32_t));
+  l.starts = take(2 * (kStepMaxWorkers + 1) * 2 * sizeof(int32_t));
   l.cuts = take(l.max_units * sizeof(int32_t));
-  l.cut_units = take(kStepMaxWorkers * sizeof(int32_t));
-  l.cut_row0 = take((kStepMaxWorkers + 1) * sizeof(int32_t));
+  l.cut_units = take(2 * kStepMaxWorkers * sizeof(int32_t));
+  l.cut_row0 = take((2 * kStepMaxWorkers + 1) * sizeof(int32_t));
   l.bytes = at;
   return l;
 }
 
-// The workspace: two slots of partial rows a worker (its first and its last unit, where cut),
+// The workspace: two slots of partial rows a worker of either kind (its first and its last unit, where cut),
 // then the rows of tokens behind shared prefixes, their own part and the prefix's.
 struct WorkLayout {
   int32_t slot_rows;
@@ -128,7 +129,7 @@ WorkLayout work_layout(const StepShape& s, int workers) {
     at += up256(floats * sizeof(float));
     return here;
   };
-  const size_t slots = 2 * static_cast<size_t>(workers) * w.slot_rows;
+  const size_t slots = 4 * static_cast<size_t>(workers + 1) * w.slot_rows;  // by the worker's place in the plan's starts
   const size_t rows = static_cast<size_t>(plan_layout(s).max_shared) * s.hq;
   w.slot_o = take(slots * s.d);
   w.slot_lse = take(slots);
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
       g_nar[kStepMaxPrefixes];
   __shared__ int64_t tmp64[kPlanThreads / 64];
   __shared__ int tmp[kPlanThreads / 64];
-  __shared__ int st_unit[kStepMaxWorkers + 1], st_step[kStepMaxWorkers + 1];
+  __shared__ int st_unit[2 * (kStepMaxWorkers + 1)], st_step[2 * (kStepMaxWorkers + 1)];
   __shared__ int n_cut;
 
   const int tid = threadIdx.x;
@@ -399,18 +400,21 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
   for (int i = tid; i < units; i += kPlanThreads) cuts[i] = 0;
   __syncthreads();
 
-  // ---- the axis, and every worker's start on it ----
+  // ---- the two axes, and every worker's start on them: worker w of the wide ones at w, of the
+  // narrow ones at W + 1 + w, the ends behind each ----
   const int64_t all_w = scan_costs(cum_w, n_wide, [&](int i) { return static_cast<int64_t>(kWideFixed + tiles[i].steps * kWideStep); }, tmp64);
   const int64_t all_n = scan_costs(cum_n, n_nar, [&](int i) { return static_cast<int64_t>(kNarrowFixed + tiles[n_wide + i].steps * kNarrowStep); }, tmp64);
-  const int64_t total = (all_w + all_n) * hkv;
   const int W = a.workers;
-  for (int w = tid; w <= W; w += kPlanThreads) {
-    int unit = units, step = 0;
+  for (int i = tid; i < 2 * (W + 1); i += kPlanThreads) {
+    const bool narrow = i > W;
+    const int w = narrow ? i - W - 1 : i;
+    const int64_t all = narrow ? all_n : all_w, total = all * hkv;
+    int unit = narrow ? units : units_w, step = 0;
     if (w < W && total > 0) {
       const int64_t x = total / W * w + total % W * w / W;
       int t, fixed, each;
       int64_t off;
-      if (x < all_w * hkv) {
+      if (!narrow) {
         const int kvh = static_cast<int>(x / all_w);
         const int64_t y = x - kvh * all_w;
         t = last_at_most(cum_w, n_wide, y);
@@ -419,13 +423,12 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
         fixed = kWideFixed;
         each = kWideStep;
       } else {
-        const int64_t y = x - all_w * hkv;
-        const int i = last_at_most(cum_n, n_nar, y / hkv);
-        const int64_t cost = cum_n[i + 1] - cum_n[i], z = y - cum_n[i] * hkv;
+        const int k = last_at_most(cum_n, n_nar, x / hkv);
+        const int64_t cost = cum_n[k + 1] - cum_n[k], z = x - cum_n[k] * hkv;
         const int kvh = static_cast<int>(z / cost);
-        t = n_wide + i;
+        t = n_wide + k;
         off = z - kvh * cost;
-        unit = units_w + i * hkv + kvh;
+        unit = units_w + k * hkv + kvh;
         fixed = kNarrowFixed;
         each = kNarrowStep;
       }
@@ -435,20 +438,20 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
         step = 0;
       }
     }
-    st_unit[w] = unit;
-    st_step[w] = step;
-    starts[2 * w] = unit;
-    starts[2 * w + 1] = step;
+    st_unit[i] = unit;
+    st_step[i] = step;
+    starts[2 * i] = unit;
+    starts[2 * i + 1] = step;
   }
   __syncthreads();
   // ---- units that several workers share: the first of them and their number ----
   auto tile_of = [&](int unit) { return unit < units_w ? unit % n_wide : n_wide + (unit - units_w) / hkv; };
-  for (int w = 1 + tid; w < W; w += kPlanThreads) {
-    const int unit = st_unit[w];
-    if (st_step[w] == 0 || (st_unit[w - 1] == unit && st_step[w - 1] > 0)) continue;
-    int k = w + 1;
-    while (k < W && st_unit[k] == unit) ++k;
-    cuts[unit] = w | (k - w + 1) << 16;  // first worker + 1, workers
+  for (int i = tid; i < 2 * (W + 1); i += kPlanThreads) {
+    const int unit = st_unit[i];
+    if (st_step[i] == 0 || (st_unit[i - 1] == unit && st_step[i - 1] > 0)) continue;  // an axis starts at step 0
+    int k = i + 1;
+    while (st_unit[k] == unit) ++k;
+    cuts[unit] = i | (k - i + 1) << 16;  // first worker's place + 1, workers
     if (tiles[tile_of(unit)].dest == kToOut) cut_units[atomicAdd(&n_cut, 1)] = unit;
   }
   __syncthreads();
@@ -524,35 +527,52 @@ struct KeyGroup {
   int rows;
 };
 
-template <int DT, int DW>
-struct StepCtx {
-  const StepArgs& a;
+// The kernel's arguments as they lie in memory.  Read through `again`, a value is loaded where
+// it is used, not kept in scalar registers across a unit's loop.
+typedef const __attribute__((address_space(4))) StepArgs* args_ptr;
+__device__ __forceinline__ args_ptr again(args_ptr a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+s"(a));
+#endif
+  return a;
+}
+
+// What the loads of a unit go by.
+struct StepKeys {
   scalar_i32 p_tab, s_tab;  // table rows of the tile
-  int kvh, d, row_bytes;
+  int p_len, s_len;
+  uint64_t base;            // the kv head's first K row of block 0
+  int64_t plane_bytes;
+  int num_blocks, gpb, gpb_shift, row_bytes, span_bytes;  // span_bytes: of a row's head
+  __device__ __forceinline__ StepKeys(args_ptr a, const StepTile& t, int kvh)
+      : p_tab(scalar_ptr(a->prefix_tables + t.p_row * a->prefix_stride)), s_tab(scalar_ptr(a->tables + t.s_row * a->table_stride)),
+        p_len(t.p_len), s_len(t.s_len), base(reinterpret_cast<uint64_t>(a->pool) + static_cast<uint64_t>(kvh) * a->s.d * 2),
+        plane_bytes(a->plane_bytes), num_blocks(static_cast<int>(a->num_blocks)), gpb(a->gpb), gpb_shift(a->gpb_shift),
+        row_bytes(a->s.hkv * a->s.d * 2), span_bytes(a->s.d * 2) {}
   __device__ __forceinline__ int entry(int key0) const {
     const int g = key0 >> 4;
-    return a.gpb_shift >= 0 ? g >> a.gpb_shift : g / a.gpb;
+    return gpb_shift >= 0 ? g >> gpb_shift : g / gpb;
   }
-  // block id of the group at key0 (end: keys of the span), -1 past the end
-  __device__ __forceinline__ int block(scalar_i32 tab, int key0, int end) const {
-    return key0 < end ? tab[entry(key0)] : -1;
+  // block id of the group at key0 of the prefix or the own keys, -1 past the end
+  __device__ __forceinline__ int block(bool pre, int key0) const {
+    return key0 < (pre ? p_len : s_len) ? (pre ? p_tab : s_tab)[entry(key0)] : -1;
   }
-  __device__ __forceinline__ KeyGroup group(int blk, int key0, int end) const {
-    int rows = min(max(end - key0, 0), 16);
-    if (rows > 0 && (blk < 0 || blk >= a.num_blocks)) {
-      if ((threadIdx.x & 63) == 0) atomicOr(a.err, 1);
+  __device__ __forceinline__ KeyGroup group(int blk, bool pre, int key0, args_ptr a) const {
+    int rows = min(max((pre ? p_len : s_len) - key0, 0), 16);
+    if (rows > 0 && (blk < 0 || blk >= num_blocks)) {
+      if ((threadIdx.x & 63) == 0) atomicOr(again(a)->err, 1);
       rows = 0;
     }
-    const int slot = key0 - entry(key0) * (a.gpb << 4);
-    const int64_t row = rows > 0 ? static_cast<int64_t>(blk) * (a.gpb << 4) + slot : 0;
-    return {reinterpret_cast<uint64_t>(a.pool) + static_cast<uint64_t>(row) * row_bytes + static_cast<uint64_t>(kvh) * d * 2, rows};
+    const int slot = key0 - entry(key0) * (gpb << 4);
+    const int64_t row = rows > 0 ? static_cast<int64_t>(blk) * (gpb << 4) + slot : 0;
+    return {base + static_cast<uint64_t>(row) * row_bytes, rows};
   }
   __device__ __forceinline__ u32x4 srd(const KeyGroup& g, bool v) const {
-    const uint64_t at = g.addr + (v ? a.plane_bytes : 0);
+    const uint64_t at = g.addr + (v ? plane_bytes : 0);
     u32x4 r;
     r[0] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
     r[1] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32) & 0xffffu);
-    r[2] = __builtin_amdgcn_readfirstlane(g.rows > 0 ? static_cast<uint32_t>((g.rows - 1) * row_bytes + d * 2) : 0u);
+    r[2] = __builtin_amdgcn_readfirstlane(g.rows > 0 ? static_cast<uint32_t>((g.rows - 1) * row_bytes + span_bytes) : 0u);
     r[3] = 0x00020000u;
     return r;
   }
@@ -565,16 +585,104 @@ struct RowDest {
   int64_t o_off;
   float* lse;
 };
-__device__ __forceinline__ RowDest row_dest(const StepArgs& a, const StepTile& t, int kvh, int slot, int row, int token, int i, int h) {
-  const int head = kvh * a.rep + h;
+__device__ __forceinline__ RowDest row_dest(args_ptr a, const StepTile& t, int kvh, int slot, int row, int token, int i, int h) {
+  const int head = kvh * a->rep + h, d = a->s.d;
   if (slot >= 0) {
-    const int64_t at = static_cast<int64_t>(slot) * a.slot_rows + row;
-    return {a.slot_o, kF32, at * a.s.d, a.slot_lse + at};
+    const int64_t at = static_cast<int64_t>(slot) * a->slot_rows + row;
+    return {a->slot_o, kF32, at * d, a->slot_lse + at};
   }
   if (t.dest == kToOut)
-    return {a.out, a.out_dtype, head * a.out_hs + token * a.out_ss, a.lse != nullptr ? a.lse + head * a.s.tokens + token : nullptr};
-  const int64_t at = static_cast<int64_t>(t.list0 + i) * a.s.hq + head;
-  return t.dest == kToOwn ? RowDest{a.own_o, kF32, at * a.s.d, a.own_lse + at} : RowDest{a.pre_o, kF32, at * a.s.d, a.pre_lse + at};
+    return {a->out, a->out_dtype, head * a->out_hs + token * a->out_ss, a->lse != nullptr ? a->lse + head * a->s.tokens + token : nullptr};
+  const int64_t at = static_cast<int64_t>(t.list0 + i) * a->s.hq + head;
+  return t.dest == kToOwn ? RowDest{a->own_o, kF32, at * d, a->own_lse + at} : RowDest{a->pre_o, kF32, at * d, a->pre_lse + at};
+}
+
+// Row `row` of a tile: token i of its source and query head h of the group, and the token's row
+// of the query.
+struct RowOf {
+  int i, h, token;
+};
+__device__ __forceinline__ RowOf row_of(args_ptr a, const StepTile& t, int row) {
+  const int r = t.row0 + min(row, t.rows - 1), i = r / a->rep;
+  int token = t.tok0 + i;
+  if (t.list) token = reinterpret_cast<const StepShared*>(a->plan + a->p_shared)[token].token;
+  return {i, r - i * a->rep, token};
+}
+
+__device__ __forceinline__ StepTile read_tile(args_ptr a, int ti) {
+  const scalar_i32 tp = scalar_ptr(a->plan + a->p_tiles) + ti * 16;
+  StepTile t;
+  t.tok0 = tp[0]; t.row0 = tp[1]; t.rows = tp[2]; t.p_row = tp[3]; t.p_len = tp[4]; t.s_row = tp[5]; t.s_len = tp[6];
+  t.vis0 = tp[7]; t.vis_step = tp[8]; t.steps = tp[9]; t.dest = tp[10]; t.list0 = tp[11]; t.list = tp[12];
+  return t;
+}
+
+// Own keys that token i of the tile's source sees.
+__device__ __forceinline__ int sees(const StepTile& t, int i) { return min(max(t.vis0 + i * t.vis_step, 0), t.s_len); }
+
+// An opaque copy: what is worked out from it stays where it is used.  Hoisted out of the loops, the
+// lane constants of a unit's loads and stores are registers that the wide tiles do not have: they
+// went through scratch memory, whose loads wait for the K and V loads before them (a prompt of
+// 16384 tokens, 32/8 heads, 4.4 ms so).
+template <typename T>
+__device__ __forceinline__ T fresh(T x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(x));
+#endif
+  return x;
+}
+__device__ __forceinline__ uint32_t fresh_lane() {
+  return fresh(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)));
+}
+
+// Where a lane reads and writes K and V rows in LDS: the swizzles and fragment addresses of the
+// ring kernels (rows of 256 or 128 bytes).  A group of 16 keys takes NJ loads of RPI rows
+// (1 KiB); load j holds row j RPI + r0 in lane r0 CPR + p, whose chunk is p ^ swizzle(row).
+template <int DW>
+struct StepLanes {
+  static constexpr int PW = DW * 2, CPR = PW / 16, RPI = 1024 / PW, NJ = 16 / RPI, DB = DW / 32;
+  uint32_t k_rd, v_rd0;
+  __device__ __forceinline__ explicit StepLanes(int lane) {
+    const int krow = kperm(lane & 31), g16 = lane >> 4, sl = lane & 15;
+    k_rd = krow * PW + (((lane >> 5) ^ (PW == 256 ? (krow & 15) : ((krow >> 1) & 7))) << 4);
+    const int vs = PW == 256 ? (sl >> 2) : ((sl >> 3) & 1);
+    v_rd0 = (8 * (g16 >> 1) + (sl >> 2)) * PW + ((4 * vs + 2 * (g16 & 1) + ((sl & 3) >> 1)) << 4) + 8 * (sl & 1);
+  }
+  // The NJ loads of a group's K or V rows to LDS at `to`: the K swizzle of row j RPI + r0 is that
+  // of r0 with bits 2 and 3 of the chunk flipped by j, the V swizzle the same for all j.  Chunks
+  // past the head dim (span_bytes) lie out of range and give zeros.
+  static __device__ __forceinline__ void load_k(u32x4 srd, uint32_t to, uint32_t row_bytes, uint32_t span_bytes) {
+    const uint32_t lane = fresh_lane(), r0 = lane / CPR, c0 = ((lane % CPR) ^ (PW == 256 ? r0 : r0 >> 1)) << 4, row0 = r0 * row_bytes;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const uint32_t ch = c0 ^ (j << 6);
+      dma16(srd, ch < span_bytes ? ch + row0 + j * RPI * row_bytes : 0x80000000u, to + j * 1024);
+    }
+  }
+  static __device__ __forceinline__ void load_v(u32x4 srd, uint32_t to, uint32_t row_bytes, uint32_t span_bytes) {
+    const uint32_t lane = fresh_lane(), r0 = lane / CPR, ch = ((lane % CPR) ^ (PW == 256 ? 4 * r0 : 4 * ((r0 >> 1) & 1))) << 4;
+    const uint32_t v0 = ch < span_bytes ? ch + r0 * row_bytes : 0x80000000u;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) dma16(srd, v0 + j * RPI * row_bytes, to + j * 1024);
+  }
+  // LDS byte of this lane's half of the V^T fragment of dims 32 b .. + 31, key step 0
+  static __device__ __forceinline__ uint32_t v_rd(uint32_t rd0, int b) { return rd0 ^ (b << 6); }
+};
+
+// Q fragments of a row: dims 16 s + 8 (lane / 32) .. + 7 of step s, zeros past the head dim.
+template <int DT, int DW>
+__device__ __forceinline__ void load_q(args_ptr a, const RowOf& r, int kvh, int lhalf, typename MfmaOps<DT>::frag (&qf)[DW / 16]) {
+  const int dn = a->s.d;
+  const uint16_t* qrow = a->q + (kvh * a->rep + r.h) * a->q_hs + r.token * a->q_ss;
+  u32x4 x[DW / 16];
+#pragma unroll
+  for (int s = 0; s < DW / 16; ++s) {
+    const int at = 16 * s + 8 * lhalf;
+    x[s] = *reinterpret_cast<const u32x4*>(qrow + (at < dn ? at : 0));
+  }
+#pragma unroll
+  for (int s = 0; s < DW / 16; ++s)
+    qf[s] = as_frag<typename MfmaOps<DT>::frag>(16 * s + 8 * lhalf < dn ? x[s] : u32x4{0u, 0u, 0u, 0u});
 }
 
 template <int DT>
@@ -584,98 +692,34 @@ __device__ __forceinline__ float frag_value(typename MfmaOps<DT>::frag f, int i)
 
 }  // namespace
 
-// TN, TW: terms of 16 bits in which a softmax weight enters the product with V, in narrow and
-// wide tiles.
-template <int DT, int DW, int TN, int TW>
-__global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs a) {
+// The narrow units of the worker at `place` of the plan's starts.  TN: terms of 16 bits in which
+// a softmax weight enters the product with V.
+template <int DT, int DW, int TN>
+__device__ __forceinline__ void step_narrow(args_ptr a, int place, char* lds) {
   using Ops = MfmaOps<DT>;
   using frag = typename Ops::frag;
-  constexpr int KS = DW / 16, DB = DW / 32;
-  constexpr int PW = DW * 2, CPR = PW / 16, RPI = 1024 / PW;
-  constexpr int NJ = 16 / RPI;  // DMA instructions of a 16-key group
-  __shared__ __attribute__((aligned(1024))) char lds[kStepLds<DW>];
-
+  using Lanes = StepLanes<DW>;
+  constexpr int KS = DW / 16, DB = Lanes::DB, PW = Lanes::PW, NJ = Lanes::NJ;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lcol = lane & 31, lhalf = lane >> 5;
-  const scalar_i32 head = scalar_ptr(a.plan);
-  if (!plan_fits(head, a.s, a.workers)) {
-    if (blockIdx.x == 0 && tid == 0) atomicOr(a.err, 8);
-    return;
-  }
-  const int n_wide = head[12], units_w = n_wide * a.s.hkv;
-  const int worker = xcd_remap(blockIdx.x, gridDim.x);
-  const scalar_i32 starts = scalar_ptr(a.plan + a.p_starts) + 2 * worker;
+  const int n_wide = scalar_ptr(a->plan)[12];
+  const scalar_i32 starts = scalar_ptr(a->plan + a->p_starts) + 2 * place;
   const int end_unit = starts[2], end_step = starts[3];
-
-  // Swizzles and fragment addresses as in the ring kernels (rows of 256 or 128 bytes).
-  auto swz_k = [](int r) __attribute__((always_inline)) { return PW == 256 ? (r & 15) : ((r >> 1) & 7); };
-  auto swz_v = [](int r) __attribute__((always_inline)) { return PW == 256 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
-  const int dn = a.s.d, row_bytes = a.s.hkv * dn * 2;
-  uint32_t k_voff[NJ], v_voff[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int r = j * RPI + lane / CPR, p = lane % CPR, kc = p ^ swz_k(r), vc = p ^ swz_v(r);
-    k_voff[j] = kc * 8 < dn ? static_cast<uint32_t>(r * row_bytes + (kc << 4)) : 0x80000000u;
-    v_voff[j] = vc * 8 < dn ? static_cast<uint32_t>(r * row_bytes + (vc << 4)) : 0x80000000u;
-  }
-  const int krow = kperm(lcol);
-  const uint32_t k_rd = krow * PW + ((lhalf ^ swz_k(krow)) << 4);
-  const int g16 = lane >> 4, sl = lane & 15;
-  uint32_t v_rd[DB];
-#pragma unroll
-  for (int b = 0; b < DB; ++b) {
-    const int vs = PW == 256 ? (sl >> 2) : ((sl >> 3) & 1);
-    v_rd[b] = (8 * (g16 >> 1) + (sl >> 2)) * PW + ((4 * (b ^ vs) + 2 * (g16 & 1) + ((sl & 3) >> 1)) << 4) + 8 * (sl & 1);
-  }
+  const Lanes at(lane);
   const uint32_t lds0 = lds_offset(lds);
-  const float c = a.scale_log2;
-
+  const float c = a->scale_log2;
   for (int unit = starts[0], s0 = starts[1]; unit < end_unit || (unit == end_unit && s0 < end_step); ++unit, s0 = 0) {
-    const bool wide = unit < units_w;
-    int ti, kvh;
-    if (wide) {
-      kvh = unit / n_wide;
-      ti = unit - kvh * n_wide;
-    } else {
-      ti = (unit - units_w) / a.s.hkv;
-      kvh = unit - units_w - ti * a.s.hkv;
-      ti += n_wide;
-    }
-    StepTile t;
-    {
-      const scalar_i32 tp = scalar_ptr(a.plan + a.p_tiles) + ti * 16;
-      t.tok0 = tp[0]; t.row0 = tp[1]; t.rows = tp[2]; t.p_row = tp[3]; t.p_len = tp[4]; t.s_row = tp[5]; t.s_len = tp[6];
-      t.vis0 = tp[7]; t.vis_step = tp[8]; t.steps = tp[9]; t.dest = tp[10]; t.list0 = tp[11]; t.list = tp[12];
-    }
+    const args_ptr b0 = again(a);
+    const int un = unit - n_wide * b0->s.hkv, ti = un / b0->s.hkv, kvh = un - ti * b0->s.hkv;
+    const StepTile t = read_tile(b0, n_wide + ti);
     const int s1 = unit == end_unit ? min(end_step, t.steps) : t.steps;
-    const int slot = s0 > 0 ? 2 * worker : s1 < t.steps ? 2 * worker + 1 : -1;
-    StepCtx<DT, DW> ctx{a, scalar_ptr(a.prefix_tables + t.p_row * a.prefix_stride), scalar_ptr(a.tables + t.s_row * a.table_stride),
-                        kvh, dn, row_bytes};
-
-    // this lane's row of the unit
-    const int row = (wide ? wave * 32 : 0) + lcol;
-    const bool has_row = row < t.rows;
-    const int src_row = t.row0 + min(row, t.rows - 1);
-    const int li = src_row / a.rep, lh = src_row - li * a.rep;  // token of the source, head of the group
-    int token = t.tok0 + li;
-    if (t.list) token = reinterpret_cast<const StepShared*>(a.plan + a.p_shared)[token].token;
+    const int slot = s0 > 0 ? 2 * place : s1 < t.steps ? 2 * place + 1 : -1;
+    const StepKeys keys(b0, t, kvh);
     frag qf[KS];
-    {
-      const uint16_t* qrow = a.q + (kvh * a.rep + lh) * a.q_hs + token * a.q_ss;
-      u32x4 x[KS];
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int at = 16 * s + 8 * lhalf;
-        x[s] = *reinterpret_cast<const u32x4*>(qrow + (at < dn ? at : 0));
-      }
-#pragma unroll
-      for (int s = 0; s < KS; ++s) qf[s] = as_frag<frag>(16 * s + 8 * lhalf < dn ? x[s] : u32x4{0u, 0u, 0u, 0u});
-    }
-    const int vis = min(max(t.vis0 + li * t.vis_step, 0), t.s_len);                      // own keys this row sees
-    const int first_i = (t.row0 + (wide ? min(wave * 32, t.rows - 1) : 0)) / a.rep;
-    const int vis_min = min(max(t.vis0 + first_i * t.vis_step, 0), t.s_len);             // the wave's fewest
-
+    const RowOf mine = row_of(b0, t, lcol);
+    load_q<DT, DW>(b0, mine, kvh, lhalf, qf);
+    const int vis = sees(t, mine.i), vis_min = sees(t, t.row0 / b0->rep);  // own keys this row and the first one see
     f32x16 oacc[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b)
@@ -684,195 +728,211 @@ __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs a) 
     float m_run = kInitMax, l_run = 0.f;
     __syncthreads();  // the previous unit's reads of LDS are over
 
-    if (!wide) {
-      // ---- narrow: this wave's groups of 32 keys, s0 * 8 + wave, + 8, ... ----
-      const int np = (t.p_len + 31) >> 5, ng = min(np + ((t.s_len + 31) >> 5), s1 * kStepWaves);
-      const uint32_t kbuf = lds0 + wave * (64 * PW), vbuf = kbuf + 32 * PW;
-      constexpr int kDma = 2 * NJ;
-      KeyGroup g0, g1;     // the two 16-key groups being loaded
-      int id0, id1;        // block ids of the ones after them
-      auto span = [&](int g, scalar_i32& tab, int& key0, int& end) __attribute__((always_inline)) {
-        const bool pre = g < np;
-        tab = pre ? ctx.p_tab : ctx.s_tab;
-        key0 = 32 * (pre ? g : g - np);
-        end = g >= ng ? 0 : pre ? t.p_len : t.s_len;
-      };
-      auto fetch = [&](int g) __attribute__((always_inline)) {
-        scalar_i32 tab;
-        int key0, end;
-        span(g, tab, key0, end);
-        id0 = ctx.block(tab, key0, end);
-        id1 = ctx.block(tab, key0 + 16, end);
-      };
-      auto locate = [&](int g) __attribute__((always_inline)) {
-        scalar_i32 tab;
-        int key0, end;
-        span(g, tab, key0, end);
-        g0 = ctx.group(id0, key0, end);
-        g1 = ctx.group(id1, key0 + 16, end);
-      };
-      auto load_k = [&] __attribute__((always_inline)) {
-        const u32x4 a0 = ctx.srd(g0, false), a1 = ctx.srd(g1, false);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) dma16(a0, k_voff[j], kbuf + j * 1024);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) dma16(a1, k_voff[j], kbuf + (NJ + j) * 1024);
-      };
-      auto load_v = [&] __attribute__((always_inline)) {
-        const u32x4 a0 = ctx.srd(g0, true), a1 = ctx.srd(g1, true);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) dma16(a0, v_voff[j], vbuf + j * 1024);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) dma16(a1, v_voff[j], vbuf + (NJ + j) * 1024);
-      };
-      int g = s0 * kStepWaves + wave;
-      bool first = true;
-      if (g < ng) {
-        fetch(g);
-        locate(g);
-        load_k();
-        load_v();
-        fetch(g + kStepWaves);
-      }
-      for (; g < ng; g += kStepWaves) {
-        const bool more = g + kStepWaves < ng;
-        scalar_i32 tab;
-        int key0, end;
-        span(g, tab, key0, end);
-        wait_dma(kDma);  // K is there, V may still be on its way
-        f32x16 sacc;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sacc[r] = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const frag kf = as_frag<frag>(*reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
-              static_cast<uintptr_t>((kbuf + k_rd) ^ static_cast<uint32_t>(s << 5))));
-          sacc = Ops::mma(kf, qf[s], sacc);
-        }
-        pin(sacc);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's last reads are done
-        if (more) {
-          locate(g + kStepWaves);
-          load_k();
-          fetch(g + 2 * kStepWaves);
-        }
-        const bool own = g >= np;
-        if (end - key0 < 32 || (own && vis_min < key0 + 32)) {
-          const int lim = min(end - key0, own ? vis - key0 : 32) - 1 - 8 * lhalf;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sacc[r] = 16 * (r >> 3) + 4 * ((r >> 2) & 1) + (r & 3) <= lim ? sacc[r] : -INFINITY;
-        }
-        float p[16];
-        auto weigh = [&] __attribute__((always_inline)) {
-          float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[r], c, -m_run));
-            l4[r & 3] += p[r];
-          }
-          return (l4[0] + l4[1]) + (l4[2] + l4[3]);
-        };
-        float lsum = 0.f;
-        bool redo = first;
-        if (!redo) {
-          lsum = weigh();
-          redo = __any(!(lsum <= kGrowSum));
-        }
-        if (redo) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, sacc[r]);
-          const float m_new = fmaxf(m_run, max_xor32(top) * c);
-          const float alpha = exp2f(m_run - m_new);
-          l_run *= alpha;
-#pragma unroll
-          for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) oacc[b][r] *= alpha;
-          m_run = m_new;
-          lsum = weigh();
-        }
-        l_run += lsum;
-        first = false;
-        wait_dma(more ? kDma : 0);  // V is there
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          frag pf[TN];
-          float rest[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) rest[i] = p[8 * s + i];
-#pragma unroll
-          for (int k = 0; k < TN; ++k) {
-            pf[k] = Ops::pack(rest);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) rest[i] -= frag_value<DT>(pf[k], i);
-          }
-#pragma unroll
-          for (int b = 0; b < DB; ++b) {
-            const char* p0 = lds + (vbuf - lds0) + v_rd[b] + s * 16 * PW;
-            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0));
-            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0 + 4 * PW));
-            const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
-            const frag vf = as_frag<frag>(u32x4{lo2[0], lo2[1], hi2[0], hi2[1]});
-#pragma unroll
-            for (int k = 0; k < TN; ++k) oacc[b] = Ops::mma(vf, pf[k], oacc[b]);
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < DB; ++b) pin(oacc[b]);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (more) load_v();
-      }
-      // ---- the waves' results meet in LDS: [wave][row][DW + 4] and m, l of every row ----
-      constexpr int OS = DW + 4;
-      float* const os = reinterpret_cast<float*>(lds);
-      float* const ml = os + kStepWaves * kNarrowRows * OS;
-      static_assert((kStepWaves * kNarrowRows * (OS + 2)) * 4 <= kStepLds<DW>, "results fit");
-      const float l_tot = sum_xor32(l_run);
-      __syncthreads();
-      if (has_row) {
-        if (lhalf == 0) {
-          ml[(wave * kNarrowRows + row) * 2] = m_run;
-          ml[(wave * kNarrowRows + row) * 2 + 1] = l_tot;
-        }
-        if (l_tot != 0.f) {
-#pragma unroll
-          for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<f32x4*>(os + (wave * kNarrowRows + row) * OS + 32 * b + 8 * j + 4 * lhalf) =
-                  f32x4{oacc[b][4 * j], oacc[b][4 * j + 1], oacc[b][4 * j + 2], oacc[b][4 * j + 3]};
-        }
-      }
-      __syncthreads();
-      const int d4 = dn / 4;
-      for (int i = tid; i < t.rows * (DW / 4); i += kStepThreads) {
-        const int r = i / (DW / 4), d = (i - r * (DW / 4));
-        if (d >= d4) continue;
-        float m = kInitMax;
-#pragma unroll
-        for (int w = 0; w < kStepWaves; ++w) m = fmaxf(m, ml[(w * kNarrowRows + r) * 2]);
-        float den = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kStepWaves; ++w) {
-          const float lw = ml[(w * kNarrowRows + r) * 2 + 1];
-          if (lw == 0.f) continue;  // took no key
-          const float f = exp2f(ml[(w * kNarrowRows + r) * 2] - m);
-          den += f * lw;
-          const f32x4 o = *reinterpret_cast<const f32x4*>(os + (w * kNarrowRows + r) * OS + 4 * d);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] += f * o[e];
-        }
-        const float inv = den == 0.f ? 0.f : 1.f / den;
-        const int sr = t.row0 + r, ri = sr / a.rep, rh = sr - ri * a.rep;
-        int tok = t.tok0 + ri;
-        if (t.list) tok = reinterpret_cast<const StepShared*>(a.plan + a.p_shared)[tok].token;
-        const RowDest dst = row_dest(a, t, kvh, slot, r, tok, ri, rh);
-        store4(dst.o, dst.dtype, dst.o_off + 4 * d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-        if (d == 0 && dst.lse != nullptr) *dst.lse = den == 0.f ? -INFINITY : (m + __log2f(den)) * kLn2;
-      }
-      continue;
+    // ---- narrow: this wave's groups of 32 keys, s0 * 8 + wave, + 8, ... ----
+    const int np = (t.p_len + 31) >> 5, ng = min(np + ((t.s_len + 31) >> 5), s1 * kStepWaves);
+    const uint32_t kbuf = lds0 + wave * (64 * PW), vbuf = kbuf + 32 * PW;
+    constexpr int kDma = 2 * NJ;
+    KeyGroup g0, g1;     // the two 16-key groups being loaded
+    int id0, id1;        // block ids of the ones after them
+    auto key_of = [&](int g) __attribute__((always_inline)) { return 32 * (g < np ? g : g - np); };
+    auto fetch = [&](int g) __attribute__((always_inline)) {
+      if (g >= ng) return;
+      id0 = keys.block(g < np, key_of(g));
+      id1 = keys.block(g < np, key_of(g) + 16);
+    };
+    auto locate = [&](int g) __attribute__((always_inline)) {
+      g0 = keys.group(id0, g < np, key_of(g), a);
+      g1 = keys.group(id1, g < np, key_of(g) + 16, a);
+    };
+    auto load_k = [&] __attribute__((always_inline)) {
+      Lanes::load_k(keys.srd(g0, false), kbuf, keys.row_bytes, keys.span_bytes);
+      Lanes::load_k(keys.srd(g1, false), kbuf + NJ * 1024, keys.row_bytes, keys.span_bytes);
+    };
+    auto load_v = [&] __attribute__((always_inline)) {
+      Lanes::load_v(keys.srd(g0, true), vbuf, keys.row_bytes, keys.span_bytes);
+      Lanes::load_v(keys.srd(g1, true), vbuf + NJ * 1024, keys.row_bytes, keys.span_bytes);
+    };
+    int g = s0 * kStepWaves + wave;
+    bool first = true;
+    if (g < ng) {
+      fetch(g);
+      locate(g);
+      load_k();
+      load_v();
+      fetch(g + kStepWaves);
     }
+    for (; g < ng; g += kStepWaves) {
+      const bool more = g + kStepWaves < ng;
+      const bool own = g >= np;
+      const int key0 = key_of(g), end = own ? t.s_len : t.p_len;
+      wait_dma(kDma);  // K is there, V may still be on its way
+      f32x16 sacc;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sacc[r] = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const frag kf = as_frag<frag>(*reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
+            static_cast<uintptr_t>((kbuf + at.k_rd) ^ static_cast<uint32_t>(s << 5))));
+        sacc = Ops::mma(kf, qf[s], sacc);
+      }
+      pin(sacc);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's last reads are done
+      if (more) {
+        locate(g + kStepWaves);
+        load_k();
+        fetch(g + 2 * kStepWaves);
+      }
+      if (end - key0 < 32 || (own && vis_min < key0 + 32)) {
+        const int lim = min(end - key0, own ? vis - key0 : 32) - 1 - 8 * lhalf;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sacc[r] = 16 * (r >> 3) + 4 * ((r >> 2) & 1) + (r & 3) <= lim ? sacc[r] : -INFINITY;
+      }
+      float p[16];
+      auto weigh = [&] __attribute__((always_inline)) {
+        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[r], c, -m_run));
+          l4[r & 3] += p[r];
+        }
+        return (l4[0] + l4[1]) + (l4[2] + l4[3]);
+      };
+      float lsum = 0.f;
+      bool redo = first;
+      if (!redo) {
+        lsum = weigh();
+        redo = __any(!(lsum <= kGrowSum));
+      }
+      if (redo) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, sacc[r]);
+        const float m_new = fmaxf(m_run, max_xor32(top) * c);
+        const float alpha = exp2f(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) oacc[b][r] *= alpha;
+        m_run = m_new;
+        lsum = weigh();
+      }
+      l_run += lsum;
+      first = false;
+      wait_dma(more ? kDma : 0);  // V is there
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        frag pf[TN];
+        float rest[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rest[i] = p[8 * s + i];
+#pragma unroll
+        for (int k = 0; k < TN; ++k) {
+          pf[k] = Ops::pack(rest);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) rest[i] -= frag_value<DT>(pf[k], i);
+        }
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          const char* p0 = lds + (vbuf - lds0) + Lanes::v_rd(at.v_rd0, b) + s * 16 * PW;
+          const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0));
+          const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0 + 4 * PW));
+          const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
+          const frag vf = as_frag<frag>(u32x4{lo2[0], lo2[1], hi2[0], hi2[1]});
+#pragma unroll
+          for (int k = 0; k < TN; ++k) oacc[b] = Ops::mma(vf, pf[k], oacc[b]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < DB; ++b) pin(oacc[b]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) load_v();
+    }
+    // ---- the waves' results meet in LDS: [wave][row][DW + 4] and m, l of every row ----
+    constexpr int OS = DW + 4;
+    float* const os = reinterpret_cast<float*>(lds);
+    float* const ml = os + kStepWaves * kNarrowRows * OS;
+    static_assert((kStepWaves * kNarrowRows * (OS + 2)) * 4 <= kStepLds<DW>, "results fit");
+    const float l_tot = sum_xor32(l_run);
+    __syncthreads();
+    if (lcol < t.rows) {
+      if (lhalf == 0) {
+        ml[(wave * kNarrowRows + lcol) * 2] = m_run;
+        ml[(wave * kNarrowRows + lcol) * 2 + 1] = l_tot;
+      }
+      if (l_tot != 0.f) {
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<f32x4*>(os + (wave * kNarrowRows + lcol) * OS + 32 * b + 8 * j + 4 * lhalf) =
+                f32x4{oacc[b][4 * j], oacc[b][4 * j + 1], oacc[b][4 * j + 2], oacc[b][4 * j + 3]};
+      }
+    }
+    __syncthreads();
+    const args_ptr e = again(a);
+    const int d4 = e->s.d / 4;
+    for (int i = tid; i < t.rows * (DW / 4); i += kStepThreads) {
+      const int r = i / (DW / 4), d = i - r * (DW / 4);
+      if (d >= d4) continue;
+      float m = kInitMax;
+#pragma unroll
+      for (int w = 0; w < kStepWaves; ++w) m = fmaxf(m, ml[(w * kNarrowRows + r) * 2]);
+      float den = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kStepWaves; ++w) {
+        const float lw = ml[(w * kNarrowRows + r) * 2 + 1];
+        if (lw == 0.f) continue;  // took no key
+        const float f = exp2f(ml[(w * kNarrowRows + r) * 2] - m);
+        den += f * lw;
+        const f32x4 o = *reinterpret_cast<const f32x4*>(os + (w * kNarrowRows + r) * OS + 4 * d);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] += f * o[k];
+      }
+      const float inv = den == 0.f ? 0.f : 1.f / den;
+      const RowOf ro = row_of(e, t, r);
+      const RowDest dst = row_dest(e, t, kvh, slot, r, ro.token, ro.i, ro.h);
+      store4(dst.o, dst.dtype, dst.o_off + 4 * d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+      if (d == 0 && dst.lse != nullptr) *dst.lse = den == 0.f ? -INFINITY : (m + __log2f(den)) * kLn2;
+    }
+  }
+}
+
+// The wide units of the worker at `place`.  TW: as TN.
+template <int DT, int DW, int TW>
+__device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
+  using Ops = MfmaOps<DT>;
+  using frag = typename Ops::frag;
+  using Lanes = StepLanes<DW>;
+  constexpr int KS = DW / 16, DB = Lanes::DB, PW = Lanes::PW, NJ = Lanes::NJ;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lcol = lane & 31, lhalf = lane >> 5;
+  const int n_wide = scalar_ptr(a->plan)[12];
+  const scalar_i32 starts = scalar_ptr(a->plan + a->p_starts) + 2 * place;
+  const int end_unit = starts[2], end_step = starts[3];
+  const Lanes at(lane);
+  const uint32_t lds0 = lds_offset(lds);
+  const float c = a->scale_log2;
+  for (int unit = starts[0], s0 = starts[1]; unit < end_unit || (unit == end_unit && s0 < end_step); ++unit, s0 = 0) {
+    const args_ptr b0 = again(a);
+    const int kvh = unit / n_wide;
+    const StepTile t = read_tile(b0, unit - kvh * n_wide);
+    const int s1 = unit == end_unit ? min(end_step, t.steps) : t.steps;
+    const int slot = s0 > 0 ? 2 * place : s1 < t.steps ? 2 * place + 1 : -1;
+    const StepKeys keys(b0, t, kvh);
+    frag qf[KS];
+    const RowOf mine = row_of(b0, t, wave * 32 + lcol);
+    load_q<DT, DW>(b0, mine, kvh, lhalf, qf);
+    // own keys that this row and the wave's first one see
+    const int vis = sees(t, mine.i), vis_min = sees(t, (t.row0 + min(wave * 32, t.rows - 1)) / b0->rep);
+    f32x16 oacc[DB];
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) oacc[b][r] = 0.f;
+    float m_run = kInitMax, l_run = 0.f;
+    __syncthreads();  // the previous unit's reads of LDS are over
 
     // ---- wide: tiles of 128 keys, [0, np) of the prefix, then the sequence's own ----
     constexpr int BK = kWideKeys, NKB = BK / 32, NPS = BK / 16;
@@ -882,33 +942,18 @@ __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs a) 
     const uint32_t k_lds0 = lds0, v_lds0 = lds0 + NBK * kTile;
     const char* v_lds_c = lds + NBK * kTile;
     int* const simd_of = reinterpret_cast<int*>(lds + (NBK + NBV - 1) * kTile);  // in the last V buffer, first written in super-step 1
-    auto span = [&](int u, scalar_i32& tab, int& key0, int& end) __attribute__((always_inline)) {
-      const int at = s0 + u;
-      const bool pre = at < np;
-      tab = pre ? ctx.p_tab : ctx.s_tab;
-      key0 = BK * (pre ? at : at - np);
-      end = pre ? t.p_len : t.s_len;
-    };
+    auto key_of = [&](int u) __attribute__((always_inline)) { return BK * (s0 + u < np ? s0 + u : s0 + u - np); };
     int next_id;
     auto fetch = [&](int u) __attribute__((always_inline)) {
-      if (u >= n_tiles) return;
-      scalar_i32 tab;
-      int key0, end;
-      span(u, tab, key0, end);
-      next_id = ctx.block(tab, key0 + 16 * wave, end);
+      if (u < n_tiles) next_id = keys.block(s0 + u < np, key_of(u) + 16 * wave);
     };
     // wave w loads rows 16 w .. 16 w + 15 of the tile: one 16-key group
     auto issue_tile = [&](int u) __attribute__((always_inline)) {
-      scalar_i32 tab;
-      int key0, end;
-      span(u, tab, key0, end);
-      const KeyGroup g = ctx.group(next_id, key0 + 16 * wave, end);
-      const u32x4 ks = ctx.srd(g, false), vs = ctx.srd(g, true);
+      const KeyGroup g = keys.group(next_id, s0 + u < np, key_of(u) + 16 * wave, a);
+      const u32x4 ks = keys.srd(g, false), vs = keys.srd(g, true);
       const uint32_t kb = k_lds0 + (u % NBK) * kTile + wave * 16 * PW, vb = v_lds0 + (u % NBV) * kTile + wave * 16 * PW;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) dma16(ks, k_voff[j], kb + j * 1024);
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) dma16(vs, v_voff[j], vb + j * 1024);
+      Lanes::load_k(ks, kb, keys.row_bytes, keys.span_bytes);
+      Lanes::load_v(vs, vb, keys.row_bytes, keys.span_bytes);
       fetch(u + 1);
     };
     fetch(0);
@@ -929,14 +974,14 @@ __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs a) 
     // last tile with a key that some row of this wave sees
     int last_live = -1;
     if (wave * 32 < t.rows) {
-      const int last_i = (t.row0 + min(wave * 32 + 31, t.rows - 1)) / a.rep;
-      const int most = min(max(t.vis0 + last_i * t.vis_step, 0), t.s_len);
+      const int most = sees(t, (t.row0 + min(wave * 32 + 31, t.rows - 1)) / a->rep);
       last_live = min(n_tiles, np + (most + BK - 1) / BK - s0) - 1;
     }
     auto live = [&](int u) __attribute__((always_inline)) { return u >= 0 && u <= last_live; };
 
     auto pv_part = [&](int vb) __attribute__((always_inline)) {
       const char* vl = v_lds_c + vb * kTile;
+      const uint32_t rd0 = fresh(at.v_rd0);
 #pragma unroll
       for (int s = 0; s < NPS; ++s) {
         frag pk[TW];
@@ -955,7 +1000,7 @@ __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs a) 
         }
 #pragma unroll
         for (int b = 0; b < DB; ++b) {
-          const char* p0 = vl + v_rd[b] + s * 16 * PW;
+          const char* p0 = vl + Lanes::v_rd(rd0, b) + s * 16 * PW;
           const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0));
           const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p0 + 4 * PW));
           const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
@@ -966,7 +1011,7 @@ __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs a) 
       }
     };
     auto s_part = [&](int kb) __attribute__((always_inline)) {
-      const uint32_t kl = k_lds0 + kb * kTile + k_rd;
+      const uint32_t kl = k_lds0 + kb * kTile + at.k_rd;
 #pragma unroll
       for (int b = 0; b < NKB; ++b)
 #pragma unroll
@@ -1008,12 +1053,10 @@ __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs a) 
       for (int b = 0; b < NKB; ++b) pin(sacc[b]);
     };
     auto xphase = [&](int u) __attribute__((always_inline)) {
-      scalar_i32 tab;
-      int key0, end;
-      span(u, tab, key0, end);
       const bool own = s0 + u >= np;
+      const int key0 = key_of(u), end = own ? t.s_len : t.p_len;
       if (end - key0 < BK || (own && vis_min < key0 + BK)) {
-        const int lim = min(min(end - key0, BK), own ? vis - key0 : BK) - 1 - 8 * lhalf;
+        const int lim = min(min(end - key0, BK), own ? vis - key0 : BK) - 1 - 8 * static_cast<int>(fresh_lane() >> 5);
 #pragma unroll
         for (int b = 0; b < NKB; ++b)
 #pragma unroll
@@ -1112,11 +1155,29 @@ __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs a) 
       settle(u);
       if (!lead) issue(u + 1);
     }
-    if (has_row) {
-      const RowDest dst = row_dest(a, t, kvh, slot, row, token, li, lh);
-      write_final_row<DW>(dst.o, dst.dtype, dst.o_off, dst.lse, lhalf, oacc, m_run, sum_xor32(l_run), dn);
+    const args_ptr e = again(a);
+    const int row = wave * 32 + (static_cast<int>(fresh_lane()) & 31);
+    if (row < t.rows) {
+      const RowOf ro = row_of(e, t, row);
+      const RowDest dst = row_dest(e, t, kvh, slot, row, ro.token, ro.i, ro.h);
+      write_final_row<DW>(dst.o, dst.dtype, dst.o_off, dst.lse, static_cast<int>(fresh_lane() >> 5), oacc, m_run, sum_xor32(l_run), e->s.d);
     }
   }
+}
+
+// Workgroups 0 .. W - 1 hold the wide units, W .. 2 W - 1 the narrow ones.
+template <int DT, int DW, int TN, int TW>
+__global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs args) {
+  __shared__ __attribute__((aligned(1024))) char lds[kStepLds<DW>];
+  const args_ptr a = (args_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  const scalar_i32 head = scalar_ptr(a->plan);
+  if (!plan_fits(head, args.s, args.workers)) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(args.err, 8);
+    return;
+  }
+  const int workers = a->workers, bid = blockIdx.x;
+  if (bid < workers) step_wide<DT, DW, TW>(a, xcd_remap(bid, workers), lds);
+  else step_narrow<DT, DW, TN>(a, workers + 1 + xcd_remap(bid - workers, workers), lds);
 }
 
 // ----------------------------------------------------------------------------------
@@ -1168,7 +1229,7 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
       token = tiles[ti].tok0 + ri;
       hd = kvh * a.rep + sr - ri * a.rep;
     }
-    const int w1 = (c1 & 0xffff) - 1, w2 = (c2 & 0xffff) - 1;
+    const int w1 = (c1 & 0xffff) - 1, w2 = (c2 & 0xffff) - 1;  // place of the first worker
     const int n1 = c1 != 0 ? c1 >> 16 : 1, n2 = o2 == nullptr ? 0 : c2 != 0 ? c2 >> 16 : 1, n = n1 + n2;
     // part k: its LSE's and its row's address; a worker without steps left nothing
     auto at = [&](int k, const float*& o) -> const float* {
@@ -1230,8 +1291,8 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
 
 template <int DT, int DW>
 static void launch_step_d(const StepArgs& a, hipStream_t stream) {
-  if (a.out_dtype == kF32) step_attn_kernel<DT, DW, DT == kBF16 ? 3 : 2, DT == kBF16 ? 3 : 2><<<a.workers, kStepThreads, 0, stream>>>(a);
-  else step_attn_kernel<DT, DW, 2, 1><<<a.workers, kStepThreads, 0, stream>>>(a);
+  if (a.out_dtype == kF32) step_attn_kernel<DT, DW, DT == kBF16 ? 3 : 2, DT == kBF16 ? 3 : 2><<<2 * a.workers, kStepThreads, 0, stream>>>(a);
+  else step_attn_kernel<DT, DW, 2, 1><<<2 * a.workers, kStepThreads, 0, stream>>>(a);
 }
 
 void launch_step_attn(const StepLaunch& L, hipStream_t stream) {
