@@ -2109,6 +2109,7 @@ StepShape step_call(const hcp_paged_decode_desc* d, const hcp_paged_pool* pool, 
   require(d->num_kv_heads == pool->num_kv_heads && d->head_dim == pool->head_dim && pool->elem_bytes == 2,
           "pool does not match the descriptor");
   require(pool->num_blocks <= INT32_MAX, "num_blocks must be in [1, 2^31)");
+  require(static_cast<int64_t>(pool->block_size) * pool->num_kv_heads * pool->head_dim < (int64_t(1) << 30), "blocks of 2^31 bytes or more");
   require(aligned(pool->data, 16), "the pool must be 16-byte aligned");
   const size_t need = step_plan_bytes(s);
   if (plan == nullptr || plan_bytes < need) throw Error(-6, "plan too small: need " + std::to_string(need) + " bytes");

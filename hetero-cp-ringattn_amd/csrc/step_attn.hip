@@ -13,11 +13,11 @@
 // with no barrier until their results meet.
 //
 // Work.  The (tile, kv head) units of each kind are laid end to end on an axis of modelled time,
-// the wide ones by kv head first (workgroups of one XCD then read one head's K and V), and
-// dealt in equal parts to one workgroup a CU: a unit that falls to several is joined afterwards
-// (step_join_kernel), as is a row's part behind a shared prefix with its own part.  One launch
-// holds the wide workers and, behind them, the narrow ones.  The plan (step_plan_kernel) lays
-// both axes out once a step for the calls of all layers.
+// the wide ones by kv head first (workgroups of one XCD then read one head's K and V).  Every XCD
+// gets an eighth of both, and its workgroups, one a CU, equal parts of that: a unit that falls to
+// several is joined afterwards (step_join_kernel), as is a row's part behind a shared prefix with
+// its own part.  The
+// plan (step_plan_kernel) lays both axes out once a step for the calls of all layers.
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -33,13 +33,30 @@ constexpr int kStepThreads = 64 * kStepWaves;
 constexpr int kWideRows = 32 * kStepWaves;  // rows of a wide tile
 constexpr int kWideKeys = 128;              // keys of its steps
 constexpr int kNarrowRows = 32;
+#ifndef NMOST
+#define NMOST 128
+#endif
+constexpr int kNarrowMost = NMOST;             // most rows of a source that is cut into narrow tiles
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMagic = 0x53544550;
 
 // Modelled time in 0.1 us: of a unit beside its steps, and of a step of 128 (wide) or up to
 // 8 x 32 keys (narrow).
-constexpr int kWideFixed = 60, kWideStep = 22;
-constexpr int kNarrowFixed = 30, kNarrowStep = 45;
+#ifndef CWF
+#define CWF 100
+#define CWS 36
+#endif
+#ifndef CNF
+#define CNF 55
+#define CNS 40
+#endif
+constexpr int kWideFixed = CWF, kWideStep = CWS;
+constexpr int kNarrowFixed = CNF, kNarrowStep = CNS;
+#ifndef LSH
+#define LSH 130
+#endif
+constexpr int kLeastShare = LSH;  // of a worker: less is not worth another part to join
+constexpr int kXcds = 8;
 
 // Where a unit's rows go when it is not cut.
 enum { kToOut = 0, kToOwn = 1, kToPrefix = 2 };
@@ -60,8 +77,8 @@ static_assert(sizeof(StepTile) == 64, "a tile is a cache line");
 // A token behind a shared prefix: its own narrow tile, and its rows in the prefix's tiles.
 struct StepShared {
   int32_t token;
-  int32_t own_tile, own_row;           // narrow tile (counted from 0), row of its first head
-  int32_t pre_tile, pre_row, pre_wide; // the prefix's first tile (wide or narrow), row of its first head
+  int32_t own_tile, own_row;           // the sequence's first narrow tile (counted from 0), row of the token's first head
+  int32_t pre_tile, pre_row, pre_wide; // the same of the prefix's tiles, wide or narrow
   int32_t pad[2];
 };
 
@@ -91,9 +108,10 @@ size_t up256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 PlanLayout plan_layout(const StepShape& s) {
   const int64_t rep = s.hq / s.hkv, live = std::min<int64_t>(s.batch, s.tokens);
   PlanLayout l;
-  l.max_shared = s.prefixes > 0 ? std::min<int64_t>(s.tokens, live * std::max<int64_t>(1, kNarrowRows / rep)) : 0;
+  l.max_shared = s.prefixes > 0 ? std::min<int64_t>(s.tokens, live * (kNarrowMost / rep)) : 0;
   l.max_wide = s.tokens * rep / kWideRows + live + (s.prefixes > 0 ? l.max_shared * rep / kWideRows + std::min<int64_t>(s.prefixes, live) : 0);
-  l.max_narrow = live + std::min<int64_t>(s.prefixes, live);
+  const int64_t each = kNarrowMost / kNarrowRows;  // narrow tiles of a source
+  l.max_narrow = std::min(s.tokens * rep / kNarrowRows + live, live * each) + std::min<int64_t>(s.prefixes, live) * each;
   l.max_units = (l.max_wide + l.max_narrow) * s.hkv;
   size_t at = up256(sizeof(StepHead));
   auto take = [&](size_t bytes) {
@@ -292,7 +310,7 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
     s_vis[b] = a.s.causal ? static_cast<int>(max(len - (static_cast<int64_t>(t1) - t0) + 1, static_cast<int64_t>(INT32_MIN / 2)))
                           : static_cast<int>(len);
     s_pid[b] = pid;
-    const bool narrow = n > 0 && static_cast<int64_t>(n) * rep <= kNarrowRows;
+    const bool narrow = n > 0 && static_cast<int64_t>(n) * rep <= kNarrowMost;
     if (narrow && pid >= 0) {
       atomicAdd(&g_seq[pid], 1);
       atomicAdd(&g_tok[pid], n);
@@ -305,8 +323,8 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
     const int rows = on ? g_tok[p] * rep : 0;
     if (!on) g_seq[p] = 0;
     g_list[p] = on ? g_tok[p] : 0;
-    g_wide[p] = rows > kNarrowRows ? (rows + kWideRows - 1) / kWideRows : 0;
-    g_nar[p] = rows > 0 && rows <= kNarrowRows ? 1 : 0;
+    g_wide[p] = rows > kNarrowMost ? (rows + kWideRows - 1) / kWideRows : 0;
+    g_nar[p] = rows <= kNarrowMost ? (rows + kNarrowRows - 1) / kNarrowRows : 0;
   }
   __syncthreads();
   const int n_shared = NP > 0 ? scan_lds(g_list, NP, tmp) : 0;
@@ -314,8 +332,8 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
   const int pre_nar = NP > 0 ? scan_lds(g_nar, NP, tmp) : 0;
   for (int b = tid; b < B; b += kPlanThreads) {
     const int64_t rows = static_cast<int64_t>(s_n[b]) * rep;
-    s_wide[b] = rows > kNarrowRows ? static_cast<int>((rows + kWideRows - 1) / kWideRows) : 0;
-    s_nar[b] = rows > 0 && rows <= kNarrowRows ? 1 : 0;
+    s_wide[b] = rows > kNarrowMost ? static_cast<int>((rows + kWideRows - 1) / kWideRows) : 0;
+    s_nar[b] = rows <= kNarrowMost ? static_cast<int>((rows + kNarrowRows - 1) / kNarrowRows) : 0;
   }
   __syncthreads();
   const int n_wide = pre_wide + scan_lds(s_wide, B, tmp);
@@ -324,7 +342,7 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
   // ---- the list of tokens behind shared prefixes, and the narrow tiles of sequences ----
   for (int b = tid; b < B; b += kPlanThreads) {
     const int n = s_n[b], rows = n * rep;
-    if (n == 0 || static_cast<int64_t>(n) * rep > kNarrowRows) continue;
+    if (n == 0 || static_cast<int64_t>(n) * rep > kNarrowMost) continue;
     const int p = s_pid[b];
     const bool on = p >= 0 && g_seq[p] > 0;
     const int own = pre_nar + s_nar[b];
@@ -333,42 +351,54 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
       // place behind the earlier sequences of the same prefix
       at = g_list[p];
       for (int c = 0; c < b; ++c)
-        if (s_pid[c] == p && static_cast<int64_t>(s_n[c]) * rep <= kNarrowRows) at += s_n[c];
-      const int wide = g_tok[p] * rep > kNarrowRows;
+        if (s_pid[c] == p && static_cast<int64_t>(s_n[c]) * rep <= kNarrowMost) at += s_n[c];
+      const int wide = g_tok[p] * rep > kNarrowMost;
       for (int i = 0; i < n; ++i)
         shared[at + i] = StepShared{s_tok[b] + i, own, i * rep, wide ? g_wide[p] : g_nar[p], (at + i - g_list[p]) * rep, wide, {0, 0}};
     }
     const int vstep = a.s.causal ? 1 : 0;
-    StepTile t{};
-    t.tok0 = s_tok[b];
-    t.rows = rows;
-    t.p_row = max(p, 0);
-    t.p_len = p >= 0 && !on ? prefix_len(p) : 0;
-    t.s_row = b;
-    t.s_len = max(0, min(s_len[b], s_vis[b] + (n - 1) * vstep));
-    t.vis0 = s_vis[b];
-    t.vis_step = vstep;
-    t.steps = max(1, ((t.p_len + 31) / 32 + (t.s_len + 31) / 32 + kStepWaves - 1) / kStepWaves);
-    t.dest = on ? kToOwn : kToOut;
-    t.list0 = at;
-    tiles[n_wide + own] = t;
+    for (int k = 0; k * kNarrowRows < rows; ++k) {
+      StepTile t{};
+      t.tok0 = s_tok[b];
+      t.row0 = k * kNarrowRows;
+      t.rows = min(kNarrowRows, rows - t.row0);
+      t.p_row = max(p, 0);
+      t.p_len = p >= 0 && !on ? prefix_len(p) : 0;
+      t.s_row = b;
+      t.s_len = max(0, min(s_len[b], s_vis[b] + (t.row0 + t.rows - 1) / rep * vstep));
+      t.vis0 = s_vis[b];
+      t.vis_step = vstep;
+      t.steps = max(1, ((t.p_len + 31) / 32 + (t.s_len + 31) / 32 + kStepWaves - 1) / kStepWaves);
+      t.dest = on ? kToOwn : kToOut;
+      t.list0 = at;
+      tiles[n_wide + own + k] = t;
+    }
   }
   // ---- narrow tiles of prefixes ----
   for (int p = tid; p < NP; p += kPlanThreads) {
     const int rows = g_seq[p] > 0 ? g_tok[p] * rep : 0;
-    if (rows == 0 || rows > kNarrowRows) continue;
-    StepTile t{};
-    t.tok0 = g_list[p];
-    t.rows = rows;
-    t.p_row = p;
-    t.p_len = prefix_len(p);
-    t.steps = max(1, ((t.p_len + 31) / 32 + kStepWaves - 1) / kStepWaves);
-    t.dest = kToPrefix;
-    t.list0 = g_list[p];
-    t.list = 1;
-    tiles[n_wide + g_nar[p]] = t;
+    if (rows == 0 || rows > kNarrowMost) continue;
+    for (int k = 0; k * kNarrowRows < rows; ++k) {
+      StepTile t{};
+      t.tok0 = g_list[p];
+      t.row0 = k * kNarrowRows;
+      t.rows = min(kNarrowRows, rows - t.row0);
+      t.p_row = p;
+      t.p_len = prefix_len(p);
+      t.steps = max(1, ((t.p_len + 31) / 32 + kStepWaves - 1) / kStepWaves);
+      t.dest = kToPrefix;
+      t.list0 = g_list[p];
+      t.list = 1;
+      tiles[n_wide + g_nar[p] + k] = t;
+    }
   }
-  // ---- wide tiles, one a thread ----
+  // ---- wide tiles, one a thread.  Those of sequences are laid out column by column: dealt to the
+  // columns (the workers of a kv head) to and fro, the last of a sequence first, so that a worker
+  // starts with a long tile and all get about as much; the workgroups of an XCD then go through
+  // the keys side by side and find them in its L2 (a prompt of 16384 tokens, 32/8 heads: 2.16 ms in
+  // the order of the rows, WIDEORD so). ----
+  const int own_wide = n_wide - pre_wide, cols = max(1, min(own_wide, a.workers / hkv)), rounds = (own_wide + cols - 1) / cols;
+  const int rest = own_wide - (rounds - 1) * cols;  // tiles of the last round
   for (int i = tid; i < n_wide; i += kPlanThreads) {
     StepTile t{};
     if (i < pre_wide) {
@@ -394,7 +424,12 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
       t.dest = kToOut;
     }
     t.steps = max(1, (t.p_len + kWideKeys - 1) / kWideKeys + (t.s_len + kWideKeys - 1) / kWideKeys);
-    tiles[i] = t;
+    int to = i;
+    if (i >= pre_wide) {
+      const int k = n_wide - 1 - i, r = k / cols, c = r & 1 ? cols - 1 - k % cols : k % cols;
+      to = pre_wide + c * (rounds - 1) + (rounds & 1 ? min(c, rest) : max(0, c - (cols - rest))) + r;
+    }
+    tiles[to] = t;
   }
   const int units_w = n_wide * hkv, units = units_w + n_nar * hkv;
   for (int i = tid; i < units; i += kPlanThreads) cuts[i] = 0;
@@ -405,13 +440,24 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
   const int64_t all_w = scan_costs(cum_w, n_wide, [&](int i) { return static_cast<int64_t>(kWideFixed + tiles[i].steps * kWideStep); }, tmp64);
   const int64_t all_n = scan_costs(cum_n, n_nar, [&](int i) { return static_cast<int64_t>(kNarrowFixed + tiles[n_wide + i].steps * kNarrowStep); }, tmp64);
   const int W = a.workers;
+  // Each XCD's workers (a run of W / 8) take an eighth of both axes: the wide part first, so that
+  // all but one of them have units of one kind.
+  const int slices = W % kXcds == 0 ? kXcds : 1, per = W / slices;
+  const int64_t share = max(((all_w + all_n) * hkv + W - 1) / W, static_cast<int64_t>(kLeastShare));
+#ifndef SLK
+#define SLK 64
+#endif
+  const int64_t slack = share / SLK;
   for (int i = tid; i < 2 * (W + 1); i += kPlanThreads) {
     const bool narrow = i > W;
     const int w = narrow ? i - W - 1 : i;
     const int64_t all = narrow ? all_n : all_w, total = all * hkv;
+    const int xcd = w / per;
+    const int64_t w0 = all_w * hkv * xcd / slices, w1 = all_w * hkv * (xcd + 1) / slices;
+    const int64_t n0 = all_n * hkv * xcd / slices, n1 = all_n * hkv * (xcd + 1) / slices, p = share * (w - xcd * per);
+    const int64_t x = narrow ? min(n1, n0 + max(p - (w1 - w0), static_cast<int64_t>(0))) : min(w1, w0 + p);
     int unit = narrow ? units : units_w, step = 0;
-    if (w < W && total > 0) {
-      const int64_t x = total / W * w + total % W * w / W;
+    if (w < W && x < total) {
       int t, fixed, each;
       int64_t off;
       if (!narrow) {
@@ -432,8 +478,9 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
         fixed = kNarrowFixed;
         each = kNarrowStep;
       }
-      step = off <= fixed ? 0 : static_cast<int>((off - fixed + each / 2) / each);
-      if (step >= tiles[t].steps) {
+      // a cut so near a unit's end that it costs more than it evens out is moved there
+      step = off <= fixed + slack ? 0 : static_cast<int>((off - fixed + each / 2) / each);
+      if (static_cast<int64_t>(tiles[t].steps - step) * each <= slack) {
         ++unit;
         step = 0;
       }
@@ -485,7 +532,8 @@ struct StepArgs {
   int64_t q_hs, q_ss;
   const uint16_t* pool;
   int64_t plane_bytes, num_blocks;
-  int32_t rep, gpb, gpb_shift;  // 16-token groups of a block, its log2 or -1
+  int32_t rep;
+  uint32_t gpb, gpb_inv, block_bytes;  // 16-token groups of a block, (2^32 - 1) / gpb, bytes of a block in a plane
   const int32_t *tables, *prefix_tables;
   int64_t table_stride, prefix_stride;
   float scale_log2;
@@ -519,12 +567,10 @@ __device__ __forceinline__ void wait_dma(int left) {  // at most `left` (0 or on
 template <int DW>
 constexpr int kStepLds = 5 * kWideKeys * DW * 2;
 
-// A 16-key group of the paged cache for one kv head: address of its first K row and how many
-// of its rows count; one with a bad block id counts none (its bit is set), so reads of its
-// rows give zeros.
+// A group of 16 keys of the paged cache: its block's id as the table has it, its first token's
+// place in the block and how many of its tokens count.
 struct KeyGroup {
-  uint64_t addr;
-  int rows;
+  int id, slot, rows;
 };
 
 // The kernel's arguments as they lie in memory.  Read through `again`, a value is loaded where
@@ -537,44 +583,51 @@ __device__ __forceinline__ args_ptr again(args_ptr a) {
   return a;
 }
 
-// What the loads of a unit go by.
+// What the loads of a unit go by.  All of it is the same for a wave's lanes: some 30 scalar
+// instructions a 16-key group, which the wide tiles' loop has to fit beside its softmax.
 struct StepKeys {
   scalar_i32 p_tab, s_tab;  // table rows of the tile
   int p_len, s_len;
   uint64_t base;            // the kv head's first K row of block 0
   int64_t plane_bytes;
-  int num_blocks, gpb, gpb_shift, row_bytes, span_bytes;  // span_bytes: of a row's head
+  uint32_t num_blocks, gpb, gpb_inv, block_bytes;
+  int row_bytes, span_bytes;  // span_bytes: of a row's head
+  bool bad;                   // a block id outside the pool was met
+  StepKeys() = default;
   __device__ __forceinline__ StepKeys(args_ptr a, const StepTile& t, int kvh)
       : p_tab(scalar_ptr(a->prefix_tables + t.p_row * a->prefix_stride)), s_tab(scalar_ptr(a->tables + t.s_row * a->table_stride)),
         p_len(t.p_len), s_len(t.s_len), base(reinterpret_cast<uint64_t>(a->pool) + static_cast<uint64_t>(kvh) * a->s.d * 2),
-        plane_bytes(a->plane_bytes), num_blocks(static_cast<int>(a->num_blocks)), gpb(a->gpb), gpb_shift(a->gpb_shift),
-        row_bytes(a->s.hkv * a->s.d * 2), span_bytes(a->s.d * 2) {}
-  __device__ __forceinline__ int entry(int key0) const {
-    const int g = key0 >> 4;
-    return gpb_shift >= 0 ? g >> gpb_shift : g / gpb;
-  }
-  // block id of the group at key0 of the prefix or the own keys, -1 past the end
-  __device__ __forceinline__ int block(bool pre, int key0) const {
-    return key0 < (pre ? p_len : s_len) ? (pre ? p_tab : s_tab)[entry(key0)] : -1;
-  }
-  __device__ __forceinline__ KeyGroup group(int blk, bool pre, int key0, args_ptr a) const {
-    int rows = min(max((pre ? p_len : s_len) - key0, 0), 16);
-    if (rows > 0 && (blk < 0 || blk >= num_blocks)) {
-      if ((threadIdx.x & 63) == 0) atomicOr(again(a)->err, 1);
-      rows = 0;
+        plane_bytes(a->plane_bytes), num_blocks(static_cast<uint32_t>(a->num_blocks)), gpb(a->gpb), gpb_inv(a->gpb_inv),
+        block_bytes(a->block_bytes), row_bytes(a->s.hkv * a->s.d * 2), span_bytes(a->s.d * 2), bad(false) {}
+  // The group at key0 of the prefix or the own keys.  Its table entry is (key0 / 16) / gpb: the
+  // product with floor((2^32 - 1) / gpb) is at most one too low.
+  __device__ __forceinline__ KeyGroup fetch(bool pre, int key0) const {
+    const uint32_t g = static_cast<uint32_t>(key0) >> 4;
+    uint32_t e = __umulhi(g, gpb_inv), r = g - e * gpb;
+    if (r >= gpb) {
+      ++e;
+      r -= gpb;
     }
-    const int slot = key0 - entry(key0) * (gpb << 4);
-    const int64_t row = rows > 0 ? static_cast<int64_t>(blk) * (gpb << 4) + slot : 0;
-    return {base + static_cast<uint64_t>(row) * row_bytes, rows};
+    const int rows = min((pre ? p_len : s_len) - key0, 16);
+    return {rows > 0 ? (pre ? p_tab : s_tab)[e] : 0, static_cast<int>(r << 4), max(rows, 0)};
   }
-  __device__ __forceinline__ u32x4 srd(const KeyGroup& g, bool v) const {
-    const uint64_t at = g.addr + (v ? plane_bytes : 0);
-    u32x4 r;
-    r[0] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
-    r[1] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32) & 0xffffu);
-    r[2] = __builtin_amdgcn_readfirstlane(g.rows > 0 ? static_cast<uint32_t>((g.rows - 1) * row_bytes + span_bytes) : 0u);
-    r[3] = 0x00020000u;
-    return r;
+  // Buffer descriptors of its K and V rows; rows past the last that counts, and all of a bad
+  // block, lie out of range and give zeros.
+  __device__ __forceinline__ void srd(const KeyGroup& g, u32x4& k, u32x4& v) {
+    const bool ok = static_cast<uint32_t>(g.id) < num_blocks;
+    bad = bad || !ok;
+    const uint64_t at = base + static_cast<uint64_t>(static_cast<uint32_t>(g.id)) * block_bytes + static_cast<uint32_t>(g.slot * row_bytes);
+    const uint32_t bytes = ok && g.rows > 0 ? static_cast<uint32_t>((g.rows - 1) * row_bytes + span_bytes) : 0u;
+    const uint64_t vat = at + plane_bytes;
+    k[0] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+    k[1] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32) & 0xffffu);
+    v[0] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(vat));
+    v[1] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(vat >> 32) & 0xffffu);
+    k[2] = v[2] = __builtin_amdgcn_readfirstlane(bytes);
+    k[3] = v[3] = 0x00020000u;
+  }
+  __device__ __forceinline__ void report(args_ptr a) const {
+    if (bad && (threadIdx.x & 63) == 0) atomicOr(again(a)->err, 1);
   }
 };
 
@@ -649,19 +702,21 @@ struct StepLanes {
     v_rd0 = (8 * (g16 >> 1) + (sl >> 2)) * PW + ((4 * vs + 2 * (g16 & 1) + ((sl & 3) >> 1)) << 4) + 8 * (sl & 1);
   }
   // The NJ loads of a group's K or V rows to LDS at `to`: the K swizzle of row j RPI + r0 is that
-  // of r0 with bits 2 and 3 of the chunk flipped by j, the V swizzle the same for all j.  Chunks
-  // past the head dim (span_bytes) lie out of range and give zeros.
+  // of r0 with bits 2 and 3 of the chunk flipped by j, the V swizzle the same for all j.  With
+  // PAD (a head dim below DW) chunks past span_bytes lie out of range and give zeros.
+  template <bool PAD>
   static __device__ __forceinline__ void load_k(u32x4 srd, uint32_t to, uint32_t row_bytes, uint32_t span_bytes) {
     const uint32_t lane = fresh_lane(), r0 = lane / CPR, c0 = ((lane % CPR) ^ (PW == 256 ? r0 : r0 >> 1)) << 4, row0 = r0 * row_bytes;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const uint32_t ch = c0 ^ (j << 6);
-      dma16(srd, ch < span_bytes ? ch + row0 + j * RPI * row_bytes : 0x80000000u, to + j * 1024);
+      dma16(srd, !PAD || ch < span_bytes ? ch + row0 + j * RPI * row_bytes : 0x80000000u, to + j * 1024);
     }
   }
+  template <bool PAD>
   static __device__ __forceinline__ void load_v(u32x4 srd, uint32_t to, uint32_t row_bytes, uint32_t span_bytes) {
     const uint32_t lane = fresh_lane(), r0 = lane / CPR, ch = ((lane % CPR) ^ (PW == 256 ? 4 * r0 : 4 * ((r0 >> 1) & 1))) << 4;
-    const uint32_t v0 = ch < span_bytes ? ch + r0 * row_bytes : 0x80000000u;
+    const uint32_t v0 = !PAD || ch < span_bytes ? ch + r0 * row_bytes : 0x80000000u;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) dma16(srd, v0 + j * RPI * row_bytes, to + j * 1024);
   }
@@ -670,7 +725,7 @@ struct StepLanes {
 };
 
 // Q fragments of a row: dims 16 s + 8 (lane / 32) .. + 7 of step s, zeros past the head dim.
-template <int DT, int DW>
+template <int DT, int DW, bool PAD>
 __device__ __forceinline__ void load_q(args_ptr a, const RowOf& r, int kvh, int lhalf, typename MfmaOps<DT>::frag (&qf)[DW / 16]) {
   const int dn = a->s.d;
   const uint16_t* qrow = a->q + (kvh * a->rep + r.h) * a->q_hs + r.token * a->q_ss;
@@ -678,11 +733,11 @@ __device__ __forceinline__ void load_q(args_ptr a, const RowOf& r, int kvh, int 
 #pragma unroll
   for (int s = 0; s < DW / 16; ++s) {
     const int at = 16 * s + 8 * lhalf;
-    x[s] = *reinterpret_cast<const u32x4*>(qrow + (at < dn ? at : 0));
+    x[s] = *reinterpret_cast<const u32x4*>(qrow + (!PAD || at < dn ? at : 0));
   }
 #pragma unroll
   for (int s = 0; s < DW / 16; ++s)
-    qf[s] = as_frag<typename MfmaOps<DT>::frag>(16 * s + 8 * lhalf < dn ? x[s] : u32x4{0u, 0u, 0u, 0u});
+    qf[s] = as_frag<typename MfmaOps<DT>::frag>(!PAD || 16 * s + 8 * lhalf < dn ? x[s] : u32x4{0u, 0u, 0u, 0u});
 }
 
 template <int DT>
@@ -694,7 +749,7 @@ __device__ __forceinline__ float frag_value(typename MfmaOps<DT>::frag f, int i)
 
 // The narrow units of the worker at `place` of the plan's starts.  TN: terms of 16 bits in which
 // a softmax weight enters the product with V.
-template <int DT, int DW, int TN>
+template <int DT, int DW, bool PAD, int TN>
 __device__ __forceinline__ void step_narrow(args_ptr a, int place, char* lds) {
   using Ops = MfmaOps<DT>;
   using frag = typename Ops::frag;
@@ -709,58 +764,73 @@ __device__ __forceinline__ void step_narrow(args_ptr a, int place, char* lds) {
   const Lanes at(lane);
   const uint32_t lds0 = lds_offset(lds);
   const float c = a->scale_log2;
-  for (int unit = starts[0], s0 = starts[1]; unit < end_unit || (unit == end_unit && s0 < end_step); ++unit, s0 = 0) {
+  auto some = [&](int unit, int step) __attribute__((always_inline)) { return unit < end_unit || (unit == end_unit && step < end_step); };
+  int unit = starts[0];
+  if (!some(unit, starts[1])) return;
+  constexpr int kDma = 2 * NJ;
+  constexpr int kStage = kStepWaves * 64 * PW;  // LDS: 32 K and 32 V rows of each wave, then the small results
+  const uint32_t kbuf = lds0 + wave * (64 * PW), vbuf = kbuf + 32 * PW;
+
+  // ---- the unit being worked on ----
+  StepTile t;
+  int kvh, slot, np, ng, g;       // this wave's groups of 32 keys: g, g + 8, ..., the first np of the unit's of the prefix
+  int vis, vis_min;               // own keys that this lane's row and the tile's first row see
+  StepKeys keys;
+  frag qf[KS];
+  KeyGroup n0, n1;                // the two 16-key groups to load next
+  u32x4 ks0, ks1, vs0, vs1;       // descriptors of those being loaded
+  auto key_of = [&](int g) __attribute__((always_inline)) { return 32 * (g < np ? g : g - np); };
+  auto fetch = [&](int g) __attribute__((always_inline)) {
+    if (g >= ng) return;
+    n0 = keys.fetch(g < np, key_of(g));
+    n1 = keys.fetch(g < np, key_of(g) + 16);
+  };
+  auto locate = [&] __attribute__((always_inline)) {
+    keys.srd(n0, ks0, vs0);
+    keys.srd(n1, ks1, vs1);
+  };
+  auto load_k = [&] __attribute__((always_inline)) {
+    Lanes::template load_k<PAD>(ks0, kbuf, keys.row_bytes, keys.span_bytes);
+    Lanes::template load_k<PAD>(ks1, kbuf + NJ * 1024, keys.row_bytes, keys.span_bytes);
+  };
+  auto load_v = [&] __attribute__((always_inline)) {
+    Lanes::template load_v<PAD>(vs0, vbuf, keys.row_bytes, keys.span_bytes);
+    Lanes::template load_v<PAD>(vs1, vbuf + NJ * 1024, keys.row_bytes, keys.span_bytes);
+  };
+  // Takes up a unit from step s0 on: its first keys are on their way when this returns.
+  auto begin = [&](int u, int s0) __attribute__((always_inline)) {
     const args_ptr b0 = again(a);
-    const int un = unit - n_wide * b0->s.hkv, ti = un / b0->s.hkv, kvh = un - ti * b0->s.hkv;
-    const StepTile t = read_tile(b0, n_wide + ti);
-    const int s1 = unit == end_unit ? min(end_step, t.steps) : t.steps;
-    const int slot = s0 > 0 ? 2 * place : s1 < t.steps ? 2 * place + 1 : -1;
-    const StepKeys keys(b0, t, kvh);
-    frag qf[KS];
+    const int un = u - n_wide * b0->s.hkv, ti = un / b0->s.hkv;
+    kvh = un - ti * b0->s.hkv;
+    t = read_tile(b0, n_wide + ti);
+    const int s1 = u == end_unit ? min(end_step, t.steps) : t.steps;
+    slot = s0 > 0 ? 2 * place : s1 < t.steps ? 2 * place + 1 : -1;
+    np = (t.p_len + 31) >> 5;
+    ng = min(np + ((t.s_len + 31) >> 5), s1 * kStepWaves);
+    g = s0 * kStepWaves + wave;
+    keys = StepKeys(b0, t, kvh);
+    fetch(g);
     const RowOf mine = row_of(b0, t, lcol);
-    load_q<DT, DW>(b0, mine, kvh, lhalf, qf);
-    const int vis = sees(t, mine.i), vis_min = sees(t, t.row0 / b0->rep);  // own keys this row and the first one see
+    load_q<DT, DW, PAD>(b0, mine, kvh, lhalf, qf);
+    vis = sees(t, mine.i);
+    vis_min = sees(t, t.row0 / b0->rep);
+    if (g < ng) {
+      locate();
+      load_k();
+      load_v();
+      fetch(g + kStepWaves);
+    }
+  };
+  __syncthreads();  // the wide units' reads of LDS are over
+  begin(unit, starts[1]);
+  while (true) {
     f32x16 oacc[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) oacc[b][r] = 0.f;
     float m_run = kInitMax, l_run = 0.f;
-    __syncthreads();  // the previous unit's reads of LDS are over
-
-    // ---- narrow: this wave's groups of 32 keys, s0 * 8 + wave, + 8, ... ----
-    const int np = (t.p_len + 31) >> 5, ng = min(np + ((t.s_len + 31) >> 5), s1 * kStepWaves);
-    const uint32_t kbuf = lds0 + wave * (64 * PW), vbuf = kbuf + 32 * PW;
-    constexpr int kDma = 2 * NJ;
-    KeyGroup g0, g1;     // the two 16-key groups being loaded
-    int id0, id1;        // block ids of the ones after them
-    auto key_of = [&](int g) __attribute__((always_inline)) { return 32 * (g < np ? g : g - np); };
-    auto fetch = [&](int g) __attribute__((always_inline)) {
-      if (g >= ng) return;
-      id0 = keys.block(g < np, key_of(g));
-      id1 = keys.block(g < np, key_of(g) + 16);
-    };
-    auto locate = [&](int g) __attribute__((always_inline)) {
-      g0 = keys.group(id0, g < np, key_of(g), a);
-      g1 = keys.group(id1, g < np, key_of(g) + 16, a);
-    };
-    auto load_k = [&] __attribute__((always_inline)) {
-      Lanes::load_k(keys.srd(g0, false), kbuf, keys.row_bytes, keys.span_bytes);
-      Lanes::load_k(keys.srd(g1, false), kbuf + NJ * 1024, keys.row_bytes, keys.span_bytes);
-    };
-    auto load_v = [&] __attribute__((always_inline)) {
-      Lanes::load_v(keys.srd(g0, true), vbuf, keys.row_bytes, keys.span_bytes);
-      Lanes::load_v(keys.srd(g1, true), vbuf + NJ * 1024, keys.row_bytes, keys.span_bytes);
-    };
-    int g = s0 * kStepWaves + wave;
     bool first = true;
-    if (g < ng) {
-      fetch(g);
-      locate(g);
-      load_k();
-      load_v();
-      fetch(g + kStepWaves);
-    }
     for (; g < ng; g += kStepWaves) {
       const bool more = g + kStepWaves < ng;
       const bool own = g >= np;
@@ -778,7 +848,7 @@ __device__ __forceinline__ void step_narrow(args_ptr a, int place, char* lds) {
       pin(sacc);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's last reads are done
       if (more) {
-        locate(g + kStepWaves);
+        locate();
         load_k();
         fetch(g + 2 * kStepWaves);
       }
@@ -848,58 +918,75 @@ __device__ __forceinline__ void step_narrow(args_ptr a, int place, char* lds) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (more) load_v();
     }
-    // ---- the waves' results meet in LDS: [wave][row][DW + 4] and m, l of every row ----
-    constexpr int OS = DW + 4;
-    float* const os = reinterpret_cast<float*>(lds);
-    float* const ml = os + kStepWaves * kNarrowRows * OS;
-    static_assert((kStepWaves * kNarrowRows * (OS + 2)) * 4 <= kStepLds<DW>, "results fit");
+    keys.report(a);
+    // ---- the waves' results meet in LDS: [wave][row][DW + 4] and m, l of every row.  Few rows
+    // meet behind the waves' K and V, up to kFew at a time, while the next unit's first keys load
+    // there; more take the place of K and V, all at once ----
+    constexpr int OS = DW + 4, kFew = 7;
+    static_assert(kStage + kStepWaves * kFew * (OS + 2) * 4 <= kStepLds<DW> && kStepWaves * kNarrowRows * (OS + 2) * 4 <= kStepLds<DW>,
+                  "results fit");
+    const StepTile et = t;
+    const int ekvh = kvh, eslot = slot;
+    const bool few = et.rows <= 2 * kFew, more_units = some(++unit, 0);
+    if (few && more_units) begin(unit, 0);
+    const int most = few ? kFew : kNarrowRows;
+    float* const os = reinterpret_cast<float*>(lds + (few ? kStage : 0));
+    float* const ml = os + kStepWaves * most * OS;
     const float l_tot = sum_xor32(l_run);
-    __syncthreads();
-    if (lcol < t.rows) {
-      if (lhalf == 0) {
-        ml[(wave * kNarrowRows + lcol) * 2] = m_run;
-        ml[(wave * kNarrowRows + lcol) * 2 + 1] = l_tot;
+    const args_ptr e = again(a);
+    for (int r0 = 0; r0 < et.rows; r0 += most) {
+      const int n_rows = min(most, et.rows - r0);
+      __syncthreads();  // earlier reads of this place are over
+      const int lr = lcol - r0;
+      if (lr >= 0 && lr < n_rows) {
+        if (lhalf == 0) {
+          ml[(wave * most + lr) * 2] = m_run;
+          ml[(wave * most + lr) * 2 + 1] = l_tot;
+        }
+        if (l_tot != 0.f) {
+#pragma unroll
+          for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<f32x4*>(os + (wave * most + lr) * OS + 32 * b + 8 * j + 4 * lhalf) =
+                  f32x4{oacc[b][4 * j], oacc[b][4 * j + 1], oacc[b][4 * j + 2], oacc[b][4 * j + 3]};
+        }
       }
-      if (l_tot != 0.f) {
+      __syncthreads();
+      for (int i = tid; i < n_rows * (DW / 4); i += kStepThreads) {
+        const int r = i / (DW / 4), d = i - r * (DW / 4);
+        if (PAD && 4 * d >= e->s.d) continue;
+        float m = kInitMax;
 #pragma unroll
-        for (int b = 0; b < DB; ++b)
+        for (int w = 0; w < kStepWaves; ++w) m = fmaxf(m, ml[(w * most + r) * 2]);
+        float den = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<f32x4*>(os + (wave * kNarrowRows + lcol) * OS + 32 * b + 8 * j + 4 * lhalf) =
-                f32x4{oacc[b][4 * j], oacc[b][4 * j + 1], oacc[b][4 * j + 2], oacc[b][4 * j + 3]};
+        for (int w = 0; w < kStepWaves; ++w) {
+          const float lw = ml[(w * most + r) * 2 + 1];
+          if (lw == 0.f) continue;  // took no key
+          const float f = exp2f(ml[(w * most + r) * 2] - m);
+          den += f * lw;
+          const f32x4 o = *reinterpret_cast<const f32x4*>(os + (w * most + r) * OS + 4 * d);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] += f * o[k];
+        }
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        const RowOf ro = row_of(e, et, r0 + r);
+        const RowDest dst = row_dest(e, et, ekvh, eslot, r0 + r, ro.token, ro.i, ro.h);
+        store4(dst.o, dst.dtype, dst.o_off + 4 * d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        if (d == 0 && dst.lse != nullptr) *dst.lse = den == 0.f ? -INFINITY : (m + __log2f(den)) * kLn2;
       }
     }
-    __syncthreads();
-    const args_ptr e = again(a);
-    const int d4 = e->s.d / 4;
-    for (int i = tid; i < t.rows * (DW / 4); i += kStepThreads) {
-      const int r = i / (DW / 4), d = i - r * (DW / 4);
-      if (d >= d4) continue;
-      float m = kInitMax;
-#pragma unroll
-      for (int w = 0; w < kStepWaves; ++w) m = fmaxf(m, ml[(w * kNarrowRows + r) * 2]);
-      float den = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < kStepWaves; ++w) {
-        const float lw = ml[(w * kNarrowRows + r) * 2 + 1];
-        if (lw == 0.f) continue;  // took no key
-        const float f = exp2f(ml[(w * kNarrowRows + r) * 2] - m);
-        den += f * lw;
-        const f32x4 o = *reinterpret_cast<const f32x4*>(os + (w * kNarrowRows + r) * OS + 4 * d);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] += f * o[k];
-      }
-      const float inv = den == 0.f ? 0.f : 1.f / den;
-      const RowOf ro = row_of(e, t, r);
-      const RowDest dst = row_dest(e, t, kvh, slot, r, ro.token, ro.i, ro.h);
-      store4(dst.o, dst.dtype, dst.o_off + 4 * d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-      if (d == 0 && dst.lse != nullptr) *dst.lse = den == 0.f ? -INFINITY : (m + __log2f(den)) * kLn2;
+    if (!more_units) return;
+    if (!few) {
+      __syncthreads();
+      begin(unit, 0);
     }
   }
 }
 
 // The wide units of the worker at `place`.  TW: as TN.
-template <int DT, int DW, int TW>
+template <int DT, int DW, bool PAD, int TW>
 __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
   using Ops = MfmaOps<DT>;
   using frag = typename Ops::frag;
@@ -920,10 +1007,10 @@ __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
     const StepTile t = read_tile(b0, unit - kvh * n_wide);
     const int s1 = unit == end_unit ? min(end_step, t.steps) : t.steps;
     const int slot = s0 > 0 ? 2 * place : s1 < t.steps ? 2 * place + 1 : -1;
-    const StepKeys keys(b0, t, kvh);
+    StepKeys keys(b0, t, kvh);
     frag qf[KS];
     const RowOf mine = row_of(b0, t, wave * 32 + lcol);
-    load_q<DT, DW>(b0, mine, kvh, lhalf, qf);
+    load_q<DT, DW, PAD>(b0, mine, kvh, lhalf, qf);
     // own keys that this row and the wave's first one see
     const int vis = sees(t, mine.i), vis_min = sees(t, (t.row0 + min(wave * 32, t.rows - 1)) / b0->rep);
     f32x16 oacc[DB];
@@ -943,17 +1030,15 @@ __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
     const char* v_lds_c = lds + NBK * kTile;
     int* const simd_of = reinterpret_cast<int*>(lds + (NBK + NBV - 1) * kTile);  // in the last V buffer, first written in super-step 1
     auto key_of = [&](int u) __attribute__((always_inline)) { return BK * (s0 + u < np ? s0 + u : s0 + u - np); };
-    int next_id;
+    KeyGroup nx;  // wave w loads rows 16 w .. 16 w + 15 of a tile: one 16-key group
     auto fetch = [&](int u) __attribute__((always_inline)) {
-      if (u < n_tiles) next_id = keys.block(s0 + u < np, key_of(u) + 16 * wave);
+      if (u < n_tiles) nx = keys.fetch(s0 + u < np, key_of(u) + 16 * wave);
     };
-    // wave w loads rows 16 w .. 16 w + 15 of the tile: one 16-key group
     auto issue_tile = [&](int u) __attribute__((always_inline)) {
-      const KeyGroup g = keys.group(next_id, s0 + u < np, key_of(u) + 16 * wave, a);
-      const u32x4 ks = keys.srd(g, false), vs = keys.srd(g, true);
-      const uint32_t kb = k_lds0 + (u % NBK) * kTile + wave * 16 * PW, vb = v_lds0 + (u % NBV) * kTile + wave * 16 * PW;
-      Lanes::load_k(ks, kb, keys.row_bytes, keys.span_bytes);
-      Lanes::load_v(vs, vb, keys.row_bytes, keys.span_bytes);
+      u32x4 ks, vs;
+      keys.srd(nx, ks, vs);
+      Lanes::template load_k<PAD>(ks, k_lds0 + (u % NBK) * kTile + wave * 16 * PW, keys.row_bytes, keys.span_bytes);
+      Lanes::template load_v<PAD>(vs, v_lds0 + (u % NBV) * kTile + wave * 16 * PW, keys.row_bytes, keys.span_bytes);
       fetch(u + 1);
     };
     fetch(0);
@@ -1155,6 +1240,7 @@ __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
       settle(u);
       if (!lead) issue(u + 1);
     }
+    keys.report(a);
     const args_ptr e = again(a);
     const int row = wave * 32 + (static_cast<int>(fresh_lane()) & 31);
     if (row < t.rows) {
@@ -1165,25 +1251,27 @@ __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
   }
 }
 
-// Workgroups 0 .. W - 1 hold the wide units, W .. 2 W - 1 the narrow ones.
-template <int DT, int DW, int TN, int TW>
+// A workgroup takes its share of the wide units, then of the narrow ones (mostly one of the two).
+template <int DT, int DW, bool PAD, int TN, int TW>
 __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs args) {
   __shared__ __attribute__((aligned(1024))) char lds[kStepLds<DW>];
   const args_ptr a = (args_ptr)__builtin_amdgcn_kernarg_segment_ptr();
-  const scalar_i32 head = scalar_ptr(a->plan);
-  if (!plan_fits(head, args.s, args.workers)) {
+  if (!plan_fits(scalar_ptr(a->plan), args.s, args.workers)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(args.err, 8);
     return;
   }
-  const int workers = a->workers, bid = blockIdx.x;
-  if (bid < workers) step_wide<DT, DW, TW>(a, xcd_remap(bid, workers), lds);
-  else step_narrow<DT, DW, TN>(a, workers + 1 + xcd_remap(bid - workers, workers), lds);
+  const int worker = xcd_remap(blockIdx.x, gridDim.x);
+  step_wide<DT, DW, PAD, TW>(a, worker, lds);
+  step_narrow<DT, DW, PAD, TN>(a, static_cast<int>(gridDim.x) + 1 + worker, lds);
 }
 
 // ----------------------------------------------------------------------------------
-// Join: a wave a row.  The rows of tokens behind shared prefixes (own part and prefix part),
-// then those of cut units; a part is a unit's rows as one worker left them.
+// Join: 16 lanes a row.  The rows of tokens behind shared prefixes (own part and prefix part),
+// then those of cut units; a part is a unit's rows as one worker left them.  Bound by the chain
+// of loads that finds a row's parts (five), so as many rows as the GPU holds are under way.
 // ----------------------------------------------------------------------------------
+constexpr int kJoinLanes = 16, kJoinRows = 256 / kJoinLanes;
+
 __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
   const int32_t* head = reinterpret_cast<const int32_t*>(a.plan);
   if (!plan_fits(head, a.s, a.workers)) return;  // the attention kernel has said so
@@ -1191,13 +1279,14 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
   const int units_w = n_wide * a.s.hkv, hkv = a.s.hkv, hq = a.s.hq, d = a.s.d;
   const StepTile* tiles = reinterpret_cast<const StepTile*>(a.plan + a.p_tiles);
   const StepShared* shared = reinterpret_cast<const StepShared*>(a.plan + a.p_shared);
-  const int32_t* starts = reinterpret_cast<const int32_t*>(a.plan + a.p_starts);
+  const int2* starts = reinterpret_cast<const int2*>(a.plan + a.p_starts);
   const int32_t* cuts = reinterpret_cast<const int32_t*>(a.plan + a.p_cuts);
   const int32_t* cut_units = reinterpret_cast<const int32_t*>(a.plan + a.p_cut_units);
   const int32_t* cut_row0 = reinterpret_cast<const int32_t*>(a.plan + a.p_cut_row0);
-  const int lane = threadIdx.x & 63;
+  const int sub = threadIdx.x % kJoinLanes;
   const int64_t shared_rows = static_cast<int64_t>(n_shared) * hq, rows = shared_rows + cut_rows;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); i < rows; i += static_cast<int64_t>(gridDim.x) * 4) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kJoinRows + threadIdx.x / kJoinLanes; i < rows;
+       i += static_cast<int64_t>(gridDim.x) * kJoinRows) {
     // up to two sources of parts: a cut unit's slots or one row
     const float *o1 = nullptr, *l1 = nullptr;  // an uncut row
     const float *o2 = nullptr, *l2 = nullptr;
@@ -1208,14 +1297,13 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
       hd = static_cast<int>(i - static_cast<int64_t>(li) * hq);
       const StepShared s = shared[li];
       token = s.token;
-      const int kvh = hd / a.rep, h = hd - kvh * a.rep;
-      c1 = cuts[units_w + s.own_tile * hkv + kvh];
-      r1 = s.own_row + h;
+      const int kvh = hd / a.rep, h = hd - kvh * a.rep, own = s.own_row + h, pre = s.pre_row + h;
+      c1 = cuts[units_w + (s.own_tile + own / kNarrowRows) * hkv + kvh];
+      r1 = own % kNarrowRows;
       o1 = a.own_o + i * d;
       l1 = a.own_lse + i;
-      const int pr = s.pre_row + h;
-      c2 = s.pre_wide ? cuts[kvh * n_wide + s.pre_tile + pr / kWideRows] : cuts[units_w + s.pre_tile * hkv + kvh];
-      r2 = s.pre_wide ? pr % kWideRows : pr;
+      c2 = s.pre_wide ? cuts[kvh * n_wide + s.pre_tile + pre / kWideRows] : cuts[units_w + (s.pre_tile + pre / kNarrowRows) * hkv + kvh];
+      r2 = s.pre_wide ? pre % kWideRows : pre % kNarrowRows;
       o2 = a.pre_o + i * d;
       l2 = a.pre_lse + i;
     } else {
@@ -1231,68 +1319,75 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
     }
     const int w1 = (c1 & 0xffff) - 1, w2 = (c2 & 0xffff) - 1;  // place of the first worker
     const int n1 = c1 != 0 ? c1 >> 16 : 1, n2 = o2 == nullptr ? 0 : c2 != 0 ? c2 >> 16 : 1, n = n1 + n2;
-    // part k: its LSE's and its row's address; a worker without steps left nothing
-    auto at = [&](int k, const float*& o) -> const float* {
-      const bool one = k < n1;
-      const int w = one ? w1 : w2, j = one ? k : k - n1;
-      if ((one ? c1 : c2) == 0) {
-        o = one ? o1 : o2;
-        return one ? l1 : l2;
-      }
-      const int worker = w + j;
-      if (starts[2 * worker] == starts[2 * worker + 2] && starts[2 * worker + 1] == starts[2 * worker + 3]) return nullptr;
-      const int64_t row = static_cast<int64_t>(2 * worker + (j == 0 ? 1 : 0)) * a.slot_rows + (one ? r1 : r2);
-      o = a.slot_o + row * d;
-      return a.slot_lse + row;
-    };
-    float m = -INFINITY, den = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int k0 = 0; k0 < n; k0 += 64) {
+    float m = -INFINITY, den = 0.f, x[8] = {};
+    for (int k0 = 0; k0 < n; k0 += kJoinLanes) {
+      // part k0 + sub: its row and LSE; a worker without steps left nothing
       const float* o = nullptr;
-      const float* lp = k0 + lane < n ? at(k0 + lane, o) : nullptr;
-      const float l = lp != nullptr ? *lp : -INFINITY;
+      float l = -INFINITY;
+      if (k0 + sub < n) {
+        const bool one = k0 + sub < n1;
+        const int j = one ? k0 + sub : k0 + sub - n1;
+        if ((one ? c1 : c2) == 0) {
+          o = one ? o1 : o2;
+          l = *(one ? l1 : l2);
+        } else {
+          const int worker = (one ? w1 : w2) + j;
+          const int64_t row = static_cast<int64_t>(2 * worker + (j == 0 ? 1 : 0)) * a.slot_rows + (one ? r1 : r2);
+          const int2 from = starts[worker], to = starts[worker + 1];
+          const float got = a.slot_lse[row];
+          o = a.slot_o + row * d;
+          if (from.x != to.x || from.y != to.y) l = got;
+        }
+      }
       float top = l;
-      for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+      for (int off = 1; off < kJoinLanes; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
       const float m_new = fmaxf(m, top);
       const float keep = m == -INFINITY ? 0.f : __expf(m - m_new);
-      // a NaN part (a NaN key) stays one
-      const float f = l == -INFINITY ? 0.f : __expf(l - m_new);
+      const float f = l == -INFINITY ? 0.f : __expf(l - m_new);  // a NaN part (a NaN key) stays one
       m = m_new;
       float fs = f;
-      for (int off = 32; off >= 1; off >>= 1) fs += __shfl_xor(fs, off);
+      for (int off = 1; off < kJoinLanes; off <<= 1) fs += __shfl_xor(fs, off);
       den = den * keep + fs;
-      x0 *= keep;
-      x1 *= keep;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= keep;
       const uint64_t ptr = reinterpret_cast<uint64_t>(o);
-      for (int k = 0; k < min(64, n - k0); ++k) {
-        const float fk = __shfl(f, k);
-        const uint64_t pk = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr), k)) |
-                            static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr >> 32), k)) << 32;
-        if (fk == 0.f) continue;
-        const float* ok = reinterpret_cast<const float*>(pk);
-        if (2 * lane < d) {
-          const float2 v = *reinterpret_cast<const float2*>(ok + 2 * lane);
-          x0 += fk * v.x;
-          x1 += fk * v.y;
+      const int parts = min(kJoinLanes, n - k0), lane0 = (threadIdx.x & 63) - sub;
+#pragma unroll 4
+      for (int k = 0; k < parts; ++k) {
+        const float fk = __shfl(f, lane0 + k);
+        const uint64_t pk = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr), lane0 + k)) |
+                            static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr >> 32), lane0 + k)) << 32;
+        if (fk == 0.f || 8 * sub >= d) continue;
+        const f32x4* ok = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(pk) + 8 * sub);
+        const f32x4 a0 = ok[0], a1 = ok[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] += fk * a0[e];
+          x[4 + e] += fk * a1[e];
         }
       }
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    if (2 * lane < d) {
-      const int64_t off = hd * a.out_hs + token * a.out_ss + 2 * lane;
-      if (a.out_dtype == kF32) *reinterpret_cast<float2*>(static_cast<float*>(a.out) + off) = make_float2(x0 * inv, x1 * inv);
-      else
-        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + off) =
-            a.out_dtype == kBF16 ? f32x2_to_bf16x2_bits(x0 * inv, x1 * inv)
-                                 : static_cast<uint32_t>(f32_to_f16_bits(x0 * inv)) | static_cast<uint32_t>(f32_to_f16_bits(x1 * inv)) << 16;
+    if (8 * sub < d) {
+      const int64_t off = hd * a.out_hs + token * a.out_ss + 8 * sub;
+      store4(a.out, a.out_dtype, off, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+      store4(a.out, a.out_dtype, off + 4, x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
     }
-    if (lane == 0 && a.lse != nullptr) a.lse[hd * a.s.tokens + token] = den == 0.f ? -INFINITY : m + __logf(den);
+    if (sub == 0 && a.lse != nullptr) a.lse[hd * a.s.tokens + token] = den == 0.f ? -INFINITY : m + __logf(den);
   }
 }
 
-template <int DT, int DW>
+template <int DT, int DW, bool PAD>
 static void launch_step_d(const StepArgs& a, hipStream_t stream) {
-  if (a.out_dtype == kF32) step_attn_kernel<DT, DW, DT == kBF16 ? 3 : 2, DT == kBF16 ? 3 : 2><<<2 * a.workers, kStepThreads, 0, stream>>>(a);
-  else step_attn_kernel<DT, DW, 2, 1><<<2 * a.workers, kStepThreads, 0, stream>>>(a);
+  if (a.out_dtype == kF32) step_attn_kernel<DT, DW, PAD, DT == kBF16 ? 3 : 2, DT == kBF16 ? 3 : 2><<<a.workers, kStepThreads, 0, stream>>>(a);
+  else step_attn_kernel<DT, DW, PAD, 2, 1><<<a.workers, kStepThreads, 0, stream>>>(a);
+}
+template <int DT>
+static void launch_step(const StepArgs& a, hipStream_t stream) {
+  if (a.s.d == 128) launch_step_d<DT, 128, false>(a, stream);
+  else if (a.s.d == 64) launch_step_d<DT, 64, false>(a, stream);
+  else if (a.s.d < 64) launch_step_d<DT, 64, true>(a, stream);
+  else launch_step_d<DT, 128, true>(a, stream);
 }
 
 void launch_step_attn(const StepLaunch& L, hipStream_t stream) {
@@ -1311,7 +1406,8 @@ void launch_step_attn(const StepLaunch& L, hipStream_t stream) {
   a.plane_bytes = L.num_blocks * L.s.bs * L.s.hkv * static_cast<int64_t>(L.s.d) * 2;
   a.rep = L.s.hq / L.s.hkv;
   a.gpb = L.s.bs / 16;
-  a.gpb_shift = (a.gpb & (a.gpb - 1)) == 0 ? __builtin_ctz(a.gpb) : -1;
+  a.gpb_inv = 0xffffffffu / a.gpb;
+  a.block_bytes = static_cast<uint32_t>(L.s.bs) * L.s.hkv * L.s.d * 2;
   a.tables = L.tables; a.prefix_tables = L.prefix_tables;
   a.table_stride = L.table_stride; a.prefix_stride = L.prefix_stride;
   a.scale_log2 = L.scale * kLog2e;
@@ -1323,15 +1419,13 @@ void launch_step_attn(const StepLaunch& L, hipStream_t stream) {
   a.pre_o = f(w.pre_o); a.pre_lse = f(w.pre_lse);
   a.slot_rows = w.slot_rows;
   a.err = L.err;
-  if (L.dtype == kBF16) {
-    if (L.s.d <= 64) launch_step_d<kBF16, 64>(a, stream);
-    else launch_step_d<kBF16, 128>(a, stream);
-  } else {
-    if (L.s.d <= 64) launch_step_d<kF16, 64>(a, stream);
-    else launch_step_d<kF16, 128>(a, stream);
-  }
+  if (L.dtype == kBF16) launch_step<kBF16>(a, stream);
+  else launch_step<kF16>(a, stream);
   HCP_HIP(hipGetLastError());
-  step_join_kernel<<<2 * workers, 256, 0, stream>>>(a);
+  // no more rows are joined than the query has, nor than shared ones and two cut units a worker
+  const int64_t rows = std::min(L.s.tokens * L.s.hq, l.max_shared * L.s.hq + 2 * static_cast<int64_t>(workers) * w.slot_rows);
+  const int64_t grid = std::min<int64_t>(ceil_div(rows, kJoinRows), 8 * workers);
+  step_join_kernel<<<static_cast<unsigned>(grid), 256, 0, stream>>>(a);
   HCP_HIP(hipGetLastError());
 }
 
