@@ -33,29 +33,17 @@ constexpr int kStepThreads = 64 * kStepWaves;
 constexpr int kWideRows = 32 * kStepWaves;  // rows of a wide tile
 constexpr int kWideKeys = 128;              // keys of its steps
 constexpr int kNarrowRows = 32;
-#ifndef NMOST
-#define NMOST 128
-#endif
-constexpr int kNarrowMost = NMOST;             // most rows of a source that is cut into narrow tiles
+constexpr int kNarrowMost = 128;            // most rows of a source that is cut into narrow tiles
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMagic = 0x53544550;
 
 // Modelled time in 0.1 us: of a unit beside its steps, and of a step of 128 (wide) or up to
-// 8 x 32 keys (narrow).
-#ifndef CWF
-#define CWF 100
-#define CWS 36
-#endif
-#ifndef CNF
-#define CNF 55
-#define CNS 40
-#endif
-constexpr int kWideFixed = CWF, kWideStep = CWS;
-constexpr int kNarrowFixed = CNF, kNarrowStep = CNS;
-#ifndef LSH
-#define LSH 130
-#endif
-constexpr int kLeastShare = LSH;  // of a worker: less is not worth another part to join
+// 8 x 32 keys (narrow).  Measured with all CUs busy: wide 60-130 and 33-43, narrow 30-45 and 16-51
+// (keys in the L2; HBM reads at their limit).
+constexpr int kWideFixed = 70, kWideStep = 40;
+constexpr int kNarrowFixed = 32, kNarrowStep = 26;
+// Of a worker: less is not worth another part to join.
+constexpr int kLeastShare = 50;
 constexpr int kXcds = 8;
 
 // Where a unit's rows go when it is not cut.
@@ -444,10 +432,7 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
   // all but one of them have units of one kind.
   const int slices = W % kXcds == 0 ? kXcds : 1, per = W / slices;
   const int64_t share = max(((all_w + all_n) * hkv + W - 1) / W, static_cast<int64_t>(kLeastShare));
-#ifndef SLK
-#define SLK 64
-#endif
-  const int64_t slack = share / SLK;
+  const int64_t slack = share / 64;
   for (int i = tid; i < 2 * (W + 1); i += kPlanThreads) {
     const bool narrow = i > W;
     const int w = narrow ? i - W - 1 : i;
@@ -747,10 +732,23 @@ __device__ __forceinline__ float frag_value(typename MfmaOps<DT>::frag f, int i)
 
 }  // namespace
 
+// Where a worker's units of one kind start and end.
+struct StepRun {
+  int n_wide, unit, step, end_unit, end_step;
+  __device__ __forceinline__ StepRun(args_ptr a, int place) {
+    const scalar_i32 s = scalar_ptr(a->plan + a->p_starts) + 2 * place;
+    n_wide = scalar_ptr(a->plan)[12];
+    unit = s[0];
+    step = s[1];
+    end_unit = s[2];
+    end_step = s[3];
+  }
+};
+
 // The narrow units of the worker at `place` of the plan's starts.  TN: terms of 16 bits in which
 // a softmax weight enters the product with V.
 template <int DT, int DW, bool PAD, int TN>
-__device__ __forceinline__ void step_narrow(args_ptr a, int place, char* lds) {
+__device__ __forceinline__ void step_narrow(args_ptr a, const StepRun& run, int place, char* lds) {
   using Ops = MfmaOps<DT>;
   using frag = typename Ops::frag;
   using Lanes = StepLanes<DW>;
@@ -758,15 +756,13 @@ __device__ __forceinline__ void step_narrow(args_ptr a, int place, char* lds) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lcol = lane & 31, lhalf = lane >> 5;
-  const int n_wide = scalar_ptr(a->plan)[12];
-  const scalar_i32 starts = scalar_ptr(a->plan + a->p_starts) + 2 * place;
-  const int end_unit = starts[2], end_step = starts[3];
+  const int n_wide = run.n_wide, end_unit = run.end_unit, end_step = run.end_step;
   const Lanes at(lane);
   const uint32_t lds0 = lds_offset(lds);
   const float c = a->scale_log2;
   auto some = [&](int unit, int step) __attribute__((always_inline)) { return unit < end_unit || (unit == end_unit && step < end_step); };
-  int unit = starts[0];
-  if (!some(unit, starts[1])) return;
+  int unit = run.unit;
+  if (!some(unit, run.step)) return;
   constexpr int kDma = 2 * NJ;
   constexpr int kStage = kStepWaves * 64 * PW;  // LDS: 32 K and 32 V rows of each wave, then the small results
   const uint32_t kbuf = lds0 + wave * (64 * PW), vbuf = kbuf + 32 * PW;
@@ -822,7 +818,7 @@ __device__ __forceinline__ void step_narrow(args_ptr a, int place, char* lds) {
     }
   };
   __syncthreads();  // the wide units' reads of LDS are over
-  begin(unit, starts[1]);
+  begin(unit, run.step);
   while (true) {
     f32x16 oacc[DB];
 #pragma unroll
@@ -987,7 +983,7 @@ __device__ __forceinline__ void step_narrow(args_ptr a, int place, char* lds) {
 
 // The wide units of the worker at `place`.  TW: as TN.
 template <int DT, int DW, bool PAD, int TW>
-__device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
+__device__ __forceinline__ void step_wide(args_ptr a, const StepRun& run, int place, char* lds) {
   using Ops = MfmaOps<DT>;
   using frag = typename Ops::frag;
   using Lanes = StepLanes<DW>;
@@ -995,13 +991,11 @@ __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lcol = lane & 31, lhalf = lane >> 5;
-  const int n_wide = scalar_ptr(a->plan)[12];
-  const scalar_i32 starts = scalar_ptr(a->plan + a->p_starts) + 2 * place;
-  const int end_unit = starts[2], end_step = starts[3];
+  const int n_wide = run.n_wide, end_unit = run.end_unit, end_step = run.end_step;
   const Lanes at(lane);
   const uint32_t lds0 = lds_offset(lds);
   const float c = a->scale_log2;
-  for (int unit = starts[0], s0 = starts[1]; unit < end_unit || (unit == end_unit && s0 < end_step); ++unit, s0 = 0) {
+  for (int unit = run.unit, s0 = run.step; unit < end_unit || (unit == end_unit && s0 < end_step); ++unit, s0 = 0) {
     const args_ptr b0 = again(a);
     const int kvh = unit / n_wide;
     const StepTile t = read_tile(b0, unit - kvh * n_wide);
@@ -1045,7 +1039,7 @@ __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
     issue_tile(0);
     if (lane == 0) simd_of[wave] = simd_id();
     f32x16 sacc[NKB];
-    frag pf[TW == 1 ? NPS : 1];
+    frag pf[TW == 1 ? NPS : 1];  // several terms are made from P, left in place of S, as V is read
 
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -1149,8 +1143,7 @@ __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
             sacc[b][r] = 32 * b + 16 * (r >> 3) + 4 * ((r >> 2) & 1) + (r & 3) <= lim ? sacc[b][r] : -INFINITY;
       }
       float lsum = 0.f;
-      // P = 2^(s c - m); the terms for several of them are made from s later, so it stays in place
-      auto weigh = [&](bool keep) __attribute__((always_inline)) {
+      auto weigh = [&] __attribute__((always_inline)) {  // P = 2^(s c - m)
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int b = 0; b < NKB; ++b) {
@@ -1163,25 +1156,34 @@ __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
           if constexpr (TW == 1) {
             pf[2 * b] = Ops::pack(p);
             pf[2 * b + 1] = Ops::pack(p + 8);
-          } else if (keep) {
+          } else {
 #pragma unroll
             for (int r = 0; r < 16; ++r) sacc[b][r] = p[r];
           }
         }
         lsum = (ls[0] + ls[1]) + (ls[2] + ls[3]);
       };
-      bool redo = u == 0;
-      if (!redo) {
-        weigh(false);
-        redo = __any(!(lsum <= kGrowSum));
-      }
-      if (redo) {
+      auto highest = [&] __attribute__((always_inline)) {
         float top = -INFINITY;
 #pragma unroll
         for (int b = 0; b < NKB; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r) top = fmaxf(top, sacc[b][r]);
-        const float m_new = fmaxf(m_run, max_xor32(top) * c);
+        return max_xor32(top) * c;
+      };
+      // The maximum moves where it has to: seen from the sums of the weights where S outlives
+      // them, from S itself where P takes its place.
+      bool redo = u == 0;
+      if constexpr (TW == 1) {
+        if (!redo) {
+          weigh();
+          redo = __any(!(lsum <= kGrowSum));
+        }
+      }
+      const float top = TW > 1 || redo ? highest() : 0.f;
+      if (TW > 1) redo = redo || __any(!(top <= m_run + 8.f));
+      if (redo) {
+        const float m_new = fmaxf(m_run, top);
         const float alpha = exp2f(m_run - m_new);
         l_run *= alpha;
 #pragma unroll
@@ -1190,7 +1192,7 @@ __device__ __forceinline__ void step_wide(args_ptr a, int place, char* lds) {
           for (int r = 0; r < 16; ++r) oacc[b][r] *= alpha;
         m_run = m_new;
       }
-      if (redo || TW > 1) weigh(true);
+      if (redo || TW > 1) weigh();
       l_run += lsum;
       if constexpr (TW == 1) {
 #pragma unroll
@@ -1256,13 +1258,14 @@ template <int DT, int DW, bool PAD, int TN, int TW>
 __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs args) {
   __shared__ __attribute__((aligned(1024))) char lds[kStepLds<DW>];
   const args_ptr a = (args_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  const int workers = a->workers, worker = xcd_remap(blockIdx.x, workers), narrow = workers + 1 + worker;
+  const StepRun wide_run(a, worker), narrow_run(a, narrow);  // loaded beside the head
   if (!plan_fits(scalar_ptr(a->plan), args.s, args.workers)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(args.err, 8);
     return;
   }
-  const int worker = xcd_remap(blockIdx.x, gridDim.x);
-  step_wide<DT, DW, PAD, TW>(a, worker, lds);
-  step_narrow<DT, DW, PAD, TN>(a, static_cast<int>(gridDim.x) + 1 + worker, lds);
+  step_wide<DT, DW, PAD, TW>(a, wide_run, worker, lds);
+  step_narrow<DT, DW, PAD, TN>(a, narrow_run, narrow, lds);
 }
 
 // ----------------------------------------------------------------------------------
@@ -1350,21 +1353,32 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
       den = den * keep + fs;
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= keep;
-      const uint64_t ptr = reinterpret_cast<uint64_t>(o);
-      const int parts = min(kJoinLanes, n - k0), lane0 = (threadIdx.x & 63) - sub;
-#pragma unroll 4
-      for (int k = 0; k < parts; ++k) {
-        const float fk = __shfl(f, lane0 + k);
-        const uint64_t pk = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr), lane0 + k)) |
-                            static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr >> 32), lane0 + k)) << 32;
-        if (fk == 0.f || 8 * sub >= d) continue;
-        const f32x4* ok = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(pk) + 8 * sub);
-        const f32x4 a0 = ok[0], a1 = ok[1];
+      // every lane has its part of a row loaded, four parts at a time; a part without weight is
+      // read from where its address would be (the slots' start where it has none) and left out
+      const uint64_t ptr = reinterpret_cast<uint64_t>(o != nullptr ? o : a.slot_o);
+      const int parts = min(kJoinLanes, n - k0), lane0 = (threadIdx.x & 63) - sub, col = 8 * sub < d ? 8 * sub : 0;
+      for (int k = 0; k < parts; k += 4) {
+        f32x4 v[4][2];
+        float fk[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] += fk * a0[e];
-          x[4 + e] += fk * a1[e];
+          const int src = lane0 + min(k + e, parts - 1);
+          fk[e] = k + e < parts ? __shfl(f, src) : 0.f;
+          const uint64_t pk = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr), src)) |
+                              static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr >> 32), src)) << 32;
+          const f32x4* ok = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(pk) + col);
+          v[e][0] = ok[0];
+          v[e][1] = ok[1];
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (fk[e] != 0.f) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x[i] += fk[e] * v[e][0][i];
+              x[4 + i] += fk[e] * v[e][1][i];
+            }
+          }
       }
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
