@@ -70,9 +70,14 @@ struct StepShared {
   int32_t pad[2];
 };
 
+// A cut unit whose rows go to the output: where they are, and its entry of cuts.
+struct StepCut {
+  int32_t cut, row0, rows, tok0, head0, pad[3];
+};
+
 struct StepHead {
   int32_t magic, batch, tokens, hq, hkv, d, bs, causal, prefixes, max_own, max_prefix, workers;
-  int32_t n_wide, n_narrow, n_shared, n_cut, cut_rows, pad[3];
+  int32_t n_wide, n_narrow, n_shared, cut_wide, cut_narrow, pad[3];
 };
 // Whether the plan was made for this shape and number of workers.
 template <typename P>
@@ -88,7 +93,7 @@ __device__ bool plan_fits(P head, const StepShape& s, int workers) {
 // Offsets of the plan's arrays, from host-known bounds alone.
 struct PlanLayout {
   int64_t max_wide, max_narrow, max_shared, max_units;
-  size_t tiles, cum_wide, cum_narrow, shared, starts, cuts, cut_units, cut_row0, bytes;
+  size_t tiles, cum_wide, cum_narrow, shared, starts, cuts, cut_wide, cut_narrow, bytes;
 };
 
 size_t up256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
@@ -113,8 +118,8 @@ PlanLayout plan_layout(const StepShape& s) {
   l.shared = take(l.max_shared * sizeof(StepShared));
   l.starts = take(2 * (kStepMaxWorkers + 1) * 2 * sizeof(int32_t));
   l.cuts = take(l.max_units * sizeof(int32_t));
-  l.cut_units = take(2 * kStepMaxWorkers * sizeof(int32_t));
-  l.cut_row0 = take((2 * kStepMaxWorkers + 1) * sizeof(int32_t));
+  l.cut_wide = take(kStepMaxWorkers * sizeof(StepCut));
+  l.cut_narrow = take(kStepMaxWorkers * sizeof(StepCut));
   l.bytes = at;
   return l;
 }
@@ -245,7 +250,7 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
   __shared__ int64_t tmp64[kPlanThreads / 64];
   __shared__ int tmp[kPlanThreads / 64];
   __shared__ int st_unit[2 * (kStepMaxWorkers + 1)], st_step[2 * (kStepMaxWorkers + 1)];
-  __shared__ int n_cut;
+  __shared__ int n_cut[2];
 
   const int tid = threadIdx.x;
   const int B = a.s.batch, NP = a.s.prefixes, rep = a.s.hq / a.s.hkv, hkv = a.s.hkv;
@@ -257,8 +262,8 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
   StepShared* shared = reinterpret_cast<StepShared*>(a.plan + a.l.shared);
   int32_t* starts = reinterpret_cast<int32_t*>(a.plan + a.l.starts);
   int32_t* cuts = reinterpret_cast<int32_t*>(a.plan + a.l.cuts);
-  int32_t* cut_units = reinterpret_cast<int32_t*>(a.plan + a.l.cut_units);
-  int32_t* cut_row0 = reinterpret_cast<int32_t*>(a.plan + a.l.cut_row0);
+  StepCut* cut_wide = reinterpret_cast<StepCut*>(a.plan + a.l.cut_wide);
+  StepCut* cut_narrow = reinterpret_cast<StepCut*>(a.plan + a.l.cut_narrow);
   auto flag = [&] { atomicOr(a.err, 8); };
   auto prefix_len = [&](int p) {  // of prefix p, within its table
     const int64_t n = a.prefix_lens[p];
@@ -271,7 +276,7 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
     const int n = a.prefix_lens[p];
     if (n < 0 || n > a.s.max_prefix) flag();
   }
-  if (tid == 0) n_cut = 0;
+  if (tid < 2) n_cut[tid] = 0;
   __syncthreads();
   for (int b = tid; b < B; b += kPlanThreads) {
     int t0 = a.token_starts[b], t1 = a.token_starts[b + 1];
@@ -477,25 +482,23 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
   }
   __syncthreads();
   // ---- units that several workers share: the first of them and their number ----
-  auto tile_of = [&](int unit) { return unit < units_w ? unit % n_wide : n_wide + (unit - units_w) / hkv; };
   for (int i = tid; i < 2 * (W + 1); i += kPlanThreads) {
     const int unit = st_unit[i];
     if (st_step[i] == 0 || (st_unit[i - 1] == unit && st_step[i - 1] > 0)) continue;  // an axis starts at step 0
     int k = i + 1;
     while (st_unit[k] == unit) ++k;
-    cuts[unit] = i | (k - i + 1) << 16;  // first worker's place + 1, workers
-    if (tiles[tile_of(unit)].dest == kToOut) cut_units[atomicAdd(&n_cut, 1)] = unit;
+    const int cut = i | (k - i + 1) << 16;  // first worker's place + 1, workers
+    cuts[unit] = cut;
+    const bool wide = unit < units_w;
+    const int ti = wide ? unit % n_wide : n_wide + (unit - units_w) / hkv, kvh = wide ? unit / n_wide : (unit - units_w) % hkv;
+    const StepTile& t = tiles[ti];
+    if (t.dest == kToOut)
+      (wide ? cut_wide : cut_narrow)[atomicAdd(&n_cut[wide ? 0 : 1], 1)] = StepCut{cut, t.row0, t.rows, t.tok0, kvh * rep, {0, 0, 0}};
   }
   __syncthreads();
-  for (int i = tid; i < n_cut; i += kPlanThreads) st_step[i] = tiles[tile_of(cut_units[i])].rows;
-  __syncthreads();
-  const int rows = scan_lds(st_step, n_cut, tmp);
-  for (int i = tid; i < n_cut; i += kPlanThreads) cut_row0[i] = st_step[i];
-  if (tid == 0) {
-    cut_row0[n_cut] = rows;
+  if (tid == 0)
     *head = StepHead{kPlanMagic, B, tokens, a.s.hq, hkv, a.s.d, a.s.bs, a.s.causal, NP, static_cast<int>(a.s.max_own),
-                     static_cast<int>(a.s.max_prefix), W, n_wide, n_nar, n_shared, n_cut, rows, {0, 0, 0}};
-  }
+                     static_cast<int>(a.s.max_prefix), W, n_wide, n_nar, n_shared, n_cut[0], n_cut[1], {0, 0, 0}};
 }
 
 void launch_step_plan(const StepShape& s, const int32_t* token_starts, const int32_t* seq_lens, const int32_t* prefix_ids,
@@ -510,7 +513,7 @@ void launch_step_plan(const StepShape& s, const int32_t* token_starts, const int
 // ----------------------------------------------------------------------------------
 struct StepArgs {
   const char* plan;
-  size_t p_tiles, p_shared, p_starts, p_cuts, p_cut_units, p_cut_row0;
+  size_t p_tiles, p_shared, p_starts, p_cuts, p_cut_wide, p_cut_narrow;
   StepShape s;
   int32_t workers;
   const uint16_t* q;
@@ -1269,25 +1272,21 @@ __global__ __launch_bounds__(kStepThreads, 1) void step_attn_kernel(StepArgs arg
 }
 
 // ----------------------------------------------------------------------------------
-// Join: 16 lanes a row.  The rows of tokens behind shared prefixes (own part and prefix part),
-// then those of cut units; a part is a unit's rows as one worker left them.  Bound by the chain
-// of loads that finds a row's parts (five), so as many rows as the GPU holds are under way.
+// Join: 32 lanes a row, 16 for every other part of it.  The rows of tokens behind shared prefixes
+// (own part and prefix part), then those of cut units; a part is a unit's rows as one worker left
+// them.  Bound by the chain of loads that finds a row's parts (three or four, some 0.7 us each).
 // ----------------------------------------------------------------------------------
-constexpr int kJoinLanes = 16, kJoinRows = 256 / kJoinLanes;
+constexpr int kJoinLanes = 32, kJoinRows = 256 / kJoinLanes;
 
 __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
   const int32_t* head = reinterpret_cast<const int32_t*>(a.plan);
+  const int n_wide = head[12], n_shared = head[14], cut_wide = head[15], cut_narrow = head[16];
   if (!plan_fits(head, a.s, a.workers)) return;  // the attention kernel has said so
-  const int n_wide = head[12], n_shared = head[14], n_cut = head[15], cut_rows = head[16];
   const int units_w = n_wide * a.s.hkv, hkv = a.s.hkv, hq = a.s.hq, d = a.s.d;
-  const StepTile* tiles = reinterpret_cast<const StepTile*>(a.plan + a.p_tiles);
-  const StepShared* shared = reinterpret_cast<const StepShared*>(a.plan + a.p_shared);
   const int2* starts = reinterpret_cast<const int2*>(a.plan + a.p_starts);
-  const int32_t* cuts = reinterpret_cast<const int32_t*>(a.plan + a.p_cuts);
-  const int32_t* cut_units = reinterpret_cast<const int32_t*>(a.plan + a.p_cut_units);
-  const int32_t* cut_row0 = reinterpret_cast<const int32_t*>(a.plan + a.p_cut_row0);
-  const int sub = threadIdx.x % kJoinLanes;
-  const int64_t shared_rows = static_cast<int64_t>(n_shared) * hq, rows = shared_rows + cut_rows;
+  const int sub = threadIdx.x % kJoinLanes, col = sub % 16 * 8 < d ? sub % 16 * 8 : 0;
+  const int64_t shared_rows = static_cast<int64_t>(n_shared) * hq;
+  const int64_t rows = shared_rows + cut_wide * kWideRows + cut_narrow * kNarrowRows;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kJoinRows + threadIdx.x / kJoinLanes; i < rows;
        i += static_cast<int64_t>(gridDim.x) * kJoinRows) {
     // up to two sources of parts: a cut unit's slots or one row
@@ -1296,9 +1295,10 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
     int c1 = 0, r1 = 0, c2 = 0, r2 = 0;        // cuts entry and row in the slots
     int token, hd;
     if (i < shared_rows) {
+      const int32_t* cuts = reinterpret_cast<const int32_t*>(a.plan + a.p_cuts);
       const int li = static_cast<int>(i / hq);
       hd = static_cast<int>(i - static_cast<int64_t>(li) * hq);
-      const StepShared s = shared[li];
+      const StepShared s = reinterpret_cast<const StepShared*>(a.plan + a.p_shared)[li];
       token = s.token;
       const int kvh = hd / a.rep, h = hd - kvh * a.rep, own = s.own_row + h, pre = s.pre_row + h;
       c1 = cuts[units_w + (s.own_tile + own / kNarrowRows) * hkv + kvh];
@@ -1310,15 +1310,16 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
       o2 = a.pre_o + i * d;
       l2 = a.pre_lse + i;
     } else {
-      const int x = static_cast<int>(i - shared_rows);
-      const int e = last_at_most(cut_row0, n_cut, x), unit = cut_units[e];
-      const int ti = unit < units_w ? unit % n_wide : n_wide + (unit - units_w) / hkv;
-      const int kvh = unit < units_w ? unit / n_wide : (unit - units_w) % hkv;
-      r1 = x - cut_row0[e];
-      c1 = cuts[unit];
-      const int sr = tiles[ti].row0 + r1, ri = sr / a.rep;
-      token = tiles[ti].tok0 + ri;
-      hd = kvh * a.rep + sr - ri * a.rep;
+      int x = static_cast<int>(i - shared_rows);
+      const bool wide = x < cut_wide * kWideRows;
+      if (!wide) x -= cut_wide * kWideRows;
+      const StepCut t = reinterpret_cast<const StepCut*>(a.plan + (wide ? a.p_cut_wide : a.p_cut_narrow))[wide ? x / kWideRows : x / kNarrowRows];
+      r1 = wide ? x % kWideRows : x % kNarrowRows;
+      if (r1 >= t.rows) continue;  // for all of a row's lanes
+      c1 = t.cut;
+      const int sr = t.row0 + r1, ri = sr / a.rep;
+      token = t.tok0 + ri;
+      hd = t.head0 + sr - ri * a.rep;
     }
     const int w1 = (c1 & 0xffff) - 1, w2 = (c2 & 0xffff) - 1;  // place of the first worker
     const int n1 = c1 != 0 ? c1 >> 16 : 1, n2 = o2 == nullptr ? 0 : c2 != 0 ? c2 >> 16 : 1, n = n1 + n2;
@@ -1353,17 +1354,20 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
       den = den * keep + fs;
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= keep;
-      // every lane has its part of a row loaded, four parts at a time; a part without weight is
-      // read from where its address would be (the slots' start where it has none) and left out
+      // A lane loads four parts at a time; one without weight from where its address would be (the
+      // slots' start where it has none), to be left out.
       const uint64_t ptr = reinterpret_cast<uint64_t>(o != nullptr ? o : a.slot_o);
-      const int parts = min(kJoinLanes, n - k0), lane0 = (threadIdx.x & 63) - sub, col = 8 * sub < d ? 8 * sub : 0;
-      for (int k = 0; k < parts; k += 4) {
+      const int parts = min(kJoinLanes, n - k0), lane0 = (threadIdx.x & 63) - sub;
+      // The same number of rounds for all of a row's lanes: they read each other's addresses.
+      for (int round = 0; round < parts; round += 8) {
+        const int k = round + sub / 16;
         f32x4 v[4][2];
         float fk[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int src = lane0 + min(k + e, parts - 1);
-          fk[e] = k + e < parts ? __shfl(f, src) : 0.f;
+          const int src = lane0 + min(k + 2 * e, parts - 1);
+          fk[e] = __shfl(f, src);
+          if (k + 2 * e >= parts) fk[e] = 0.f;
           const uint64_t pk = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr), src)) |
                               static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ptr >> 32), src)) << 32;
           const f32x4* ok = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(pk) + col);
@@ -1381,8 +1385,10 @@ __global__ __launch_bounds__(256) void step_join_kernel(StepArgs a) {
           }
       }
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += __shfl_xor(x[e], 16);
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    if (8 * sub < d) {
+    if (sub < 16 && 8 * sub < d) {
       const int64_t off = hd * a.out_hs + token * a.out_ss + 8 * sub;
       store4(a.out, a.out_dtype, off, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
       store4(a.out, a.out_dtype, off + 4, x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
@@ -1410,7 +1416,7 @@ void launch_step_attn(const StepLaunch& L, hipStream_t stream) {
   const WorkLayout w = work_layout(L.s, workers);
   StepArgs a;
   a.plan = static_cast<const char*>(L.plan);
-  a.p_tiles = l.tiles; a.p_shared = l.shared; a.p_starts = l.starts; a.p_cuts = l.cuts; a.p_cut_units = l.cut_units; a.p_cut_row0 = l.cut_row0;
+  a.p_tiles = l.tiles; a.p_shared = l.shared; a.p_starts = l.starts; a.p_cuts = l.cuts; a.p_cut_wide = l.cut_wide; a.p_cut_narrow = l.cut_narrow;
   a.s = L.s;
   a.workers = workers;
   a.q = static_cast<const uint16_t*>(L.q);
@@ -1438,7 +1444,7 @@ void launch_step_attn(const StepLaunch& L, hipStream_t stream) {
   HCP_HIP(hipGetLastError());
   // no more rows are joined than the query has, nor than shared ones and two cut units a worker
   const int64_t rows = std::min(L.s.tokens * L.s.hq, l.max_shared * L.s.hq + 2 * static_cast<int64_t>(workers) * w.slot_rows);
-  const int64_t grid = std::min<int64_t>(ceil_div(rows, kJoinRows), 8 * workers);
+  const int64_t grid = std::min<int64_t>(ceil_div(rows, kJoinRows) + 1, 8 * workers);
   step_join_kernel<<<static_cast<unsigned>(grid), 256, 0, stream>>>(a);
   HCP_HIP(hipGetLastError());
 }

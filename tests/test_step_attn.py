@@ -146,3 +146,15 @@ def test_shared_prefixes(gpu, heads, dtype):
     step = Step([1, 1, 2, 1, 1, 1, 1, 40, 1, 1, 1, 0], [1, 20, 3, 70, 5, 33, 9, 60, 64, 18, 1, 4], hq, hkv, d, ids=ids,
                 plens=[517, 64, 31, 0, 16], dtype=dtype, seed=3)
     check(step, *step.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ctx", [1000, 4500, 9000, 40000])
+@pytest.mark.parametrize("heads", [(8, 1, 128), (4, 2, 64), (12, 3, 96)])
+def test_one_sequence_over_the_whole_gpu(gpu, heads, ctx):
+    """A few units cut among all workgroups: up to 256 parts of a row are joined, of a number that
+    is no multiple of what a lane loads at a time."""
+    hq, hkv, d = heads
+    for new in (1, 2, 40):
+        step = Step([new], [ctx + new], hq, hkv, d, seed=ctx)
+        check(step, *step.run())
