@@ -33,7 +33,7 @@ constexpr int kStepThreads = 64 * kStepWaves;
 constexpr int kWideRows = 32 * kStepWaves;  // rows of a wide tile
 constexpr int kWideKeys = 128;              // keys of its steps
 constexpr int kNarrowRows = 32;
-constexpr int kNarrowMost = 128;            // most rows of a source that is cut into narrow tiles
+constexpr int kNarrowMost = 128;            // most rows of a source that is cut into narrow tiles in any step
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMagic = 0x53544550;
 
@@ -44,6 +44,11 @@ constexpr int kWideFixed = 70, kWideStep = 40;
 constexpr int kNarrowFixed = 32, kNarrowStep = 26;
 // Of a worker: less is not worth another part to join.
 constexpr int kLeastShare = 50;
+// Sources of more rows are narrow tiles too where that is this much longer at most per worker: a
+// step of few wide units cuts them among many workers, each of which leaves 256 rows to join.  512
+// queries x 2085 keys, 8/1 heads of 96 dims, fp32 rows: 32 us as 16 wide units, 22.6 as 128 narrow
+// ones; 1500-token prefixes behind 16 sequences of 5 tokens, 14/2 heads of 64: 24.5 and 23.3.
+constexpr int kNarrowMore = 150;
 constexpr int kXcds = 8;
 
 // Where a unit's rows go when it is not cut.
@@ -103,8 +108,7 @@ PlanLayout plan_layout(const StepShape& s) {
   PlanLayout l;
   l.max_shared = s.prefixes > 0 ? std::min<int64_t>(s.tokens, live * (kNarrowMost / rep)) : 0;
   l.max_wide = s.tokens * rep / kWideRows + live + (s.prefixes > 0 ? l.max_shared * rep / kWideRows + std::min<int64_t>(s.prefixes, live) : 0);
-  const int64_t each = kNarrowMost / kNarrowRows;  // narrow tiles of a source
-  l.max_narrow = std::min(s.tokens * rep / kNarrowRows + live, live * each) + std::min<int64_t>(s.prefixes, live) * each;
+  l.max_narrow = s.tokens * rep / kNarrowRows + live + (s.prefixes > 0 ? l.max_shared * rep / kNarrowRows + std::min<int64_t>(s.prefixes, live) : 0);
   l.max_units = (l.max_wide + l.max_narrow) * s.hkv;
   size_t at = up256(sizeof(StepHead));
   auto take = [&](size_t bytes) {
@@ -244,13 +248,14 @@ __device__ int last_at_most(const T* a, int n, T x) {
 
 __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs a) {
   __shared__ int s_tok[kStepMaxBatch], s_n[kStepMaxBatch], s_vis[kStepMaxBatch], s_len[kStepMaxBatch];
-  __shared__ int s_pid[kStepMaxBatch], s_wide[kStepMaxBatch], s_nar[kStepMaxBatch];
+  __shared__ int s_pid[kStepMaxBatch], s_wide[kStepMaxBatch], s_nar[kStepMaxBatch], s_list[kStepMaxBatch];
   __shared__ int g_seq[kStepMaxPrefixes], g_tok[kStepMaxPrefixes], g_list[kStepMaxPrefixes], g_wide[kStepMaxPrefixes],
       g_nar[kStepMaxPrefixes];
   __shared__ int64_t tmp64[kPlanThreads / 64];
   __shared__ int tmp[kPlanThreads / 64];
   __shared__ int st_unit[2 * (kStepMaxWorkers + 1)], st_step[2 * (kStepMaxWorkers + 1)];
   __shared__ int n_cut[2];
+  __shared__ unsigned long long more[2];  // modelled time of the sources above kNarrowMost rows: wide, narrow
 
   const int tid = threadIdx.x;
   const int B = a.s.batch, NP = a.s.prefixes, rep = a.s.hq / a.s.hkv, hkv = a.s.hkv;
@@ -276,7 +281,7 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
     const int n = a.prefix_lens[p];
     if (n < 0 || n > a.s.max_prefix) flag();
   }
-  if (tid < 2) n_cut[tid] = 0;
+  if (tid < 2) n_cut[tid] = more[tid] = 0;
   __syncthreads();
   for (int b = tid; b < B; b += kPlanThreads) {
     int t0 = a.token_starts[b], t1 = a.token_starts[b + 1];
@@ -310,14 +315,29 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
     }
   }
   __syncthreads();
-  // ---- prefixes with tokens of several sequences behind them: list places and tiles ----
+  // ---- prefixes with tokens of several sequences behind them; which sources are wide ----
+  auto weigh = [&](int64_t rows, int64_t keys) {
+    if (rows <= kNarrowMost) return;
+    atomicAdd(&more[0], static_cast<unsigned long long>((rows + kWideRows - 1) / kWideRows * (kWideFixed + (keys + kWideKeys - 1) / kWideKeys * kWideStep)));
+    atomicAdd(&more[1], static_cast<unsigned long long>((rows + kNarrowRows - 1) / kNarrowRows * (kNarrowFixed + (keys + 255) / 256 * kNarrowStep)));
+  };
   for (int p = tid; p < NP; p += kPlanThreads) {
     const bool on = g_seq[p] >= 2;
-    const int rows = on ? g_tok[p] * rep : 0;
     if (!on) g_seq[p] = 0;
+    else weigh(static_cast<int64_t>(g_tok[p]) * rep, prefix_len(p));
     g_list[p] = on ? g_tok[p] : 0;
-    g_wide[p] = rows > kNarrowMost ? (rows + kWideRows - 1) / kWideRows : 0;
-    g_nar[p] = rows <= kNarrowMost ? (rows + kNarrowRows - 1) / kNarrowRows : 0;
+  }
+  for (int b = tid; b < B; b += kPlanThreads)
+    if (s_n[b] > 0)
+      weigh(static_cast<int64_t>(s_n[b]) * rep,
+            (s_pid[b] >= 0 ? prefix_len(s_pid[b]) : 0) + max(s_len[b] - (a.s.causal ? s_n[b] / 2 : 0), 0));
+  __syncthreads();
+  const int64_t narrow_more = static_cast<int64_t>(more[1] - more[0]) * hkv / a.workers;
+  const int64_t most = narrow_more <= kNarrowMore ? INT64_MAX : kNarrowMost;  // rows of a source in narrow tiles
+  for (int p = tid; p < NP; p += kPlanThreads) {
+    const int rows = g_list[p] * rep;
+    g_wide[p] = rows > most ? (rows + kWideRows - 1) / kWideRows : 0;
+    g_nar[p] = rows <= most ? (rows + kNarrowRows - 1) / kNarrowRows : 0;
   }
   __syncthreads();
   const int n_shared = NP > 0 ? scan_lds(g_list, NP, tmp) : 0;
@@ -325,96 +345,85 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
   const int pre_nar = NP > 0 ? scan_lds(g_nar, NP, tmp) : 0;
   for (int b = tid; b < B; b += kPlanThreads) {
     const int64_t rows = static_cast<int64_t>(s_n[b]) * rep;
-    s_wide[b] = rows > kNarrowMost ? static_cast<int>((rows + kWideRows - 1) / kWideRows) : 0;
-    s_nar[b] = rows <= kNarrowMost ? static_cast<int>((rows + kNarrowRows - 1) / kNarrowRows) : 0;
+    s_wide[b] = rows > most ? static_cast<int>((rows + kWideRows - 1) / kWideRows) : 0;
+    s_nar[b] = rows <= most ? static_cast<int>((rows + kNarrowRows - 1) / kNarrowRows) : 0;
   }
   __syncthreads();
   const int n_wide = pre_wide + scan_lds(s_wide, B, tmp);
   const int n_nar = pre_nar + scan_lds(s_nar, B, tmp);
 
-  // ---- the list of tokens behind shared prefixes, and the narrow tiles of sequences ----
+  // ---- the list of tokens behind shared prefixes ----
   for (int b = tid; b < B; b += kPlanThreads) {
-    const int n = s_n[b], rows = n * rep;
-    if (n == 0 || static_cast<int64_t>(n) * rep > kNarrowMost) continue;
-    const int p = s_pid[b];
-    const bool on = p >= 0 && g_seq[p] > 0;
-    const int own = pre_nar + s_nar[b];
-    int at = 0;
-    if (on) {
-      // place behind the earlier sequences of the same prefix
-      at = g_list[p];
-      for (int c = 0; c < b; ++c)
-        if (s_pid[c] == p && static_cast<int64_t>(s_n[c]) * rep <= kNarrowMost) at += s_n[c];
-      const int wide = g_tok[p] * rep > kNarrowMost;
-      for (int i = 0; i < n; ++i)
-        shared[at + i] = StepShared{s_tok[b] + i, own, i * rep, wide ? g_wide[p] : g_nar[p], (at + i - g_list[p]) * rep, wide, {0, 0}};
-    }
-    const int vstep = a.s.causal ? 1 : 0;
-    for (int k = 0; k * kNarrowRows < rows; ++k) {
-      StepTile t{};
-      t.tok0 = s_tok[b];
-      t.row0 = k * kNarrowRows;
-      t.rows = min(kNarrowRows, rows - t.row0);
-      t.p_row = max(p, 0);
-      t.p_len = p >= 0 && !on ? prefix_len(p) : 0;
-      t.s_row = b;
-      t.s_len = max(0, min(s_len[b], s_vis[b] + (t.row0 + t.rows - 1) / rep * vstep));
-      t.vis0 = s_vis[b];
-      t.vis_step = vstep;
-      t.steps = max(1, ((t.p_len + 31) / 32 + (t.s_len + 31) / 32 + kStepWaves - 1) / kStepWaves);
-      t.dest = on ? kToOwn : kToOut;
-      t.list0 = at;
-      tiles[n_wide + own + k] = t;
-    }
+    const int n = s_n[b], p = s_pid[b];
+    s_list[b] = -1;
+    if (n == 0 || p < 0 || g_seq[p] == 0 || static_cast<int64_t>(n) * rep > kNarrowMost) continue;
+    int at = g_list[p];  // behind the earlier sequences of the same prefix
+    for (int c = 0; c < b; ++c)
+      if (s_pid[c] == p && static_cast<int64_t>(s_n[c]) * rep <= kNarrowMost) at += s_n[c];
+    const int wide = static_cast<int64_t>(g_tok[p]) * rep > most;
+    for (int i = 0; i < n; ++i)
+      shared[at + i] = StepShared{s_tok[b] + i, pre_nar + s_nar[b], i * rep, wide ? g_wide[p] : g_nar[p], (at + i - g_list[p]) * rep, wide, {0, 0}};
+    s_list[b] = at;
   }
-  // ---- narrow tiles of prefixes ----
-  for (int p = tid; p < NP; p += kPlanThreads) {
-    const int rows = g_seq[p] > 0 ? g_tok[p] * rep : 0;
-    if (rows == 0 || rows > kNarrowMost) continue;
-    for (int k = 0; k * kNarrowRows < rows; ++k) {
-      StepTile t{};
-      t.tok0 = g_list[p];
-      t.row0 = k * kNarrowRows;
-      t.rows = min(kNarrowRows, rows - t.row0);
-      t.p_row = p;
-      t.p_len = prefix_len(p);
-      t.steps = max(1, ((t.p_len + 31) / 32 + kStepWaves - 1) / kStepWaves);
-      t.dest = kToPrefix;
-      t.list0 = g_list[p];
-      t.list = 1;
-      tiles[n_wide + g_nar[p] + k] = t;
+  __syncthreads();
+  const int vstep = a.s.causal ? 1 : 0;
+  // rows row0 .. of a sequence or of a prefix's tokens as a tile of up to `size` rows
+  auto own_tile = [&](int b, int row0, int size) {
+    StepTile t{};
+    const int p = s_pid[b];
+    const bool shares = s_list[b] >= 0;
+    t.tok0 = s_tok[b];
+    t.row0 = row0;
+    t.rows = min(size, s_n[b] * rep - row0);
+    t.p_row = max(p, 0);
+    t.p_len = p >= 0 && !shares ? prefix_len(p) : 0;
+    t.s_row = b;
+    t.s_len = max(0, min(s_len[b], s_vis[b] + (row0 + t.rows - 1) / rep * vstep));
+    t.vis0 = s_vis[b];
+    t.vis_step = vstep;
+    t.dest = shares ? kToOwn : kToOut;
+    t.list0 = max(s_list[b], 0);
+    return t;
+  };
+  auto prefix_tile = [&](int p, int row0, int size) {
+    StepTile t{};
+    t.tok0 = t.list0 = g_list[p];
+    t.list = 1;
+    t.row0 = row0;
+    t.rows = min(size, g_tok[p] * rep - row0);
+    t.p_row = p;
+    t.p_len = prefix_len(p);
+    t.dest = kToPrefix;
+    return t;
+  };
+  // ---- narrow tiles, one a thread ----
+  for (int i = tid; i < n_nar; i += kPlanThreads) {
+    StepTile t;
+    if (i < pre_nar) {
+      const int p = last_at_most(g_nar, NP, i);
+      t = prefix_tile(p, (i - g_nar[p]) * kNarrowRows, kNarrowRows);
+    } else {
+      const int b = last_at_most(s_nar, B, i - pre_nar);
+      t = own_tile(b, (i - pre_nar - s_nar[b]) * kNarrowRows, kNarrowRows);
     }
+    t.steps = max(1, ((t.p_len + 31) / 32 + (t.s_len + 31) / 32 + kStepWaves - 1) / kStepWaves);
+    tiles[n_wide + i] = t;
   }
   // ---- wide tiles, one a thread.  Those of sequences are laid out column by column: dealt to the
   // columns (the workers of a kv head) to and fro, the last of a sequence first, so that a worker
   // starts with a long tile and all get about as much; the workgroups of an XCD then go through
   // the keys side by side and find them in its L2 (a prompt of 16384 tokens, 32/8 heads: 2.16 ms in
-  // the order of the rows, WIDEORD so). ----
+  // the order of the rows, 2.04 so). ----
   const int own_wide = n_wide - pre_wide, cols = max(1, min(own_wide, a.workers / hkv)), rounds = (own_wide + cols - 1) / cols;
   const int rest = own_wide - (rounds - 1) * cols;  // tiles of the last round
   for (int i = tid; i < n_wide; i += kPlanThreads) {
-    StepTile t{};
+    StepTile t;
     if (i < pre_wide) {
       const int p = last_at_most(g_wide, NP, i);
-      t.tok0 = t.list0 = g_list[p];
-      t.list = 1;
-      t.row0 = (i - g_wide[p]) * kWideRows;
-      t.rows = min(kWideRows, g_tok[p] * rep - t.row0);
-      t.p_row = p;
-      t.p_len = prefix_len(p);
-      t.dest = kToPrefix;
+      t = prefix_tile(p, (i - g_wide[p]) * kWideRows, kWideRows);
     } else {
-      const int b = last_at_most(s_wide, B, i - pre_wide), vstep = a.s.causal ? 1 : 0;
-      t.tok0 = s_tok[b];
-      t.row0 = (i - pre_wide - s_wide[b]) * kWideRows;
-      t.rows = min(kWideRows, s_n[b] * rep - t.row0);
-      t.p_row = max(s_pid[b], 0);
-      t.p_len = s_pid[b] >= 0 ? prefix_len(s_pid[b]) : 0;
-      t.s_row = b;
-      t.s_len = max(0, min(s_len[b], s_vis[b] + (t.row0 + t.rows - 1) / rep * vstep));
-      t.vis0 = s_vis[b];
-      t.vis_step = vstep;
-      t.dest = kToOut;
+      const int b = last_at_most(s_wide, B, i - pre_wide);
+      t = own_tile(b, (i - pre_wide - s_wide[b]) * kWideRows, kWideRows);
     }
     t.steps = max(1, (t.p_len + kWideKeys - 1) / kWideKeys + (t.s_len + kWideKeys - 1) / kWideKeys);
     int to = i;
