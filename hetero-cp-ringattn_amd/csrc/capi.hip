@@ -2097,8 +2097,8 @@ StepShape step_shape(const hcp_paged_decode_desc* d, int64_t tokens, int32_t cau
     require(prefixes->table_len <= (int64_t(1) << 30) / bs, "prefix tables of more than 2^30 tokens");
     s.max_prefix = prefixes->table_len * bs;
   }
-  // a plan counts (tile, kv head) units in 32 bits: a tile a 256 rows, up to three a sequence
-  require((tokens * (s.hq / s.hkv) / 128 + 4 * static_cast<int64_t>(s.batch)) * s.hkv < (int64_t(1) << 30), "too many rows for one step");
+  // a plan counts (tile, kv head) units in 32 bits: at most a tile every 16 rows and four a sequence
+  require((tokens * (s.hq / s.hkv) / 8 + 4 * static_cast<int64_t>(s.batch)) * s.hkv < (int64_t(1) << 30), "too many rows for one step");
   return s;
 }
 StepShape step_call(const hcp_paged_decode_desc* d, const hcp_paged_pool* pool, int64_t tokens, int32_t causal,

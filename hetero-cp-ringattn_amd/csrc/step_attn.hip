@@ -737,6 +737,14 @@ __device__ __forceinline__ void load_q(args_ptr a, const RowOf& r, int kvh, int 
     qf[s] = as_frag<typename MfmaOps<DT>::frag>(!PAD || 16 * s + 8 * lhalf < dn ? x[s] : u32x4{0u, 0u, 0u, 0u});
 }
 
+// The largest weight of a row is 2^kBias where its maximum was last taken, and no sum of a lane's
+// weights passes kMostSum: f16 holds weights down to 2^-31 of the largest so, whose sum over a long
+// row is still within fp32's needs (with the largest at 1 all below 2^-24 were lost).
+template <int DT>
+constexpr float kBias = DT == kF16 ? 7.f : 0.f;
+template <int DT>
+constexpr float kMostSum = kGrowSum * (DT == kF16 ? 128.f : 1.f);
+
 template <int DT>
 __device__ __forceinline__ float frag_value(typename MfmaOps<DT>::frag f, int i) {
   return static_cast<float>(f[i]);
@@ -879,13 +887,13 @@ __device__ __forceinline__ void step_narrow(args_ptr a, const StepRun& run, int 
       bool redo = first;
       if (!redo) {
         lsum = weigh();
-        redo = __any(!(lsum <= kGrowSum));
+        redo = __any(!(lsum <= kMostSum<DT>));
       }
       if (redo) {
         float top = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, sacc[r]);
-        const float m_new = fmaxf(m_run, max_xor32(top) * c);
+        const float m_new = fmaxf(m_run, max_xor32(top) * c - kBias<DT>);
         const float alpha = exp2f(m_run - m_new);
         l_run *= alpha;
 #pragma unroll
@@ -1189,13 +1197,13 @@ __device__ __forceinline__ void step_wide(args_ptr a, const StepRun& run, int pl
       if constexpr (TW == 1) {
         if (!redo) {
           weigh();
-          redo = __any(!(lsum <= kGrowSum));
+          redo = __any(!(lsum <= kMostSum<DT>));
         }
       }
       const float top = TW > 1 || redo ? highest() : 0.f;
-      if (TW > 1) redo = redo || __any(!(top <= m_run + 8.f));
+      if (TW > 1) redo = redo || __any(!(top <= m_run + 8.f + kBias<DT>));
       if (redo) {
-        const float m_new = fmaxf(m_run, top);
+        const float m_new = fmaxf(m_run, top - kBias<DT>);
         const float alpha = exp2f(m_run - m_new);
         l_run *= alpha;
 #pragma unroll

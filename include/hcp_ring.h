@@ -840,6 +840,9 @@ int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float e
  * or all of them (0, a peer domain's shard).  out [Hq, tokens, D] (out_dtype: dtype, or F32 for
  * a partial) gets softmax(q k^T scale) v and lse [Hq, tokens] fp32 (may be NULL) the natural
  * log-sum-exp: 0 and -inf where nothing is seen.  Rows of no sequence are left as they are.
+ * Slots past a length are not read.  A K row that is not finite reaches only the tokens that see
+ * it; a V row that is not finite may reach the new tokens before it, too, of its own sequence
+ * alone (a weight of 0 times it).
  *
  * A prefix is read once for all the tokens behind it of sequences with up to 32 / (Hq / Hkv)
  * new tokens; longer runs of tokens read it for themselves.
