@@ -868,6 +868,16 @@ def _rows_of(name, t, shape, dev, dtype=None):
                          + (f" in {dtype}" if dtype is not None else ""))
 
 
+def _row_view(name, t, shape, dev, dtype):
+    """hcp_ring_view of rows [heads, tokens, head_dim], checked (one pass over what a call asks of them)."""
+    a, b, c = t.stride()
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be [{', '.join(str(n) for n in shape)}] on {_place(dev)} in {dtype}")
+    if c != 1 and shape[2] > 1:
+        raise ValueError("head_dim must be the contiguous dimension")
+    return View(t.data_ptr(), a, b)
+
+
 def kv8_append(pool, scales, k, v, slots, stream=None):
     """Quantise the rows of k / v [Hkv, T, D] into the slots [T] int64 of an 8-bit cache
     (:func:`kv_plan_step`; negative: skipped).  A block's scale is a power of two that only
@@ -1004,31 +1014,34 @@ def kv8_ring_attention_replay_paged(q, pool, scales, block_table, chunks, causal
 # (11) norms of q and k with the rotation
 # ---------------------------------------------------------------------------------
 def _qk_norm(q, k, q_weight, k_weight, positions, table, eps, pairs, q_out, stream):
-    """(GPU, q_out, arguments up to k, arguments from the weights to q_out), the tensors checked."""
-    torch = _torch()
-    dev = q.get_device()
-    hq, tokens, d = q.shape
+    """(GPU, k's shape and dtype, q_out, arguments up to k, arguments from the weights to q_out), the
+    tensors checked."""
+    dev, dtype, shape = q.get_device(), q.dtype, q.shape
+    hq, tokens, d = shape
     hkv = k.shape[0]
-    _rows_of("k", k, (hkv, tokens, d), dev, q.dtype)
+    k_shape = (hkv, tokens, d)
     if q_out is None:
-        q_out = _empty((hq, tokens, d), q.dtype, q.device, stream)
-    else:
-        _rows_of("q_out", q_out, (hq, tokens, d), dev, q.dtype)
+        q_out = _empty(shape, dtype, q.device, stream)
+    weights = []
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None:
-            _want(name, w, q.dtype, (d,), dev)
+            _want(name, w, dtype, (d,), dev)
+            w = w.data_ptr()
+        weights.append(w)
     rows = rot = 0
+    pos = cos = None
     if table is not None:
-        if table.dim() != 3 or table.shape[0] != 2 or positions is None:
+        torch = _torch()
+        two, rows, half = table.shape if table.dim() == 3 else (0, 0, 0)
+        if two != 2 or positions is None:
             raise ValueError("the rotation needs positions and a table [2, rows, rope_dims / 2]")
-        rows, rot = table.shape[1], 2 * table.shape[2]
-        _want("table", table, torch.float32, (2, rows, rot // 2), dev)
+        rot = 2 * half
+        _want("table", table, torch.float32, (2, rows, half), dev)
         _want("positions", positions, torch.int64, (tokens,), dev)
-    desc = QkvDesc(dtype_code(q.dtype), 0, hq, hkv, d, (2 if pairs else 1) if rot else 0, tokens, rows)
-    args = (ctypes.byref(desc), rot, eps, view(q), view(k))
-    more = (None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-            positions.data_ptr() if rot else None, table.data_ptr() if rot else None, view(q_out))
-    return dev, q_out, args, more
+        pos, cos = positions.data_ptr(), table.data_ptr()
+    desc = QkvDesc(dtype_code(dtype), 0, hq, hkv, d, (2 if pairs else 1) if rot else 0, tokens, rows)
+    args = (desc, rot, eps, _row_view("q", q, shape, dev, dtype), _row_view("k", k, k_shape, dev, dtype))
+    return dev, k_shape, dtype, q_out, args, (*weights, pos, cos, _row_view("q_out", q_out, shape, dev, dtype))
 
 
 def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, table=None, eps=1e-6, pairs=False, q_out=None,
@@ -1037,12 +1050,10 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, table=None,
     turned at ``positions`` [T] int64 by the ``table`` of :func:`rope_table` (its rope_dims may be
     less than D; None: no rotation; ``pairs``: planes of neighbouring dims instead of halves)
     -> (q_out, k_out), which may be q and k themselves."""
-    dev, q_out, args, more = _qk_norm(q, k, q_weight, k_weight, positions, table, eps, pairs, q_out, stream)
+    dev, k_shape, dtype, q_out, args, more = _qk_norm(q, k, q_weight, k_weight, positions, table, eps, pairs, q_out, stream)
     if k_out is None:
-        k_out = _empty(k.shape, k.dtype, k.device, stream)
-    else:
-        _rows_of("k_out", k_out, k.shape, dev, k.dtype)
-    _launch(lib().hcp_qk_norm_rope, dev, stream, *args, *more, view(k_out))
+        k_out = _empty(k_shape, dtype, k.device, stream)
+    _launch(lib().hcp_qk_norm_rope, dev, stream, *args, *more, _row_view("k_out", k_out, k_shape, dev, dtype))
     return q_out, k_out
 
 
@@ -1051,13 +1062,12 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, pool, slots, positions=None
     """As :func:`qk_norm_rope`, with the K rows and v [Hkv, T, D] as it is appended to the paged
     ``pool`` [2, num_blocks, block_size, Hkv, D] at ``slots`` [T] int64 (:func:`kv_plan_step`;
     negative: skipped) -> q_out."""
-    dev, q_out, args, more = _qk_norm(q, k, q_weight, k_weight, positions, table, eps, pairs, q_out, stream)
+    dev, k_shape, dtype, q_out, args, more = _qk_norm(q, k, q_weight, k_weight, positions, table, eps, pairs, q_out, stream)
     pp = paged_pool(pool)
-    _rows_of("v", v, k.shape, dev, k.dtype)
-    if pool.dtype != q.dtype or pool.get_device() != dev:
-        raise ValueError(f"pool must be {q.dtype} on {_place(dev)}")
-    _want("slots", slots, _torch().int64, (q.shape[1],), dev)
-    _launch(lib().hcp_qk_norm_rope_append, dev, stream, *args, view(v), *more, ctypes.byref(pp), slots.data_ptr())
+    if pool.dtype != dtype or pool.get_device() != dev:
+        raise ValueError(f"pool must be {dtype} on {_place(dev)}")
+    _want("slots", slots, _torch().int64, k_shape[1:2], dev)
+    _launch(lib().hcp_qk_norm_rope_append, dev, stream, *args, _row_view("v", v, k_shape, dev, dtype), *more, pp, slots.data_ptr())
     return q_out
 
 
@@ -1067,22 +1077,21 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, pool, slots, positions=None
 def _step_args(q, pool, block_tables, prefix_tables, prefix_lens=None, scale=None):
     """(descriptor, pool, number of prefixes, hcp_decode_shard of them or None, GPU), checked."""
     pp = paged_pool(pool)
-    dev = pool.get_device()
+    dev, dtype = pool.get_device(), pool.dtype
     hq, _, d = q.shape
-    if q.dtype != pool.dtype or q.get_device() != dev:
-        raise ValueError(f"q must be {pool.dtype} on {_place(dev)}")
-    b = block_tables.shape[0]
+    if q.dtype != dtype or q.get_device() != dev:
+        raise ValueError(f"q must be {dtype} on {_place(dev)}")
+    b, width = block_tables.shape if block_tables.dim() == 2 else (0, 0)
     _decode_tables("block_tables", block_tables, None, b, dev)
-    n = 0 if prefix_tables is None else prefix_tables.shape[0]
-    shard = None
-    if n:
+    n, shard = 0, None
+    if prefix_tables is not None and prefix_tables.shape[0] > 0:
+        n, m = prefix_tables.shape if prefix_tables.dim() == 2 else (0, 0)
         _decode_tables("prefix_tables", prefix_tables, None, n, dev)
         if prefix_lens is not None:
             _want("prefix_lens", prefix_lens, _torch().int32, (n,), dev)
-        shard = DecodeShard(prefix_tables.data_ptr(), max(prefix_tables.stride(0), prefix_tables.shape[1]), prefix_tables.shape[1],
+        shard = DecodeShard(prefix_tables.data_ptr(), max(prefix_tables.stride(0), m), m,
                             None if prefix_lens is None else prefix_lens.data_ptr(), 0)
-    desc = DecodeDesc(dtype_code(q.dtype), b, hq, pp.num_kv_heads, d, 0, 0, 0,
-                      max(block_tables.stride(0), block_tables.shape[1]), block_tables.shape[1],
+    desc = DecodeDesc(dtype_code(dtype), b, hq, pp.num_kv_heads, d, 0, 0, 0, max(block_tables.stride(0), width), width,
                       scale if scale is not None else 1.0 / math.sqrt(d))
     return desc, pp, n, shard, dev
 
@@ -1138,22 +1147,20 @@ def step_attn(q, pool, block_tables, plan, prefix_tables=None, causal=True, scal
     :func:`step_attn_plan` for the same shapes -> (out [Hq, T, D] in q's type, or fp32 if an fp32
     ``out`` is given, lse [Hq, T] fp32).  Rows of no sequence are left as they are."""
     desc, pp, n, shard, dev = _step_args(q, pool, block_tables, prefix_tables, None, scale)
-    torch = _torch()
-    hq, tokens, d = shape = q.shape
+    shape, dtype, f32 = q.shape, q.dtype, _torch().float32
+    tokens = shape[1]
     if out is None:
-        out = _empty(shape, q.dtype, q.device, stream)
-    _rows_of("out", out, shape, dev)
+        out = _empty(shape, dtype, q.device, stream)
     if lse is None:
-        lse = _empty((hq, tokens), torch.float32, q.device, stream)
-    _want("lse", lse, torch.float32, (hq, tokens), dev)
+        lse = _empty(shape[:2], f32, q.device, stream)
+    _want("lse", lse, f32, shape[:2], dev)
     if plan.get_device() != dev or not plan.is_contiguous():
         raise ValueError(f"plan must be contiguous on {_place(dev)}")
     fns = lib()
-    _ws, ws, ws_bytes = _workspace(workspace, lambda: _size(fns.hcp_step_attn_workspace_size(ctypes.byref(desc), tokens, n)),
-                                   dev, stream)
-    _launch(fns.hcp_step_attn, dev, stream, ctypes.byref(desc), ctypes.byref(pp), tokens, 1 if causal else 0, view(q),
-            block_tables.data_ptr(), n, None if shard is None else ctypes.byref(shard), plan.data_ptr(),
-            plan.numel() * plan.element_size(), dtype_code(out.dtype), view(out), lse.data_ptr(), ws, ws_bytes)
+    _ws, ws, ws_bytes = _workspace(workspace, lambda: _size(fns.hcp_step_attn_workspace_size(desc, tokens, n)), dev, stream)
+    _launch(fns.hcp_step_attn, dev, stream, desc, pp, tokens, 1 if causal else 0, _row_view("q", q, shape, dev, dtype),
+            block_tables.data_ptr(), n, shard, plan.data_ptr(), plan.numel() * plan.element_size(), dtype_code(out.dtype),
+            _row_view("out", out, shape, dev, out.dtype), lse.data_ptr(), ws, ws_bytes)
     return out, lse
 
 
