@@ -358,8 +358,11 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
     s_list[b] = -1;
     if (n == 0 || p < 0 || g_seq[p] == 0 || static_cast<int64_t>(n) * rep > kNarrowMost) continue;
     int at = g_list[p];  // behind the earlier sequences of the same prefix
-    for (int c = 0; c < b; ++c)
-      if (s_pid[c] == p && static_cast<int64_t>(s_n[c]) * rep <= kNarrowMost) at += s_n[c];
+#pragma unroll 8
+    for (int c = 0; c < b; ++c) {
+      const int there = s_pid[c], k = s_n[c];
+      at += there == p && k <= kNarrowMost / rep ? k : 0;
+    }
     const int wide = static_cast<int64_t>(g_tok[p]) * rep > most;
     for (int i = 0; i < n; ++i)
       shared[at + i] = StepShared{s_tok[b] + i, pre_nar + s_nar[b], i * rep, wide ? g_wide[p] : g_nar[p], (at + i - g_list[p]) * rep, wide, {0, 0}};
@@ -1461,7 +1464,7 @@ void launch_step_attn(const StepLaunch& L, hipStream_t stream) {
   HCP_HIP(hipGetLastError());
   // no more rows are joined than the query has, nor than shared ones and two cut units a worker
   const int64_t rows = std::min(L.s.tokens * L.s.hq, l.max_shared * L.s.hq + 2 * static_cast<int64_t>(workers) * w.slot_rows);
-  const int64_t grid = std::min<int64_t>(ceil_div(rows, kJoinRows) + 1, 8 * workers);
+  const int64_t grid = std::min<int64_t>(ceil_div(rows, kJoinRows) + 1, 32 * workers);
   step_join_kernel<<<static_cast<unsigned>(grid), 256, 0, stream>>>(a);
   HCP_HIP(hipGetLastError());
 }
