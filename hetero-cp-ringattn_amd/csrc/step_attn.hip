@@ -482,7 +482,7 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
       }
       // a cut so near a unit's end that it costs more than it evens out is moved there
       step = off <= fixed + slack ? 0 : static_cast<int>((off - fixed + each / 2) / each);
-      if (static_cast<int64_t>(tiles[t].steps - step) * each <= slack) {
+      if (step > 0 && static_cast<int64_t>(tiles[t].steps - step) * each <= slack) {
         ++unit;
         step = 0;
       }
@@ -1271,7 +1271,11 @@ __device__ __forceinline__ void step_wide(args_ptr a, const StepRun& run, int pl
     if (row < t.rows) {
       const RowOf ro = row_of(e, t, row);
       const RowDest dst = row_dest(e, t, kvh, slot, row, ro.token, ro.i, ro.h);
-      write_final_row<DW>(dst.o, dst.dtype, dst.o_off, dst.lse, static_cast<int>(fresh_lane() >> 5), oacc, m_run, sum_xor32(l_run), e->s.d);
+      const float l_tot = sum_xor32(l_run);
+      const int half = static_cast<int>(fresh_lane() >> 5);
+      write_final_row<DW>(dst.o, dst.dtype, dst.o_off, dst.lse, half, oacc, m_run, l_tot, e->s.d);
+      // a row that met a NaN key says so, or a join would take it for one without keys
+      if (half == 0 && dst.lse != nullptr && l_tot != l_tot) *dst.lse = l_tot;
     }
   }
 }

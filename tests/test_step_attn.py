@@ -92,8 +92,9 @@ class Step:
         return o, mag, lse, s
 
 
-def check(step, out, lse, ref=None, terms=1):
-    o, mag, want, s = ref or step.reference()
+def check(step, out, lse, ref=None, terms=1, rows=slice(None)):
+    o, mag, want, s = (t[:, rows] for t in (ref or step.reference()))
+    out, lse = out[:, rows], lse[:, rows]
     live = ~torch.isnan(want)
     half = torch.finfo(step.q.dtype).eps / 2
     r = half ** terms
@@ -281,6 +282,36 @@ def test_values_that_are_not_finite_stay_with_their_sequence(gpu):
     # own key 60 of sequence 1 is seen by its tokens 30 .. 39; its K reaches no other's LSE
     assert torch.equal(lse[:, 1: 31], want_lse[:, 1: 31]) and bool(lse[:, 31: 41].isnan().all())
     assert not bool(out[:, 1: 41].isfinite().all(-1).any())
+
+
+@pytest.mark.gpu
+def test_a_nan_key_in_a_long_chunk_is_not_lost(gpu):
+    """Tiles of 256 rows, some of them joined of parts: the rows that see the key are NaN, and their
+    LSE too, the ones before it as they were.  The 8 tokens of a wave take their maxima anew
+    together, so those beside token 700 may round otherwise: they stay within the bounds."""
+    step = Step([1500, 1], [5500, 40], 32, 8, 128, seed=16)
+    ref = step.reference()
+    x = step.device()
+    want, want_lse = (t.clone() for t in step.run(x=x))
+    x["pool"][0, int(step.tables[0, 4700 // 16]), 4700 % 16] = float("nan")  # seen by tokens 700 ..
+    out, lse = step.run(x=x)
+    assert torch.equal(lse[:, :696], want_lse[:, :696]) and torch.equal(out[:, :696], want[:, :696])
+    check(step, out, lse, ref=ref, rows=slice(0, 700))
+    assert bool(lse[:, 700: 1500].isnan().all()) and bool(out[:, 700: 1500].isnan().all())
+    assert torch.equal(out[:, 1500:], want[:, 1500:]) and torch.equal(lse[:, 1500:], want_lse[:, 1500:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [1, 200, 600])
+def test_a_short_sequence_before_long_ones(gpu, first):
+    """The first unit of the work is short against a worker's share, and is still done."""
+    for new, lens in (([1] * 24, [first] + [12000] * 23), ([1] * 24, [12000] * 23 + [first])):
+        step = Step(new, lens, 16, 8, 64, seed=17)
+        out = torch.full((16, 24, 64), float("nan"), dtype=torch.bfloat16, device="cuda")
+        check(step, *step.run(out=out))
+    step = Step([40, 3000], [40 + first, 6000], 16, 8, 64, seed=18)
+    out = torch.full((16, 3040, 64), float("nan"), dtype=torch.bfloat16, device="cuda")
+    check(step, *step.run(out=out))
 
 
 @pytest.mark.gpu
