@@ -4,20 +4,29 @@
 //   o = softmax(q K^T scale) V over a sequence's prefix keys and those of its own keys that a
 //   token sees; a prefix's K and V are read once for all of the step's tokens behind it.
 //
-// Rows.  The query heads of a kv head are packed token-major: row r of a source is token
-// r / rep, head r % rep of the group.  A source of more than 32 rows (a prompt chunk, or the
-// tokens behind one prefix) is cut into wide tiles of 256 rows, 32 a wave, whose K and V
-// tiles of 128 keys are shared through LDS (the ping-pong of the ring kernels, with the rows of
-// a tile fetched block by block).  One of up to 32 rows (a decoding sequence) is a narrow
-// tile: 8 waves hold the same rows and take 32 keys each in turn, out of LDS of their own,
-// with no barrier until their results meet.
+// Rows.  The query heads of a kv head are packed token-major: row r of a source (a sequence's new
+// tokens, or all the tokens behind one prefix) is token r / rep, head r % rep of the group.  A long
+// source is cut into wide tiles of 256 rows, 32 a wave, whose K and V tiles of 128 keys are shared
+// through LDS: the ping-pong of the ring kernels, with the rows of a tile fetched block by block,
+// bound by the MFMA rate and the softmax's VALU work beside it (16384 tokens of 32/8 heads of 128
+// dims: 1.90 ms, 1157 TFLOP/s; the ring kernel on contiguous K and V 1240-1280).  A short one is cut
+// into narrow tiles of 32 rows: 8 waves hold the same rows and take 32 keys each in turn, out of
+// LDS of their own, with no barrier until their results meet, bound by HBM reads (64 sequences of
+// up to 16384 tokens, 32/8 heads: 592 us, 5.7 TB/s) or, in short steps, by the chain of loads that
+// leads to the keys.  64 sequences behind one prefix of 16384 tokens: 56 us, where every one reading
+// it for itself would take some 700.
 //
 // Work.  The (tile, kv head) units of each kind are laid end to end on an axis of modelled time,
 // the wide ones by kv head first (workgroups of one XCD then read one head's K and V).  Every XCD
 // gets an eighth of both, and its workgroups, one a CU, equal parts of that: a unit that falls to
 // several is joined afterwards (step_join_kernel), as is a row's part behind a shared prefix with
-// its own part.  The
-// plan (step_plan_kernel) lays both axes out once a step for the calls of all layers.
+// its own part.  The plan (step_plan_kernel) lays both axes out once a step for the calls of all
+// layers.
+//
+// Rounding.  Scores, statistics, sums and joins are fp32.  A weight enters the product with V in 16
+// bits: one term in wide tiles of 16-bit output (its rounding is as large as the output's own;
+// errors add to 1.4 times that), two in narrow ones, whose matrix cores wait for HBM anyway, and for
+// fp32 output as many as hold 22 bits or more (two of f16, three of bf16).
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -65,7 +74,7 @@ struct StepTile {
   int32_t list;             // tokens through the list
   int32_t pad[3];
 };
-static_assert(sizeof(StepTile) == 64, "a tile is a cache line");
+static_assert(sizeof(StepTile) == 64, "read_tile counts 16 words");
 
 // A token behind a shared prefix: its own narrow tile, and its rows in the prefix's tiles.
 struct StepShared {
