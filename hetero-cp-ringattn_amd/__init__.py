@@ -1074,6 +1074,17 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, pool, slots, positions=None
 # ---------------------------------------------------------------------------------
 # (12) attention of a serving step
 # ---------------------------------------------------------------------------------
+def _table_rows(name, t, dev):
+    """(rows, entries, stride) of a table [rows, entries] int32, checked."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or t.dtype != _torch().int32 or t.get_device() != dev or (strides[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{name} must be an int32 tensor of contiguous rows on {_place(dev)}")
+    rows, width = shape
+    if rows > 1 and strides[0] < width:  # an expanded row, say: the kernels want rows that stand apart
+        raise ValueError(f"the rows of {name} must not overlap")
+    return rows, width, strides[0] if rows > 1 else width
+
+
 def _step_args(q, pool, block_tables, prefix_tables, prefix_lens=None, scale=None):
     """(descriptor, pool, number of prefixes, hcp_decode_shard of them or None, GPU), checked."""
     pp = paged_pool(pool)
@@ -1081,17 +1092,14 @@ def _step_args(q, pool, block_tables, prefix_tables, prefix_lens=None, scale=Non
     hq, _, d = q.shape
     if q.dtype != dtype or q.get_device() != dev:
         raise ValueError(f"q must be {dtype} on {_place(dev)}")
-    b, width = block_tables.shape if block_tables.dim() == 2 else (0, 0)
-    _decode_tables("block_tables", block_tables, None, b, dev)
+    b, width, stride = _table_rows("block_tables", block_tables, dev)
     n, shard = 0, None
     if prefix_tables is not None and prefix_tables.shape[0] > 0:
-        n, m = prefix_tables.shape if prefix_tables.dim() == 2 else (0, 0)
-        _decode_tables("prefix_tables", prefix_tables, None, n, dev)
+        n, m, step = _table_rows("prefix_tables", prefix_tables, dev)
         if prefix_lens is not None:
             _want("prefix_lens", prefix_lens, _torch().int32, (n,), dev)
-        shard = DecodeShard(prefix_tables.data_ptr(), max(prefix_tables.stride(0), m), m,
-                            None if prefix_lens is None else prefix_lens.data_ptr(), 0)
-    desc = DecodeDesc(dtype_code(dtype), b, hq, pp.num_kv_heads, d, 0, 0, 0, max(block_tables.stride(0), width), width,
+        shard = DecodeShard(prefix_tables.data_ptr(), step, m, None if prefix_lens is None else prefix_lens.data_ptr(), 0)
+    desc = DecodeDesc(dtype_code(dtype), b, hq, pp.num_kv_heads, d, 0, 0, 0, stride, width,
                       scale if scale is not None else 1.0 / math.sqrt(d))
     return desc, pp, n, shard, dev
 

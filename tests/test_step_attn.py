@@ -504,3 +504,17 @@ def test_bindings_refuse_what_does_not_fit(hcp):
     for kw in (dict(out=torch.zeros(4, 3, 32)), dict(lse=torch.zeros(4, 2)), dict(lse=torch.zeros(4, 3).half()), dict(plan=plan[::2]), dict()):
         with pytest.raises(ValueError):
             H.step_attn(x["q"], x["pool"], x["tables"], kw.pop("plan", plan), x["ptables"], **kw)
+
+
+def test_bindings_refuse_tables_whose_rows_overlap(hcp):
+    """An expanded row, or rows closer than their length, would be read at other places than the tensor's."""
+    step = Step([1, 2], [3, 4], 4, 2, 64, ids=[0, -1], plens=[5, 3])
+    x = step.device("cpu")
+    for key in ("tables", "ptables"):
+        row = torch.zeros(64, dtype=torch.int32)
+        for bad in (row[:5].expand(2, 5), row.as_strided((2, 5), (4, 1))):
+            y = dict(x, **{key: bad})
+            with pytest.raises(ValueError, match="overlap"):
+                H.step_attn_plan(*(y[k] for k in ("q", "pool", "tables", "starts", "lens", "ptables", "ids", "plens")))
+            with pytest.raises(ValueError, match="overlap"):
+                H.step_attn(y["q"], y["pool"], y["tables"], torch.zeros(1 << 16, dtype=torch.uint8), y["ptables"])
