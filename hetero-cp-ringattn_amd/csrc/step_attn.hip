@@ -291,12 +291,20 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanKernelArgs 
     if (n < 0 || n > a.s.max_prefix) flag();
   }
   if (tid < 2) n_cut[tid] = more[tid] = 0;
-  __syncthreads();
+  int falls = 0;
+  for (int b = tid; b < B; b += kPlanThreads) falls |= a.token_starts[b + 1] < a.token_starts[b];
+  falls = __syncthreads_or(falls);
   for (int b = tid; b < B; b += kPlanThreads) {
     int t0 = a.token_starts[b], t1 = a.token_starts[b + 1];
     if (t0 < 0 || t1 < t0) {
       flag();
       t0 = t1 = 0;
+    }
+    // Where the starts fall somewhere, a later sequence may name the tokens of an earlier one again: it
+    // keeps those behind all earlier starts, since the plan has room for every token once.
+    if (falls) {
+      for (int c = 0; c < b; ++c) t0 = max(t0, a.token_starts[c]);
+      t1 = max(t0, t1);
     }
     int64_t len = a.seq_lens[b];
     if (len < 0 || len > a.s.max_own) {

@@ -853,7 +853,8 @@ int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float e
  * (descriptor, tokens, causal, table lengths, num_prefixes; desc->t0 / t1 are ignored, as is
  * prefixes->max_len).  A plan of another shape sets device error bit 3 and writes nothing.
  * Lengths outside their tables, decreasing token_starts and prefix ids outside
- * [-1, num_prefixes) set bit 3 too and are cut to what fits (an id: none).  A block id outside
+ * [-1, num_prefixes) set bit 3 too and are cut to what fits (an id: none; where token_starts
+ * fall, a later sequence keeps the tokens behind all earlier starts).  A block id outside
  * [0, num_blocks) sets bit 0, and its tokens count as rows of zeros.
  * dtype BF16 or F16; head_dim a multiple of 8 up to 128; block_size a multiple of 16; up to
  * 4096 sequences and 1024 prefixes; Hq / Hkv up to 256.  q and out 16-byte aligned with strides

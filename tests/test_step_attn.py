@@ -348,6 +348,25 @@ def test_bad_ids_lengths_and_plans_set_their_flags(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("starts", [[0, 200, 0, 200, 0, 200, 0, 200, 0], [0, 30, 10, 200, 199, 200, -4, 200, 200],
+                                    [0, 3, 0, 4, 1, 5, 2, 200, 0]])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_starts_that_fall_give_every_token_to_one_sequence(gpu, starts, prefix):
+    """What earlier sequences have is left out of later ones: the plan has room for every token once."""
+    new = [0 if t0 < 0 or t1 < t0 else max(t1 - max(starts[: b + 1]), 0) for b, (t0, t1) in enumerate(zip(starts, starts[1:]))]
+    assert sum(new) == 200
+    step = Step(new, [260 + 7 * b for b in range(8)], 8, 2, 64, ids=[b // 2 % 2 for b in range(8)] if prefix else None,
+                plens=[40, 300] if prefix else (), seed=17)
+    x = step.device()
+    x["starts"] = torch.tensor(starts, dtype=I32, device="cuda")
+    size = H.step_attn_plan_size(x["q"], x["pool"], x["tables"], x["ptables"])
+    room = torch.full((size + (1 << 20),), 90, dtype=torch.uint8, device="cuda")
+    plan = H.step_attn_plan(x["q"], x["pool"], x["tables"], x["starts"], x["lens"], x["ptables"], x["ids"], x["plens"], plan=room[:size])
+    assert H.fetch_device_errors() == 8 and bool((room[size:] == 90).all())
+    check(step, *H.step_attn(x["q"], x["pool"], x["tables"], plan, x["ptables"]))
+
+
+@pytest.mark.gpu
 def test_two_calls_at_once_share_a_plan(gpu):
     """One plan, two streams, each with a workspace of its own."""
     step = Step([1, 1, 300, 5], [9000, 700, 2000, 40], 16, 2, 128, ids=[0, 0, -1, 0], plens=[3000], seed=13)
