@@ -2155,10 +2155,10 @@ int hcp_step_attn(const hcp_paged_decode_desc* desc, const hcp_paged_pool* pool,
     require(desc->scale > 0.f && desc->scale <= FLT_MAX, "scale must be positive");
     require(out_dtype == desc->dtype || out_dtype == kF32, "out_dtype must be dtype or F32");
     require(block_tables != nullptr && (num_prefixes == 0 || prefixes->block_tables != nullptr), "null block tables");
+    if (tokens == 0) return;
     const size_t need = step_work_bytes(s);
     if (workspace == nullptr || workspace_bytes < need) throw Error(-6, "workspace too small: need " + std::to_string(need) + " bytes");
     require(aligned(workspace, 256), "the workspace must be 256-byte aligned");
-    if (tokens == 0) return;
     check_view(q, "q", tokens);
     check_view(out, "out", tokens);
     require(mfma_layout_ok(q), "q must be 16-byte aligned with strides multiple of 8");

@@ -161,7 +161,7 @@ WorkLayout work_layout(const StepShape& s, int workers) {
   w.own_lse = take(rows);
   w.pre_o = take(rows * s.d);
   w.pre_lse = take(rows);
-  w.bytes = at;
+  w.bytes = std::max<size_t>(at, 256);  // without tokens too: a size of 0 says that the shape is bad
   return w;
 }
 

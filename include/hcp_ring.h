@@ -860,7 +860,8 @@ int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float e
  * 4096 sequences and 1024 prefixes; Hq / Hkv up to 256.  q and out 16-byte aligned with strides
  * of whole 16 bytes.  plan and workspace: DEVICE memory, 256-byte aligned, of the bytes that
  * the size queries report (0 for a bad shape); the workspace is scratch of one call, the plan
- * is only read.
+ * is only read.  A step of no tokens is a shape like any other: its plan is made, and
+ * hcp_step_attn has nothing to do and asks for no workspace.
  * ------------------------------------------------------------------------------- */
 size_t hcp_step_attn_plan_size(const hcp_paged_decode_desc* desc, int64_t tokens, int32_t num_prefixes);
 
