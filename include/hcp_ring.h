@@ -843,6 +843,8 @@ int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float e
  * Slots past a length are not read.  A K row that is not finite reaches only the tokens that see
  * it; a V row that is not finite may reach the new tokens before it, too, of its own sequence
  * alone (a weight of 0 times it).
+ * Scores (q k^T scale) have to lie within 2^20 of 0: past that fp32 scores are steps of an eighth
+ * and more apart, and a row's weights, and whether it counts as empty, undefined.
  *
  * A prefix is read once for all the tokens behind it of sequences with up to 32 / (Hq / Hkv)
  * new tokens; longer runs of tokens read it for themselves.

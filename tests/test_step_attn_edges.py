@@ -35,3 +35,61 @@ def test_an_empty_step_runs(gpu, prefix):
     out, lse = step.run()
     assert out.shape == (8, 0, 64) and lse.shape == (8, 0)
     assert H.fetch_device_errors() == 0
+
+
+# ---------------------------------------------------------------------------------
+# the range of scores
+# ---------------------------------------------------------------------------------
+RANGE = {"narrow": dict(new=[1, 1, 5], lens=[300, 33, 2000]), "cut": dict(new=[1], lens=[20000]),
+         "prefix": dict(new=[1] * 40, lens=[200 + b for b in range(40)], ids=[0] * 40, plens=[3000]),
+         "wide": dict(new=[1500, 700], lens=[3500, 2700])}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("kind", RANGE)
+def test_scores_of_the_largest_size(gpu, kind, sign, dtype, f32):
+    """Scores of one sign, 2^19.5 in size, that rise by 5 (2^7.2 of a weight) every 128 keys, eight
+    times over, and one key of each sequence 29 above all others.  Dim 0 gives the size and dim 1
+    the steps: every product and sum is exact in fp32 (multiples of 4 below 2^23).
+
+    The other keys weigh up to 20000 e^-29 < 2^-27 of a row together, and what their own weights are
+    off by (parts are joined by LSEs that are rounded to 2^-5) leaves them below 2^-25.  The winner's
+    weight is within 2^-19 of 1 (exponential, sums, reciprocal) and enters the product within
+    eps / 2 of it (one term); the output rounds once more.  The LSE is a product of the score's fp32
+    image with ln 2, joined and rounded: 8 roundings of its size."""
+    kw = RANGE[kind]
+    step = Step(hq=8, hkv=2, d=64, dtype=dtype, seed=31, **kw)
+    step.q.zero_()
+    step.q[..., 0], step.q[..., 1] = sign * 1024.0, 32.0
+    k = step.pool[0]
+    k[~torch.isnan(k)] = 0.0
+
+    def keys(table, n, best):
+        j = torch.arange(n)
+        at = torch.from_numpy(table)[j // step.bs].long(), j % step.bs
+        k1 = 1.25 * (j // 128 % 8)
+        if best is not None:
+            k1[best] = 16.0
+        k[at[0], at[1], :, 0] = 5632.0
+        k[at[0], at[1], :, 1] = k1.to(k.dtype)[:, None]
+        return at
+
+    won = torch.zeros(step.tokens, 2, 64, dtype=torch.float64)
+    for b, n in enumerate(step.new):
+        best = int(step.lens[b] - n)  # the last key that all new tokens see
+        at = keys(step.tables[b], int(step.lens[b]), best)
+        won[int(step.starts[b]): int(step.starts[b]) + int(n)] = step.pool[1, at[0][best], at[1][best]].double()
+    for p, n in enumerate(step.plens):
+        keys(step.ptables[p], int(n), None)
+    won = won.repeat_interleave(4, 1).permute(1, 0, 2)
+    out = torch.empty(8, step.tokens, 64, dtype=torch.float32, device="cuda") if f32 else None
+    out, lse = step.run(out=out)
+    assert H.fetch_device_errors() == 0
+    got, eps = out.double().cpu(), torch.finfo(out.dtype).eps
+    bound = (torch.finfo(step.q.dtype).eps / 2 + 2.0 ** -19 + eps / 2) * won.abs() + 2.0 ** -25 * 6.0
+    assert bool(((got - won).abs() <= bound).all()), float(((got - won).abs() / bound).nan_to_num(1e30).max())
+    want = (sign * 1024.0 * 5632.0 + 32.0 * 16.0) / 8.0  # ln of 1 + 2^-27 behind it
+    assert bool(((lse.double().cpu() - want).abs() <= 8 * 2.0 ** -24 * abs(want)).all())
