@@ -846,8 +846,9 @@ int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float e
  * Scores (q k^T scale) have to lie within 2^20 of 0: past that fp32 scores are steps of an eighth
  * and more apart, and a row's weights, and whether it counts as empty, undefined.
  *
- * A prefix is read once for all the tokens behind it of sequences with up to 32 / (Hq / Hkv)
- * new tokens; longer runs of tokens read it for themselves.
+ * A prefix is read once for all the tokens behind it of sequences with up to 128 / (Hq / Hkv) new
+ * tokens (none where Hq / Hkv is above 128), if there are two such sequences at least; a lone
+ * sequence and longer runs of tokens read it for themselves.
  *
  * hcp_step_attn_plan lays the step's work out over the GPU from the lengths (DEVICE memory,
  * nothing is read on the host: a captured graph follows them); hcp_step_attn then takes the

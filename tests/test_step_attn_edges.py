@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import hcp_ring_amd as H
-from test_step_attn import AT, DESC, POOL, Step
+from test_step_attn import AT, DESC, POOL, Step, check
 
 
 # ---------------------------------------------------------------------------------
@@ -93,3 +93,22 @@ def test_scores_of_the_largest_size(gpu, kind, sign, dtype, f32):
     assert bool(((got - won).abs() <= bound).all()), float(((got - won).abs() / bound).nan_to_num(1e30).max())
     want = (sign * 1024.0 * 5632.0 + 32.0 * 16.0) / 8.0  # ln of 1 + 2^-27 behind it
     assert bool(((lse.double().cpu() - want).abs() <= 8 * 2.0 ** -24 * abs(want)).all())
+
+
+# ---------------------------------------------------------------------------------
+# which sequences share a prefix's read
+# ---------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,heads,shared", [
+    ([32, 1, 32], (8, 2), 65),      # 128 rows at most: all three
+    ([33, 1, 32], (8, 2), 33),      # 132 rows: reads the prefix for itself
+    ([33, 1, 40], (8, 2), 0),       # one sequence is left, and reads it alone
+    ([1, 0, 33], (8, 2), 0),
+    ([1, 1, 1], (128, 1), 3), ([2, 1, 1], (128, 1), 2), ([1, 1, 1], (130, 1), 0), ([3, 1, 2], (256, 1), 0)])
+def test_what_shares_a_prefix(gpu, new, heads, shared):
+    """The plan's own count of the tokens behind shared prefixes (word 14 of its head), and the outputs."""
+    step = Step(new, [70, 9, 90], *heads, 64, ids=[0, 0, 0], plens=[300], seed=32)
+    x = step.device()
+    plan = H.step_attn_plan(x["q"], x["pool"], x["tables"], x["starts"], x["lens"], x["ptables"], x["ids"], x["plens"])
+    assert int(plan[:64].view(torch.int32)[14]) == shared
+    check(step, *H.step_attn(x["q"], x["pool"], x["tables"], plan, x["ptables"]))
