@@ -2097,7 +2097,9 @@ StepShape step_shape(const hcp_paged_decode_desc* d, int64_t tokens, int32_t cau
     require(prefixes->table_len <= (int64_t(1) << 30) / bs, "prefix tables of more than 2^30 tokens");
     s.max_prefix = prefixes->table_len * bs;
   }
-  // a plan counts (tile, kv head) units in 32 bits: at most a tile every 16 rows and four a sequence
+  // A plan counts (tile, kv head) units in 32 bits.  It has room for a wide tile every 256 rows and a narrow
+  // one every 32, twice where there are prefixes (own rows and shared ones): 9 in 128 rows, and four a
+  // sequence for tiles that are not full.  Checked with 16 in 128.
   require((tokens * (s.hq / s.hkv) / 8 + 4 * static_cast<int64_t>(s.batch)) * s.hkv < (int64_t(1) << 30), "too many rows for one step");
   return s;
 }

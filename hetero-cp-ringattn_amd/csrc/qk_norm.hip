@@ -9,8 +9,9 @@
 // Bound by HBM: a row is read once and written once, ~10 flops an element.  A lane holds two
 // chunks of C elements r/2 apart (16 bytes each), so that in the halves form both ends of a
 // plane are in one lane and nothing is exchanged but the sum of squares; a row takes
-// D / (2 C) lanes, a wave 64 / that rows of one token at a time, whose cos, sin and weights
-// its lanes hold for all of them, and the next run's rows load while one is turned.  Stores
+// D / (2 C) lanes, a wave 64 / that rows of one token at a time.  Its lanes hold the token's cos and
+// sin for all of them and load the weights for every run (from the L1: q's and k's differ); the next
+// run's rows load while one is turned.  Stores
 // stream (nt): 32768 tokens of 32/8 heads of 128 dims take 189 us so, 198 with plain ones (805 MB
 // of rows and 17 MB of angles: 4.35 TB/s; a copy of 2 GiB reaches 4.97), 2048 tokens 12 and 14.5.
 // Streaming loads as well: 184 and 11-14 (what the projection wrote last is still in the caches).
