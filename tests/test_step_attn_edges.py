@@ -112,3 +112,81 @@ def test_what_shares_a_prefix(gpu, new, heads, shared):
     plan = H.step_attn_plan(x["q"], x["pool"], x["tables"], x["starts"], x["lens"], x["ptables"], x["ids"], x["plens"])
     assert int(plan[:64].view(torch.int32)[14]) == shared
     check(step, *H.step_attn(x["q"], x["pool"], x["tables"], plan, x["ptables"]))
+
+
+# ---------------------------------------------------------------------------------
+# the bits of a softmax weight
+# ---------------------------------------------------------------------------------
+# Two keys a row, and scores that are one product each, exact in fp32 and in [-2, 2] (dim 0 alone, a scale
+# of 1/8).  Units of 2^-24, an error of a weight relative to it: log2 e in fp32 times the distance of two
+# scores, 4; the exponent's rounding (at most 8 + 7 in size: 2^-21 of a factor, times ln 2), 6; the
+# exponential, 2^-22: 4.  Normalised, twice that: 28.  The sum of two weights, its reciprocal and the
+# product with it, 4; two keys of up to three terms added up, 6.  38 in all, below 2^-18 of A = sum w |v|,
+# beside what a weight of `terms` 16-bit terms is off by, (eps / 2)^terms, and the output's own half step.
+# Nothing is joined: a unit of two keys has one step.
+def _two_keys(new, dtype, out):
+    """A step over two keys a sequence, V of the second the negative of the first's, so that an output of
+    close weights is small beside A and its own rounding hides nothing."""
+    step = Step(new, [2] * len(new), 8, 2, 64, dtype=dtype, causal=False, seed=33)
+    g = torch.Generator().manual_seed(34)
+    step.q.zero_()
+    step.q[..., 0] = (1 + torch.rand(step.tokens, 8, generator=g)).to(step.q.dtype)
+    for b in range(len(new)):
+        k, v = (step.pool[p, int(step.tables[b, 0])] for p in (0, 1))
+        k[:2] = 0.0
+        k[:2, :, 0] = ((torch.rand(2, 2, generator=g) - 0.5) * (16 if out == "f32" else 1)).to(k.dtype)
+        v[1] = -v[0]
+    return step
+
+
+def _weights_and_values(step):
+    """(w [Hq, T, 2], v [Hq, T, 2, D]) in fp64."""
+    seq = torch.repeat_interleave(torch.arange(len(step.new)), torch.from_numpy(step.new))
+    k, v = (step.pool[p, torch.from_numpy(step.tables[:, 0]).long(), :2].double()[seq].repeat_interleave(4, 2).permute(2, 0, 1, 3)
+            for p in (0, 1))
+    return torch.softmax((step.q.double().permute(1, 0, 2)[:, :, None] * k).sum(-1) / 8, -1), v
+
+
+def _bound(step, w, v, terms, out):
+    half = torch.finfo(step.q.dtype).eps / 2
+    o, mag = (w[..., None] * v).sum(2), (w[..., None] * v.abs()).sum(2)
+    b = (2.0 ** -18 + half ** terms) * mag + torch.finfo(out).eps / 2 * o.abs()
+    return o, b + (2.0 ** -25 if out == torch.float16 else 0.0)
+
+
+# kind: (new tokens, terms of a weight by type of the rows and of the output)
+KINDS = {"narrow": ([1, 1, 3, 5, 7, 1, 2, 32], {("bf16", "f32"): 3, ("f16", "f32"): 2, ("bf16", "same"): 2, ("f16", "same"): 2}),
+         "wide": ([6000, 1, 3], {("bf16", "f32"): 3, ("f16", "f32"): 2})}
+WEIGHTS = [(kind, dtype, out, terms) for kind, (_, t) in KINDS.items() for (dtype, out), terms in t.items()]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype,out,terms", WEIGHTS)
+def test_bits_of_a_weight(gpu, kind, dtype, out, terms):
+    step = _two_keys(KINDS[kind][0], dtype, out)
+    x = step.device()
+    otype = torch.float32 if out == "f32" else step.q.dtype
+    plan = H.step_attn_plan(x["q"], x["pool"], x["tables"], x["starts"], x["lens"], causal=False)
+    assert (int(plan[:64].view(torch.int32)[12]) > 0) == (kind == "wide")  # word 12 of a plan's head: wide tiles
+    got, _ = H.step_attn(x["q"], x["pool"], x["tables"], plan, causal=False,
+                         out=torch.empty(8, step.tokens, 64, dtype=otype, device="cuda"))
+    o, bound = _bound(step, *_weights_and_values(step), terms, otype)
+    worst = ((got.double().cpu() - o).abs() / bound).max()
+    assert float(worst) <= 1.0, float(worst)
+    assert H.fetch_device_errors() == 0
+
+
+@pytest.mark.parametrize("kind,dtype,out,terms", WEIGHTS)
+def test_a_term_less_would_be_seen(kind, dtype, out, terms):
+    """The oracle with weights of one term less is outside the bound, with all of them within."""
+    step = _two_keys(KINDS[kind][0], dtype, out)
+    otype = torch.float32 if out == "f32" else step.q.dtype
+    w, v = _weights_and_values(step)
+    o, bound = _bound(step, w, v, terms, otype)
+    for n, seen in ((terms, False), (terms - 1, True)):
+        kept, rest = torch.zeros_like(w), (w * 100).float().double()  # as beside a maximum taken elsewhere
+        for _ in range(n):
+            t = rest.to(step.q.dtype).double()
+            kept, rest = kept + t, rest - t
+        got = ((kept / 100)[..., None] * v).sum(2).to(otype).double()
+        assert bool(((got - o).abs() > bound).any()) == seen, n
