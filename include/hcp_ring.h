@@ -843,6 +843,12 @@ int hcp_qk_norm_rope_append(const hcp_qkv_desc* desc, int32_t rope_dims, float e
  * Slots past a length are not read.  A K row that is not finite reaches only the tokens that see
  * it; a V row that is not finite may reach the new tokens before it, too, of its own sequence
  * alone (a weight of 0 times it).
+ * Scores, sums and statistics are fp32, and parts of a row are joined by their fp32 LSEs.  A softmax
+ * weight enters the product with V in 16-bit terms: with F32 out, as many as hold 22 bits or
+ * more; with 16-bit out, two in tiles of 32 rows and one (off by half a step of dtype, as out
+ * itself) in tiles of 256.  Which tiles a sequence gets, and where its keys are cut into parts, goes by
+ * the whole step: the same step gives the same bits, but beside other sequences a row may
+ * differ by these roundings, with 16-bit out by eps / 2 of the sum of w |v|, and out's own.
  * Scores (q k^T scale) have to lie within 2^20 of 0: past that fp32 scores are steps of an eighth
  * and more apart, and a row's weights, and whether it counts as empty, undefined.
  *

@@ -190,3 +190,35 @@ def test_a_term_less_would_be_seen(kind, dtype, out, terms):
             kept, rest = kept + t, rest - t
         got = ((kept / 100)[..., None] * v).sum(2).to(otype).double()
         assert bool(((got - o).abs() > bound).any()) == seen, n
+
+
+# ---------------------------------------------------------------------------------
+# the same step, the same bits
+# ---------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("kw", [
+    dict(new=[1], lens=[30000]), dict(new=[1] * 50 + [5] * 9, lens=[300 + 17 * b for b in range(59)], ids=[0] * 40 + [1] * 19, plens=[4000, 333]),
+    dict(new=[1] * 9 + [2000, 1100], lens=[900 + 300 * b for b in range(9)] + [3000, 1100], ids=[0] * 5 + [-1] * 5 + [0], plens=[700])])
+def test_the_same_step_gives_the_same_bits(gpu, kw, dtype, f32):
+    """Cut units and shared prefixes, by the same plan and by others of the same lengths, whatever the
+    workspace, the plan's memory and the outputs held before."""
+    step = Step(hq=8, hkv=2, d=128, dtype=dtype, seed=35, **kw)
+    x = step.device()
+    out = torch.empty(8, step.tokens, 128, dtype=torch.float32 if f32 else step.q.dtype, device="cuda")
+    lse = torch.empty(8, step.tokens, device="cuda")
+    ws = torch.empty(H.step_attn_workspace_size(x["q"], x["pool"], x["tables"], x["ptables"]), dtype=torch.uint8, device="cuda")
+    plan = torch.empty(H.step_attn_plan_size(x["q"], x["pool"], x["tables"], x["ptables"]), dtype=torch.uint8, device="cuda")
+    first = None
+    for i, fill in enumerate((0, 255, 0x3f, 255)):
+        for t in (ws, out.view(torch.uint8), lse.view(torch.uint8)):
+            t.fill_(fill)
+        if i % 2 == 0:
+            plan.fill_(fill)
+            H.step_attn_plan(x["q"], x["pool"], x["tables"], x["starts"], x["lens"], x["ptables"], x["ids"], x["plens"], plan=plan)
+        H.step_attn(x["q"], x["pool"], x["tables"], plan, x["ptables"], out=out, lse=lse, workspace=ws)
+        got = out.clone(), lse.clone()
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first)), i
+    check(step, *first, terms=2 if f32 else 1)
