@@ -132,3 +132,15 @@ def test_more_tokens_than_one_grid_takes(gpu):
         ref, mag = reference(src, w, cos, sin, d, False, 1e-6)
         check(got, ref.cpu(), mag.cpu(), torch.bfloat16)
     assert H.fetch_device_errors() == 0
+
+
+@pytest.mark.gpu
+def test_no_tokens(gpu):
+    """Steps without tokens come through the bindings too."""
+    x, wq, wk, pos, tab = device_inputs(46, 4, 2, 0, 64, torch.bfloat16, 64)
+    q, k, v = parts(x, 4, 2)
+    pool = torch.ones(2, 2, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+    qo, ko = H.qk_norm_rope(q, k, wq, wk, pos, tab)
+    qa = H.qk_norm_rope_append(q, k, v, wq, wk, pool, pos, pos, tab)
+    assert qo.shape == qa.shape == (4, 0, 64) and ko.shape == (2, 0, 64)
+    assert bool((pool == 1).all()) and H.fetch_device_errors() == 0
